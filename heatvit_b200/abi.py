@@ -35,6 +35,15 @@ HV_ERR_CUDA = 4
 HV_ERR_NOMEM = 5
 HV_ERR_STATE = 6
 
+# element types and device error bits of the decode operators
+HV_BF16 = 0
+HV_F16 = 1
+HV_F32 = 2
+HV_DECODE_BAD_PAGE = 1
+HV_DECODE_BAD_POSITION = 2
+HV_DECODE_BAD_LENGTH = 4
+HV_DECODE_STALLED = 8
+
 WARN_HEAD_DEN_ZERO = 1
 WARN_PACKAGE_DEN_ZERO = 2
 WARN_LN_NEG_VARIANCE = 4

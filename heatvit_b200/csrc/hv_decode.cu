@@ -1,0 +1,45 @@
+// hv_decode.cu — the decode operators' device error word.
+#include <atomic>
+
+#include "hv_decode.cuh"
+
+namespace hv {
+namespace {
+
+__device__ int g_decode_error;
+
+constexpr int MAX_DEVICES = 64;
+std::atomic<int *> g_address[MAX_DEVICES];
+
+}  // namespace
+
+namespace dec {
+
+int *error_word() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return nullptr;
+    int *p = g_address[dev].load(std::memory_order_acquire);
+    if (!p) {
+        void *v = nullptr;
+        if (cudaGetSymbolAddress(&v, g_decode_error) != cudaSuccess) return nullptr;
+        p = (int *)v;
+        g_address[dev].store(p, std::memory_order_release);
+    }
+    return p;
+}
+
+}  // namespace dec
+}  // namespace hv
+
+extern "C" int hv_decode_error(int *bits) {
+    using namespace hv;
+    if (!bits) return fail(HV_ERR_VALUE, "null argument");
+    int *p = dec::error_word();
+    if (!p) return fail(HV_ERR_CUDA, "cannot resolve the device error word");
+    const int zero = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpy(bits, p, sizeof(int), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && *bits) e = cudaMemcpy(p, &zero, sizeof(int), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "decode error word: %s", cudaGetErrorString(e));
+    return HV_OK;
+}

@@ -8,6 +8,9 @@
 
 namespace hv {
 
+// Sets hv_last_error() of the calling thread and returns `code`.
+int fail(int code, const char *fmt, ...);
+
 // LayerNorm constants of one LN layer (nonlinear.py:136-186), host-derived.
 struct LnParams {
     const int8_t *gamma, *beta;    // [192]

@@ -23,16 +23,18 @@
 using namespace hv;
 
 namespace {
-
 thread_local char g_err[512] = "";
+}
 
-int fail(int code, const char *fmt, ...) {
+int hv::fail(int code, const char *fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
     va_end(ap);
     return code;
 }
+
+namespace {
 
 #define CUDA_TRY(expr)                                                                      \
     do {                                                                                    \

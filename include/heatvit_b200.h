@@ -390,6 +390,84 @@ HV_API int hv_token_selector(hv_model *model, int selector_index, const int8_t *
 HV_API int hv_selector_h2(hv_model *model, int selector_index, const int8_t *d_x,
                           const int32_t *d_offsets, int images, int8_t *d_h2, void *stream);
 
+/* ---- decode operators ------------------------------------------------------------
+ * The serving step of a language decoder that reads the encoder's tokens: floating
+ * point, with no counterpart in the reference.  They enqueue on `stream` and return;
+ * none allocates, synchronises or keeps anything between calls.  Strides are in elements
+ * and the innermost dimension is always contiguous.  What only the device can see (a page
+ * number outside the cache, a position past a table, a bounded wait that gave up) faults
+ * nothing: the access is left out, and a bit is set in the device's error word. */
+#define HV_BF16 0
+#define HV_F16 1
+#define HV_F32 2
+
+#define HV_DECODE_BAD_PAGE 1     /* a page table entry outside [0, num_pages): not read, not written */
+#define HV_DECODE_BAD_POSITION 2 /* a position, or a sequence, past the page table or the rotation table */
+#define HV_DECODE_BAD_LENGTH 4   /* a length above max_pages * page_size: taken as that */
+#define HV_DECODE_STALLED 8      /* a GEMM's bounded wait gave up: that output is invalid */
+
+/* Read and clear the current device's error word (synchronises with the device). */
+HV_API int hv_decode_error(int *bits);
+
+/* h = x + residual; residual_out = h; y = h * rsqrt(mean(h^2) + eps) * weight, and y in e4m3
+ * with a scale for each 128 channels of a row: scale = max(amax |y|, 2^-100) / 448,
+ * q = e4m3(y / scale).  Sums in 32 bits; the norm is of the unrounded h.
+ *   d_x, d_residual, d_residual_out [rows][dim], d_weight [dim], all of `dtype`; d_residual
+ *   and d_residual_out both NULL for a plain norm, and may be the same buffer.
+ *   d_q [rows][dim] e4m3; the scale of row r, group g at r * row stride + g * group stride.
+ * dim in [1, 32768]. */
+HV_API int hv_add_rmsnorm_fp8(const void *d_x, int64_t x_stride, const void *d_residual, int64_t residual_stride,
+                              const void *d_weight, int64_t rows, int dim, int dtype, float eps,
+                              void *d_residual_out, int64_t residual_out_stride, void *d_q, int64_t q_stride,
+                              float *d_scale, int64_t scale_row_stride, int64_t scale_group_stride, void *stream);
+
+/* Keys and values of new tokens into a paged cache, q and k rotated by position.
+ * Token t of sequence d_seq_ids[t] (t itself when NULL) at d_positions[t] is stored in page
+ * d_page_table[seq][position / page_size], slot position % page_size.  A negative position
+ * marks a padding token: nothing is stored, its q_out row is zeros.  The first `rot` elements of
+ * each q and k head turn in pairs, (i, i + rot/2) or, interleaved, (2i, 2i + 1); d_rope
+ * [rope_rows][rot] float holds rot/2 cosines, then rot/2 sines, for each position.  rot = 0: no
+ * rotation, d_rope unused.  heads = 0: no q. */
+typedef struct hv_append_args {
+    const void *d_q, *d_k, *d_v;             /* [tokens][heads or kv_heads][dim] */
+    void *d_q_out;                           /* [tokens][heads][dim], may be d_q */
+    void *d_k_cache, *d_v_cache;             /* [num_pages][page_size][kv_heads][dim], by strides */
+    const float *d_rope;
+    const int32_t *d_page_table;             /* [seqs][max_pages] */
+    const int32_t *d_seq_ids, *d_positions;  /* [tokens] */
+    int64_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2]; /* token, head */
+    int64_t k_cache_strides[3], v_cache_strides[3];                     /* page, slot, head */
+    int64_t rope_stride, page_table_stride;
+    int32_t tokens, heads, kv_heads, dim, rot, interleaved, dtype;
+    int32_t num_pages, page_size, seqs, max_pages, rope_rows;
+} hv_append_args;
+HV_API int hv_append_kv(const hv_append_args *args, void *stream);
+
+/* Attention of one new token per sequence over a paged cache: softmax(scale * q K^T) V over the
+ * first d_lens[seq] cached tokens, `heads / kv_heads` query heads sharing a key head.  A length
+ * of zero (or less) gives zeros, and -inf in d_lse.
+ * dim one of 32, 64, 96, 128, 192, 256; cache rows start on 16 bytes.
+ * d_workspace: hv_paged_attention_workspace bytes, 256-byte aligned, zeroed once after it is
+ * allocated; calls of any sizes may share it one after another, calls that overlap in time not. */
+typedef struct hv_attention_args {
+    const void *d_q;                   /* [seqs][heads][dim] */
+    void *d_out;                       /* [seqs][heads][dim] */
+    float *d_lse;                      /* [seqs][heads] log-sum-exp of the scaled scores, may be NULL */
+    const void *d_k_cache, *d_v_cache; /* [num_pages][page_size][kv_heads][dim], by strides */
+    const int32_t *d_page_table;       /* [seqs][max_pages] */
+    const int32_t *d_lens;             /* [seqs] */
+    void *d_workspace;
+    int64_t workspace_bytes;
+    int64_t q_strides[2], out_strides[2], lse_strides[2]; /* sequence, head */
+    int64_t k_cache_strides[3], v_cache_strides[3];       /* page, slot, head */
+    int64_t page_table_stride;
+    int32_t seqs, heads, kv_heads, dim, dtype;
+    int32_t num_pages, page_size, max_pages;
+    float scale;
+} hv_attention_args;
+HV_API int hv_paged_attention_workspace(int dim, int64_t *bytes);
+HV_API int hv_paged_attention(const hv_attention_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
