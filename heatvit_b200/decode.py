@@ -128,6 +128,70 @@ def add_rmsnorm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None):
     return Fp8Rows(q if wide == dim else q[:, :dim], scale.t(), residual_out)
 
 
+def quantize_weight_fp8(weight):
+    """A weight [n, k] as e4m3 with a float32 scale for each 128 x 128 block, as
+    ``gemm_fp8`` takes it -> (q [n, k] with 16-byte aligned rows, scale [ceil(n/128),
+    ceil(k/128)]).  Done once, when weights are loaded."""
+    torch = _torch()
+    if weight.dim() != 2:
+        raise ValueError("weight must be 2-dimensional")
+    n, k = weight.shape
+    nb, kb = -(-n // GROUP), -(-k // GROUP)
+    w = torch.zeros((nb * GROUP, kb * GROUP), dtype=torch.float32, device=weight.device)
+    w[:n, :k] = weight
+    blocks = w.view(nb, GROUP, kb, GROUP)
+    scale = blocks.abs().amax((1, 3)).clamp_(min=2.0 ** -100) / E4M3_MAX
+    q = torch.empty((n, -(-k // 16) * 16), dtype=torch.float8_e4m3fn, device=weight.device)[:, :k]
+    q.copy_((blocks / scale[:, None, :, None]).clamp_(-E4M3_MAX, E4M3_MAX).view_as(w)[:n, :k])
+    return q, scale
+
+
+def gemm_fp8(a, a_scale, b, b_scale, out_dtype=None, out=None):
+    """``out[m, n] = sum_k a[m, k] b[n, k]`` of e4m3 operands, where a_scale [m, groups]
+    scales each 128 channels of a row of a, and b_scale [ceil(n / 128), groups] each
+    128 x 128 block of b; groups = ceil(k / 128).
+
+    Operand rows start on 16 bytes (as ``add_rmsnorm_fp8`` and ``quantize_weight_fp8``
+    lay them out); scales are float32 of any strides.  Sums in 32 bits, rounded once to
+    ``out_dtype`` (bfloat16 unless given; float16, float32) or to ``out``'s type."""
+    torch = _torch()
+    dev = a.device
+    fp8 = torch.float8_e4m3fn
+    for t, name in ((a, "a"), (b, "b")):
+        _need(t, name, 2, dev)
+        if t.dtype != fp8:
+            raise TypeError(f"{name} must be float8_e4m3fn")
+    m, k = a.shape
+    n = b.shape[0]
+    if b.shape[1] != k:
+        raise ValueError(f"K mismatch: a has {k}, b has {b.shape[1]}")
+    if k < 1:
+        raise ValueError("k must be positive")
+    groups = -(-k // GROUP)
+    for t, name, rows in ((a_scale, "a_scale", m), (b_scale, "b_scale", -(-n // GROUP))):
+        if t.device != dev:
+            raise ValueError(f"{name} must live on {dev}")
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32")
+        if t.shape != (rows, groups):
+            raise ValueError(f"{name} must be [{rows}, {groups}]")
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=dev)
+    else:
+        _need(out, "out", 2, dev)
+        if out.shape != (m, n):
+            raise ValueError(f"out must be [{m}, {n}]")
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise TypeError("out has another type than out_dtype")
+    code = _dtype_codes().get(out.dtype)
+    if code is None:
+        raise TypeError("out must be bfloat16, float16 or float32")
+    _call(lib().hv_gemm_fp8, dev, a.data_ptr(), a.stride(0), a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1),
+          b.data_ptr(), b.stride(0), b_scale.data_ptr(), b_scale.stride(0), b_scale.stride(1), m, n, k, out.data_ptr(),
+          out.stride(0), code)
+    return out
+
+
 def rope_table(positions, rot, base=10000.0, device="cuda"):
     """Cosines, then sines, of ``position * base^(-2 i / rot)``: float32 [positions, rot],
     angles in 64 bits.  Built once and kept by the caller."""

@@ -421,6 +421,17 @@ HV_API int hv_add_rmsnorm_fp8(const void *d_x, int64_t x_stride, const void *d_r
                               void *d_residual_out, int64_t residual_out_stride, void *d_q, int64_t q_stride,
                               float *d_scale, int64_t scale_row_stride, int64_t scale_group_stride, void *stream);
 
+/* e4m3 product with block scales: out[m][n] = sum over groups g of 128 along K of
+ * a_scale[m][g] * b_scale[n / 128][g] * sum_k a[m][k] b[n][k], sums in 32 bits, rounded once.
+ *   d_a [m][k], d_b [n][k] e4m3 (B as the weights' rows of output channels); rows start on 16
+ *   bytes (strides in bytes, a multiple of 16), k need not be a multiple of anything.
+ *   A scale of row r (of A) or block r (of 128 rows of B), group g at r * row stride +
+ *   g * group stride.  out_dtype HV_BF16, HV_F16 or HV_F32. */
+HV_API int hv_gemm_fp8(const void *d_a, int64_t a_stride, const float *d_a_scale, int64_t a_scale_row_stride,
+                       int64_t a_scale_group_stride, const void *d_b, int64_t b_stride, const float *d_b_scale,
+                       int64_t b_scale_row_stride, int64_t b_scale_group_stride, int64_t m, int64_t n, int k,
+                       void *d_out, int64_t out_stride, int out_dtype, void *stream);
+
 /* Keys and values of new tokens into a paged cache, q and k rotated by position.
  * Token t of sequence d_seq_ids[t] (t itself when NULL) at d_positions[t] is stored in page
  * d_page_table[seq][position / page_size], slot position % page_size.  A negative position
