@@ -53,6 +53,10 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
     const int head = is_q ? hh : is_k ? hh - a.heads : hh - a.heads - a.kv_heads;
     const int pos = a.positions[tok];
     if (pos < 0 && !is_q) return;  // a padding token stores nothing
+    if (a.rot && pos >= a.table_rows) {  // nor does one that the rotation table does not reach
+        atomicOr(a.err, HV_DECODE_BAD_POSITION);
+        return;
+    }
 
     T *dst;
     const T *src;
@@ -63,12 +67,12 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
         const int s = a.seq_ids ? a.seq_ids[tok] : tok;
         const int col = pos / a.page, slot = pos - col * a.page;
         if (s < 0 || s >= a.seqs || col >= a.max_pages) {
-            if (a.err) atomicOr(a.err, HV_DECODE_BAD_POSITION);
+            atomicOr(a.err, HV_DECODE_BAD_POSITION);
             return;
         }
         const int pg = a.pages[s * a.pages_stride + col];
         if (pg < 0 || pg >= a.num_pages) {
-            if (a.err) atomicOr(a.err, HV_DECODE_BAD_PAGE);
+            atomicOr(a.err, HV_DECODE_BAD_PAGE);
             return;
         }
         if (is_k) {
@@ -89,13 +93,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
     }
     const bool turned = c0 < rot;
     const float *tab = nullptr;
-    if (turned) {
-        if (pos >= a.table_rows) {
-            if (a.err) atomicOr(a.err, HV_DECODE_BAD_POSITION);
-            return;
-        }
-        tab = a.table + (pos < 0 ? 0 : pos) * a.table_stride;
-    }
+    if (turned) tab = a.table + (pos < 0 ? 0 : pos) * a.table_stride;
     float x0[PAIR], x1[PAIR];
     if constexpr (PAIR == 8) {
         load8(src + c0, a.dim - c0, true, x0);

@@ -499,14 +499,15 @@ extern "C" int hv_paged_attention(const hv_attention_args *p, void *stream) {
     if (p->dtype != HV_BF16 && p->dtype != HV_F16) return fail(HV_ERR_TYPE, "dtype must be HV_BF16 or HV_F16");
     if (p->seqs < 0 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads)
         return fail(HV_ERR_VALUE, "heads must be a positive multiple of kv_heads");
-    int64_t need = 0;
-    const int rc = hv_paged_attention_workspace(p->dim, &need);
-    if (rc) return rc;
+    if (!known_dim(p->dim)) return fail(HV_ERR_VALUE, "dim must be 32, 64, 96, 128, 192 or 256");
     if (p->page_size < 1 || p->num_pages < 0 || p->max_pages < 0) return fail(HV_ERR_VALUE, "bad cache geometry");
     if (p->seqs == 0) return HV_OK;
     if (!p->d_q || !p->d_out || !p->d_lens || (p->max_pages && !p->d_page_table) ||
         (p->num_pages && (!p->d_k_cache || !p->d_v_cache)))
         return fail(HV_ERR_VALUE, "null buffer");
+    int64_t need = 0;
+    const int rc = hv_paged_attention_workspace(p->dim, &need);
+    if (rc) return rc;
     if (!p->d_workspace || p->workspace_bytes < need)
         return fail(HV_ERR_VALUE, "the workspace has %lld bytes of %lld", (long long)p->workspace_bytes, (long long)need);
     if (!dec::aligned(p->d_workspace, 256)) return fail(HV_ERR_VALUE, "the workspace must be 256-byte aligned");

@@ -1,0 +1,104 @@
+"""Decode operators without a GPU: struct layouts, exports and the refusals that need no device."""
+
+import ctypes as C
+import os
+import struct
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+SYMBOLS = ("hv_decode_error", "hv_add_rmsnorm_fp8", "hv_gemm_fp8", "hv_append_kv", "hv_paged_attention",
+           "hv_paged_attention_workspace")
+
+
+@pytest.fixture(scope="module")
+def library():
+    from heatvit_b200 import build
+    build.build()
+    from heatvit_b200 import _lib
+    return _lib.lib()
+
+
+def test_packed_structs_match_the_header(tmp_path):
+    from heatvit_b200 import decode
+    prog = tmp_path / "sz.c"
+    prog.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "heatvit_b200.h"\nint main(){printf("'
+                    + '%zu ' * 10 + '\\n", sizeof(hv_append_args), offsetof(hv_append_args, d_positions), '
+                    'offsetof(hv_append_args, q_strides), offsetof(hv_append_args, rope_stride), '
+                    'offsetof(hv_append_args, tokens), sizeof(hv_attention_args), '
+                    'offsetof(hv_attention_args, workspace_bytes), offsetof(hv_attention_args, page_table_stride), '
+                    'offsetof(hv_attention_args, seqs), offsetof(hv_attention_args, scale));return 0;}\n')
+    exe = tmp_path / "sz"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(prog), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True).stdout.split()]
+
+    def round8(n):
+        return -(-n // 8) * 8
+    assert got == [round8(decode._APPEND.size), 72, 80, struct.calcsize("@10P14q"), struct.calcsize("@10P16q"),
+                   round8(decode._ATTEND.size), struct.calcsize("@8P"), struct.calcsize("@8P13q"),
+                   struct.calcsize("@8P14q"), struct.calcsize("@8P14q8i")]
+
+
+def test_every_symbol_has_a_signature(library):
+    from heatvit_b200 import _lib
+    for name in SYMBOLS:
+        assert name in _lib._SIGNATURES and getattr(library, name)
+
+
+def test_c_entries_refuse_before_they_touch_a_device(library):
+    """Status codes of mistakes that are visible on the host."""
+    from heatvit_b200 import abi
+    none = [None] * 1
+
+    def norm(rows=1, dim=64, dtype=0, eps=1e-6, x=16, res=None, out=None):
+        return library.hv_add_rmsnorm_fp8(x, dim, res, dim, 16, rows, dim, dtype, eps, out, dim, 16, dim, 16, 1, rows,
+                                          none[0])
+    assert norm(dtype=7) == abi.HV_ERR_TYPE
+    assert norm(dim=0) == abi.HV_ERR_VALUE and norm(dim=32769) == abi.HV_ERR_VALUE
+    assert norm(rows=-1) == abi.HV_ERR_VALUE and norm(x=None) == abi.HV_ERR_VALUE
+    assert norm(eps=-1.0) == abi.HV_ERR_VALUE and norm(eps=float("nan")) == abi.HV_ERR_VALUE
+    assert norm(res=16) == abi.HV_ERR_VALUE and b"together" in library.hv_last_error()
+    assert norm(rows=0) == abi.HV_OK
+
+    def gemm(m=1, n=1, k=16, a=16, lda=16, dtype=0):
+        return library.hv_gemm_fp8(a, lda, 16, 1, 1, 16, 16, 16, 1, 1, m, n, k, 16, n, dtype, None)
+    assert gemm(dtype=3) == abi.HV_ERR_TYPE
+    assert gemm(k=0) == abi.HV_ERR_VALUE and gemm(m=-1) == abi.HV_ERR_VALUE and gemm(a=None) == abi.HV_ERR_VALUE
+    assert gemm(a=24) == abi.HV_ERR_VALUE and b"16 bytes" in library.hv_last_error()
+    assert gemm(m=2, lda=24) == abi.HV_ERR_VALUE and gemm(m=2, k=32, lda=16) == abi.HV_ERR_VALUE
+    assert gemm(m=0) == abi.HV_OK and gemm(n=0) == abi.HV_OK
+
+    from heatvit_b200 import decode
+
+    def append(tokens=1, heads=0, kv=1, dim=8, rot=0, dtype=0, pages=1, page=1, k=16):
+        return library.hv_append_kv(decode._APPEND.pack(0, k, 16, 0, 16, 16, 0, 16, 0, 16, *[8] * 16, tokens, heads, kv,
+                                                        dim, rot, 0, dtype, pages, page, 1, 1, 0), None)
+    assert append(dtype=2) == abi.HV_ERR_TYPE
+    for bad in (dict(tokens=-1), dict(kv=0), dict(dim=0), dict(rot=3), dict(rot=16), dict(rot=2), dict(page=0),
+                dict(heads=1), dict(k=0), dict(pages=-1)):
+        assert append(**bad) == abi.HV_ERR_VALUE, bad
+    assert append(tokens=0) == abi.HV_OK
+
+    def attend(seqs=1, heads=1, kv=1, dim=64, dtype=0, pages=1, page=1, ws=256, wsb=0, stride=8, q=16):
+        return library.hv_paged_attention(decode._ATTEND.pack(q, 16, 0, 16, 16, 16, 16, ws, wsb, *[8] * 6,
+                                                              *[stride] * 6, 1, seqs, heads, kv, dim, dtype, pages,
+                                                              page, 1, 1.0), None)
+    assert attend(dtype=2) == abi.HV_ERR_TYPE
+    for bad in (dict(seqs=-1), dict(heads=3, kv=2), dict(kv=0), dict(dim=80), dict(page=0), dict(q=0)):
+        assert attend(**bad) == abi.HV_ERR_VALUE, bad
+    assert library.hv_paged_attention(None, None) == abi.HV_ERR_VALUE
+    assert library.hv_append_kv(None, None) == abi.HV_ERR_VALUE
+    assert library.hv_decode_error(None) == abi.HV_ERR_VALUE
+    assert library.hv_paged_attention_workspace(80, C.byref(C.c_int64())) == abi.HV_ERR_VALUE
+    assert library.hv_paged_attention_workspace(64, None) == abi.HV_ERR_VALUE
+
+
+def test_python_needs_a_device():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a CUDA device is present")
+    from heatvit_b200 import decode
+    with pytest.raises(RuntimeError, match="CUDA"):
+        decode.add_rmsnorm_fp8(torch.zeros(1, 8), torch.zeros(8))
