@@ -29,8 +29,10 @@ namespace {
 
 using namespace dec;
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, ROWS = 16, WTOK = 16, TILE = WARPS * WTOK;
+constexpr int ROWS = 16, WTOK = 16, SLICES = 4, TILE = SLICES * WTOK;
 constexpr int MIN_SHARE = 4;  // tiles: a part costs more than the loads of fewer
+constexpr int FAN = 16;       // parts that one CTA joins at a time
+constexpr int MAX_GRID = 1024;
 
 struct AttendArgs {
     const void *q, *kc, *vc;
@@ -39,28 +41,40 @@ struct AttendArgs {
     const int32_t *pages, *lens;
     long long q_seq, q_head, o_seq, o_head, lse_seq, lse_head;
     long long kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head, pages_stride;
-    int seqs, heads, kv_heads, group, head_tiles, num_pages, page, max_pages, q_pairs;
+    int seqs, heads, kv_heads, group, head_tiles, num_pages, page, max_pages, q_pairs, o_vec;
+    int page16, page_shift;  // the page is a multiple of 16 tokens; log2 of a page that is a power of two, or -1
     float scale_log2;
     float *parts;      // [grid][2][ROWS][D], then [grid][2][ROWS][2]
-    uint32_t *counts;  // [grid], by the share that a cut item starts in; zero between calls
+    uint32_t *counts;  // [3][MAX_GRID], see the end of an item; zero between calls
     int *err;
 };
 
+// A head of over 128 dimensions is split between two warps (HALVES), which add their halves of
+// the scores through shared memory: one warp's sums and q would take all of its registers.
 template <int D>
 struct Lay {
-    static constexpr int ROW = D * 2 + 16;  // bytes: rows 16 bytes apart modulo 128 (ldmatrix without conflicts)
-    static constexpr int STAGES = D <= 64 ? 4 : 3;
+    static constexpr int HALVES = D > 128 ? 2 : 1, DH = D / HALVES;
+    static constexpr int WARPS = SLICES * HALVES, THREADS = WARPS * 32;
+    static constexpr int ROW = DH * 2 + 16;  // bytes: rows 16 bytes apart modulo 128 (ldmatrix without conflicts)
+    static constexpr int STAGES = 3;
     static constexpr int STAGE = 2 * WTOK * ROW;
-    static constexpr int SUM = WARPS * STAGES * STAGE;  // [ROWS][D + 4] float
-    static constexpr int STAT = SUM + ROWS * (D + 4) * 4;  // [WARPS][ROWS][2] float
-    static constexpr int MISC = STAT + WARPS * ROWS * 2 * 4;
+    static constexpr int SUM_ROW = D + 4;
+    static constexpr int SUM = WARPS * STAGES * STAGE;  // [ROWS][SUM_ROW] float, at an item's end
+    static constexpr int EXCHANGE = HALVES == 1 ? 0 : 2 * WARPS * 32 * 8 * 4;  // halves of scores, before it
+    static constexpr int STAT = SUM + (ROWS * SUM_ROW * 4 > EXCHANGE ? ROWS * SUM_ROW * 4 : EXCHANGE);
+    static constexpr int MISC = STAT + SLICES * ROWS * 2 * 4;  // stat: [SLICES][ROWS][2] float
     static constexpr int BYTES = MISC + 32;
-    // registers cap it at two or three, shared memory at one for D = 256
     static constexpr int PER_SM = D <= 64 ? 3 : D <= 128 ? 2 : 1;
+    static_assert(PER_SM * (BYTES + 1024) <= 228 * 1024, "the CTAs of a wave are resident together");
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float exp2_(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
@@ -73,6 +87,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(a)
                  : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t load_pair(const T *p, bool pairs) {
+    if (pairs) return *(const uint32_t *)p;
+    return *(const uint16_t *)p | (uint32_t) * (const uint16_t *)(p + 1) << 16;
 }
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -128,17 +147,134 @@ struct Place {
     }
 };
 
+template <typename T>
+__device__ __forceinline__ void store4(T *p, bool vec, float4 v, float f) {
+    T e[4] = {from_f32<T>(v.x * f), from_f32<T>(v.y * f), from_f32<T>(v.z * f), from_f32<T>(v.w * f)};
+    if (vec) {
+        *(uint2 *)p = *(const uint2 *)e;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = e[i];
+    }
+}
+
+// Joins n parts of one item, by the whole CTA: FAN parts at a time, the loads of a round
+// issued together (the parts come from L2, and its latency under load, once a part, would be
+// the time).  Part k is in slot(k).  The order of every sum is that of the parts.  Goes to the
+// output if `out`, else back to slot(0).  `sum` has room for 2 * FAN * ROWS, `stat` for
+// 3 * ROWS numbers.
+template <typename T, int D, typename Slot>
+__device__ __forceinline__ void join_parts(float *parts, float *sum, float *stat, Slot slot, int n, int nrows, T *out,
+                                           long long o_head, bool o_vec, float *lse, long long lse_head) {
+    constexpr int THREADS = Lay<D>::THREADS, PER = FAN * ROWS / THREADS;  // (part, row) pairs of a thread
+    constexpr int NV = ROWS * D / 4 / THREADS;
+    const int tid = threadIdx.x;
+    float4 *po = (float4 *)parts;
+    float2 *pst = (float2 *)(parts + 2ll * gridDim.x * (ROWS * D));
+    const int nvec = nrows * (D / 4);
+    float *factor = stat + 2 * ROWS;
+    float4 acc[NV] = {};
+    for (int k0 = 0; k0 < n; k0 += FAN) {
+        const int m = min(FAN, n - k0);
+        float2 v[PER];
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int k = (tid + e * THREADS) / ROWS, r = tid % ROWS;
+            v[e] = k < m && r < nrows ? __ldcg(pst + slot(k0 + k) * ROWS + r) : make_float2(-CUDART_INF_F, 0.f);
+        }
+        float4 x[FAN];
+        auto fetch = [&](int t) {
+#pragma unroll
+            for (int k = 0; k < FAN; ++k)
+                x[k] = k < m && t < nvec ? __ldcg(po + slot(k0 + k) * (ROWS * D / 4) + t) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        fetch(tid);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            sum[tid + e * THREADS] = v[e].x;
+            sum[FAN * ROWS + tid + e * THREADS] = v[e].y;
+        }
+        __syncthreads();
+        if (tid < ROWS) {  // weights of the parts of row `tid`
+            const float was = k0 ? stat[2 * tid] : -CUDART_INF_F;
+            float M = was;
+            for (int k = 0; k < FAN; ++k) M = fmaxf(M, sum[k * ROWS + tid]);
+            const float f = k0 ? exp2_(was - M) : 0.f;
+            float S = k0 ? stat[2 * tid + 1] * f : 0.f;
+            for (int k = 0; k < FAN; ++k) {
+                const float w = k < m ? exp2_(sum[k * ROWS + tid] - M) : 0.f;
+                if (k < m) S += w * sum[(FAN + k) * ROWS + tid];
+                sum[k * ROWS + tid] = w;
+            }
+            stat[2 * tid] = M;
+            stat[2 * tid + 1] = S;
+            factor[tid] = f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int t = tid + i * THREADS;
+            if (t >= nvec) break;
+            if (i) fetch(t);
+            const int row = t / (D / 4);
+            const float f = factor[row];
+            acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
+#pragma unroll
+            for (int k = 0; k < FAN; ++k) {
+                if (k >= m) break;
+                const float w = sum[k * ROWS + row];
+                acc[i].x += w * x[k].x;
+                acc[i].y += w * x[k].y;
+                acc[i].z += w * x[k].z;
+                acc[i].w += w * x[k].w;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int t = tid + i * THREADS, row = t / (D / 4);
+        if (t >= nvec) break;
+        if (out) store4(out + row * o_head + (t - row * (D / 4)) * 4, o_vec, acc[i], 1.f / stat[2 * row + 1]);
+        else __stcg(po + slot(0) * (ROWS * D / 4) + t, acc[i]);
+    }
+    if (tid < nrows) {
+        if (!out) __stcg(pst + slot(0) * ROWS + tid, make_float2(stat[2 * tid], stat[2 * tid + 1]));
+        else if (lse) lse[tid * lse_head] = (stat[2 * tid] + log2f(stat[2 * tid + 1])) * 0.69314718055994531f;
+    }
+}
+
+// Counts this CTA in; true in the one that comes last, for which the counter is zero again
+// and the others' stores are visible.
+__device__ __forceinline__ bool comes_last(uint32_t *counter, uint32_t of, long long *flag) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const bool last = atomicAdd(counter, 1u) == of - 1;
+        if (last) *counter = 0;
+        *flag = last;
+    }
+    __syncthreads();
+    const bool last = *flag;
+    if (last) __threadfence();
+    __syncthreads();
+    return last;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
+    attend_kernel(const __grid_constant__ AttendArgs a) {
     griddep_wait();
     griddep_launch();
     using L = Lay<D>;
+    constexpr int DH = L::DH, THREADS = L::THREADS;
     extern __shared__ __align__(128) uint8_t smem[];
     float *sum = (float *)(smem + L::SUM);
     float *stat = (float *)(smem + L::STAT);
     long long *misc = (long long *)(smem + L::MISC);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int items = a.kv_heads * a.head_tiles;  // of a sequence
+    const int slice = warp % SLICES, half = warp / SLICES;  // tokens and dimensions of this warp
+    const int items = a.kv_heads * a.head_tiles;            // of a sequence
 
     // Sequences of no tokens: nobody's share holds them.
     for (int b = blockIdx.x; b < a.seqs; b += gridDim.x)
@@ -152,11 +288,11 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
     // The line's length, this CTA's share of it, and the share's first place.
     if (warp == 0) {
         long long total = 0;
+        int held = 0;  // this lane's sequence of the last 32
         for (int b0 = 0; b0 < a.seqs; b0 += 32) {
             const int b = b0 + lane;
-            int n = b < a.seqs ? (length_of(a, b) + TILE - 1) / TILE : 0;
-            for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
-            total += n;
+            held = b < a.seqs ? (length_of(a, b) + TILE - 1) / TILE : 0;
+            total += __reduce_add_sync(~0u, held);
         }
         total *= items;
         long long share = (total + gridDim.x - 1) / gridDim.x;
@@ -166,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
         int found = -1;
         for (int b0 = 0; b0 < a.seqs && found < 0 && first < total; b0 += 32) {
             const int b = b0 + lane;
-            const int n = b < a.seqs ? (length_of(a, b) + TILE - 1) / TILE : 0;
+            const int n = a.seqs <= 32 ? held : b < a.seqs ? (length_of(a, b) + TILE - 1) / TILE : 0;
             int incl = n;
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(~0u, incl, o);
@@ -206,25 +342,63 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
     uint8_t *ring = smem + warp * L::STAGES * L::STAGE;
     const T *kc = (const T *)a.kc, *vc = (const T *)a.vc;
 
-    // The page of this lane's token (lane & 15) at place p; -1 past the length.
+    // The page of this warp's tokens (page16: they share one), or of this lane's token (lane
+    // & 15), at place p; -1 past the length.
     auto page_of = [&](const Place &p) {
-        const int t = p.tile * TILE + warp * WTOK + (lane & 15);
-        return t < p.len ? a.pages[p.b * a.pages_stride + t / a.page] : -1;
+        const int t0 = p.tile * TILE + slice * WTOK, t = a.page16 ? t0 : t0 + (lane & 15);
+        if (t >= p.len) return -1;
+        const int col = a.page16 ? (a.page_shift >= 0 ? t >> a.page_shift : t / a.page) : t / a.page;
+        return a.pages[p.b * a.pages_stride + col];
     };
     auto load = [&](int stage, const Place &p, int pg) {
-        const int t = p.tile * TILE + warp * WTOK + (lane & 15);
+        const int t0 = p.tile * TILE + slice * WTOK;
+        if (t0 >= p.len) return;  // not read either
         const int head = p.h / a.head_tiles;
+        const uint32_t dst = tc05::smem_u32(ring + stage * L::STAGE);
+        constexpr int CH = DH / 8;  // 16-byte pieces of a row
+        constexpr int N = WTOK * CH / 32;
+        if (a.page16) {
+            const bool ok = pg >= 0 && pg < a.num_pages;
+            if (!ok) {
+                atomicOr(a.err, HV_DECODE_BAD_PAGE);
+                pg = 0;
+            }
+            const int live = ok ? p.len - t0 : 0;  // rows of the 16 that exist
+            const int slot = a.page_shift >= 0 ? t0 & (a.page - 1) : t0 % a.page;
+            const T *k = kc + (pg * a.kc_page + slot * a.kc_slot + head * a.kc_head + half * DH);
+            const T *v = vc + (pg * a.vc_page + slot * a.vc_slot + head * a.vc_head + half * DH);
+            if constexpr (32 % CH == 0) {
+                const int row0 = lane / CH, col = lane % CH;
+                k += row0 * a.kc_slot + col * 8;
+                v += row0 * a.vc_slot + col * 8;
+                const uint32_t to = dst + row0 * L::ROW + col * 16;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int n = row0 + i * (32 / CH) < live ? 16 : 0;
+                    cp16(to + i * (32 / CH) * L::ROW, k, n);
+                    cp16(to + (WTOK + i * (32 / CH)) * L::ROW, v, n);
+                    k += (32 / CH) * a.kc_slot;
+                    v += (32 / CH) * a.vc_slot;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int c = i * 32 + lane, row = c / CH, col = c % CH, n = row < live ? 16 : 0;
+                    cp16(dst + row * L::ROW + col * 16, k + row * a.kc_slot + col * 8, n);
+                    cp16(dst + (WTOK + row) * L::ROW + col * 16, v + row * a.vc_slot + col * 8, n);
+                }
+            }
+            return;
+        }
+        const int t = t0 + (lane & 15);
         bool ok = t < p.len;
         if (ok && (pg < 0 || pg >= a.num_pages)) {
             atomicOr(a.err, HV_DECODE_BAD_PAGE);
             ok = false;
         }
         const int slot = t % a.page;
-        const long long ko = ok ? pg * a.kc_page + slot * a.kc_slot + head * a.kc_head : -1;
-        const long long vo = ok ? pg * a.vc_page + slot * a.vc_slot + head * a.vc_head : -1;
-        const uint32_t dst = tc05::smem_u32(ring + stage * L::STAGE);
-        constexpr int CH = D / 8;  // 16-byte pieces of a row
-        constexpr int N = WTOK * CH / 32;
+        const long long ko = ok ? pg * a.kc_page + slot * a.kc_slot + head * a.kc_head + half * DH : -1;
+        const long long vo = ok ? pg * a.vc_page + slot * a.vc_slot + head * a.vc_head + half * DH : -1;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = i * 32 + lane, row = c / CH, col = c % CH;
@@ -248,8 +422,8 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
     };
     for (int s = 0; s < L::STAGES - 1; ++s) load_next();
 
-    uint32_t qf[D / 16][4];
-    float o[D / 8][4];
+    uint32_t qf[DH / 16][4];
+    float o[DH / 8][4];
     float m[2], l[2];
     bool fresh = true;
     for (int u = 0; u < count; ++u) {
@@ -257,81 +431,97 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
         const int nrows = min(ROWS, a.group - ht * ROWS);
         const int h0 = head * a.group + ht * ROWS;
         if (fresh) {
-            const T *q = (const T *)a.q + cur.b * a.q_seq;
+            const T *q = (const T *)a.q + cur.b * a.q_seq + h0 * a.q_head;
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j)
+            for (int j = 0; j < DH / 16; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = (lane >> 2) + (i & 1) * 8, c = j * 16 + (lane & 3) * 2 + (i >> 1) * 8;
-                    uint32_t w = 0;
-                    if (r < nrows) {
-                        const T *p = q + (h0 + r) * a.q_head + c;
-                        if (a.q_pairs) w = *(const uint32_t *)p;
-                        else w = *(const uint16_t *)p | (uint32_t) * (const uint16_t *)(p + 1) << 16;
-                    }
-                    qf[j][i] = w;
+                    const int r = (lane >> 2) + (i & 1) * 8, c = half * DH + j * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+                    qf[j][i] = r < nrows ? load_pair(q + r * a.q_head + c, a.q_pairs) : 0;
                 }
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+            for (int j = 0; j < DH / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
             m[0] = m[1] = -CUDART_INF_F;
             l[0] = l[1] = 0.f;
             fresh = false;
         }
         asm volatile("cp.async.wait_group %0;\n" ::"n"(L::STAGES - 2) : "memory");
         __syncwarp();
-        const int t0 = cur.tile * TILE + warp * WTOK;
+        const int t0 = cur.tile * TILE + slice * WTOK;
         if (t0 < cur.len) {
             const uint32_t kb = tc05::smem_u32(ring + (u % L::STAGES) * L::STAGE), vb = kb + WTOK * L::ROW;
             float s[2][4] = {};
             const uint32_t ka = kb + ((lane >> 4) * 8 + (lane & 7)) * L::ROW + ((lane >> 3) & 1) * 16;
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
+            for (int j = 0; j < DH / 16; ++j) {
                 uint32_t r[4];
                 ldsm4(ka + j * 32, r);
                 mma<T>(s[0], qf[j], r[0], r[1]);
                 mma<T>(s[1], qf[j], r[2], r[3]);
             }
+            if constexpr (L::HALVES == 2) {
+                // two buffers in turn: the partner has read a buffer before the step's barrier
+                // after the one that filled it
+                float4 *mine = (float4 *)sum + ((u & 1) * L::WARPS + warp) * 64 + lane;
+                const float4 *its = (float4 *)sum + ((u & 1) * L::WARPS + (warp ^ SLICES)) * 64 + lane;
+                mine[0] = make_float4(s[0][0], s[0][1], s[0][2], s[0][3]);
+                mine[32] = make_float4(s[1][0], s[1][1], s[1][2], s[1][3]);
+                asm volatile("bar.sync %0, 64;\n" ::"r"(1 + slice) : "memory");
+                const float4 x = its[0], y = its[32];
+                s[0][0] += x.x, s[0][1] += x.y, s[0][2] += x.z, s[0][3] += x.w;
+                s[1][0] += y.x, s[1][1] += y.y, s[1][2] += y.z, s[1][3] += y.w;
+            }
             // s[n][2 * i + e]: row lane / 4 + 8 i, token t0 + 8 n + 2 (lane % 4) + e
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    s[n][e] = t0 + n * 8 + (lane & 3) * 2 + (e & 1) < cur.len ? s[n][e] * a.scale_log2 : -CUDART_INF_F;
-            float f[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float x = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-                x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
-                x = fmaxf(x, m[i]);
-                f[i] = exp2f(m[i] - x);
-                m[i] = x;
-                float p = 0.f;
+                for (int e = 0; e < 4; ++e) s[n][e] *= a.scale_log2;
+            if (t0 + WTOK > cur.len)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        s[n][2 * i + e] = exp2f(s[n][2 * i + e] - x);
-                        p += s[n][2 * i + e];
-                    }
-                l[i] = l[i] * f[i] + p;
-            }
-            if (__any_sync(~0u, f[0] != 1.f || f[1] != 1.f)) {
+                    for (int e = 0; e < 4; ++e)
+                        if (t0 + n * 8 + (lane & 3) * 2 + (e & 1) >= cur.len) s[n][e] = -CUDART_INF_F;
+            // The reference of the weights moves only when a maximum passes it by more than 2^6:
+            // until then weights are at most 64, exact powers apart from what they would be.
+            float x[2];
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
+            for (int i = 0; i < 2; ++i) {
+                x[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+                x[i] = fmaxf(x[i], __shfl_xor_sync(~0u, x[i], 1));
+                x[i] = fmaxf(x[i], __shfl_xor_sync(~0u, x[i], 2));
+            }
+            if (__any_sync(~0u, x[0] > m[0] + 6.f || x[1] > m[1] + 6.f)) {
+                float f[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    x[i] = fmaxf(x[i], m[i]);
+                    f[i] = exp2_(m[i] - x[i]);
+                    m[i] = x[i];
+                    l[i] *= f[i];
+                }
+#pragma unroll
+                for (int j = 0; j < DH / 8; ++j) {
                     o[j][0] *= f[0];
                     o[j][1] *= f[0];
                     o[j][2] *= f[1];
                     o[j][3] *= f[1];
                 }
             }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] = exp2_(s[n][e] - m[e >> 1]);
+                    l[e >> 1] += s[n][e];
+                }
             // weights in T for the product: each is within 2^-9 (bf16) of its 32-bit value,
             // as the values that it multiplies are of theirs; the sums stay in 32 bits
             uint32_t p[4] = {pack(s[0][0], s[0][1], T()), pack(s[0][2], s[0][3], T()), pack(s[1][0], s[1][1], T()),
                              pack(s[1][2], s[1][3], T())};
             const uint32_t va = vb + (lane & 15) * L::ROW + (lane >> 4) * 16;
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
+            for (int j = 0; j < DH / 16; ++j) {
                 uint32_t r[4];
                 ldsm4t(va + j * 32, r);
                 mma<T>(o[2 * j], p, r[0], r[1]);
@@ -343,32 +533,34 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
 
         const bool item_ends = cur.tile + 1 == cur.tiles;
         if (item_ends || u + 1 == count) {
-            // Join the four warps: rows' maxima, then the sums in the order of the warps.
+            // Join the slices of tokens: rows' maxima, then the sums in the order of the slices.
+            if (L::HALVES == 2) __syncthreads();  // the scores that were exchanged last have been read
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 l[i] += __shfl_xor_sync(~0u, l[i], 1);
                 l[i] += __shfl_xor_sync(~0u, l[i], 2);
-                if ((lane & 3) == 0) {
-                    float *st = stat + (warp * ROWS + (lane >> 2) + 8 * i) * 2;
+                if ((lane & 3) == 0 && half == 0) {
+                    float *st = stat + (slice * ROWS + (lane >> 2) + 8 * i) * 2;
                     st[0] = m[i];
                     st[1] = l[i];
                 }
             }
             __syncthreads();
-            float top[2], f[2];
+            float f[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                top[i] = -CUDART_INF_F;
-                for (int w = 0; w < WARPS; ++w) top[i] = fmaxf(top[i], stat[(w * ROWS + (lane >> 2) + 8 * i) * 2]);
-                f[i] = m[i] == -CUDART_INF_F ? 0.f : exp2f(m[i] - top[i]);
+                float top = -CUDART_INF_F;
+                for (int w = 0; w < SLICES; ++w) top = fmaxf(top, stat[(w * ROWS + (lane >> 2) + 8 * i) * 2]);
+                f[i] = m[i] == -CUDART_INF_F ? 0.f : exp2_(m[i] - top);
             }
-            for (int w = 0; w < WARPS; ++w) {
-                if (warp == w) {
+            for (int w = 0; w < SLICES; ++w) {
+                if (slice == w) {
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j)
+                    for (int j = 0; j < DH / 8; ++j)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float2 *d = (float2 *)(sum + ((lane >> 2) + 8 * i) * (D + 4) + j * 8 + (lane & 3) * 2);
+                            float2 *d = (float2 *)(sum + ((lane >> 2) + 8 * i) * L::SUM_ROW + half * DH + j * 8 +
+                                                   (lane & 3) * 2);
                             float2 v = make_float2(o[j][2 * i] * f[i], o[j][2 * i + 1] * f[i]);
                             if (w) {
                                 const float2 x = *d;
@@ -380,59 +572,51 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
                 }
                 __syncthreads();
             }
-            auto row_stat = [&](int r, float &M, float &S) {
-                M = -CUDART_INF_F;
-                S = 0.f;
-                for (int w = 0; w < WARPS; ++w) M = fmaxf(M, stat[(w * ROWS + r) * 2]);
-                for (int w = 0; w < WARPS; ++w) {
-                    const float mw = stat[(w * ROWS + r) * 2];
-                    if (mw != -CUDART_INF_F) S += stat[(w * ROWS + r) * 2 + 1] * exp2f(mw - M);
+            float M = -CUDART_INF_F, S = 0.f;
+            if (tid < ROWS) {  // a row's maximum and sum, into its first place
+                for (int w = 0; w < SLICES; ++w) M = fmaxf(M, stat[(w * ROWS + tid) * 2]);
+                for (int w = 0; w < SLICES; ++w) {
+                    const float mw = stat[(w * ROWS + tid) * 2];
+                    if (mw != -CUDART_INF_F) S += stat[(w * ROWS + tid) * 2 + 1] * exp2_(mw - M);
                 }
-            };
+                stat[tid * 2] = M;
+                stat[tid * 2 + 1] = S;
+            }
+            const int nvec = nrows * (D / 4);
             T *out = (T *)a.out + cur.b * a.o_seq + h0 * a.o_head;
             float *lse = a.lse ? a.lse + cur.b * a.lse_seq + h0 * a.lse_head : nullptr;
-            const long long c_first = item_first / share, c_last = (item_first + cur.tiles - 1) / share;
+            const int c_first = (int)(item_first / share), c_last = (int)((item_first + cur.tiles - 1) / share);
             if (c_first == c_last) {
-                for (int i = tid; i < nrows * D; i += THREADS) {
-                    const int r = i / D, c = i - r * D;
-                    float M, S;
-                    row_stat(r, M, S);
-                    out[r * a.o_head + c] = from_f32<T>(sum[r * (D + 4) + c] / S);
-                    if (lse && c == 0) lse[r * a.lse_head] = (M + log2f(S)) * 0.69314718055994531f;
+                __syncthreads();
+                for (int i = tid; i < nvec; i += THREADS) {
+                    const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+                    const float4 x = *(const float4 *)(sum + r * L::SUM_ROW + c);
+                    store4(out + r * a.o_head + c, a.o_vec, x, 1.f / stat[r * 2 + 1]);
                 }
+                if (lse && tid < nrows) lse[tid * a.lse_head] = (M + log2f(S)) * 0.69314718055994531f;
             } else {
-                const long long slot = 2ll * blockIdx.x + (blockIdx.x == c_first ? 1 : 0);
-                float *po = a.parts + slot * (ROWS * D);
-                float *pst = a.parts + 2ll * gridDim.x * (ROWS * D);
-                for (int i = tid; i < nrows * D; i += THREADS) __stcg(po + i, sum[(i / D) * (D + 4) + i % D]);
-                if (tid < nrows) {
-                    float M, S;
-                    row_stat(tid, M, S);
-                    __stcg(pst + (slot * ROWS + tid) * 2, M);
-                    __stcg(pst + (slot * ROWS + tid) * 2 + 1, S);
-                }
-                __threadfence();
-                __syncthreads();
-                uint32_t *cnt = a.counts + c_first;  // one cut item at most starts in a share
-                if (tid == 0) misc[0] = atomicAdd(cnt, 1u) == (uint32_t)(c_last - c_first);
-                __syncthreads();
-                if (misc[0]) {
-                    __threadfence();
-                    for (int i = tid; i < nrows * D; i += THREADS) {
-                        const int r = i / D, c = i - r * D;
-                        float M = -CUDART_INF_F, S = 0.f, acc = 0.f;
-                        for (long long k = c_first; k <= c_last; ++k)
-                            M = fmaxf(M, __ldcg(pst + ((2 * k + (k == c_first)) * ROWS + r) * 2));
-                        for (long long k = c_first; k <= c_last; ++k) {
-                            const long long sl = 2 * k + (k == c_first);
-                            const float w = exp2f(__ldcg(pst + (sl * ROWS + r) * 2) - M);
-                            S += w * __ldcg(pst + (sl * ROWS + r) * 2 + 1);
-                            acc += w * __ldcg(a.parts + sl * (ROWS * D) + r * D + c);
-                        }
-                        out[r * a.o_head + c] = from_f32<T>(acc / S);
-                        if (lse && c == 0) lse[r * a.lse_head] = (M + log2f(S)) * 0.69314718055994531f;
-                    }
-                    if (tid == 0) *cnt = 0;
+                // A part.  Those of FAN neighbouring shares are joined by the last of them to come,
+                // and where the item has more, their sums by the last of all.  A share leaves its
+                // second slot to the item that starts in it, its first to one that started before;
+                // likewise at most one item enters a group of shares from before.
+                auto slot = [&](int c) { return 2ll * c + (c == c_first); };
+                const long long mine = slot(blockIdx.x);
+                float4 *po = (float4 *)(a.parts + mine * (ROWS * D));
+                float2 *pst = (float2 *)(a.parts + 2ll * gridDim.x * (ROWS * D)) + mine * ROWS;
+                for (int i = tid; i < nvec; i += THREADS)
+                    __stcg(po + i, *(const float4 *)(sum + (i / (D / 4)) * L::SUM_ROW + i % (D / 4) * 4));
+                if (tid < nrows) __stcg(pst + tid, make_float2(M, S));
+                const int g = blockIdx.x / FAN, g_first = c_first / FAN, g_last = c_last / FAN;
+                const int lo = max(c_first, g * FAN), n = min(c_last, g * FAN + FAN - 1) - lo + 1;
+                if (comes_last(lo == c_first ? a.counts + c_first : a.counts + MAX_GRID + g, n, misc)) {
+                    const bool all = g_first == g_last;
+                    if (all || n > 1)
+                        join_parts<T, D>(a.parts, sum, stat, [&](int k) { return slot(lo + k); }, n, nrows,
+                                         all ? out : nullptr, a.o_head, a.o_vec, lse, a.lse_head);
+                    if (!all && comes_last(a.counts + 2 * MAX_GRID + c_first, g_last - g_first + 1, misc))
+                        join_parts<T, D>(a.parts, sum, stat,
+                                         [&](int k) { return slot(k ? (g_first + k) * FAN : c_first); },
+                                         g_last - g_first + 1, nrows, out, a.o_head, a.o_vec, lse, a.lse_head);
                 }
             }
             __syncthreads();  // sum, stat and misc are free again
@@ -446,7 +630,7 @@ __global__ void __launch_bounds__(THREADS, Lay<D>::PER_SM) attend_kernel(const A
 
 // The counters come first and take the same room for every call, so that calls of other
 // sizes with the same workspace never find a part where a zero belongs.
-constexpr int MAX_GRID = 1024, COUNT_BYTES = MAX_GRID * 4;
+constexpr int COUNT_BYTES = 3 * MAX_GRID * 4;
 
 // CTAs of one resident wave on the current device.
 int wave(int d) {
@@ -463,7 +647,7 @@ cudaError_t launch(const AttendArgs &a, int grid, cudaStream_t st) {
     const cudaError_t e =
         cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::BYTES);
     if (e != cudaSuccess) return e;
-    return launch_pdl(attend_kernel<T, D>, dim3((unsigned)grid), dim3(THREADS), Lay<D>::BYTES, st, a);
+    return launch_pdl(attend_kernel<T, D>, dim3((unsigned)grid), dim3(Lay<D>::THREADS), Lay<D>::BYTES, st, a);
 }
 
 template <typename T>
@@ -529,6 +713,9 @@ extern "C" int hv_paged_attention(const hv_attention_args *p, void *stream) {
     a.head_tiles = (group + ROWS - 1) / ROWS;
     a.num_pages = p->num_pages, a.page = p->page_size, a.max_pages = p->max_pages;
     a.q_pairs = dec::aligned(a.q, 4) && a.q_seq % 2 == 0 && a.q_head % 2 == 0;
+    a.o_vec = dec::aligned(a.out, 8) && a.o_seq % 4 == 0 && a.o_head % 4 == 0;
+    a.page16 = a.page % WTOK == 0;
+    a.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.counts = (uint32_t *)p->d_workspace;
     a.parts = (float *)((char *)p->d_workspace + COUNT_BYTES);

@@ -17,6 +17,7 @@ TypeError.  What only the device can see (a page number outside the cache, a
 position past a table) faults nothing and is reported by ``device_error``.
 """
 
+import ctypes as C
 import struct
 from collections import namedtuple
 
@@ -35,40 +36,66 @@ Fp8Rows.__doc__ = "q [rows, dim] e4m3, scale [rows, ceil(dim / 128)] float32, re
 _APPEND = struct.Struct("@10P16q12i")
 _ATTEND = struct.Struct("@8P14q8if")
 
-_types = None
+_torch_module = None
+_types = _raw_stream = _current_device = _c = None
 
 
-def _dtype_codes():
-    global _types
-    if _types is None:
+def _ready():
+    """torch, once a CUDA device and the library are known to be there; small calls cost
+    what the host does, so the look-ups are made once."""
+    global _torch_module, _types, _raw_stream, _current_device, _c
+    if _torch_module is None:
         torch = _torch()
+        _c = lib()
         _types = {torch.bfloat16: abi.HV_BF16, torch.float16: abi.HV_F16, torch.float32: abi.HV_F32}
-    return _types
+        _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+        _torch_module = torch
+    return _torch_module
 
 
-def _need(t, name, dims, device):
-    if not t.is_cuda or t.device != device:
-        raise ValueError(f"{name} must live on {device}")
-    if t.dim() != dims:
+def _index(t, name):
+    """The CUDA device of an operator's first tensor, which the others share."""
+    i = t.get_device()
+    if i < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return i
+
+
+def _strides(t, name, dims, index):
+    """t's strides, after the checks that every operand passes."""
+    if t.get_device() != index:
+        raise ValueError(f"{name} must live on cuda:{index}")
+    s = t.stride()
+    if len(s) != dims:
         raise ValueError(f"{name} must be {dims}-dimensional")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if s[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
+    return s
 
 
-def _ints(t, name, dims, device):
-    _need(t, name, dims, device)
-    if t.dtype != _torch().int32:
+def _int_strides(t, name, dims, index):
+    if t.dtype is not _torch_module.int32:
         raise TypeError(f"{name} must be int32")
+    return _strides(t, name, dims, index)
 
 
-def _call(fn, device, *args):
-    """fn(*args, stream) with `device` current; raises on a status."""
-    torch = _torch()
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _like(t, name, other, its_name, index):
+    """t's strides; t has the shape and the type of another operand."""
+    s = _strides(t, name, len(other.shape), index)
+    if t.shape != other.shape:
+        raise ValueError(f"{name} must have {its_name}'s shape")
+    if t.dtype is not other.dtype:
+        raise TypeError(f"{name} must have {its_name}'s type")
+    return s
+
+
+def _call(fn, index, *args):
+    """fn(*args, stream) with the device current; raises on a status."""
+    if _current_device() == index:
+        status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with _torch_module.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
     if status:
         check(status)
 
@@ -76,11 +103,10 @@ def _call(fn, device, *args):
 def device_error(device=None):
     """Read and clear the decode error bits of a device (synchronises with it):
     abi.HV_DECODE_BAD_PAGE, _BAD_POSITION, _BAD_LENGTH, _STALLED; 0 when all went well."""
-    import ctypes as C
-    torch = _torch()
+    torch = _ready()
     bits = C.c_int()
     with torch.cuda.device(device):
-        check(lib().hv_decode_error(C.byref(bits)))
+        check(_c.hv_decode_error(C.byref(bits)))
     return bits.value
 
 
@@ -93,46 +119,44 @@ def add_rmsnorm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None):
     bfloat16, float16, float32; ``residual_out`` (a new tensor unless given, and it may
     be ``residual``) receives h rounded to that type.  q's row stride is a multiple of 16,
     scale is stored group by group: both as ``gemm_fp8`` reads them best."""
-    torch = _torch()
-    dev = x.device
-    _need(x, "x", 2, dev)
-    _need(weight, "weight", 1, dev)
-    code = _dtype_codes().get(x.dtype)
+    torch = _ready()
+    dev = _index(x, "x")
+    x_stride = _strides(x, "x", 2, dev)[0]
+    _strides(weight, "weight", 1, dev)
+    dtype = x.dtype
+    code = _types.get(dtype)
     if code is None:
         raise TypeError("x must be bfloat16, float16 or float32")
     rows, dim = x.shape
     if weight.shape[0] != dim:
         raise ValueError(f"weight has {weight.shape[0]} channels, x {dim}")
-    if weight.dtype != x.dtype:
+    if weight.dtype is not dtype:
         raise TypeError("weight must have x's type")
     r_ptr = ro_ptr = None
     r_stride = ro_stride = 0
     if residual is not None:
+        r_stride = _like(residual, "residual", x, "x", dev)[0]
         if residual_out is None:
-            residual_out = torch.empty((rows, dim), dtype=x.dtype, device=dev)
-        for t, name in ((residual, "residual"), (residual_out, "residual_out")):
-            _need(t, name, 2, dev)
-            if t.shape != x.shape:
-                raise ValueError(f"{name} must have x's shape")
-            if t.dtype != x.dtype:
-                raise TypeError(f"{name} must have x's type")
-        r_ptr, r_stride = residual.data_ptr(), residual.stride(0)
-        ro_ptr, ro_stride = residual_out.data_ptr(), residual_out.stride(0)
+            residual_out = torch.empty((rows, dim), dtype=dtype, device=x.device)
+            ro_stride = dim
+        else:
+            ro_stride = _like(residual_out, "residual_out", x, "x", dev)[0]
+        r_ptr, ro_ptr = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
     wide = -(-dim // 16) * 16
-    q = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty((-(-dim // GROUP), rows), dtype=torch.float32, device=dev)
-    _call(lib().hv_add_rmsnorm_fp8, dev, x.data_ptr(), x.stride(0), r_ptr, r_stride, weight.data_ptr(), rows, dim,
+    q = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty_strided((rows, -(-dim // GROUP)), (1, rows), dtype=torch.float32, device=x.device)
+    _call(_c.hv_add_rmsnorm_fp8, dev, x.data_ptr(), x_stride, r_ptr, r_stride, weight.data_ptr(), rows, dim,
           code, eps, ro_ptr, ro_stride, q.data_ptr(), wide, scale.data_ptr(), 1, rows)
-    return Fp8Rows(q if wide == dim else q[:, :dim], scale.t(), residual_out)
+    return Fp8Rows(q if wide == dim else q[:, :dim], scale, residual_out)
 
 
 def quantize_weight_fp8(weight):
     """A weight [n, k] as e4m3 with a float32 scale for each 128 x 128 block, as
     ``gemm_fp8`` takes it -> (q [n, k] with 16-byte aligned rows, scale [ceil(n/128),
     ceil(k/128)]).  Done once, when weights are loaded."""
-    torch = _torch()
+    torch = _ready()
     if weight.dim() != 2:
         raise ValueError("weight must be 2-dimensional")
     n, k = weight.shape
@@ -154,13 +178,12 @@ def gemm_fp8(a, a_scale, b, b_scale, out_dtype=None, out=None):
     Operand rows start on 16 bytes (as ``add_rmsnorm_fp8`` and ``quantize_weight_fp8``
     lay them out); scales are float32 of any strides.  Sums in 32 bits, rounded once to
     ``out_dtype`` (bfloat16 unless given; float16, float32) or to ``out``'s type."""
-    torch = _torch()
-    dev = a.device
+    torch = _ready()
+    dev = _index(a, "a")
+    a_stride, b_stride = _strides(a, "a", 2, dev)[0], _strides(b, "b", 2, dev)[0]
     fp8 = torch.float8_e4m3fn
-    for t, name in ((a, "a"), (b, "b")):
-        _need(t, name, 2, dev)
-        if t.dtype != fp8:
-            raise TypeError(f"{name} must be float8_e4m3fn")
+    if a.dtype is not fp8 or b.dtype is not fp8:
+        raise TypeError("a and b must be float8_e4m3fn")
     m, k = a.shape
     n = b.shape[0]
     if b.shape[1] != k:
@@ -169,33 +192,33 @@ def gemm_fp8(a, a_scale, b, b_scale, out_dtype=None, out=None):
         raise ValueError("k must be positive")
     groups = -(-k // GROUP)
     for t, name, rows in ((a_scale, "a_scale", m), (b_scale, "b_scale", -(-n // GROUP))):
-        if t.device != dev:
-            raise ValueError(f"{name} must live on {dev}")
-        if t.dtype != torch.float32:
+        if t.get_device() != dev:
+            raise ValueError(f"{name} must live on cuda:{dev}")
+        if t.dtype is not torch.float32:
             raise TypeError(f"{name} must be float32")
         if t.shape != (rows, groups):
             raise ValueError(f"{name} must be [{rows}, {groups}]")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=dev)
+        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=a.device)
+        out_stride = n
     else:
-        _need(out, "out", 2, dev)
+        out_stride = _strides(out, "out", 2, dev)[0]
         if out.shape != (m, n):
             raise ValueError(f"out must be [{m}, {n}]")
-        if out_dtype is not None and out.dtype != out_dtype:
+        if out_dtype is not None and out.dtype is not out_dtype:
             raise TypeError("out has another type than out_dtype")
-    code = _dtype_codes().get(out.dtype)
+    code = _types.get(out.dtype)
     if code is None:
         raise TypeError("out must be bfloat16, float16 or float32")
-    _call(lib().hv_gemm_fp8, dev, a.data_ptr(), a.stride(0), a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1),
-          b.data_ptr(), b.stride(0), b_scale.data_ptr(), b_scale.stride(0), b_scale.stride(1), m, n, k, out.data_ptr(),
-          out.stride(0), code)
+    _call(_c.hv_gemm_fp8, dev, a.data_ptr(), a_stride, a_scale.data_ptr(), *a_scale.stride(), b.data_ptr(),
+          b_stride, b_scale.data_ptr(), *b_scale.stride(), m, n, k, out.data_ptr(), out_stride, code)
     return out
 
 
 def rope_table(positions, rot, base=10000.0, device="cuda"):
     """Cosines, then sines, of ``position * base^(-2 i / rot)``: float32 [positions, rot],
     angles in 64 bits.  Built once and kept by the caller."""
-    torch = _torch()
+    torch = _ready()
     if rot < 2 or rot % 2:
         raise ValueError("rot must be even and positive")
     i = torch.arange(rot // 2, dtype=torch.float64, device=device)
@@ -203,14 +226,9 @@ def rope_table(positions, rot, base=10000.0, device="cuda"):
     return torch.cat([angle.cos(), angle.sin()], 1).float()
 
 
-def _cache_strides(k_cache, v_cache, device):
-    _need(k_cache, "k_cache", 4, device)
-    _need(v_cache, "v_cache", 4, device)
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("k_cache and v_cache must have the same shape")
-    if k_cache.dtype != v_cache.dtype:
-        raise TypeError("k_cache and v_cache must have the same type")
-    return (*k_cache.stride()[:3], *v_cache.stride()[:3])
+def _cache_strides(k_cache, v_cache, index):
+    ks = _strides(k_cache, "k_cache", 4, index)
+    return (*ks[:3], *_like(v_cache, "v_cache", k_cache, "k_cache", index)[:3])
 
 
 def append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, rope=None, q=None, interleaved=False,
@@ -225,60 +243,61 @@ def append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, rope=
     float32 (see ``rope_table``) turns the first rot elements of each head in pairs
     (i, i + rot/2), or (2i, 2i + 1) when interleaved; v is stored as it is.  Returns the
     rotated q (a new tensor, or q_out, which may be q), None without q."""
-    torch = _torch()
-    dev = k.device
-    _need(k, "k", 3, dev)
-    _need(v, "v", 3, dev)
+    torch = _ready()
+    dev = _index(k, "k")
+    k_str, v_str = _strides(k, "k", 3, dev), _like(v, "v", k, "k", dev)
     cache = _cache_strides(k_cache, v_cache, dev)
-    _ints(page_table, "page_table", 2, dev)
-    _ints(positions, "positions", 1, dev)
-    code = _dtype_codes().get(k.dtype)
+    table_stride = _int_strides(page_table, "page_table", 2, dev)[0]
+    _int_strides(positions, "positions", 1, dev)
+    dtype = k.dtype
+    code = _types.get(dtype)
     if code not in (abi.HV_BF16, abi.HV_F16):
         raise TypeError("k must be bfloat16 or float16")
-    if v.dtype != k.dtype or k_cache.dtype != k.dtype:
+    if k_cache.dtype is not dtype:
         raise TypeError("k, v and the caches must have the same type")
     tokens, kv_heads, dim = k.shape
-    if v.shape != k.shape:
-        raise ValueError("k and v must have the same shape")
-    if k_cache.shape[2:] != (kv_heads, dim):
+    pages, page, cache_heads, cache_dim = k_cache.shape
+    if cache_heads != kv_heads or cache_dim != dim:
         raise ValueError("the caches hold other heads or another head dimension")
     if positions.shape[0] != tokens:
         raise ValueError("one position per token")
-    ids = None
+    seqs, max_pages = page_table.shape
+    ids = 0
     if seq_ids is not None:
-        _ints(seq_ids, "seq_ids", 1, dev)
+        _int_strides(seq_ids, "seq_ids", 1, dev)
         if seq_ids.shape[0] != tokens:
             raise ValueError("one sequence id per token")
         ids = seq_ids.data_ptr()
-    elif page_table.shape[0] < tokens:
+    elif seqs < tokens:
         raise ValueError("without seq_ids the page table has one row per token")
     heads, q_ptr, qo_ptr, q_str, qo_str = 0, 0, 0, (0, 0), (0, 0)
     if q is not None:
+        q_str = _strides(q, "q", 3, dev)
+        if q.shape[0] != tokens or q.shape[2] != dim:
+            raise ValueError("q must be [tokens, heads, dim]")
+        if q.dtype is not dtype:
+            raise TypeError("q must have k's type")
+        heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        for t, name in ((q, "q"), (q_out, "q_out")):
-            _need(t, name, 3, dev)
-            if t.shape[0] != tokens or t.shape[2] != dim or t.shape != q.shape:
-                raise ValueError(f"{name} must be [tokens, heads, dim]")
-            if t.dtype != k.dtype:
-                raise TypeError(f"{name} must have k's type")
-        heads, q_ptr, qo_ptr = q.shape[1], q.data_ptr(), q_out.data_ptr()
-        q_str, qo_str = q.stride()[:2], q_out.stride()[:2]
+            q_out = torch.empty((tokens, heads, dim), dtype=dtype, device=q.device)
+            qo_str = (heads * dim, dim)
+        else:
+            qo_str = _like(q_out, "q_out", q, "q", dev)
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
     rot, rope_ptr, rope_stride, rope_rows = 0, 0, 0, 0
     if rope is not None:
-        _need(rope, "rope", 2, dev)
-        if rope.dtype != torch.float32:
+        rope_stride = _strides(rope, "rope", 2, dev)[0]
+        if rope.dtype is not torch.float32:
             raise TypeError("rope must be float32")
         rope_rows, rot = rope.shape
-        rope_ptr, rope_stride = rope.data_ptr(), rope.stride(0)
+        rope_ptr = rope.data_ptr()
     args = _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, k_cache.data_ptr(), v_cache.data_ptr(), rope_ptr,
-                        page_table.data_ptr(), ids or 0, positions.data_ptr(), *q_str, *k.stride()[:2],
-                        *v.stride()[:2], *qo_str, *cache, rope_stride, page_table.stride(0), tokens, heads, kv_heads,
-                        dim, rot, bool(interleaved), code, k_cache.shape[0], k_cache.shape[1], page_table.shape[0],
-                        page_table.shape[1], rope_rows)
-    _call(lib().hv_append_kv, dev, args)
+                        page_table.data_ptr(), ids, positions.data_ptr(), *q_str[:2], *k_str[:2], *v_str[:2],
+                        *qo_str[:2], *cache, rope_stride, table_stride, tokens, heads, kv_heads, dim, rot,
+                        bool(interleaved), code, pages, page, seqs, max_pages, rope_rows)
+    _call(_c.hv_append_kv, dev, args)
     return q_out
 
 
@@ -287,14 +306,13 @@ class AttentionWorkspace:
     and any sizes.  Calls that share one must not overlap in time (one per stream)."""
 
     def __init__(self, device=None):
-        import ctypes as C
-        torch = _torch()
+        torch = _ready()
         self.device = torch.device("cuda", torch.cuda.current_device() if device is None else
                                    torch.device(device).index or 0)
         need, most = C.c_int64(), 0
         with torch.cuda.device(self.device):
             for dim in HEAD_DIMS:
-                check(lib().hv_paged_attention_workspace(dim, C.byref(need)))
+                check(_c.hv_paged_attention_workspace(dim, C.byref(need)))
                 most = max(most, need.value)
             self.buffer = torch.zeros(most, dtype=torch.uint8, device=self.device)
         self.bytes = most
@@ -304,15 +322,15 @@ class AttentionWorkspace:
 _workspaces = {}  # (device index, stream handle) -> AttentionWorkspace
 
 
-def _workspace(torch, device):
+def _workspace(torch, index):
     """The current stream's own workspace, made at its first call; a fresh one while the
     stream is being captured, since a graph may be replayed on any stream."""
     if torch.cuda.is_current_stream_capturing():
-        return AttentionWorkspace(device)
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+        return AttentionWorkspace(f"cuda:{index}")
+    key = (index, _raw_stream(index))
     ws = _workspaces.get(key)
     if ws is None:
-        ws = _workspaces[key] = AttentionWorkspace(device)
+        ws = _workspaces[key] = AttentionWorkspace(f"cuda:{index}")
     return ws
 
 
@@ -327,16 +345,17 @@ def paged_attention(q, k_cache, v_cache, page_table, lens, scale=None, workspace
     float32 [seqs, heads] (-inf for no tokens).
 
     ``workspace``: an AttentionWorkspace; by default the module keeps one per stream."""
-    torch = _torch()
-    dev = q.device
-    _need(q, "q", 3, dev)
+    torch = _ready()
+    dev = _index(q, "q")
+    q_str = _strides(q, "q", 3, dev)
     cache = _cache_strides(k_cache, v_cache, dev)
-    _ints(page_table, "page_table", 2, dev)
-    _ints(lens, "lens", 1, dev)
-    code = _dtype_codes().get(q.dtype)
+    table_stride = _int_strides(page_table, "page_table", 2, dev)[0]
+    _int_strides(lens, "lens", 1, dev)
+    dtype = q.dtype
+    code = _types.get(dtype)
     if code not in (abi.HV_BF16, abi.HV_F16):
         raise TypeError("q must be bfloat16 or float16")
-    if k_cache.dtype != q.dtype:
+    if k_cache.dtype is not dtype:
         raise TypeError("q and the caches must have the same type")
     seqs, heads, dim = q.shape
     pages, page, kv_heads, cache_dim = k_cache.shape
@@ -346,24 +365,22 @@ def paged_attention(q, k_cache, v_cache, page_table, lens, scale=None, workspace
         raise ValueError(f"dim must be one of {HEAD_DIMS}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("heads must be a positive multiple of kv_heads")
-    if page_table.shape[0] != seqs or lens.shape[0] != seqs:
+    rows, max_pages = page_table.shape
+    if rows != seqs or lens.shape[0] != seqs:
         raise ValueError("page_table and lens have one row per sequence")
     if out is None:
-        out = torch.empty((seqs, heads, dim), dtype=q.dtype, device=dev)
+        out = torch.empty((seqs, heads, dim), dtype=dtype, device=q.device)
+        out_str = (heads * dim, dim)
     else:
-        _need(out, "out", 3, dev)
-        if out.shape != q.shape:
-            raise ValueError("out must have q's shape")
-        if out.dtype != q.dtype:
-            raise TypeError("out must have q's type")
+        out_str = _like(out, "out", q, "q", dev)
     if workspace is None:
         workspace = _workspace(torch, dev)
-    elif workspace.device != dev:
-        raise ValueError(f"the workspace must live on {dev}")
-    lse = torch.empty((seqs, heads), dtype=torch.float32, device=dev) if return_lse else None
+    elif workspace.device.index != dev:
+        raise ValueError(f"the workspace must live on cuda:{dev}")
+    lse = torch.empty((seqs, heads), dtype=torch.float32, device=q.device) if return_lse else None
     args = _ATTEND.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, k_cache.data_ptr(),
                         v_cache.data_ptr(), page_table.data_ptr(), lens.data_ptr(), workspace.ptr, workspace.bytes,
-                        *q.stride()[:2], *out.stride()[:2], heads, 1, *cache, page_table.stride(0), seqs, heads,
-                        kv_heads, dim, code, pages, page, page_table.shape[1], dim ** -0.5 if scale is None else scale)
-    _call(lib().hv_paged_attention, dev, args)
+                        *q_str[:2], *out_str[:2], heads, 1, *cache, table_stride, seqs, heads, kv_heads, dim, code,
+                        pages, page, max_pages, dim ** -0.5 if scale is None else scale)
+    _call(_c.hv_paged_attention, dev, args)
     return (out, lse) if return_lse else out
