@@ -29,9 +29,11 @@ namespace {
 
 using namespace dec;
 
-constexpr int ROWS = 16, WTOK = 16, SLICES = 4, TILE = SLICES * WTOK;
-constexpr int MIN_SHARE = 4;  // tiles: a part costs more than the loads of fewer
-constexpr int FAN = 16;       // parts that one CTA joins at a time
+constexpr int ROWS = 16, BLOCK = 16, SLICES = 4;
+constexpr int MIN_SHARE = 256;  // tokens: a part costs more than the loads of fewer
+constexpr int FAN = 16;       // parts whose loads a joining CTA has in flight together
+// A further FAN parts cost a joining CTA about 1.5 us, a second level about 7.
+constexpr int ONE_LEVEL = 4 * FAN, GROUP = FAN;
 constexpr int MAX_GRID = 1024;
 
 struct AttendArgs {
@@ -55,6 +57,9 @@ template <int D>
 struct Lay {
     static constexpr int HALVES = D > 128 ? 2 : 1, DH = D / HALVES;
     static constexpr int WARPS = SLICES * HALVES, THREADS = WARPS * 32;
+    // 16-token blocks of a warp's step: a step costs about the same for 32 tokens of 64
+    // dimensions (16 heads of 64 over 64 x 4000 tokens: BEFORE -> AFTER us) as for 16 of 128
+    static constexpr int BLOCKS = D <= 64 ? 2 : 1, WTOK = BLOCKS * BLOCK, TILE = SLICES * WTOK;
     static constexpr int ROW = DH * 2 + 16;  // bytes: rows 16 bytes apart modulo 128 (ldmatrix without conflicts)
     static constexpr int STAGES = 3;
     static constexpr int STAGE = 2 * WTOK * ROW;
@@ -64,7 +69,7 @@ struct Lay {
     static constexpr int STAT = SUM + (ROWS * SUM_ROW * 4 > EXCHANGE ? ROWS * SUM_ROW * 4 : EXCHANGE);
     static constexpr int MISC = STAT + SLICES * ROWS * 2 * 4;  // stat: [SLICES][ROWS][2] float
     static constexpr int BYTES = MISC + 32;
-    static constexpr int PER_SM = D <= 64 ? 3 : D <= 128 ? 2 : 1;
+    static constexpr int PER_SM = D <= 128 ? 2 : 1;
     static_assert(PER_SM * (BYTES + 1024) <= 228 * 1024, "the CTAs of a wave are resident together");
 };
 
@@ -130,6 +135,7 @@ __device__ __forceinline__ int length_of(const AttendArgs &a, int b) {
 }
 
 // A place on the line of tiles: tile `tile` of item (sequence b, head tile h).
+template <int TILE>
 struct Place {
     int b, h, tile, len, tiles;
     __device__ __forceinline__ void set(const AttendArgs &a, int seq) {
@@ -267,7 +273,8 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
     griddep_wait();
     griddep_launch();
     using L = Lay<D>;
-    constexpr int DH = L::DH, THREADS = L::THREADS;
+    constexpr int DH = L::DH, THREADS = L::THREADS, BLOCKS = L::BLOCKS, WTOK = L::WTOK, TILE = L::TILE;
+    using Place = Place<L::TILE>;
     extern __shared__ __align__(128) uint8_t smem[];
     float *sum = (float *)(smem + L::SUM);
     float *stat = (float *)(smem + L::STAT);
@@ -296,7 +303,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
         }
         total *= items;
         long long share = (total + gridDim.x - 1) / gridDim.x;
-        if (share < MIN_SHARE) share = MIN_SHARE;
+        if (share < MIN_SHARE / TILE) share = MIN_SHARE / TILE;
         const long long first = share * blockIdx.x;
         long long before = 0;  // tiles of the sequences ahead of b0
         int found = -1;
@@ -342,80 +349,89 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
     uint8_t *ring = smem + warp * L::STAGES * L::STAGE;
     const T *kc = (const T *)a.kc, *vc = (const T *)a.vc;
 
-    // The page of this warp's tokens (page16: they share one), or of this lane's token (lane
-    // & 15), at place p; -1 past the length.
-    auto page_of = [&](const Place &p) {
-        const int t0 = p.tile * TILE + slice * WTOK, t = a.page16 ? t0 : t0 + (lane & 15);
-        if (t >= p.len) return -1;
-        const int col = a.page16 ? (a.page_shift >= 0 ? t >> a.page_shift : t / a.page) : t / a.page;
-        return a.pages[p.b * a.pages_stride + col];
+    // The page of a block of 16 tokens (page16: they share one), or of this lane's token of it
+    // (lane & 15), at place p; -1 past the length.
+    struct Pages {
+        int of[BLOCKS];
     };
-    auto load = [&](int stage, const Place &p, int pg) {
+    auto pages_of = [&](const Place &p) {
+        Pages r;
+#pragma unroll
+        for (int k = 0; k < BLOCKS; ++k) {
+            const int t = p.tile * TILE + slice * WTOK + k * BLOCK + (a.page16 ? 0 : lane & 15);
+            r.of[k] = t < p.len ? a.pages[p.b * a.pages_stride + (a.page_shift >= 0 ? t >> a.page_shift : t / a.page)] : -1;
+        }
+        return r;
+    };
+    auto load = [&](int stage, const Place &p, const Pages &pgs) {
         const int t0 = p.tile * TILE + slice * WTOK;
         if (t0 >= p.len) return;  // not read either
         const int head = p.h / a.head_tiles;
-        const uint32_t dst = tc05::smem_u32(ring + stage * L::STAGE);
         constexpr int CH = DH / 8;  // 16-byte pieces of a row
-        constexpr int N = WTOK * CH / 32;
-        if (a.page16) {
-            const bool ok = pg >= 0 && pg < a.num_pages;
-            if (!ok) {
+        constexpr int N = BLOCK * CH / 32;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            const uint32_t dst = tc05::smem_u32(ring + stage * L::STAGE) + b * BLOCK * L::ROW;
+            const int t1 = t0 + b * BLOCK;
+            if (a.page16) {
+                int pg = pgs.of[b], live = p.len - t1;  // rows of the 16 that exist
+                if (pg < 0 || pg >= a.num_pages) {
+                    if (live > 0) atomicOr(a.err, HV_DECODE_BAD_PAGE);
+                    pg = live = 0;
+                }
+                const int slot = a.page_shift >= 0 ? t1 & (a.page - 1) : t1 % a.page;
+                const T *k = kc + (pg * a.kc_page + slot * a.kc_slot + head * a.kc_head + half * DH);
+                const T *v = vc + (pg * a.vc_page + slot * a.vc_slot + head * a.vc_head + half * DH);
+                if constexpr (32 % CH == 0) {
+                    const int row0 = lane / CH, col = lane % CH;
+                    k += row0 * a.kc_slot + col * 8;
+                    v += row0 * a.vc_slot + col * 8;
+                    const uint32_t to = dst + row0 * L::ROW + col * 16;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int n = row0 + i * (32 / CH) < live ? 16 : 0;
+                        cp16(to + i * (32 / CH) * L::ROW, k, n);
+                        cp16(to + (WTOK + i * (32 / CH)) * L::ROW, v, n);
+                        k += (32 / CH) * a.kc_slot;
+                        v += (32 / CH) * a.vc_slot;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int c = i * 32 + lane, row = c / CH, col = c % CH, n = row < live ? 16 : 0;
+                        cp16(dst + row * L::ROW + col * 16, k + row * a.kc_slot + col * 8, n);
+                        cp16(dst + (WTOK + row) * L::ROW + col * 16, v + row * a.vc_slot + col * 8, n);
+                    }
+                }
+                continue;
+            }
+            const int t = t1 + (lane & 15), pg = pgs.of[b];
+            bool ok = t < p.len;
+            if (ok && (pg < 0 || pg >= a.num_pages)) {
                 atomicOr(a.err, HV_DECODE_BAD_PAGE);
-                pg = 0;
+                ok = false;
             }
-            const int live = ok ? p.len - t0 : 0;  // rows of the 16 that exist
-            const int slot = a.page_shift >= 0 ? t0 & (a.page - 1) : t0 % a.page;
-            const T *k = kc + (pg * a.kc_page + slot * a.kc_slot + head * a.kc_head + half * DH);
-            const T *v = vc + (pg * a.vc_page + slot * a.vc_slot + head * a.vc_head + half * DH);
-            if constexpr (32 % CH == 0) {
-                const int row0 = lane / CH, col = lane % CH;
-                k += row0 * a.kc_slot + col * 8;
-                v += row0 * a.vc_slot + col * 8;
-                const uint32_t to = dst + row0 * L::ROW + col * 16;
+            const int slot = a.page_shift >= 0 ? t & (a.page - 1) : t % a.page;
+            const long long ko = ok ? pg * a.kc_page + slot * a.kc_slot + head * a.kc_head + half * DH : -1;
+            const long long vo = ok ? pg * a.vc_page + slot * a.vc_slot + head * a.vc_head + half * DH : -1;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int n = row0 + i * (32 / CH) < live ? 16 : 0;
-                    cp16(to + i * (32 / CH) * L::ROW, k, n);
-                    cp16(to + (WTOK + i * (32 / CH)) * L::ROW, v, n);
-                    k += (32 / CH) * a.kc_slot;
-                    v += (32 / CH) * a.vc_slot;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int c = i * 32 + lane, row = c / CH, col = c % CH, n = row < live ? 16 : 0;
-                    cp16(dst + row * L::ROW + col * 16, k + row * a.kc_slot + col * 8, n);
-                    cp16(dst + (WTOK + row) * L::ROW + col * 16, v + row * a.vc_slot + col * 8, n);
-                }
+            for (int i = 0; i < N; ++i) {
+                const int c = i * 32 + lane, row = c / CH, col = c % CH;
+                const long long k = __shfl_sync(~0u, ko, row), v = __shfl_sync(~0u, vo, row);
+                cp16(dst + row * L::ROW + col * 16, kc + (k < 0 ? 0 : k + col * 8), k < 0 ? 0 : 16);
+                cp16(dst + (WTOK + row) * L::ROW + col * 16, vc + (v < 0 ? 0 : v + col * 8), v < 0 ? 0 : 16);
             }
-            return;
-        }
-        const int t = t0 + (lane & 15);
-        bool ok = t < p.len;
-        if (ok && (pg < 0 || pg >= a.num_pages)) {
-            atomicOr(a.err, HV_DECODE_BAD_PAGE);
-            ok = false;
-        }
-        const int slot = t % a.page;
-        const long long ko = ok ? pg * a.kc_page + slot * a.kc_slot + head * a.kc_head + half * DH : -1;
-        const long long vo = ok ? pg * a.vc_page + slot * a.vc_slot + head * a.vc_head + half * DH : -1;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = i * 32 + lane, row = c / CH, col = c % CH;
-            const long long k = __shfl_sync(~0u, ko, row), v = __shfl_sync(~0u, vo, row);
-            cp16(dst + row * L::ROW + col * 16, kc + (k < 0 ? 0 : k + col * 8), k < 0 ? 0 : 16);
-            cp16(dst + (WTOK + row) * L::ROW + col * 16, vc + (v < 0 ? 0 : v + col * 8), v < 0 ? 0 : 16);
         }
     };
 
-    int pg = page_of(ld);
+    Pages pg = pages_of(ld);
     int loaded = 0;
     auto load_next = [&]() {
         if (loaded < count) {
             load(loaded % L::STAGES, ld, pg);
             if (++loaded < count) {
                 ld.next(a, items);
-                pg = page_of(ld);
+                pg = pages_of(ld);
             }
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
@@ -450,15 +466,17 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
         const int t0 = cur.tile * TILE + slice * WTOK;
         if (t0 < cur.len) {
             const uint32_t kb = tc05::smem_u32(ring + (u % L::STAGES) * L::STAGE), vb = kb + WTOK * L::ROW;
-            float s[2][4] = {};
+            float s[2 * BLOCKS][4] = {};
             const uint32_t ka = kb + ((lane >> 4) * 8 + (lane & 7)) * L::ROW + ((lane >> 3) & 1) * 16;
 #pragma unroll
-            for (int j = 0; j < DH / 16; ++j) {
-                uint32_t r[4];
-                ldsm4(ka + j * 32, r);
-                mma<T>(s[0], qf[j], r[0], r[1]);
-                mma<T>(s[1], qf[j], r[2], r[3]);
-            }
+            for (int j = 0; j < DH / 16; ++j)
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) {
+                    uint32_t r[4];
+                    ldsm4(ka + b * BLOCK * L::ROW + j * 32, r);
+                    mma<T>(s[2 * b], qf[j], r[0], r[1]);
+                    mma<T>(s[2 * b + 1], qf[j], r[2], r[3]);
+                }
             if constexpr (L::HALVES == 2) {
                 // two buffers in turn: the partner has read a buffer before the step's barrier
                 // after the one that filled it
@@ -473,12 +491,12 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
             }
             // s[n][2 * i + e]: row lane / 4 + 8 i, token t0 + 8 n + 2 (lane % 4) + e
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2 * BLOCKS; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[n][e] *= a.scale_log2;
             if (t0 + WTOK > cur.len)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 2 * BLOCKS; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (t0 + n * 8 + (lane & 3) * 2 + (e & 1) >= cur.len) s[n][e] = -CUDART_INF_F;
@@ -487,7 +505,9 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
             float x[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                x[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+                x[i] = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+#pragma unroll
+                for (int n = 1; n < 2 * BLOCKS; ++n) x[i] = fmaxf(x[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
                 x[i] = fmaxf(x[i], __shfl_xor_sync(~0u, x[i], 1));
                 x[i] = fmaxf(x[i], __shfl_xor_sync(~0u, x[i], 2));
             }
@@ -509,7 +529,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2 * BLOCKS; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[n][e] = exp2_(s[n][e] - m[e >> 1]);
@@ -517,15 +537,19 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 }
             // weights in T for the product: each is within 2^-9 (bf16) of its 32-bit value,
             // as the values that it multiplies are of theirs; the sums stay in 32 bits
-            uint32_t p[4] = {pack(s[0][0], s[0][1], T()), pack(s[0][2], s[0][3], T()), pack(s[1][0], s[1][1], T()),
-                             pack(s[1][2], s[1][3], T())};
-            const uint32_t va = vb + (lane & 15) * L::ROW + (lane >> 4) * 16;
 #pragma unroll
-            for (int j = 0; j < DH / 16; ++j) {
-                uint32_t r[4];
-                ldsm4t(va + j * 32, r);
-                mma<T>(o[2 * j], p, r[0], r[1]);
-                mma<T>(o[2 * j + 1], p, r[2], r[3]);
+            for (int b = 0; b < BLOCKS; ++b) {
+                const float(&x)[4] = s[2 * b], (&y)[4] = s[2 * b + 1];
+                const uint32_t p[4] = {pack(x[0], x[1], T()), pack(x[2], x[3], T()), pack(y[0], y[1], T()),
+                                       pack(y[2], y[3], T())};
+                const uint32_t va = vb + (b * BLOCK + (lane & 15)) * L::ROW + (lane >> 4) * 16;
+#pragma unroll
+                for (int j = 0; j < DH / 16; ++j) {
+                    uint32_t r[4];
+                    ldsm4t(va + j * 32, r);
+                    mma<T>(o[2 * j], p, r[0], r[1]);
+                    mma<T>(o[2 * j + 1], p, r[2], r[3]);
+                }
             }
         }
         __syncwarp();  // the stage that is refilled next was read in the step before
@@ -595,10 +619,10 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 }
                 if (lse && tid < nrows) lse[tid * a.lse_head] = (M + log2f(S)) * 0.69314718055994531f;
             } else {
-                // A part.  Those of FAN neighbouring shares are joined by the last of them to come,
-                // and where the item has more, their sums by the last of all.  A share leaves its
-                // second slot to the item that starts in it, its first to one that started before;
-                // likewise at most one item enters a group of shares from before.
+                // A part.  The last CTA of up to ONE_LEVEL to come joins them all; of more, the last of
+                // every GROUP neighbouring shares joins theirs, and the last of those the rest.  A
+                // share leaves its second slot to the item that starts in it, its first to one that
+                // started before; likewise at most one item enters a group of shares from before.
                 auto slot = [&](int c) { return 2ll * c + (c == c_first); };
                 const long long mine = slot(blockIdx.x);
                 float4 *po = (float4 *)(a.parts + mine * (ROWS * D));
@@ -606,17 +630,23 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 for (int i = tid; i < nvec; i += THREADS)
                     __stcg(po + i, *(const float4 *)(sum + (i / (D / 4)) * L::SUM_ROW + i % (D / 4) * 4));
                 if (tid < nrows) __stcg(pst + tid, make_float2(M, S));
-                const int g = blockIdx.x / FAN, g_first = c_first / FAN, g_last = c_last / FAN;
-                const int lo = max(c_first, g * FAN), n = min(c_last, g * FAN + FAN - 1) - lo + 1;
-                if (comes_last(lo == c_first ? a.counts + c_first : a.counts + MAX_GRID + g, n, misc)) {
-                    const bool all = g_first == g_last;
-                    if (all || n > 1)
-                        join_parts<T, D>(a.parts, sum, stat, [&](int k) { return slot(lo + k); }, n, nrows,
-                                         all ? out : nullptr, a.o_head, a.o_vec, lse, a.lse_head);
-                    if (!all && comes_last(a.counts + 2 * MAX_GRID + c_first, g_last - g_first + 1, misc))
-                        join_parts<T, D>(a.parts, sum, stat,
-                                         [&](int k) { return slot(k ? (g_first + k) * FAN : c_first); },
-                                         g_last - g_first + 1, nrows, out, a.o_head, a.o_vec, lse, a.lse_head);
+                const int n = c_last - c_first + 1;
+                if (n <= ONE_LEVEL) {
+                    if (comes_last(a.counts + c_first, n, misc))
+                        join_parts<T, D>(a.parts, sum, stat, [&](int k) { return slot(c_first + k); }, n, nrows, out,
+                                         a.o_head, a.o_vec, lse, a.lse_head);
+                } else {
+                    const int g = blockIdx.x / GROUP, g_first = c_first / GROUP, groups = c_last / GROUP - g_first + 1;
+                    const int lo = max(c_first, g * GROUP), ng = min(c_last, g * GROUP + GROUP - 1) - lo + 1;
+                    if (comes_last(lo == c_first ? a.counts + c_first : a.counts + MAX_GRID + g, ng, misc)) {
+                        if (ng > 1)
+                            join_parts<T, D>(a.parts, sum, stat, [&](int k) { return slot(lo + k); }, ng, nrows,
+                                             (T *)nullptr, 0, false, nullptr, 0);
+                        if (comes_last(a.counts + 2 * MAX_GRID + c_first, groups, misc))
+                            join_parts<T, D>(a.parts, sum, stat,
+                                             [&](int k) { return slot(k ? (g_first + k) * GROUP : c_first); }, groups,
+                                             nrows, out, a.o_head, a.o_vec, lse, a.lse_head);
+                    }
                 }
             }
             __syncthreads();  // sum, stat and misc are free again
@@ -638,7 +668,7 @@ int wave(int d) {
     if (cudaGetDevice(&dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return 0;
-    const int grid = sms * (d <= 64 ? Lay<64>::PER_SM : d <= 128 ? Lay<128>::PER_SM : Lay<256>::PER_SM);
+    const int grid = sms * (d <= 128 ? Lay<128>::PER_SM : Lay<256>::PER_SM);
     return grid < MAX_GRID ? grid : MAX_GRID;
 }
 
@@ -714,7 +744,7 @@ extern "C" int hv_paged_attention(const hv_attention_args *p, void *stream) {
     a.num_pages = p->num_pages, a.page = p->page_size, a.max_pages = p->max_pages;
     a.q_pairs = dec::aligned(a.q, 4) && a.q_seq % 2 == 0 && a.q_head % 2 == 0;
     a.o_vec = dec::aligned(a.out, 8) && a.o_seq % 4 == 0 && a.o_head % 4 == 0;
-    a.page16 = a.page % WTOK == 0;
+    a.page16 = a.page % BLOCK == 0;
     a.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.counts = (uint32_t *)p->d_workspace;
