@@ -1,4 +1,4 @@
-// hv_decode.cu — the decode operators' device error word.
+// hv_decode.cu — the decode operators' device error word and device properties.
 #include <atomic>
 
 #include "hv_decode.cuh"
@@ -10,6 +10,7 @@ __device__ int g_decode_error;
 
 constexpr int MAX_DEVICES = 64;
 std::atomic<int *> g_address[MAX_DEVICES];
+std::atomic<int> g_sms[MAX_DEVICES];
 
 }  // namespace
 
@@ -26,6 +27,17 @@ int *error_word() {
         g_address[dev].store(p, std::memory_order_release);
     }
     return p;
+}
+
+int sm_count() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 0;
+    int n = g_sms[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        g_sms[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 }  // namespace dec

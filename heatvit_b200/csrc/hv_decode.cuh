@@ -15,6 +15,8 @@ namespace dec {
 // Device word that the decode kernels OR HV_DECODE_* bits into (hv_decode_error reads
 // and clears it); null when its address cannot be resolved.
 int *error_word();
+// SMs of the current device; 0 when that cannot be read.
+int sm_count();
 
 inline int elem_size(int dtype) { return dtype == HV_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == HV_BF16 || dtype == HV_F16 || dtype == HV_F32; }
