@@ -14,6 +14,8 @@
 // shuffles.  Rows of up to 1024 channels take a warp each, longer ones a CTA.
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "hv_decode.cuh"
 #include "hv_tc05.cuh"
 
@@ -29,7 +31,7 @@ struct NormArgs {
     float *scale;
     long long x_stride, res_stride, res_out_stride, q_stride;  // elements
     long long scale_row, scale_group;
-    int rows, dim, vec, q8;
+    int rows, dim, full;
     float eps;
 };
 
@@ -46,124 +48,191 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_
 
 constexpr float kE4m3Max = 448.f;
 constexpr float kAmaxFloor = 7.888609052210118e-31f;  // 2^-100
+constexpr float kSafeLow = 1e-30f, kSafeHigh = 1e30f;
 
-// Group `c / 8` of a row's output: eight channels of a thread, `n` of which exist; 16
-// neighbouring lanes hold a block of 128.  Every lane of the warp takes part.
-__device__ __forceinline__ void put_group(const NormArgs &a, long long row, int c, int n, const float (&h)[8],
-                                          const float (&w)[8], float rstd) {
-    float y[8], amax = 0.f;
+// A row is worked on in groups of eight channels, of which the group at channel c has
+// a.dim - c.  FULL: every group has eight or none, and starts on 16 bytes (8 in q).
+template <typename T, bool FULL>
+struct Group {
+    T e[8];  // as stored, so that a load can be under way while others are used
+    __device__ __forceinline__ void load(const T *p, int n) {
+        if (FULL) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        y[j] = h[j] * rstd * w[j];
-        amax = fmaxf(amax, fabsf(y[j]));
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                ((uint4 *)e)[i] = n > 0 ? ((const uint4 *)p)[i] : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : from_f32<T>(0.f);
+        }
     }
+    __device__ __forceinline__ void store(T *p, int n) const {
+        if (FULL) {
+            if (n > 0)
 #pragma unroll
-    for (int o = 8; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-    amax = fmaxf(amax, kAmaxFloor);
-    if (n <= 0) return;
-    if ((c & 127) == 0) a.scale[row * a.scale_row + (long long)(c >> 7) * a.scale_group] = amax / kE4m3Max;
-    const float inv = kE4m3Max / amax;
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4 *)p)[i] = ((const uint4 *)e)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) p[i] = e[i];
+        }
+    }
+};
+
+__device__ __forceinline__ float reciprocal(float x) {  // within one unit in the last place
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// e4m3(y * f) of a group.
+template <bool FULL>
+__device__ __forceinline__ void put_q(const NormArgs &a, long long row, int c, int n, const float (&y)[8], float f) {
     uint32_t b[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * j] * inv, y[4 * j + 1] * inv), __NV_SATFINITE,
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * j] * f, y[4 * j + 1] * f), __NV_SATFINITE,
                                                      __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * j + 2] * inv, y[4 * j + 3] * inv),
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * j + 2] * f, y[4 * j + 3] * f),
                                                      __NV_SATFINITE, __NV_E4M3);
         b[j] = lo | hi << 16;
     }
     uint8_t *q = a.q + row * a.q_stride + c;
-    if (a.q8 && n >= 8) {
-        *(uint2 *)q = make_uint2(b[0], b[1]);
+    if (FULL) {
+        if (n > 0) *(uint2 *)q = make_uint2(b[0], b[1]);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < n) q[j] = (uint8_t)(b[j >> 2] >> (8 * (j & 3)));
     }
 }
-
-// One CTA a row, or (TPR = 32) one warp for RPW rows, whose loads are issued together.
-template <typename T, int TPR, int NV, int RPW, bool RES>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_kernel(const NormArgs a) {
-    griddep_wait();
-    griddep_launch();
-    static_assert(TPR == 32 || RPW == 1, "a CTA's barrier is for one row");
-    const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const long long row0 = TPR == 32 ? ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * RPW : blockIdx.x;
-    if (row0 >= a.rows) return;  // whole warps, or none of a one-row CTA
-    float h[RPW][NV][8], ss[RPW];
+// A block's amax: 16 neighbouring lanes hold its 128 channels, and every lane of the warp
+// takes part.
+__device__ __forceinline__ float block_amax(const float (&y)[8]) {
+    float m = 0.f;
 #pragma unroll
-    for (int k = 0; k < RPW; ++k) {
-        const long long row = min(row0 + k, (long long)a.rows - 1);
-        const T *x = (const T *)a.x + row * a.x_stride;
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(y[j]));
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (t + i * TPR) * 8;
-            load8(x + c, a.dim - c, a.vec, h[k][i]);
-        }
-    }
-    if (RES) {
+    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    return m;
+}
+// A row's 1 / rms cancels in y / scale, so q goes out before the row's sum is known:
+// q = e4m3(h w 448 / amax|h w|).  Returns amax|h w|, from which put_scales makes the scale.
+template <typename T, bool FULL>
+__device__ __forceinline__ float put_group(const NormArgs &a, long long row, int c, const float (&h)[8],
+                                           const Group<T, FULL> &w) {
+    float y[8];
 #pragma unroll
-        for (int k = 0; k < RPW; ++k) {
-            const long long row = min(row0 + k, (long long)a.rows - 1);
-            const T *res = (const T *)a.res + row * a.res_stride;
+    for (int j = 0; j < 8; ++j) y[j] = h[j] * to_f32(w.e[j]);
+    const float amax = block_amax(y);
+    put_q<FULL>(a, row, c, a.dim - c, y, kE4m3Max * reciprocal(amax));
+    return amax;
+}
+template <typename T, int TPR, int NV, bool FULL>
+__device__ __forceinline__ void put_scales(const NormArgs &a, long long row, int t, const float (&h)[NV][8],
+                                           const Group<T, FULL> (&w)[NV], const float (&amax)[NV], float rstd) {
+    // A block under the floor, or whose products or quotients may have left the range, is done
+    // again in the order of the formula.
+    bool redo = false;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (t + i * TPR) * 8;
-                float r[8];
-                load8(res + c, a.dim - c, a.vec, r);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) h[k][i][j] += r[j];
-            }
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < RPW; ++k) {
-        ss[k] = 0.f;
+    for (int i = 0; i < NV; ++i)
+        redo |= (t + i * TPR) * 8 < a.dim && !(amax[i] * rstd >= kAmaxFloor && amax[i] > kSafeLow && amax[i] < kSafeHigh);
+    if (!__any_sync(~0u, redo)) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * 8;
-            if (RES && row0 + k < a.rows)
-                store8((T *)a.res_out + (row0 + k) * a.res_out_stride + c, a.dim - c, a.vec, h[k][i]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ss[k] += h[k][i][j] * h[k][i][j];
+            if ((t & 15) == 0 && c < a.dim)
+                a.scale[row * a.scale_row + (c >> 7) * a.scale_group] = amax[i] * rstd * (1.f / kE4m3Max);
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) ss[k] += __shfl_xor_sync(~0u, ss[k], o);
+        return;
     }
-    if (TPR > 32) {
-        __shared__ float part[32];
-        if ((t & 31) == 0) part[t >> 5] = ss[0];
-        __syncthreads();
-        ss[0] = 0.f;
-#pragma unroll
-        for (int i = 0; i < TPR / 32; ++i) ss[0] += part[i];
-    }
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8;
-        float w[8];
-        load8((const T *)a.w + c, a.dim - c, a.vec, w);
+        float y[8];
 #pragma unroll
-        for (int k = 0; k < RPW; ++k)
-            put_group(a, row0 + k, c, row0 + k < a.rows ? a.dim - c : 0, h[k][i], w,
-                      rsqrtf(ss[k] / (float)a.dim + a.eps));
+        for (int k = 0; k < NV; ++k)
+            if (k == i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = h[k][j] * rstd * to_f32(w[k].e[j]);
+        const float top = fmaxf(block_amax(y), kAmaxFloor);
+        put_q<FULL>(a, row, c, a.dim - c, y, kE4m3Max / top);
+        if ((t & 15) == 0 && c < a.dim) a.scale[row * a.scale_row + (c >> 7) * a.scale_group] = top * (1.f / kE4m3Max);
+    }
+}
+
+// One row for each group of TPR threads: a CTA of it, or (TPR = 32) warps that take a row
+// after another and load the next while they work on one.
+template <typename T, int TPR, int NV, bool RES, bool FULL>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_kernel(const __grid_constant__ NormArgs a) {
+    griddep_wait();
+    griddep_launch();
+    const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const long long step = TPR == 32 ? gridDim.x * 8ll : gridDim.x;
+    long long row = TPR == 32 ? blockIdx.x * 8ll + (threadIdx.x >> 5) : blockIdx.x;
+    Group<T, FULL> x[NV], r[RES ? NV : 1], w[NV];
+    auto fetch = [&](long long k) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            x[i].load((const T *)a.x + k * a.x_stride + c, a.dim - c);
+            if (RES) r[i].load((const T *)a.res + k * a.res_stride + c, a.dim - c);
+        }
+    };
+    if (row < a.rows) fetch(row);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i].load((const T *)a.w + (t + i * TPR) * 8, a.dim - (t + i * TPR) * 8);
+    for (; row < a.rows; row += step) {  // once, where TPR > 32
+        float h[NV][8], amax[NV], ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[i][j] = to_f32(x[i].e[j]);
+                if (RES) h[i][j] += to_f32(r[i].e[j]);
+            }
+        if (TPR == 32 && row + step < a.rows) fetch(row + step);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            if (RES) {
+                Group<T, FULL> o;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o.e[j] = from_f32<T>(h[i][j]);
+                o.store((T *)a.res_out + row * a.res_out_stride + c, a.dim - c);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss += h[i][j] * h[i][j];
+            amax[i] = put_group(a, row, c, h[i], w[i]);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+        if (TPR > 32) {
+            __shared__ float part[32];
+            if ((t & 31) == 0) part[t >> 5] = ss;
+            __syncthreads();
+            ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < TPR / 32; ++i) ss += part[i];
+        }
+        put_scales<T, TPR, NV, FULL>(a, row, t, h, w, amax, rsqrtf(ss / (float)a.dim + a.eps));
+        if (TPR > 32) break;
     }
 }
 
 // Many long rows: CTAs that stay, rows copied ahead into a ring in shared memory by the bulk
 // copy engine, so that loads are on the way while a row is reduced and written (one CTA a row
-// leaves the memory idle between its phases).  Everyone has read a stage by the barrier of its
-// row's reduction, after which one thread refills it.
-constexpr int RING_THREADS = 256, MAX_STAGES = 4;
+// leaves the memory idle between its phases: 16384 x 8192 bf16 took 194 us that way, 222 with
+// 256 threads).  Everyone has read a stage by the barrier of its row's reduction, after which
+// one thread refills it.
+constexpr int MAX_STAGES = 4;
 constexpr uint32_t RING_WAIT = 1u << 22;
 
-template <typename T, int NV, bool RES>
-__global__ void __launch_bounds__(RING_THREADS) norm_ring_kernel(const NormArgs a, int stages, int stage_bytes,
-                                                                 int row_bytes, int *err) {
+template <typename T, int THREADS, int NV, bool RES>
+__global__ void __launch_bounds__(THREADS) norm_ring_kernel(const __grid_constant__ NormArgs a, int stages,
+                                                            int stage_bytes, int row_bytes, int *err) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[MAX_STAGES];
-    __shared__ float part[2][RING_THREADS / 32];
+    __shared__ float part[2][THREADS / 32];
     __shared__ volatile int stop;
     const int t = threadIdx.x;
     if (t == 0) {
@@ -175,39 +244,44 @@ __global__ void __launch_bounds__(RING_THREADS) norm_ring_kernel(const NormArgs 
     griddep_wait();
     griddep_launch();
     const int mine = (a.rows - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // rows of this CTA
-    auto fetch = [&](int i) {
+    auto fetch = [&](int i, int s) {
         const long long row = blockIdx.x + (long long)i * gridDim.x;
-        const uint32_t dst = tc05::smem_u32(smem + (i % stages) * stage_bytes);
-        uint64_t *bar = &full[i % stages];
-        mbar_expect(bar, RES ? 2 * row_bytes : row_bytes);
-        bulk_copy(dst, (const T *)a.x + row * a.x_stride, row_bytes, bar);
-        if (RES) bulk_copy(dst + stage_bytes / 2, (const T *)a.res + row * a.res_stride, row_bytes, bar);
+        const uint32_t dst = tc05::smem_u32(smem + s * stage_bytes);
+        mbar_expect(&full[s], RES ? 2 * row_bytes : row_bytes);
+        bulk_copy(dst, (const T *)a.x + row * a.x_stride, row_bytes, &full[s]);
+        if (RES) bulk_copy(dst + stage_bytes / 2, (const T *)a.res + row * a.res_stride, row_bytes, &full[s]);
     };
     if (t == 0)
-        for (int i = 0; i < min(stages, mine); ++i) fetch(i);
-    float w[NV][8];
+        for (int i = 0; i < min(stages, mine); ++i) fetch(i, i);
+    Group<T, true> w[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load8((const T *)a.w + (t + i * RING_THREADS) * 8, a.dim - (t + i * RING_THREADS) * 8, true, w[i]);
+    for (int i = 0; i < NV; ++i) w[i].load((const T *)a.w + (t + i * THREADS) * 8, a.dim - (t + i * THREADS) * 8);
 
+    int s = 0, phase = 0;
     for (int k = 0; k < mine; ++k) {
         const long long row = blockIdx.x + (long long)k * gridDim.x;
-        const T *x = (const T *)(smem + (k % stages) * stage_bytes);
-        const T *res = (const T *)(smem + (k % stages) * stage_bytes + stage_bytes / 2);
-        if (!tc05::mbar_wait(&full[k % stages], (k / stages) & 1, RING_WAIT)) stop = 1;
-        float h[NV][8], ss = 0.f;
+        const T *x = (const T *)(smem + s * stage_bytes), *res = (const T *)(smem + s * stage_bytes + stage_bytes / 2);
+        if (!tc05::mbar_wait(&full[s], phase, RING_WAIT)) stop = 1;
+        float h[NV][8], amax[NV], ss = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (t + i * RING_THREADS) * 8, n = a.dim - c;
-            load8(x + c, n, true, h[i]);
-            if (RES) {
-                float r[8];
-                load8(res + c, n, true, r);
+            const int c = (t + i * THREADS) * 8, n = a.dim - c;
+            Group<T, true> g;
+            g.load(x + c, n);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[i][j] += r[j];
-                store8((T *)a.res_out + row * a.res_out_stride + c, n, true, h[i]);
+            for (int j = 0; j < 8; ++j) h[i][j] = to_f32(g.e[j]);
+            if (RES) {
+                g.load(res + c, n);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    h[i][j] += to_f32(g.e[j]);
+                    g.e[j] = from_f32<T>(h[i][j]);
+                }
+                g.store((T *)a.res_out + row * a.res_out_stride + c, n);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss += h[i][j] * h[i][j];
+            amax[i] = put_group(a, row, c, h[i], w[i]);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
@@ -220,58 +294,64 @@ __global__ void __launch_bounds__(RING_THREADS) norm_ring_kernel(const NormArgs 
             }
             break;
         }
-        if (t == 0 && k + stages < mine) fetch(k + stages);
+        if (t == 0 && k + stages < mine) fetch(k + stages, s);
+        if (++s == stages) {
+            s = 0;
+            phase ^= 1;
+        }
         ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < RING_THREADS / 32; ++i) ss += part[k & 1][i];
-        const float rstd = rsqrtf(ss / (float)a.dim + a.eps);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (t + i * RING_THREADS) * 8;
-            put_group(a, row, c, a.dim - c, h[i], w[i], rstd);
-        }
+        for (int i = 0; i < THREADS / 32; ++i) ss += part[k & 1][i];
+        put_scales<T, THREADS, NV, true>(a, row, t, h, w, amax, rsqrtf(ss / (float)a.dim + a.eps));
     }
 }
 
-template <typename T, int TPR, int NV, int RPW = 1>
-cudaError_t launch(const NormArgs &a, cudaStream_t st) {
-    const dim3 grid((unsigned)(TPR == 32 ? (a.rows + 8ll * RPW - 1) / (8 * RPW) : a.rows)), block(TPR == 32 ? 256 : TPR);
-    return a.res ? launch_pdl(norm_kernel<T, TPR, NV, RPW, true>, grid, block, 0, st, a)
-                 : launch_pdl(norm_kernel<T, TPR, NV, RPW, false>, grid, block, 0, st, a);
+template <typename T, int TPR, int NV>
+cudaError_t launch(const NormArgs &a, int sms, cudaStream_t st) {
+    const int warps_grid = (int)std::min<long long>((a.rows + 7ll) / 8, (long long)sms * (NV == 1 ? 5 : NV == 2 ? 4 : 2));
+    const dim3 grid((unsigned)(TPR == 32 ? warps_grid : a.rows)), block(TPR == 32 ? 256 : TPR);
+    if (a.full)
+        return a.res ? launch_pdl(norm_kernel<T, TPR, NV, true, true>, grid, block, 0, st, a)
+                     : launch_pdl(norm_kernel<T, TPR, NV, false, true>, grid, block, 0, st, a);
+    return a.res ? launch_pdl(norm_kernel<T, TPR, NV, true, false>, grid, block, 0, st, a)
+                 : launch_pdl(norm_kernel<T, TPR, NV, false, false>, grid, block, 0, st, a);
 }
 
-template <typename T, int NV>
-cudaError_t launch_ring(const NormArgs &a, int sms, int per_sm, int stages, int stage_bytes, int *err, cudaStream_t st) {
-    const auto kernel = a.res ? norm_ring_kernel<T, NV, true> : norm_ring_kernel<T, NV, false>;
-    const int smem = stages * stage_bytes;
+// CTAs of an SM and stages of a ring: enough threads to keep up (16-bit rows with a residual
+// 512 an SM, without one twice as many, float32 half), and no more rows ahead than that takes:
+// 32768 x 2048 bf16 took 72 us with 8 rows ahead an SM, 83 with 12 and 94 with 16.
+template <typename T, int THREADS, int NV>
+cudaError_t launch_ring(const NormArgs &a, int sms, int row_bytes, int *err, cudaStream_t st) {
+    const auto kernel = a.res ? norm_ring_kernel<T, THREADS, NV, true> : norm_ring_kernel<T, THREADS, NV, false>;
+    const int stage = (row_bytes + 127) / 128 * 128 * (a.res ? 2 : 1);
+    const int per_sm = std::max(1, (a.res ? 512 : 1024) * 2 / (int)sizeof(T) / THREADS);
+    const int stages = per_sm > 1 ? 2 : std::max(2, std::min(MAX_STAGES, 128 * 1024 / stage)), smem = stages * stage;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    const int grid = min(a.rows, sms * per_sm);
-    return launch_pdl(kernel, dim3((unsigned)grid), dim3(RING_THREADS), smem, st, a, stages, stage_bytes,
-                      a.dim * (int)sizeof(T), err);
+    return launch_pdl(kernel, dim3((unsigned)std::min(a.rows, sms * per_sm)), dim3(THREADS), smem, st, a, stages, stage,
+                      row_bytes, err);
 }
 
 template <typename T>
 cudaError_t by_dim(const NormArgs &a, int sms, int *err, cudaStream_t st) {
     const int d = a.dim;
-    if (d <= 256) return launch<T, 32, 1, 4>(a, st);
-    if (d <= 512) return launch<T, 32, 2, 2>(a, st);
-    if (d <= 1024) return launch<T, 32, 4>(a, st);
-    // The ring wants whole 16-byte pieces, at least two stages, and some rows for each CTA.
-    const int bytes = (d * (int)sizeof(T) + 127) / 128 * 128 * (a.res ? 2 : 1);
-    if (a.vec && d * sizeof(T) % 16 == 0 && d <= 16384 && a.rows >= 4 * sms && 2 * bytes <= 220 * 1024) {
-        const int per_sm = 2 * bytes <= 110 * 1024 ? 2 : 1;
-        const int stages = min(MAX_STAGES, (per_sm == 2 ? 110 : 220) * 1024 / bytes);
-        if (d <= 2048) return launch_ring<T, 1>(a, sms, per_sm, stages, bytes, err, st);
-        if (d <= 4096) return launch_ring<T, 2>(a, sms, per_sm, stages, bytes, err, st);
-        if (d <= 8192) return launch_ring<T, 4>(a, sms, per_sm, stages, bytes, err, st);
-        return launch_ring<T, 8>(a, sms, per_sm, stages, bytes, err, st);
+    if (d <= 256) return launch<T, 32, 1>(a, sms, st);
+    if (d <= 512) return launch<T, 32, 2>(a, sms, st);
+    // The ring wants whole 16-byte pieces, room for two stages, and some rows for each CTA.
+    const int bytes = d * (int)sizeof(T);
+    if (a.full && bytes % 16 == 0 && d <= 16384 && a.rows >= 4 * sms && 2 * (a.res ? 2 : 1) * (bytes + 127) <= 222 * 1024) {
+        if (d <= 1024) return launch_ring<T, 128, 1>(a, sms, bytes, err, st);
+        if (d <= 2048) return launch_ring<T, 128, 2>(a, sms, bytes, err, st);
+        if (d <= 4096) return launch_ring<T, 256, 2>(a, sms, bytes, err, st);
+        if (d <= 8192) return launch_ring<T, 512, 2>(a, sms, bytes, err, st);
+        return launch_ring<T, 512, 4>(a, sms, bytes, err, st);
     }
-    if (d <= 2048) return launch<T, 128, 2>(a, st);
-    if (d <= 4096) return launch<T, 256, 2>(a, st);
-    if (d <= 8192) return launch<T, 512, 2>(a, st);
-    if (d <= 16384) return launch<T, 512, 4>(a, st);
-    return launch<T, 1024, 4>(a, st);
+    if (d <= 1024) return launch<T, 32, 4>(a, sms, st);
+    if (d <= 2048) return launch<T, 128, 2>(a, sms, st);
+    if (d <= 4096) return launch<T, 256, 2>(a, sms, st);
+    if (d <= 8192) return launch<T, 512, 2>(a, sms, st);
+    if (d <= 16384) return launch<T, 512, 4>(a, sms, st);
+    return launch<T, 1024, 4>(a, sms, st);
 }
 
 }  // namespace
@@ -293,14 +373,14 @@ extern "C" int hv_add_rmsnorm_fp8(const void *d_x, int64_t x_stride, const void 
         return fail(HV_ERR_VALUE, "residual and residual_out are given together or not at all");
     if (!(eps >= 0.f)) return fail(HV_ERR_VALUE, "eps must not be negative");
     NormArgs a{d_x, d_residual, d_weight, d_residual_out, (uint8_t *)d_q, d_scale, x_stride, residual_stride,
-               residual_out_stride, q_stride, scale_row_stride, scale_group_stride, (int)rows, dim, 1, 0, eps};
+               residual_out_stride, q_stride, scale_row_stride, scale_group_stride, (int)rows, dim, 0, eps};
     const int es = dec::elem_size(dtype);
     auto wide = [&](const void *p, int64_t stride) {
         return dec::aligned(p, 16) && (rows == 1 || stride * es % 16 == 0);
     };
-    a.vec = wide(d_x, x_stride) && dec::aligned(d_weight, 16) &&
-            (!d_residual || (wide(d_residual, residual_stride) && wide(d_residual_out, residual_out_stride)));
-    a.q8 = dec::aligned(d_q, 8) && (rows == 1 || q_stride % 8 == 0);
+    a.full = dim % 8 == 0 && wide(d_x, x_stride) && dec::aligned(d_weight, 16) &&
+             (!d_residual || (wide(d_residual, residual_stride) && wide(d_residual_out, residual_out_stride))) &&
+             dec::aligned(d_q, 8) && (rows == 1 || q_stride % 8 == 0);
     int *err = dec::error_word();
     const int sms = dec::sm_count();
     if (!err || !sms) return fail(HV_ERR_CUDA, "cannot read the device's properties");
