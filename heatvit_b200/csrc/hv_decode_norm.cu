@@ -53,16 +53,27 @@ constexpr float kSafeLow = 1e-30f, kSafeHigh = 1e30f;
 // A row is worked on in groups of eight channels, of which the group at channel c has
 // a.dim - c.  FULL: every group has eight or none, and starts on 16 bytes (8 in q).
 template <typename T, bool FULL>
-struct Group {
+struct alignas(16) Group {
     T e[8];  // as stored, so that a load can be under way while others are used
     __device__ __forceinline__ void load(const T *p, int n) {
         if (FULL) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i)
                 ((uint4 *)e)[i] = n > 0 ? ((const uint4 *)p)[i] : make_uint4(0, 0, 0, 0);
-        } else {
+        } else if (n < 8) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : from_f32<T>(0.f);
+        } else if ((uintptr_t)p % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4 *)e)[i] = ((const uint4 *)p)[i];
+        } else if ((uintptr_t)p % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) * 2; ++i) ((uint32_t *)e)[i] = ((const uint32_t *)p)[i];
+        } else {  // 16 bits and odd: whole words between the first element and the last
+            const uint32_t *m = (const uint32_t *)(p + 1);
+            uint32_t v[5] = {(uint32_t) * (const uint16_t *)p << 16, m[0], m[1], m[2], *(const uint16_t *)(p + 7)};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ((uint32_t *)e)[i] = __funnelshift_r(v[i], v[i + 1], 16);
         }
     }
     __device__ __forceinline__ void store(T *p, int n) const {
@@ -70,10 +81,23 @@ struct Group {
             if (n > 0)
 #pragma unroll
                 for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4 *)p)[i] = ((const uint4 *)e)[i];
-        } else {
+        } else if (n < 8) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (i < n) p[i] = e[i];
+        } else if ((uintptr_t)p % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4 *)p)[i] = ((const uint4 *)e)[i];
+        } else if ((uintptr_t)p % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) * 2; ++i) ((uint32_t *)p)[i] = ((const uint32_t *)e)[i];
+        } else {
+            const uint32_t *v = (const uint32_t *)e;
+            uint32_t *m = (uint32_t *)(p + 1);
+            p[0] = e[0];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) m[i] = __funnelshift_r(v[i], v[i + 1], 16);
+            p[7] = e[7];
         }
     }
 };
@@ -99,6 +123,8 @@ __device__ __forceinline__ void put_q(const NormArgs &a, long long row, int c, i
     uint8_t *q = a.q + row * a.q_stride + c;
     if (FULL) {
         if (n > 0) *(uint2 *)q = make_uint2(b[0], b[1]);
+    } else if (n >= 8 && (uintptr_t)q % 8 == 0) {
+        *(uint2 *)q = make_uint2(b[0], b[1]);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -224,7 +250,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_kernel(const __gri
 // leaves the memory idle between its phases: 16384 x 8192 bf16 took 194 us that way, 222 with
 // 256 threads).  Everyone has read a stage by the barrier of its row's reduction, after which
 // one thread refills it.
-constexpr int MAX_STAGES = 4;
+constexpr int MAX_STAGES = 8;
 constexpr uint32_t RING_WAIT = 1u << 22;
 
 template <typename T, int THREADS, int NV, bool RES>
@@ -318,14 +344,15 @@ cudaError_t launch(const NormArgs &a, int sms, cudaStream_t st) {
 }
 
 // CTAs of an SM and stages of a ring: enough threads to keep up (16-bit rows with a residual
-// 512 an SM, without one twice as many, float32 half), and no more rows ahead than that takes:
-// 32768 x 2048 bf16 took 72 us with 8 rows ahead an SM, 83 with 12 and 94 with 16.
+// 512 an SM, without one twice as many, float32 half), and 64 KB ahead an SM (128 where one CTA
+// has it): 32768 x 2048 bf16 took 72 us with 64 KB, 83 with 96 and 94 with 128.
 template <typename T, int THREADS, int NV>
 cudaError_t launch_ring(const NormArgs &a, int sms, int row_bytes, int *err, cudaStream_t st) {
     const auto kernel = a.res ? norm_ring_kernel<T, THREADS, NV, true> : norm_ring_kernel<T, THREADS, NV, false>;
     const int stage = (row_bytes + 127) / 128 * 128 * (a.res ? 2 : 1);
     const int per_sm = std::max(1, (a.res ? 512 : 1024) * 2 / (int)sizeof(T) / THREADS);
-    const int stages = per_sm > 1 ? 2 : std::max(2, std::min(MAX_STAGES, 128 * 1024 / stage)), smem = stages * stage;
+    const int ahead = (per_sm > 1 ? 64 : 128) * 1024 / (per_sm * stage);
+    const int stages = std::max(2, std::min(MAX_STAGES, ahead)), smem = stages * stage;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3((unsigned)std::min(a.rows, sms * per_sm)), dim3(THREADS), smem, st, a, stages, stage,
@@ -337,16 +364,15 @@ cudaError_t by_dim(const NormArgs &a, int sms, int *err, cudaStream_t st) {
     const int d = a.dim;
     if (d <= 256) return launch<T, 32, 1>(a, sms, st);
     if (d <= 512) return launch<T, 32, 2>(a, sms, st);
+    if (d <= 1024) return launch<T, 32, 4>(a, sms, st);
     // The ring wants whole 16-byte pieces, room for two stages, and some rows for each CTA.
     const int bytes = d * (int)sizeof(T);
     if (a.full && bytes % 16 == 0 && d <= 16384 && a.rows >= 4 * sms && 2 * (a.res ? 2 : 1) * (bytes + 127) <= 222 * 1024) {
-        if (d <= 1024) return launch_ring<T, 128, 1>(a, sms, bytes, err, st);
         if (d <= 2048) return launch_ring<T, 128, 2>(a, sms, bytes, err, st);
         if (d <= 4096) return launch_ring<T, 256, 2>(a, sms, bytes, err, st);
         if (d <= 8192) return launch_ring<T, 512, 2>(a, sms, bytes, err, st);
         return launch_ring<T, 512, 4>(a, sms, bytes, err, st);
     }
-    if (d <= 1024) return launch<T, 32, 4>(a, sms, st);
     if (d <= 2048) return launch<T, 128, 2>(a, sms, st);
     if (d <= 4096) return launch<T, 256, 2>(a, sms, st);
     if (d <= 8192) return launch<T, 512, 2>(a, sms, st);

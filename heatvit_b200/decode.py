@@ -117,8 +117,9 @@ def add_rmsnorm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None):
     for each 128 channels of a row ``scale = max(amax |y|, 2^-100) / 448`` and
     ``q = e4m3(y / scale)``.  x and residual [rows, dim] and weight [dim] share one of
     bfloat16, float16, float32; ``residual_out`` (a new tensor unless given, and it may
-    be ``residual``) receives h rounded to that type.  q's row stride is a multiple of 16,
-    scale is stored group by group: both as ``gemm_fp8`` reads them best."""
+    be ``residual``) receives h rounded to that type.  q's row stride is a multiple of 16 and
+    scale is stored group by group, both as ``gemm_fp8`` reads them best; a new residual's
+    row stride is a multiple of 8, since rows that start on 16 bytes go faster."""
     torch = _ready()
     dev = _index(x, "x")
     x_stride = _strides(x, "x", 2, dev)[0]
@@ -137,8 +138,10 @@ def add_rmsnorm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None):
     if residual is not None:
         r_stride = _like(residual, "residual", x, "x", dev)[0]
         if residual_out is None:
-            residual_out = torch.empty((rows, dim), dtype=dtype, device=x.device)
-            ro_stride = dim
+            ro_stride = -(-dim // 8) * 8
+            residual_out = torch.empty((rows, ro_stride), dtype=dtype, device=x.device)
+            if ro_stride != dim:
+                residual_out = residual_out[:, :dim]
         else:
             ro_stride = _like(residual_out, "residual_out", x, "x", dev)[0]
         r_ptr, ro_ptr = residual.data_ptr(), residual_out.data_ptr()
