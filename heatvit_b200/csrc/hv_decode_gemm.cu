@@ -305,6 +305,226 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
 }
 
+// ---- many tiles: persistent CTAs -------------------------------------------------
+// 128 x 256 tiles, one CTA an SM that takes a tile after another.  The rings of operand stages
+// and TMEM accumulators run on from tile to tile, so that the tensor core works through the
+// output of the tile before.  An adding thread has 128 columns of a row: its sums take 128
+// registers, so the copying and issuing warps give theirs up.  It keeps a 16-column TMEM load
+// under way while it adds the one before, with packed pairs of multiply-adds.
+constexpr int WIDE_BN = 256, WIDE_STAGES = 4, WIDE_BUFS = 2, WIDE_THREADS = 384, BAND = 16;
+constexpr int WIDE_STAGE = (BM + WIDE_BN) * GK;
+// Scales of SB groups at a time, a row's times its columns', for either half of the columns: two
+// warps fetch and multiply them (loads in the adding warps made those wait: 711 us, 8192^3).
+constexpr int SB = 8, SC_BYTES = 2 * SB * 2 * BM * 4;
+constexpr int WIDE_BYTES = WIDE_STAGES * WIDE_STAGE + SC_BYTES + 256 + 1024;
+
+__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t lo, uint32_t hi, uint64_t f) {
+    asm("{\n.reg .b64 t;\nmov.b64 t, {%1, %2};\nfma.rn.f32x2 %0, t, %3, %0;\n}\n" : "+l"(acc) : "r"(lo), "r"(hi), "l"(f));
+}
+
+// Tile `i` in bands of BAND tile rows, columns of a band one after another: the CTAs at work at
+// one time share few rows and columns of the operands, which L2 then has.
+__device__ __forceinline__ void tile_at(int i, int tiles_x, int tiles_y, int &tx, int &ty) {
+    const int band = i / (BAND * tiles_y), in = i - band * BAND * tiles_y;
+    const int h = min(BAND, tiles_x - band * BAND);
+    ty = in / h;
+    tx = band * BAND + in - ty * h;
+}
+
+__global__ void __launch_bounds__(WIDE_THREADS, 1)
+    gemm_wide_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmy,
+                     const __grid_constant__ GemmFp8Args a) {
+    extern __shared__ uint8_t raw[];
+    __shared__ uint32_t tslot;
+    __shared__ volatile int stop;
+    uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    float(*sc)[SB][2][BM] = (float(*)[SB][2][BM])(smem + WIDE_STAGES * WIDE_STAGE);
+    uint64_t *full = (uint64_t *)(smem + WIDE_STAGES * WIDE_STAGE + SC_BYTES), *empty = full + WIDE_STAGES;
+    uint64_t *tfull = empty + WIDE_STAGES, *tempty = tfull + WIDE_BUFS, *drain = tempty + WIDE_BUFS;
+    uint64_t *sfull = drain + 1, *sempty = sfull + 2;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tiles_y = (a.y_rows + WIDE_BN - 1) / WIDE_BN, tiles = a.tiles_x * tiles_y;
+
+    if (warp == 2) {
+        tc05::tmem_alloc(&tslot, 512);
+        tc05::tmem_relinquish();
+    }
+    if (tid == 0) {
+        stop = 0;
+        for (int i = 0; i < WIDE_STAGES; ++i) {
+            tc05::mbar_init(&full[i], 1);
+            tc05::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < WIDE_BUFS; ++i) {
+            tc05::mbar_init(&tfull[i], 1);
+            tc05::mbar_init(&tempty[i], EPI_WARPS);
+        }
+        tc05::mbar_init(drain, 1);
+        for (int i = 0; i < 2; ++i) {
+            tc05::mbar_init(&sfull[i], 64);
+            tc05::mbar_init(&sempty[i], EPI_WARPS);
+        }
+        tc05::fence_mbar_init();
+    }
+    tc05::fence_before();
+    __syncthreads();
+    tc05::fence_after();
+    griddep_wait();
+    griddep_launch();
+    const uint32_t tmem = tslot;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+        if (warp == 0 && lane == 0) {  // copies
+            uint32_t n = 0;  // stages filled
+            bool ok = true;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                int tx, ty;
+                tile_at(t, a.tiles_x, tiles_y, tx, ty);
+                for (int g = 0; g < a.groups; ++g, ++n) {
+                    const uint32_t s = n % WIDE_STAGES;
+                    if (n >= WIDE_STAGES && !wait_or_stop(&empty[s], (n / WIDE_STAGES - 1) & 1, &stop)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = tc05::smem_u32(smem + s * WIDE_STAGE);
+                    expect_tx(&full[s], WIDE_STAGE);
+                    tma_box(dst, &tmx, g * GK, tx * BM, &full[s]);
+                    tma_box(dst + BM * GK, &tmy, g * GK, ty * WIDE_BN, &full[s]);
+                }
+            }
+            if (!ok)  // what was issued has to land before shared memory goes
+                for (uint32_t k = n > WIDE_STAGES ? n - WIDE_STAGES : 0; k < n; ++k)
+                    tc05::mbar_wait(&full[k % WIDE_STAGES], (k / WIDE_STAGES) & 1, WAIT_ITERS);
+        } else if (warp == 1 && lane == 0) {  // products
+            constexpr uint32_t idesc = idesc_e4m3(BM, WIDE_BN);
+            uint32_t n = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+                for (int g = 0; g < a.groups; ++g, ++n) {
+                    const uint32_t s = n % WIDE_STAGES, b = n % WIDE_BUFS;
+                    ok = (n < WIDE_BUFS || wait_or_stop(&tempty[b], (n / WIDE_BUFS - 1) & 1, &stop)) &&
+                         wait_or_stop(&full[s], (n / WIDE_STAGES) & 1, &stop);
+                    if (!ok) break;
+                    tc05::fence_after();
+                    const uint32_t at = tc05::smem_u32(smem + s * WIDE_STAGE);
+                    const uint64_t da = desc_sw128(at), db = desc_sw128(at + BM * GK);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_e4m3(tmem + b * WIDE_BN, da + 2 * k, db + 2 * k, idesc, k > 0);
+                    tc05::commit(&empty[s]);
+                    tc05::commit(&tfull[b]);
+                }
+            if (!ok) {
+                tc05::commit(drain);
+                tc05::mbar_wait(drain, 0, WAIT_ITERS);
+            }
+        } else if (warp >= 2) {  // scales
+            const int r = tid - 64;  // and r + 64
+            int t = blockIdx.x, g = 0;
+            const float *x0 = nullptr, *x1 = nullptr, *y0 = nullptr, *y1 = nullptr;
+            for (uint32_t q = 0; t < tiles; ++q) {
+                const int b = q & 1;
+                if (q >= 2 && !wait_or_stop(&sempty[b], (q / 2 - 1) & 1, &stop)) break;
+#pragma unroll
+                for (int e0 = 0; e0 < SB; e0 += 4) {
+                    float vx0[4], vx1[4], vy0[4], vy1[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (t >= tiles) break;
+                        if (g == 0) {
+                            int tx, ty;
+                            tile_at(t, a.tiles_x, tiles_y, tx, ty);
+                            x0 = a.xs + min(tx * BM + r, a.x_rows - 1) * a.xs_row;
+                            x1 = a.xs + min(tx * BM + r + 64, a.x_rows - 1) * a.xs_row;
+                            y0 = a.ys + min(ty * WIDE_BN, a.y_rows - 1) / GK * a.ys_row;
+                            y1 = a.ys + min(ty * WIDE_BN + GK, a.y_rows - 1) / GK * a.ys_row;
+                        }
+                        vx0[e] = x0[g * a.xs_group];
+                        vx1[e] = x1[g * a.xs_group];
+                        vy0[e] = y0[g * a.ys_group];
+                        vy1[e] = y1[g * a.ys_group];
+                        if (++g == a.groups) {
+                            g = 0;
+                            t += gridDim.x;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sc[b][e0 + e][0][r] = vx0[e] * vy0[e];
+                        sc[b][e0 + e][1][r] = vx0[e] * vy1[e];
+                        sc[b][e0 + e][0][r + 64] = vx1[e] * vy0[e];
+                        sc[b][e0 + e][1][r + 64] = vx1[e] * vy1[e];
+                    }
+                }
+                arrive(&sfull[b]);
+            }
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
+        const int row = (warp & 3) * 32 + lane, c0 = ((warp - 4) >> 2) * 128;
+        const uint32_t tbase = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
+        const int half = (warp - 4) >> 2;
+        uint64_t acc[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[j] = 0;
+        uint32_t n = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int g = 0; g < a.groups; ++g, ++n) {
+                const uint32_t b = n % WIDE_BUFS, sb = n / SB;
+                ok = n % SB || wait_or_stop(&sfull[sb & 1], (sb / 2) & 1, &stop);
+                const float f = sc[sb & 1][n % SB][half][row];
+                uint64_t s2;
+                asm("mov.b64 %0, {%1, %1};\n" : "=l"(s2) : "f"(f));
+                ok = ok && wait_or_stop(&tfull[b], (n / WIDE_BUFS) & 1, &stop);
+                ok = __all_sync(~0u, ok);  // and every lane has its scale
+                if (!ok) break;
+                __syncwarp();
+                if (n % SB == SB - 1 && lane == 0) arrive(&sempty[sb & 1]);
+                tc05::fence_after();
+                uint32_t d[2][16];
+                tc05::ld16(tbase + b * WIDE_BN, d[0]);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    tc05::wait_ld_regs(d[c & 1]);
+                    if (c < 7) {
+                        tc05::ld16(tbase + b * WIDE_BN + (c + 1) * 16, d[(c + 1) & 1]);
+                    } else {
+                        tc05::fence_before();
+                        if (lane == 0) arrive(&tempty[b]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], d[c & 1][2 * j], d[c & 1][2 * j + 1], s2);
+                }
+            }
+            if (!ok) break;
+            int tx, ty;
+            tile_at(t, a.tiles_x, tiles_y, tx, ty);
+            const int m = tx * BM + row, col = ty * WIDE_BN + c0;
+            const long long at = (long long)m * a.ldc + col;
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(v[2 * e]), "=f"(v[2 * e + 1]) : "l"(acc[j + e]));
+                    acc[j + e] = 0;
+                }
+                if (m < a.x_rows && col + 2 * j < a.y_rows)
+                    put8_any(a.out, a.out_dtype, at + 2 * j, a.vec, a.y_rows - col - 2 * j, v);
+            }
+        }
+    }
+    if (tid == 0 && stop) atomicOr(a.err, HV_DECODE_STALLED);
+    tc05::fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc05::fence_after();
+        tc05::tmem_dealloc(tmem, 512);
+    }
+}
+
 PFN_cuTensorMapEncodeTiled encoder() {
     static PFN_cuTensorMapEncodeTiled encode = [] {
         void *fn = nullptr;
@@ -374,6 +594,24 @@ int run(const Operand &x, const Operand &y, int k, GemmFp8Args a, int sms, cudaS
     return HV_OK;
 }
 
+int run_wide(const Operand &x, const Operand &y, int k, GemmFp8Args a, int sms, cudaStream_t st) {
+    CUtensorMap tmx, tmy;
+    if (!tensor_map(&tmx, x.p, x.rows, k, x.stride, BM) || !tensor_map(&tmy, y.p, y.rows, k, y.stride, WIDE_BN))
+        return fail(HV_ERR_CUDA, "gemm_fp8: cannot encode the operands' tensor maps");
+    a.xs = x.scale, a.xs_row = x.s_row, a.xs_group = x.s_group;
+    a.ys = y.scale, a.ys_row = y.s_row, a.ys_group = y.s_group;
+    a.x_rows = (int)x.rows, a.y_rows = (int)y.rows;
+    a.tiles_x = (int)((x.rows + BM - 1) / BM);
+    const int64_t tiles = (int64_t)a.tiles_x * ((y.rows + WIDE_BN - 1) / WIDE_BN);
+    if (tiles > INT32_MAX / 2) return fail(HV_ERR_VALUE, "gemm_fp8: too many tiles");
+    cudaError_t e = cudaFuncSetAttribute(gemm_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WIDE_BYTES);
+    if (e == cudaSuccess)
+        e = launch_pdl(gemm_wide_kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(WIDE_THREADS), WIDE_BYTES, st,
+                       tmx, tmy, a);
+    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "gemm_fp8: %s", cudaGetErrorString(e));
+    return HV_OK;
+}
+
 }  // namespace
 }  // namespace hv
 
@@ -409,6 +647,6 @@ extern "C" int hv_gemm_fp8(const void *d_a, int64_t a_stride, const float *d_a_s
     if (m <= 32) return run<32, true>(b, a, k, g, sms, st);
     if (m <= 64) return run<64, true>(b, a, k, g, sms, st);
     // a 256-wide tile reads each operand byte for more products; a 128-wide one fills more SMs
-    if (((m + 127) / 128) * ((n + 255) / 256) >= sms) return run<256, false>(a, b, k, g, sms, st);
+    if (((m + 127) / 128) * ((n + 255) / 256) >= sms) return run_wide(a, b, k, g, sms, st);
     return run<128, false>(a, b, k, g, sms, st);
 }
