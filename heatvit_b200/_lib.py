@@ -52,8 +52,8 @@ _SIGNATURES = {
     "hv_selector_h2": (I, [P, I, P, P, I, P, P]),
     "hv_align_add_i8": (I, [P, I, P, I, I, I64, P, P]),
     "hv_decode_error": (I, [C.POINTER(C.c_int)]),
-    "hv_add_rmsnorm_fp8": (I, [P, I64, P, I64, P, I64, I, I, C.c_float, P, I64, P, I64, P, I64, I64, P]),
-    "hv_gemm_fp8": (I, [P, I64, P, I64, I64, P, I64, P, I64, I64, I64, I64, I, P, I64, I, P]),
+    "hv_add_rmsnorm_fp8": (I, [P, P]),
+    "hv_gemm_fp8": (I, [P, P]),
     "hv_append_kv": (I, [P, P]),
     "hv_paged_attention_workspace": (I, [I, C.POINTER(I64)]),
     "hv_paged_attention": (I, [P, P]),

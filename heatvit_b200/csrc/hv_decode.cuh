@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "hv_internal.cuh"
 #include "hv_launch.cuh"
 
@@ -17,6 +19,17 @@ namespace dec {
 int *error_word();
 // SMs of the current device; 0 when that cannot be read.
 int sm_count();
+
+// Lets `kernel` have all of an SM's shared memory, once a device: `ready` has a bit for each.
+template <typename K>
+cudaError_t allow_shared(K kernel, std::atomic<uint64_t> &ready) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && ready.load(std::memory_order_relaxed) >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 2048);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
+}
 
 inline int elem_size(int dtype) { return dtype == HV_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == HV_BF16 || dtype == HV_F16 || dtype == HV_F32; }

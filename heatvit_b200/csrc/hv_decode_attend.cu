@@ -664,18 +664,15 @@ constexpr int COUNT_BYTES = 3 * MAX_GRID * 4;
 
 // CTAs of one resident wave on the current device.
 int wave(int d) {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
+    const int sms = sm_count();
     const int grid = sms * (d <= 128 ? Lay<128>::PER_SM : Lay<256>::PER_SM);
     return grid < MAX_GRID ? grid : MAX_GRID;
 }
 
 template <typename T, int D>
 cudaError_t launch(const AttendArgs &a, int grid, cudaStream_t st) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::BYTES);
+    static std::atomic<uint64_t> ready;
+    const cudaError_t e = allow_shared(attend_kernel<T, D>, ready);
     if (e != cudaSuccess) return e;
     return launch_pdl(attend_kernel<T, D>, dim3((unsigned)grid), dim3(Lay<D>::THREADS), Lay<D>::BYTES, st, a);
 }

@@ -573,7 +573,8 @@ int run(const Operand &x, const Operand &y, int k, GemmFp8Args a, int sms, cudaS
     if (tiles * split > INT32_MAX) return fail(HV_ERR_VALUE, "gemm_fp8: too many tiles");
     a.split = split;
     auto kernel = gemm_kernel<BN, SWAP>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+    static std::atomic<uint64_t> ready;
+    cudaError_t e = allow_shared(kernel, ready);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(tiles * split));
@@ -604,7 +605,8 @@ int run_wide(const Operand &x, const Operand &y, int k, GemmFp8Args a, int sms, 
     a.tiles_x = (int)((x.rows + BM - 1) / BM);
     const int64_t tiles = (int64_t)a.tiles_x * ((y.rows + WIDE_BN - 1) / WIDE_BN);
     if (tiles > INT32_MAX / 2) return fail(HV_ERR_VALUE, "gemm_fp8: too many tiles");
-    cudaError_t e = cudaFuncSetAttribute(gemm_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WIDE_BYTES);
+    static std::atomic<uint64_t> ready;
+    cudaError_t e = allow_shared(gemm_wide_kernel, ready);
     if (e == cudaSuccess)
         e = launch_pdl(gemm_wide_kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(WIDE_THREADS), WIDE_BYTES, st,
                        tmx, tmy, a);
@@ -617,36 +619,34 @@ int run_wide(const Operand &x, const Operand &y, int k, GemmFp8Args a, int sms, 
 
 using namespace hv;
 
-extern "C" int hv_gemm_fp8(const void *d_a, int64_t a_stride, const float *d_a_scale, int64_t a_scale_row_stride,
-                           int64_t a_scale_group_stride, const void *d_b, int64_t b_stride, const float *d_b_scale,
-                           int64_t b_scale_row_stride, int64_t b_scale_group_stride, int64_t m, int64_t n, int k,
-                           void *d_out, int64_t out_stride, int out_dtype, void *stream) {
-    if (!dec::known_dtype(out_dtype)) return fail(HV_ERR_TYPE, "out_dtype must be HV_BF16, HV_F16 or HV_F32");
-    if (m < 0 || n < 0 || m > INT32_MAX - 256 || n > INT32_MAX - 256) return fail(HV_ERR_VALUE, "m or n outside [0, 2^31)");
-    if (k < 1 || k > INT32_MAX - GK) return fail(HV_ERR_VALUE, "k must be positive");
+extern "C" int hv_gemm_fp8(const hv_gemm_fp8_args *p, void *stream) {
+    if (!p) return fail(HV_ERR_VALUE, "null argument");
+    if (!dec::known_dtype(p->out_dtype)) return fail(HV_ERR_TYPE, "out_dtype must be HV_BF16, HV_F16 or HV_F32");
+    const int64_t m = p->m, n = p->n, k = p->k, most = INT32_MAX - 512;
+    if (m < 0 || n < 0 || m > most || n > most) return fail(HV_ERR_VALUE, "m or n outside [0, 2^31 - 512]");
+    if (k < 1 || k > most) return fail(HV_ERR_VALUE, "k outside [1, 2^31 - 512]");
     if (m == 0 || n == 0) return HV_OK;
-    if (!d_a || !d_a_scale || !d_b || !d_b_scale || !d_out) return fail(HV_ERR_VALUE, "null buffer");
-    if (!dec::aligned(d_a, 16) || !dec::aligned(d_b, 16) || (m > 1 && a_stride % 16) || (n > 1 && b_stride % 16))
+    if (!p->d_a || !p->d_a_scale || !p->d_b || !p->d_b_scale || !p->d_out) return fail(HV_ERR_VALUE, "null buffer");
+    if (!dec::aligned(p->d_a, 16) || !dec::aligned(p->d_b, 16) || (m > 1 && p->a_stride % 16) ||
+        (n > 1 && p->b_stride % 16))
         return fail(HV_ERR_VALUE, "operand rows must start on 16 bytes");
     const int64_t room = (k + 15) / 16 * 16;  // a one-row operand's stride is not used
-    const int64_t sa = m > 1 ? a_stride : room, sb = n > 1 ? b_stride : room;
+    const int64_t sa = m > 1 ? p->a_stride : room, sb = n > 1 ? p->b_stride : room;
     if (sa < k || sb < k) return fail(HV_ERR_VALUE, "operand rows overlap");
     int *err = dec::error_word();
-    if (!err) return fail(HV_ERR_CUDA, "cannot resolve the device error word");
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "gemm_fp8: %s", cudaGetErrorString(e));
+    const int sms = dec::sm_count();
+    if (!err || !sms) return fail(HV_ERR_CUDA, "cannot read the device's properties");
     GemmFp8Args g{};
-    g.out = d_out, g.ldc = out_stride, g.out_dtype = out_dtype, g.groups = (k + GK - 1) / GK, g.err = err;
-    g.vec = dec::aligned(d_out, 16) && (m == 1 || out_stride * dec::elem_size(out_dtype) % 16 == 0);
-    const Operand a{d_a, m, sa, d_a_scale, a_scale_row_stride, a_scale_group_stride};
-    const Operand b{d_b, n, sb, d_b_scale, b_scale_row_stride, b_scale_group_stride};
+    g.out = p->d_out, g.ldc = p->out_stride, g.out_dtype = p->out_dtype, g.groups = (int)((k + GK - 1) / GK), g.err = err;
+    g.vec = dec::aligned(p->d_out, 16) && (m == 1 || p->out_stride * dec::elem_size(p->out_dtype) % 16 == 0);
+    const Operand a{p->d_a, m, sa, p->d_a_scale, p->a_scale_strides[0], p->a_scale_strides[1]};
+    const Operand b{p->d_b, n, sb, p->d_b_scale, p->b_scale_strides[0], p->b_scale_strides[1]};
     const cudaStream_t st = (cudaStream_t)stream;
-    if (m <= 16) return run<16, true>(b, a, k, g, sms, st);
-    if (m <= 32) return run<32, true>(b, a, k, g, sms, st);
-    if (m <= 64) return run<64, true>(b, a, k, g, sms, st);
+    const int kk = (int)k;
+    if (m <= 16) return run<16, true>(b, a, kk, g, sms, st);
+    if (m <= 32) return run<32, true>(b, a, kk, g, sms, st);
+    if (m <= 64) return run<64, true>(b, a, kk, g, sms, st);
     // a 256-wide tile reads each operand byte for more products; a 128-wide one fills more SMs
-    if (((m + 127) / 128) * ((n + 255) / 256) >= sms) return run_wide(a, b, k, g, sms, st);
-    return run<128, false>(a, b, k, g, sms, st);
+    if (((m + 127) / 128) * ((n + 255) / 256) >= sms) return run_wide(a, b, kk, g, sms, st);
+    return run<128, false>(a, b, kk, g, sms, st);
 }

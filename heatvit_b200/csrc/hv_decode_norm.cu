@@ -353,7 +353,8 @@ cudaError_t launch_ring(const NormArgs &a, int sms, int row_bytes, int *err, cud
     const int per_sm = std::max(1, (a.res ? 512 : 1024) * 2 / (int)sizeof(T) / THREADS);
     const int ahead = (per_sm > 1 ? 64 : 128) * 1024 / (per_sm * stage);
     const int stages = std::max(2, std::min(MAX_STAGES, ahead)), smem = stages * stage;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> ready[2];
+    const cudaError_t e = allow_shared(kernel, ready[a.res != nullptr]);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3((unsigned)std::min(a.rows, sms * per_sm)), dim3(THREADS), smem, st, a, stages, stage,
                       row_bytes, err);
@@ -385,35 +386,33 @@ cudaError_t by_dim(const NormArgs &a, int sms, int *err, cudaStream_t st) {
 
 using namespace hv;
 
-extern "C" int hv_add_rmsnorm_fp8(const void *d_x, int64_t x_stride, const void *d_residual, int64_t residual_stride,
-                                  const void *d_weight, int64_t rows, int dim, int dtype, float eps,
-                                  void *d_residual_out, int64_t residual_out_stride, void *d_q, int64_t q_stride,
-                                  float *d_scale, int64_t scale_row_stride, int64_t scale_group_stride,
-                                  void *stream) {
-    if (!dec::known_dtype(dtype)) return fail(HV_ERR_TYPE, "dtype must be HV_BF16, HV_F16 or HV_F32");
-    if (rows < 0 || rows > INT32_MAX) return fail(HV_ERR_VALUE, "rows outside [0, 2^31)");
-    if (dim < 1 || dim > 32768) return fail(HV_ERR_VALUE, "dim outside [1, 32768]");
-    if (rows == 0) return HV_OK;
-    if (!d_x || !d_weight || !d_q || !d_scale) return fail(HV_ERR_VALUE, "null buffer");
-    if (!d_residual != !d_residual_out)
+extern "C" int hv_add_rmsnorm_fp8(const hv_norm_args *p, void *stream) {
+    if (!p) return fail(HV_ERR_VALUE, "null argument");
+    if (!dec::known_dtype(p->dtype)) return fail(HV_ERR_TYPE, "dtype must be HV_BF16, HV_F16 or HV_F32");
+    if (p->rows < 0 || p->rows > INT32_MAX) return fail(HV_ERR_VALUE, "rows outside [0, 2^31)");
+    if (p->dim < 1 || p->dim > 32768) return fail(HV_ERR_VALUE, "dim outside [1, 32768]");
+    if (!(p->eps >= 0.f)) return fail(HV_ERR_VALUE, "eps must not be negative");
+    if (!p->d_residual != !p->d_residual_out)
         return fail(HV_ERR_VALUE, "residual and residual_out are given together or not at all");
-    if (!(eps >= 0.f)) return fail(HV_ERR_VALUE, "eps must not be negative");
-    NormArgs a{d_x, d_residual, d_weight, d_residual_out, (uint8_t *)d_q, d_scale, x_stride, residual_stride,
-               residual_out_stride, q_stride, scale_row_stride, scale_group_stride, (int)rows, dim, 0, eps};
-    const int es = dec::elem_size(dtype);
-    auto wide = [&](const void *p, int64_t stride) {
-        return dec::aligned(p, 16) && (rows == 1 || stride * es % 16 == 0);
+    if (p->rows == 0) return HV_OK;
+    if (!p->d_x || !p->d_weight || !p->d_q || !p->d_scale) return fail(HV_ERR_VALUE, "null buffer");
+    NormArgs a{p->d_x, p->d_residual, p->d_weight, p->d_residual_out, (uint8_t *)p->d_q, p->d_scale, p->x_stride,
+               p->residual_stride, p->residual_out_stride, p->q_stride, p->scale_strides[0], p->scale_strides[1],
+               (int)p->rows, p->dim, 0, p->eps};
+    const int es = dec::elem_size(p->dtype);
+    auto wide = [&](const void *b, int64_t stride) {
+        return dec::aligned(b, 16) && (p->rows == 1 || stride * es % 16 == 0);
     };
-    a.full = dim % 8 == 0 && wide(d_x, x_stride) && dec::aligned(d_weight, 16) &&
-             (!d_residual || (wide(d_residual, residual_stride) && wide(d_residual_out, residual_out_stride))) &&
-             dec::aligned(d_q, 8) && (rows == 1 || q_stride % 8 == 0);
+    a.full = p->dim % 8 == 0 && wide(a.x, a.x_stride) && dec::aligned(a.w, 16) &&
+             (!a.res || (wide(a.res, a.res_stride) && wide(a.res_out, a.res_out_stride))) && dec::aligned(a.q, 8) &&
+             (p->rows == 1 || a.q_stride % 8 == 0);
     int *err = dec::error_word();
     const int sms = dec::sm_count();
     if (!err || !sms) return fail(HV_ERR_CUDA, "cannot read the device's properties");
     const cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e = dtype == HV_BF16  ? by_dim<__nv_bfloat16>(a, sms, err, st)
-                          : dtype == HV_F16 ? by_dim<__half>(a, sms, err, st)
-                                            : by_dim<float>(a, sms, err, st);
+    const cudaError_t e = p->dtype == HV_BF16  ? by_dim<__nv_bfloat16>(a, sms, err, st)
+                          : p->dtype == HV_F16 ? by_dim<__half>(a, sms, err, st)
+                                               : by_dim<float>(a, sms, err, st);
     if (e != cudaSuccess) return fail(HV_ERR_CUDA, "add_rmsnorm_fp8: %s", cudaGetErrorString(e));
     return HV_OK;
 }

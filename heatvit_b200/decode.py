@@ -32,7 +32,9 @@ HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 Fp8Rows = namedtuple("Fp8Rows", "q scale residual")
 Fp8Rows.__doc__ = "q [rows, dim] e4m3, scale [rows, ceil(dim / 128)] float32, residual [rows, dim] or None."
 
-# hv_append_args and hv_attention_args of include/heatvit_b200.h
+# hv_norm_args, hv_gemm_fp8_args, hv_append_args and hv_attention_args of include/heatvit_b200.h
+_NORM = struct.Struct("@6P7q2if")
+_GEMM = struct.Struct("@5P10qi")
 _APPEND = struct.Struct("@10P16q12i")
 _ATTEND = struct.Struct("@8P14q8if")
 
@@ -89,13 +91,13 @@ def _like(t, name, other, its_name, index):
     return s
 
 
-def _call(fn, index, *args):
-    """fn(*args, stream) with the device current; raises on a status."""
+def _call(fn, index, args):
+    """fn(args, stream) with the device current; raises on a status."""
     if _current_device() == index:
-        status = fn(*args, _raw_stream(index))
+        status = fn(args, _raw_stream(index))
     else:
         with _torch_module.cuda.device(index):
-            status = fn(*args, _raw_stream(index))
+            status = fn(args, _raw_stream(index))
     if status:
         check(status)
 
@@ -133,13 +135,13 @@ def add_rmsnorm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None):
         raise ValueError(f"weight has {weight.shape[0]} channels, x {dim}")
     if weight.dtype is not dtype:
         raise TypeError("weight must have x's type")
-    r_ptr = ro_ptr = None
-    r_stride = ro_stride = 0
+    device = x.device
+    r_ptr = ro_ptr = r_stride = ro_stride = 0
     if residual is not None:
         r_stride = _like(residual, "residual", x, "x", dev)[0]
         if residual_out is None:
             ro_stride = -(-dim // 8) * 8
-            residual_out = torch.empty((rows, ro_stride), dtype=dtype, device=x.device)
+            residual_out = torch.empty(rows, ro_stride, dtype=dtype, device=device)
             if ro_stride != dim:
                 residual_out = residual_out[:, :dim]
         else:
@@ -148,10 +150,11 @@ def add_rmsnorm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None):
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
     wide = -(-dim // 16) * 16
-    q = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty_strided((rows, -(-dim // GROUP)), (1, rows), dtype=torch.float32, device=x.device)
-    _call(_c.hv_add_rmsnorm_fp8, dev, x.data_ptr(), x_stride, r_ptr, r_stride, weight.data_ptr(), rows, dim,
-          code, eps, ro_ptr, ro_stride, q.data_ptr(), wide, scale.data_ptr(), 1, rows)
+    q = torch.empty(rows, wide, dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty_strided((rows, -(-dim // GROUP)), (1, rows), dtype=torch.float32, device=device)
+    _call(_c.hv_add_rmsnorm_fp8, dev, _NORM.pack(x.data_ptr(), r_ptr, weight.data_ptr(), ro_ptr, q.data_ptr(),
+                                                 scale.data_ptr(), rows, x_stride, r_stride, ro_stride, wide, 1, rows,
+                                                 dim, code, eps))
     return Fp8Rows(q if wide == dim else q[:, :dim], scale, residual_out)
 
 
@@ -202,7 +205,7 @@ def gemm_fp8(a, a_scale, b, b_scale, out_dtype=None, out=None):
         if t.shape != (rows, groups):
             raise ValueError(f"{name} must be [{rows}, {groups}]")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=a.device)
+        out = torch.empty(m, n, dtype=out_dtype or torch.bfloat16, device=a.device)
         out_stride = n
     else:
         out_stride = _strides(out, "out", 2, dev)[0]
@@ -213,8 +216,9 @@ def gemm_fp8(a, a_scale, b, b_scale, out_dtype=None, out=None):
     code = _types.get(out.dtype)
     if code is None:
         raise TypeError("out must be bfloat16, float16 or float32")
-    _call(_c.hv_gemm_fp8, dev, a.data_ptr(), a_stride, a_scale.data_ptr(), *a_scale.stride(), b.data_ptr(),
-          b_stride, b_scale.data_ptr(), *b_scale.stride(), m, n, k, out.data_ptr(), out_stride, code)
+    _call(_c.hv_gemm_fp8, dev, _GEMM.pack(a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
+                                          out.data_ptr(), m, n, k, a_stride, b_stride, out_stride, *a_scale.stride(),
+                                          *b_scale.stride(), code))
     return out
 
 
@@ -282,7 +286,7 @@ def append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, rope=
             raise TypeError("q must have k's type")
         heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty((tokens, heads, dim), dtype=dtype, device=q.device)
+            q_out = torch.empty(tokens, heads, dim, dtype=dtype, device=q.device)
             qo_str = (heads * dim, dim)
         else:
             qo_str = _like(q_out, "q_out", q, "q", dev)
@@ -372,7 +376,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lens, scale=None, workspace
     if rows != seqs or lens.shape[0] != seqs:
         raise ValueError("page_table and lens have one row per sequence")
     if out is None:
-        out = torch.empty((seqs, heads, dim), dtype=dtype, device=q.device)
+        out = torch.empty(seqs, heads, dim, dtype=dtype, device=q.device)
         out_str = (heads * dim, dim)
     else:
         out_str = _like(out, "out", q, "q", dev)
@@ -380,7 +384,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lens, scale=None, workspace
         workspace = _workspace(torch, dev)
     elif workspace.device.index != dev:
         raise ValueError(f"the workspace must live on cuda:{dev}")
-    lse = torch.empty((seqs, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty(seqs, heads, dtype=torch.float32, device=q.device) if return_lse else None
     args = _ATTEND.pack(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, k_cache.data_ptr(),
                         v_cache.data_ptr(), page_table.data_ptr(), lens.data_ptr(), workspace.ptr, workspace.bytes,
                         *q_str[:2], *out_str[:2], heads, 1, *cache, table_stride, seqs, heads, kv_heads, dim, code,

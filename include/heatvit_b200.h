@@ -412,25 +412,35 @@ HV_API int hv_decode_error(int *bits);
 /* h = x + residual; residual_out = h; y = h * rsqrt(mean(h^2) + eps) * weight, and y in e4m3
  * with a scale for each 128 channels of a row: scale = max(amax |y|, 2^-100) / 448,
  * q = e4m3(y / scale).  Sums in 32 bits; the norm is of the unrounded h.
- *   d_x, d_residual, d_residual_out [rows][dim], d_weight [dim], all of `dtype`; d_residual
- *   and d_residual_out both NULL for a plain norm, and may be the same buffer.
- *   d_q [rows][dim] e4m3; the scale of row r, group g at r * row stride + g * group stride.
+ * d_residual and d_residual_out both NULL for a plain norm; they may be the same buffer.
  * dim in [1, 32768]. */
-HV_API int hv_add_rmsnorm_fp8(const void *d_x, int64_t x_stride, const void *d_residual, int64_t residual_stride,
-                              const void *d_weight, int64_t rows, int dim, int dtype, float eps,
-                              void *d_residual_out, int64_t residual_out_stride, void *d_q, int64_t q_stride,
-                              float *d_scale, int64_t scale_row_stride, int64_t scale_group_stride, void *stream);
+typedef struct hv_norm_args {
+    const void *d_x, *d_residual; /* [rows][dim] of `dtype` */
+    const void *d_weight;         /* [dim] of `dtype` */
+    void *d_residual_out;         /* [rows][dim] of `dtype` */
+    void *d_q;                    /* [rows][dim] e4m3 */
+    float *d_scale;               /* [rows][ceil(dim / 128)] */
+    int64_t rows, x_stride, residual_stride, residual_out_stride, q_stride;
+    int64_t scale_strides[2];     /* row, group */
+    int32_t dim, dtype;
+    float eps;
+} hv_norm_args;
+HV_API int hv_add_rmsnorm_fp8(const hv_norm_args *args, void *stream);
 
 /* e4m3 product with block scales: out[m][n] = sum over groups g of 128 along K of
  * a_scale[m][g] * b_scale[n / 128][g] * sum_k a[m][k] b[n][k], sums in 32 bits, rounded once.
- *   d_a [m][k], d_b [n][k] e4m3 (B as the weights' rows of output channels); rows start on 16
- *   bytes (strides in bytes, a multiple of 16), k need not be a multiple of anything.
- *   A scale of row r (of A) or block r (of 128 rows of B), group g at r * row stride +
- *   g * group stride.  out_dtype HV_BF16, HV_F16 or HV_F32. */
-HV_API int hv_gemm_fp8(const void *d_a, int64_t a_stride, const float *d_a_scale, int64_t a_scale_row_stride,
-                       int64_t a_scale_group_stride, const void *d_b, int64_t b_stride, const float *d_b_scale,
-                       int64_t b_scale_row_stride, int64_t b_scale_group_stride, int64_t m, int64_t n, int k,
-                       void *d_out, int64_t out_stride, int out_dtype, void *stream);
+ * B as the weights' rows of output channels.  Operand rows start on 16 bytes (strides a
+ * multiple of 16); m, n and k need not be multiples of anything. */
+typedef struct hv_gemm_fp8_args {
+    const void *d_a, *d_b;           /* [m][k], [n][k] e4m3 */
+    const float *d_a_scale;          /* [m][ceil(k / 128)] */
+    const float *d_b_scale;          /* [ceil(n / 128)][ceil(k / 128)] */
+    void *d_out;                     /* [m][n] of `out_dtype` */
+    int64_t m, n, k, a_stride, b_stride, out_stride;
+    int64_t a_scale_strides[2], b_scale_strides[2]; /* row or block of rows, group */
+    int32_t out_dtype;               /* HV_BF16, HV_F16 or HV_F32 */
+} hv_gemm_fp8_args;
+HV_API int hv_gemm_fp8(const hv_gemm_fp8_args *args, void *stream);
 
 /* Keys and values of new tokens into a paged cache, q and k rotated by position.
  * Token t of sequence d_seq_ids[t] (t itself when NULL) at d_positions[t] is stored in page

@@ -23,22 +23,22 @@ def library():
 
 def test_packed_structs_match_the_header(tmp_path):
     from heatvit_b200 import decode
+    fields = {"hv_norm_args": ("rows", "scale_strides", "dim", "eps"),
+              "hv_gemm_fp8_args": ("m", "a_scale_strides", "out_dtype"),
+              "hv_append_args": ("d_positions", "q_strides", "rope_stride", "tokens", "rope_rows"),
+              "hv_attention_args": ("workspace_bytes", "page_table_stride", "seqs", "scale")}
+    terms = [f"sizeof({t})" for t in fields] + [f"offsetof({t}, {f})" for t, fs in fields.items() for f in fs]
     prog = tmp_path / "sz.c"
-    prog.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "heatvit_b200.h"\nint main(){printf("'
-                    + '%zu ' * 10 + '\\n", sizeof(hv_append_args), offsetof(hv_append_args, d_positions), '
-                    'offsetof(hv_append_args, q_strides), offsetof(hv_append_args, rope_stride), '
-                    'offsetof(hv_append_args, tokens), sizeof(hv_attention_args), '
-                    'offsetof(hv_attention_args, workspace_bytes), offsetof(hv_attention_args, page_table_stride), '
-                    'offsetof(hv_attention_args, seqs), offsetof(hv_attention_args, scale));return 0;}\n')
+    prog.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "heatvit_b200.h"\nint main(){'
+                    + "".join(f'printf("%zu ", {t});' for t in terms) + 'return 0;}\n')
     exe = tmp_path / "sz"
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(prog), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True).stdout.split()]
-
-    def round8(n):
-        return -(-n // 8) * 8
-    assert got == [round8(decode._APPEND.size), 72, 80, struct.calcsize("@10P14q"), struct.calcsize("@10P16q"),
-                   round8(decode._ATTEND.size), struct.calcsize("@8P"), struct.calcsize("@8P13q"),
-                   struct.calcsize("@8P14q"), struct.calcsize("@8P14q8i")]
+    sizes = [-(-s.size // 8) * 8 for s in (decode._NORM, decode._GEMM, decode._APPEND, decode._ATTEND)]
+    offsets = [struct.calcsize(f) for f in (
+        "@6P", "@6P5q", "@6P7q", "@6P7q2i", "@5P", "@5P6q", "@5P10q", "@9P", "@10P", "@10P14q", "@10P16q", "@10P16q11i",
+        "@8P", "@8P13q", "@8P14q", "@8P14q8i")]
+    assert got == sizes + offsets
 
 
 def test_every_symbol_has_a_signature(library):
@@ -50,27 +50,26 @@ def test_every_symbol_has_a_signature(library):
 def test_c_entries_refuse_before_they_touch_a_device(library):
     """Status codes of mistakes that are visible on the host."""
     from heatvit_b200 import abi
-    none = [None] * 1
+    from heatvit_b200 import decode
 
-    def norm(rows=1, dim=64, dtype=0, eps=1e-6, x=16, res=None, out=None):
-        return library.hv_add_rmsnorm_fp8(x, dim, res, dim, 16, rows, dim, dtype, eps, out, dim, 16, dim, 16, 1, rows,
-                                          none[0])
+    def norm(rows=1, dim=64, dtype=0, eps=1e-6, x=16, res=0, out=0):
+        return library.hv_add_rmsnorm_fp8(decode._NORM.pack(x, res, 16, out, 16, 16, rows, *[64] * 6, dim, dtype, eps),
+                                          None)
     assert norm(dtype=7) == abi.HV_ERR_TYPE
     assert norm(dim=0) == abi.HV_ERR_VALUE and norm(dim=32769) == abi.HV_ERR_VALUE
-    assert norm(rows=-1) == abi.HV_ERR_VALUE and norm(x=None) == abi.HV_ERR_VALUE
+    assert norm(rows=-1) == abi.HV_ERR_VALUE and norm(x=0) == abi.HV_ERR_VALUE
     assert norm(eps=-1.0) == abi.HV_ERR_VALUE and norm(eps=float("nan")) == abi.HV_ERR_VALUE
     assert norm(res=16) == abi.HV_ERR_VALUE and b"together" in library.hv_last_error()
     assert norm(rows=0) == abi.HV_OK
 
     def gemm(m=1, n=1, k=16, a=16, lda=16, dtype=0):
-        return library.hv_gemm_fp8(a, lda, 16, 1, 1, 16, 16, 16, 1, 1, m, n, k, 16, n, dtype, None)
+        return library.hv_gemm_fp8(decode._GEMM.pack(a, 16, 16, 16, 16, m, n, k, lda, 16, n, 1, 1, 1, 1, dtype), None)
     assert gemm(dtype=3) == abi.HV_ERR_TYPE
-    assert gemm(k=0) == abi.HV_ERR_VALUE and gemm(m=-1) == abi.HV_ERR_VALUE and gemm(a=None) == abi.HV_ERR_VALUE
+    assert gemm(k=0) == abi.HV_ERR_VALUE and gemm(m=-1) == abi.HV_ERR_VALUE and gemm(a=0) == abi.HV_ERR_VALUE
+    assert gemm(m=1 << 31) == abi.HV_ERR_VALUE and gemm(k=1 << 31) == abi.HV_ERR_VALUE
     assert gemm(a=24) == abi.HV_ERR_VALUE and b"16 bytes" in library.hv_last_error()
     assert gemm(m=2, lda=24) == abi.HV_ERR_VALUE and gemm(m=2, k=32, lda=16) == abi.HV_ERR_VALUE
     assert gemm(m=0) == abi.HV_OK and gemm(n=0) == abi.HV_OK
-
-    from heatvit_b200 import decode
 
     def append(tokens=1, heads=0, kv=1, dim=8, rot=0, dtype=0, pages=1, page=1, k=16):
         return library.hv_append_kv(decode._APPEND.pack(0, k, 16, 0, 16, 16, 0, 16, 0, 16, *[8] * 16, tokens, heads, kv,
@@ -90,6 +89,8 @@ def test_c_entries_refuse_before_they_touch_a_device(library):
         assert attend(**bad) == abi.HV_ERR_VALUE, bad
     assert library.hv_paged_attention(None, None) == abi.HV_ERR_VALUE
     assert library.hv_append_kv(None, None) == abi.HV_ERR_VALUE
+    assert library.hv_add_rmsnorm_fp8(None, None) == abi.HV_ERR_VALUE
+    assert library.hv_gemm_fp8(None, None) == abi.HV_ERR_VALUE
     assert library.hv_decode_error(None) == abi.HV_ERR_VALUE
     assert library.hv_paged_attention_workspace(80, C.byref(C.c_int64())) == abi.HV_ERR_VALUE
     assert library.hv_paged_attention_workspace(64, None) == abi.HV_ERR_VALUE
