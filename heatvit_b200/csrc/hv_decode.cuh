@@ -26,7 +26,7 @@ cudaError_t allow_shared(K kernel, std::atomic<uint64_t> &ready) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || (dev < 64 && ready.load(std::memory_order_relaxed) >> dev & 1)) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 2048);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512);
     if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
     return e;
 }

@@ -3,22 +3,26 @@
 //   C[m][n] = sum_g as[m][g] * bs[n / 128][g] * sum_{k in group g} A[m][k] B[n][k],
 //   g the groups of 128 along K; sums in 32 bits, one rounding to C's type.
 //
-// A CTA computes 128 rows x BN columns of the product of two K-major operands, X (rows) and
-// Y (columns).  Roles: one thread issues the TMA copies (128-byte swizzled boxes of one
-// group) into a ring of stages; one thread issues tcgen05.mma kind::f8f6f4, four of K = 32
-// for a group, into one of several TMEM accumulators; eight warps read each finished
-// accumulator and add it, times its scale, to sums in their registers, since the tensor core
-// itself cannot scale by 32-bit numbers.  Reading and adding a 128 x BN block takes half the
-// time of its MMAs, and runs beside those of the next group.
+// A CTA computes tiles of 128 rows x BN columns of the product of two K-major operands, X
+// (rows) and Y (columns).  Its warps: one thread issues the TMA copies (128-byte swizzled boxes of
+// one group) into a ring of stages; one issues tcgen05.mma kind::f8f6f4, four of K = 32 for a
+// group, into one of several TMEM accumulators; two warps fetch scales; eight read each
+// finished accumulator and add it, times its scales, to sums in their registers, since the
+// tensor core itself cannot scale by 32-bit numbers.  They keep a TMEM load under way while
+// they add the one before, with packed pairs of multiply-adds.
 //
-// Two ways round.  Many tokens: X = A, Y = B.  Few tokens (SWAP): X = B, Y = A, so that the
-// 128 rows that an MMA has anyway are weights; the time is that of reading the weights once.
-// Where the tiles are fewer than the SMs, K is split over the CTAs of a cluster, which join
-// their sums through distributed shared memory, in the order of their ranks.
+// Three shapes of work.  Many tiles: 128 x 256, one CTA an SM that takes a tile after another,
+// its rings running on from tile to tile so that the tensor core works through the output of the
+// tile before.  Fewer: 128 x 128, K split over the CTAs of a cluster, which join their sums
+// through distributed shared memory in the order of their ranks.  Few tokens (SWAP): X = B,
+// Y = A, so that the 128 rows that an MMA has anyway are weights; split as well, two CTAs an SM;
+// the time is that of reading the weights once.
 //
 // Every mbarrier wait is bounded: after a timeout the CTA waits for what it has in flight,
 // releases its TMEM and sets the device's error word.
 #include <cudaTypedefs.h>
+
+#include <algorithm>
 
 #include "hv_decode.cuh"
 #include "hv_tc05.cuh"
@@ -29,28 +33,35 @@ namespace {
 using namespace dec;
 
 constexpr int BM = 128, GK = 128;  // rows of a tile; a group of K, in elements and bytes
-constexpr int EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32;
-constexpr int THREADS = EPI_THREADS + 64;
+constexpr int EPI_WARPS = 8, THREADS = 128 + EPI_WARPS * 32;
 constexpr uint32_t WAIT_ITERS = 1u << 22;
+constexpr int SB = 8;     // groups whose scales are fetched together
+constexpr int BAND = 16;  // tile rows of a band
 
 struct GemmFp8Args {
     const float *xs, *ys;  // scales of the row and column operands
     long long xs_row, xs_group, ys_row, ys_group;
     void *out;
     long long ldc;
-    int x_rows, y_rows, groups, tiles_x, split, out_dtype, vec;
+    int x_rows, y_rows, groups, tiles_x, tiles_y, split, out_dtype, vec;
     int *err;
 };
 
-template <int BN>
+template <int BN, bool SWAP>
 struct Lay {
     static constexpr int A_ST = BM * GK, B_ST = BN * GK, STAGE = A_ST + B_ST;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int PER_SM = SWAP ? 2 : 1;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : BN == 64 ? 4 : BN == 32 ? 5 : 6;
     static constexpr int BUFS = BN == 256 ? 2 : 4;  // TMEM accumulators
     static constexpr int COLS = BN < 32 ? 32 : BN;  // TMEM columns of one
     static constexpr int TMEM = BUFS * COLS;
-    static constexpr int BARS = STAGES * STAGE;  // full[STAGES] empty[STAGES] tfull[BUFS] tempty[BUFS] drain
+    // scales: of each column (SWAP: all rows share one), or of each row with either half of the columns
+    static constexpr int SCALES = SWAP ? BN : 2 * BM;
+    static constexpr int SC = STAGES * STAGE;  // [2][SB][SCALES] float
+    static constexpr int OUT = SC + 2 * SB * SCALES * 4;  // 2 KB an adding warp (see store_rows)
+    static constexpr int BARS = OUT + (SWAP ? 0 : EPI_WARPS * 2048);
     static constexpr int BYTES = BARS + 256 + 1024;  // and room to align the ring to 1024
+    static_assert(PER_SM * TMEM <= 512 && PER_SM * (BYTES + 1024) <= 228 * 1024, "resident CTAs");
 };
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *mbar) {
@@ -101,222 +112,71 @@ __device__ __forceinline__ void put_any(void *out, int dtype, long long i, float
     else if (dtype == HV_F16) put<__half>(out, i, v);
     else put<float>(out, i, v);
 }
-__device__ __forceinline__ void put8_any(void *out, int dtype, long long i, bool vec, int n, const float (&v)[8]) {
-    if (dtype == HV_BF16) store8((__nv_bfloat16 *)out + i, n, vec, v);
-    else if (dtype == HV_F16) store8((__half *)out + i, n, vec, v);
-    else store8((float *)out + i, n, vec, v);
+template <typename T>
+__device__ __forceinline__ void put4(T *p, bool vec, int n, float4 v) {
+    alignas(16) T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+    if (vec && n >= 4) {
+        if constexpr (sizeof(T) == 2) *(uint2 *)p = *(const uint2 *)e;
+        else *(uint4 *)p = *(const uint4 *)e;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) p[i] = e[i];
+    }
+}
+__device__ __forceinline__ void put4_any(const GemmFp8Args &a, long long i, int n, float4 v) {
+    if (a.out_dtype == HV_BF16) put4((__nv_bfloat16 *)a.out + i, a.vec, n, v);
+    else if (a.out_dtype == HV_F16) put4((__half *)a.out + i, a.vec, n, v);
+    else put4((float *)a.out + i, a.vec, n, v);
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-__device__ __forceinline__ float ld_peer(uint32_t saddr, uint32_t rank) {
+__device__ __forceinline__ float4 ld_peer(uint32_t saddr, uint32_t rank) {
     uint32_t a;
-    float v;
+    float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(saddr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
     return v;
 }
-
-// gridDim.x = tiles * split, the CTAs of a cluster next to one another.
-template <int BN, bool SWAP>
-__global__ void __launch_bounds__(THREADS, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmy, const GemmFp8Args a) {
-    using L = Lay<BN>;
-    extern __shared__ uint8_t raw[];
-    __shared__ uint32_t tslot;
-    __shared__ volatile int stop;
-    uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *full = (uint64_t *)(smem + L::BARS), *empty = full + L::STAGES;
-    uint64_t *tfull = empty + L::STAGES, *tempty = tfull + L::BUFS, *drain = tempty + L::BUFS;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = a.split, rank = blockIdx.x % split, tile = blockIdx.x / split;
-    const int tx = tile % a.tiles_x, ty = tile / a.tiles_x;
-    const int x0 = tx * BM, y0 = ty * BN;
-    const int g0 = (int)((long long)a.groups * rank / split), g1 = (int)((long long)a.groups * (rank + 1) / split);
-    const int n_groups = g1 - g0;
-
-    if (warp == EPI_WARPS) {
-        tc05::tmem_alloc(&tslot, L::TMEM);
-        tc05::tmem_relinquish();
-    }
-    if (tid == 0) {
-        stop = 0;
-        for (int i = 0; i < L::STAGES; ++i) {
-            tc05::mbar_init(&full[i], 1);
-            tc05::mbar_init(&empty[i], 1);
-        }
-        for (int i = 0; i < L::BUFS; ++i) {
-            tc05::mbar_init(&tfull[i], 1);
-            tc05::mbar_init(&tempty[i], EPI_WARPS);
-        }
-        tc05::mbar_init(drain, 1);
-        tc05::fence_mbar_init();
-    }
-    tc05::fence_before();
-    __syncthreads();
-    tc05::fence_after();
-    griddep_wait();
-    griddep_launch();
-    const uint32_t tmem = tslot;
-
-    if (warp == EPI_WARPS && lane == 0) {  // copies
-        int i = 0;
-        for (; i < n_groups; ++i) {
-            const int s = i % L::STAGES;
-            if (i >= L::STAGES && !wait_or_stop(&empty[s], (i / L::STAGES - 1) & 1, &stop)) break;
-            const uint32_t dst = tc05::smem_u32(smem + s * L::STAGE);
-            expect_tx(&full[s], L::STAGE);
-            tma_box(dst, &tmx, (g0 + i) * GK, x0, &full[s]);
-            tma_box(dst + L::A_ST, &tmy, (g0 + i) * GK, y0, &full[s]);
-        }
-        if (i < n_groups)  // gave up: what was issued has to land before shared memory goes
-            for (int k = max(0, i - L::STAGES); k < i; ++k) tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, WAIT_ITERS);
-    } else if (warp == EPI_WARPS + 1 && lane == 0) {  // products
-        constexpr uint32_t idesc = idesc_e4m3(BM, BN);
-        int i = 0;
-        for (; i < n_groups; ++i) {
-            const int s = i % L::STAGES, b = i % L::BUFS;
-            if (i >= L::BUFS && !wait_or_stop(&tempty[b], (i / L::BUFS - 1) & 1, &stop)) break;
-            if (!wait_or_stop(&full[s], (i / L::STAGES) & 1, &stop)) break;
-            tc05::fence_after();
-            const uint32_t at = tc05::smem_u32(smem + s * L::STAGE);
-            const uint64_t da = desc_sw128(at), db = desc_sw128(at + L::A_ST);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_e4m3(tmem + b * L::COLS, da + 2 * k, db + 2 * k, idesc, k > 0);
-            tc05::commit(&empty[s]);
-            tc05::commit(&tfull[b]);
-        }
-        if (i < n_groups) {
-            tc05::commit(drain);
-            tc05::mbar_wait(drain, 0, WAIT_ITERS);
-        }
-    }
-
-    // Sums: thread = (tile row, half of the columns).
-    constexpr int HC = BN / 2;
-    constexpr int CH = HC < 32 ? HC : 32;  // columns of one TMEM load
-    const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * HC;
-    float acc[HC];
-    if (warp < EPI_WARPS) {
-#pragma unroll
-        for (int j = 0; j < HC; ++j) acc[j] = 0.f;
-        // Scales of a group: a row's own times its columns' (SWAP: the rows' shared one times
-        // each column's, which lane j holds for column j).
-        const int xr = SWAP ? x0 / GK : min(x0 + row, a.x_rows - 1);
-        const int yr = SWAP ? min(y0 + c0 + lane % HC, a.y_rows - 1) : min(y0 + c0, a.y_rows - 1) / GK;
-        const float *xs = a.xs + xr * a.xs_row + g0 * a.xs_group;
-        const float *ys = a.ys + yr * a.ys_row + g0 * a.ys_group;
-        const uint32_t tbase = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
-        constexpr int AHEAD = 4;  // groups whose scales are on the way
-        float sx[AHEAD], sy[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            sx[i] = i < n_groups ? xs[i * a.xs_group] : 0.f;
-            sy[i] = i < n_groups ? ys[i * a.ys_group] : 0.f;
-        }
-        bool ok = true;
-        for (int i0 = 0; i0 < n_groups && ok; i0 += AHEAD)
-#pragma unroll
-            for (int ii = 0; ii < AHEAD; ++ii) {
-                const int i = i0 + ii;
-                if (i >= n_groups || !ok) break;
-                const float s = sx[ii] * sy[ii];
-                if (i + AHEAD < n_groups) {
-                    sx[ii] = xs[(i + AHEAD) * a.xs_group];
-                    sy[ii] = ys[(i + AHEAD) * a.ys_group];
-                }
-                const int b = i % L::BUFS;
-                ok = wait_or_stop(&tfull[b], (i / L::BUFS) & 1, &stop);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                tc05::fence_after();
-#pragma unroll
-                for (int j0 = 0; j0 < HC; j0 += CH) {
-                    uint32_t d[CH];
-                    if constexpr (CH == 32) tc05::ld32(tbase + b * L::COLS + j0, d);
-                    else if constexpr (CH == 16) tc05::ld16(tbase + b * L::COLS + j0, d);
-                    else tc05::ld8(tbase + b * L::COLS + j0, d);
-                    tc05::wait_ld_regs(d);
-                    if (j0 + CH == HC) {
-                        tc05::fence_before();
-                        if (lane == 0) arrive(&tempty[b]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < CH; ++j) {
-                        const float f = SWAP ? __shfl_sync(~0u, s, j0 + j) : s;
-                        acc[j0 + j] = fmaf(__uint_as_float(d[j]), f, acc[j0 + j]);
-                    }
-                }
-            }
-    }
-
-    __syncwarp();  // the one-thread roles rejoin their warps
-    const int cols_of = a.y_rows;
-    if (split == 1) {
-        if (warp < EPI_WARPS && x0 + row < a.x_rows) {
-            if (SWAP) {
-#pragma unroll
-                for (int j = 0; j < HC; ++j) {
-                    const int c = y0 + c0 + j;
-                    if (c < cols_of) put_any(a.out, a.out_dtype, c * a.ldc + x0 + row, acc[j]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < HC; j += 8) {
-                    const int c = y0 + c0 + j;
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = acc[j + e];
-                    if (c < cols_of)
-                        put8_any(a.out, a.out_dtype, (long long)(x0 + row) * a.ldc + c, a.vec, cols_of - c, v);
-                }
-            }
-        }
-        __syncthreads();
-    } else {
-        // Every copy and product of this CTA has completed (or its waits gave up and were
-        // drained): the ring's memory takes the sums, column by column.
-        __syncthreads();
-        float *part = (float *)smem;
-        if (warp < EPI_WARPS)
-#pragma unroll
-            for (int j = 0; j < HC; ++j) part[(c0 + j) * BM + row] = acc[j];
-        cluster_sync();
-        if (warp < EPI_WARPS) {
-            const int per = BN / split, cb = rank * per;
-            for (int j = tid >> 7; j < per; j += 2) {
-                const int r = tid & 127, c = y0 + cb + j;
-                const uint32_t at = tc05::smem_u32(part + (cb + j) * BM + r);
-                float v = 0.f;
-                for (int k = 0; k < split; ++k) v += ld_peer(at, k);
-                if (x0 + r < a.x_rows && c < cols_of)
-                    put_any(a.out, a.out_dtype,
-                            SWAP ? (long long)c * a.ldc + x0 + r : (long long)(x0 + r) * a.ldc + c, v);
-            }
-        }
-        cluster_sync();  // no CTA leaves while its sums may be read
-    }
-    if (tid == 0 && stop) atomicOr(a.err, HV_DECODE_STALLED);
-    tc05::fence_before();
-    __syncthreads();
-    if (warp == EPI_WARPS) {
-        tc05::fence_after();
-        tc05::tmem_dealloc(tmem, L::TMEM);
-    }
+__device__ __forceinline__ void split2(uint64_t pair, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(pair));
 }
 
-// ---- many tiles: persistent CTAs -------------------------------------------------
-// 128 x 256 tiles, one CTA an SM that takes a tile after another.  The rings of operand stages
-// and TMEM accumulators run on from tile to tile, so that the tensor core works through the
-// output of the tile before.  An adding thread has 128 columns of a row: its sums take 128
-// registers, so the copying and issuing warps give theirs up.  It keeps a 16-column TMEM load
-// under way while it adds the one before, with packed pairs of multiply-adds.
-constexpr int WIDE_BN = 256, WIDE_STAGES = 4, WIDE_BUFS = 2, WIDE_THREADS = 384, BAND = 16;
-constexpr int WIDE_STAGE = (BM + WIDE_BN) * GK;
-// Scales of SB groups at a time, a row's times its columns', for either half of the columns: two
-// warps fetch and multiply them (loads in the adding warps made those wait: 711 us, 8192^3).
-constexpr int SB = 8, SC_BYTES = 2 * SB * 2 * BM * 4;
-constexpr int WIDE_BYTES = WIDE_STAGES * WIDE_STAGE + SC_BYTES + 256 + 1024;
+// A warp's 32 rows x 2 * N columns of sums to `out` (row `m0` + lane at column 0), through 2 KB of
+// shared memory in pieces of 64 bytes a row, so that a store writes eight rows' 64 bytes and
+// not 32 rows' 16.  Everything lies on 16 bytes, and whole groups of 16 bytes are in or out.
+template <typename T, int N>
+__device__ __forceinline__ void store_rows(T *out, long long ldc, int rows, int cols, uint4 *stage,
+                                           const uint64_t (&acc)[N]) {
+    constexpr int PER = 16 / sizeof(T);  // elements of 16 bytes
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int p = 0; p < 2 * N / (4 * PER); ++p) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            alignas(16) T e[PER];
+#pragma unroll
+            for (int i = 0; i < PER; i += 2) {
+                float lo, hi;
+                split2(acc[(p * 4 + u) * (PER / 2) + i / 2], lo, hi);
+                e[i] = from_f32<T>(lo);
+                e[i + 1] = from_f32<T>(hi);
+            }
+            stage[lane * 4 + (u ^ (lane >> 1 & 3))] = *(const uint4 *)e;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2), u = lane & 3, c = (p * 4 + u) * PER;
+            if (r < rows && c < cols) *(uint4 *)(out + r * ldc + c) = stage[r * 4 + (u ^ (r >> 1 & 3))];
+        }
+        __syncwarp();
+    }
+}
 
 __device__ __forceinline__ void fma2(uint64_t &acc, uint32_t lo, uint32_t hi, uint64_t f) {
     asm("{\n.reg .b64 t;\nmov.b64 t, {%1, %2};\nfma.rn.f32x2 %0, t, %3, %0;\n}\n" : "+l"(acc) : "r"(lo), "r"(hi), "l"(f));
@@ -331,39 +191,44 @@ __device__ __forceinline__ void tile_at(int i, int tiles_x, int tiles_y, int &tx
     tx = band * BAND + in - ty * h;
 }
 
-__global__ void __launch_bounds__(WIDE_THREADS, 1)
-    gemm_wide_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmy,
-                     const __grid_constant__ GemmFp8Args a) {
+// One tile after another (split = 1), or one tile a cluster of `split` CTAs next to one another.
+template <int BN, bool SWAP>
+__global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
+    gemm_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmy,
+                const __grid_constant__ GemmFp8Args a) {
+    using L = Lay<BN, SWAP>;
     extern __shared__ uint8_t raw[];
     __shared__ uint32_t tslot;
     __shared__ volatile int stop;
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    float(*sc)[SB][2][BM] = (float(*)[SB][2][BM])(smem + WIDE_STAGES * WIDE_STAGE);
-    uint64_t *full = (uint64_t *)(smem + WIDE_STAGES * WIDE_STAGE + SC_BYTES), *empty = full + WIDE_STAGES;
-    uint64_t *tfull = empty + WIDE_STAGES, *tempty = tfull + WIDE_BUFS, *drain = tempty + WIDE_BUFS;
-    uint64_t *sfull = drain + 1, *sempty = sfull + 2;
+    float(*sc)[SB][L::SCALES] = (float(*)[SB][L::SCALES])(smem + L::SC);
+    uint64_t *full = (uint64_t *)(smem + L::BARS), *empty = full + L::STAGES;
+    uint64_t *tfull = empty + L::STAGES, *tempty = tfull + L::BUFS, *sfull = tempty + L::BUFS, *sempty = sfull + 2;
+    uint64_t *drain = sempty + 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int tiles_y = (a.y_rows + WIDE_BN - 1) / WIDE_BN, tiles = a.tiles_x * tiles_y;
+    const int tiles = a.tiles_x * a.tiles_y, split = a.split, rank = blockIdx.x % split;
+    const int first = blockIdx.x / split, step = gridDim.x / split;  // tiles of this CTA
+    const int g0 = (int)((long long)a.groups * rank / split), g1 = (int)((long long)a.groups * (rank + 1) / split);
 
     if (warp == 2) {
-        tc05::tmem_alloc(&tslot, 512);
+        tc05::tmem_alloc(&tslot, L::TMEM);
         tc05::tmem_relinquish();
     }
     if (tid == 0) {
         stop = 0;
-        for (int i = 0; i < WIDE_STAGES; ++i) {
+        for (int i = 0; i < L::STAGES; ++i) {
             tc05::mbar_init(&full[i], 1);
             tc05::mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < WIDE_BUFS; ++i) {
+        for (int i = 0; i < L::BUFS; ++i) {
             tc05::mbar_init(&tfull[i], 1);
             tc05::mbar_init(&tempty[i], EPI_WARPS);
         }
-        tc05::mbar_init(drain, 1);
         for (int i = 0; i < 2; ++i) {
             tc05::mbar_init(&sfull[i], 64);
             tc05::mbar_init(&sempty[i], EPI_WARPS);
         }
+        tc05::mbar_init(drain, 1);
         tc05::fence_mbar_init();
     }
     tc05::fence_before();
@@ -373,44 +238,49 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
     griddep_launch();
     const uint32_t tmem = tslot;
 
+    // Sums of an adding thread: one row, half of the columns, in pairs.
+    constexpr int HC = BN / 2, CW = HC < 16 ? HC : 16;  // CW: columns of one TMEM load
+    const int row = (warp & 3) * 32 + lane, half = warp >= 8, c0 = half * HC;
+    uint64_t acc[HC / 2];
+
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+        if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         if (warp == 0 && lane == 0) {  // copies
-            uint32_t n = 0;  // stages filled
+            uint32_t n = 0;            // stages filled
             bool ok = true;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int t = first; t < tiles && ok; t += step) {
                 int tx, ty;
-                tile_at(t, a.tiles_x, tiles_y, tx, ty);
-                for (int g = 0; g < a.groups; ++g, ++n) {
-                    const uint32_t s = n % WIDE_STAGES;
-                    if (n >= WIDE_STAGES && !wait_or_stop(&empty[s], (n / WIDE_STAGES - 1) & 1, &stop)) {
+                tile_at(t, a.tiles_x, a.tiles_y, tx, ty);
+                for (int g = g0; g < g1; ++g, ++n) {
+                    const uint32_t s = n % L::STAGES;
+                    if (n >= L::STAGES && !wait_or_stop(&empty[s], (n / L::STAGES - 1) & 1, &stop)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t dst = tc05::smem_u32(smem + s * WIDE_STAGE);
-                    expect_tx(&full[s], WIDE_STAGE);
+                    const uint32_t dst = tc05::smem_u32(smem + s * L::STAGE);
+                    expect_tx(&full[s], L::STAGE);
                     tma_box(dst, &tmx, g * GK, tx * BM, &full[s]);
-                    tma_box(dst + BM * GK, &tmy, g * GK, ty * WIDE_BN, &full[s]);
+                    tma_box(dst + L::A_ST, &tmy, g * GK, ty * BN, &full[s]);
                 }
             }
             if (!ok)  // what was issued has to land before shared memory goes
-                for (uint32_t k = n > WIDE_STAGES ? n - WIDE_STAGES : 0; k < n; ++k)
-                    tc05::mbar_wait(&full[k % WIDE_STAGES], (k / WIDE_STAGES) & 1, WAIT_ITERS);
+                for (uint32_t k = n > L::STAGES ? n - L::STAGES : 0; k < n; ++k)
+                    tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, WAIT_ITERS);
         } else if (warp == 1 && lane == 0) {  // products
-            constexpr uint32_t idesc = idesc_e4m3(BM, WIDE_BN);
+            constexpr uint32_t idesc = idesc_e4m3(BM, BN);
             uint32_t n = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
-                for (int g = 0; g < a.groups; ++g, ++n) {
-                    const uint32_t s = n % WIDE_STAGES, b = n % WIDE_BUFS;
-                    ok = (n < WIDE_BUFS || wait_or_stop(&tempty[b], (n / WIDE_BUFS - 1) & 1, &stop)) &&
-                         wait_or_stop(&full[s], (n / WIDE_STAGES) & 1, &stop);
+            for (int t = first; t < tiles && ok; t += step)
+                for (int g = g0; g < g1; ++g, ++n) {
+                    const uint32_t s = n % L::STAGES, b = n % L::BUFS;
+                    ok = (n < L::BUFS || wait_or_stop(&tempty[b], (n / L::BUFS - 1) & 1, &stop)) &&
+                         wait_or_stop(&full[s], (n / L::STAGES) & 1, &stop);
                     if (!ok) break;
                     tc05::fence_after();
-                    const uint32_t at = tc05::smem_u32(smem + s * WIDE_STAGE);
-                    const uint64_t da = desc_sw128(at), db = desc_sw128(at + BM * GK);
+                    const uint32_t at = tc05::smem_u32(smem + s * L::STAGE);
+                    const uint64_t da = desc_sw128(at), db = desc_sw128(at + L::A_ST);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_e4m3(tmem + b * WIDE_BN, da + 2 * k, db + 2 * k, idesc, k > 0);
+                    for (int k = 0; k < 4; ++k) mma_e4m3(tmem + b * L::COLS, da + 2 * k, db + 2 * k, idesc, k > 0);
                     tc05::commit(&empty[s]);
                     tc05::commit(&tfull[b]);
                 }
@@ -418,9 +288,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
                 tc05::commit(drain);
                 tc05::mbar_wait(drain, 0, WAIT_ITERS);
             }
-        } else if (warp >= 2) {  // scales
-            const int r = tid - 64;  // and r + 64
-            int t = blockIdx.x, g = 0;
+        } else if (warp >= 2) {  // scales (loads of theirs in the adding warps made those wait)
+            const int r = tid - 64;  // row r and r + 64, or column r
+            int t = first, g = g0;
             const float *x0 = nullptr, *x1 = nullptr, *y0 = nullptr, *y1 = nullptr;
             for (uint32_t q = 0; t < tiles; ++q) {
                 const int b = q & 1;
@@ -431,97 +301,177 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (t >= tiles) break;
-                        if (g == 0) {
+                        if (g == g0) {
                             int tx, ty;
-                            tile_at(t, a.tiles_x, tiles_y, tx, ty);
-                            x0 = a.xs + min(tx * BM + r, a.x_rows - 1) * a.xs_row;
-                            x1 = a.xs + min(tx * BM + r + 64, a.x_rows - 1) * a.xs_row;
-                            y0 = a.ys + min(ty * WIDE_BN, a.y_rows - 1) / GK * a.ys_row;
-                            y1 = a.ys + min(ty * WIDE_BN + GK, a.y_rows - 1) / GK * a.ys_row;
+                            tile_at(t, a.tiles_x, a.tiles_y, tx, ty);
+                            if (SWAP) {
+                                x0 = a.xs + tx * a.xs_row;  // BM rows are a block
+                                y0 = a.ys + min(ty * BN + r, a.y_rows - 1) * a.ys_row;
+                            } else {
+                                x0 = a.xs + min(tx * BM + r, a.x_rows - 1) * a.xs_row;
+                                x1 = a.xs + min(tx * BM + r + 64, a.x_rows - 1) * a.xs_row;
+                                y0 = a.ys + min(ty * BN, a.y_rows - 1) / GK * a.ys_row;
+                                y1 = a.ys + min(ty * BN + HC, a.y_rows - 1) / GK * a.ys_row;
+                            }
                         }
                         vx0[e] = x0[g * a.xs_group];
-                        vx1[e] = x1[g * a.xs_group];
                         vy0[e] = y0[g * a.ys_group];
-                        vy1[e] = y1[g * a.ys_group];
-                        if (++g == a.groups) {
-                            g = 0;
-                            t += gridDim.x;
+                        if (!SWAP) {
+                            vx1[e] = x1[g * a.xs_group];
+                            vy1[e] = y1[g * a.ys_group];
+                        }
+                        if (++g == g1) {
+                            g = g0;
+                            t += step;
                         }
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        sc[b][e0 + e][0][r] = vx0[e] * vy0[e];
-                        sc[b][e0 + e][1][r] = vx0[e] * vy1[e];
-                        sc[b][e0 + e][0][r + 64] = vx1[e] * vy0[e];
-                        sc[b][e0 + e][1][r + 64] = vx1[e] * vy1[e];
+                        float *to = sc[b][e0 + e];
+                        if (SWAP) {
+                            if (r < BN) to[r] = vx0[e] * vy0[e];
+                        } else {
+                            to[r] = vx0[e] * vy0[e];
+                            to[r + 64] = vx1[e] * vy0[e];
+                            to[BM + r] = vx0[e] * vy1[e];
+                            to[BM + r + 64] = vx1[e] * vy1[e];
+                        }
                     }
                 }
                 arrive(&sfull[b]);
             }
         }
-        __syncwarp();
+        __syncwarp();  // the one-thread roles rejoin their warps
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
-        const int row = (warp & 3) * 32 + lane, c0 = ((warp - 4) >> 2) * 128;
+        if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
         const uint32_t tbase = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
-        const int half = (warp - 4) >> 2;
-        uint64_t acc[64];
 #pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = 0;
+        for (int j = 0; j < HC / 2; ++j) acc[j] = 0;
         uint32_t n = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            for (int g = 0; g < a.groups; ++g, ++n) {
-                const uint32_t b = n % WIDE_BUFS, sb = n / SB;
+        for (int t = first; t < tiles && ok; t += step) {
+            for (int g = g0; g < g1; ++g, ++n) {
+                const uint32_t b = n % L::BUFS, sb = n / SB;
                 ok = n % SB || wait_or_stop(&sfull[sb & 1], (sb / 2) & 1, &stop);
-                const float f = sc[sb & 1][n % SB][half][row];
-                uint64_t s2;
-                asm("mov.b64 %0, {%1, %1};\n" : "=l"(s2) : "f"(f));
-                ok = ok && wait_or_stop(&tfull[b], (n / WIDE_BUFS) & 1, &stop);
-                ok = __all_sync(~0u, ok);  // and every lane has its scale
+                const float *f = sc[sb & 1][n % SB] + (SWAP ? c0 : half * BM + row);
+                uint64_t s2 = 0;
+                if (!SWAP) asm("mov.b64 %0, {%1, %1};\n" : "=l"(s2) : "f"(*f));
+                ok = ok && wait_or_stop(&tfull[b], (n / L::BUFS) & 1, &stop);
+                ok = __all_sync(~0u, ok);
                 if (!ok) break;
-                __syncwarp();
-                if (n % SB == SB - 1 && lane == 0) arrive(&sempty[sb & 1]);
                 tc05::fence_after();
-                uint32_t d[2][16];
-                tc05::ld16(tbase + b * WIDE_BN, d[0]);
+                uint32_t d[2][CW];
+                auto ask = [&](int c) {
+                    if constexpr (CW == 16) tc05::ld16(tbase + b * L::COLS + c * CW, d[c & 1]);
+                    else tc05::ld8(tbase + b * L::COLS + c * CW, d[c & 1]);
+                };
+                ask(0);
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < HC / CW; ++c) {
                     tc05::wait_ld_regs(d[c & 1]);
-                    if (c < 7) {
-                        tc05::ld16(tbase + b * WIDE_BN + (c + 1) * 16, d[(c + 1) & 1]);
+                    if (c + 1 < HC / CW) {
+                        ask(c + 1);
                     } else {
                         tc05::fence_before();
                         if (lane == 0) arrive(&tempty[b]);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], d[c & 1][2 * j], d[c & 1][2 * j + 1], s2);
+                    for (int j = 0; j < CW / 2; ++j)
+                        fma2(acc[c * CW / 2 + j], d[c & 1][2 * j], d[c & 1][2 * j + 1],
+                             SWAP ? ((const uint64_t *)f)[c * CW / 2 + j] : s2);
                 }
+                __syncwarp();  // every lane has its scales
+                if (n % SB == SB - 1 && lane == 0) arrive(&sempty[sb & 1]);
             }
-            if (!ok) break;
+            if (!ok || split > 1) break;
             int tx, ty;
-            tile_at(t, a.tiles_x, tiles_y, tx, ty);
-            const int m = tx * BM + row, col = ty * WIDE_BN + c0;
-            const long long at = (long long)m * a.ldc + col;
+            tile_at(t, a.tiles_x, a.tiles_y, tx, ty);
+            const int m = tx * BM + row, col = ty * BN + c0;
+            if (SWAP) {
 #pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(v[2 * e]), "=f"(v[2 * e + 1]) : "l"(acc[j + e]));
-                    acc[j + e] = 0;
+                for (int j = 0; j < HC / 2; ++j) {
+                    float v[2];
+                    split2(acc[j], v[0], v[1]);
+                    acc[j] = 0;
+                    if (m < a.x_rows && col + 2 * j < a.y_rows) put_any(a.out, a.out_dtype, (col + 2 * j) * a.ldc + m, v[0]);
+                    if (m < a.x_rows && col + 2 * j + 1 < a.y_rows)
+                        put_any(a.out, a.out_dtype, (col + 2 * j + 1) * a.ldc + m, v[1]);
                 }
-                if (m < a.x_rows && col + 2 * j < a.y_rows)
-                    put8_any(a.out, a.out_dtype, at + 2 * j, a.vec, a.y_rows - col - 2 * j, v);
+            } else {
+                const int m0 = tx * BM + (warp & 3) * 32;
+                const long long at = (long long)m0 * a.ldc + col;
+                uint4 *stage = (uint4 *)(smem + L::OUT) + (warp - 4) * 128;
+                if (a.vec && a.out_dtype == HV_BF16) {
+                    store_rows((__nv_bfloat16 *)a.out + at, a.ldc, a.x_rows - m0, a.y_rows - col, stage, acc);
+                } else if (a.vec && a.out_dtype == HV_F16) {
+                    store_rows((__half *)a.out + at, a.ldc, a.x_rows - m0, a.y_rows - col, stage, acc);
+                } else if (a.vec) {
+                    store_rows((float *)a.out + at, a.ldc, a.x_rows - m0, a.y_rows - col, stage, acc);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < HC / 2; ++j) {
+                        float v[2];
+                        split2(acc[j], v[0], v[1]);
+                        for (int e = 0; e < 2; ++e)
+                            if (m < a.x_rows && col + 2 * j + e < a.y_rows)
+                                put_any(a.out, a.out_dtype, (long long)m * a.ldc + col + 2 * j + e, v[e]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < HC / 2; ++j) acc[j] = 0;
             }
         }
+    }
+
+    if (BN < 256 && split > 1) {
+        // Every copy and product of this CTA has completed (or its waits gave up and were
+        // drained): the ring's memory takes the sums, along the output's rows.
+        constexpr int ALONG = SWAP ? BM : BN, ACROSS = SWAP ? BN : BM, LD = ALONG + 4;
+        static_assert(BN == 256 || ACROSS * LD * 4 <= L::SC, "the sums fit where the ring was");
+        float *part = (float *)smem;
+        __syncthreads();
+        if (warp >= 4)
+#pragma unroll
+            for (int j = 0; j < HC / 2; j += 2) {
+                float4 v;
+                split2(acc[j], v.x, v.y);
+                split2(acc[j + 1], v.z, v.w);
+                const int c = c0 + 2 * j;
+                if (SWAP) {
+                    part[c * LD + row] = v.x;
+                    part[(c + 1) * LD + row] = v.y;
+                    part[(c + 2) * LD + row] = v.z;
+                    part[(c + 3) * LD + row] = v.w;
+                } else {
+                    *(float4 *)(part + row * LD + c) = v;
+                }
+            }
+        cluster_sync();
+        int tx, ty;
+        tile_at(first, a.tiles_x, a.tiles_y, tx, ty);
+        // Each rank has a share of the output's rows, four neighbouring elements a thread.
+        const int per = (ACROSS + split - 1) / split, from = rank * per, share = min(per, ACROSS - from);
+        const int p0 = SWAP ? ty * BN : tx * BM, q0 = SWAP ? tx * BM : ty * BN;
+        const int p_end = SWAP ? a.y_rows : a.x_rows, q_end = SWAP ? a.x_rows : a.y_rows;
+#pragma unroll 2
+        for (int i = tid; i < share * (ALONG / 4); i += THREADS) {
+            const int p = from + i / (ALONG / 4), q = i % (ALONG / 4) * 4;
+            const uint32_t at = tc05::smem_u32(part + p * LD + q);
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = k < split ? ld_peer(at, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 1; k < 8; ++k) v[0].x += v[k].x, v[0].y += v[k].y, v[0].z += v[k].z, v[0].w += v[k].w;
+            if (p0 + p < p_end) put4_any(a, (p0 + p) * a.ldc + q0 + q, q_end - q0 - q, v[0]);
+        }
+        cluster_sync();  // no CTA leaves while its sums may be read
     }
     if (tid == 0 && stop) atomicOr(a.err, HV_DECODE_STALLED);
     tc05::fence_before();
     __syncthreads();
     if (warp == 2) {
         tc05::fence_after();
-        tc05::tmem_dealloc(tmem, 512);
+        tc05::tmem_dealloc(tmem, L::TMEM);
     }
 }
 
@@ -558,58 +508,67 @@ struct Operand {
 };
 
 template <int BN, bool SWAP>
+cudaLaunchConfig_t config(unsigned grid, int split, cudaStream_t st, cudaLaunchAttribute (&attr)[2]) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Lay<BN, SWAP>::BYTES;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cfg;
+}
+
+// How many ways K is split: as many as leave every cluster resident at once and a CTA at least
+// two groups.  (A second wave of clusters costs more than it saves: 512 x 4096 x 4096 took 19 us
+// unsplit and 284 split eight ways.)  How many clusters a device holds is asked once.
+template <int BN, bool SWAP>
+int split_of(int64_t tiles, int groups) {
+    static std::atomic<int> held[64][9];  // clusters of each size, plus one
+    int dev = 0, best = 1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 1;
+    for (int s = 2; s <= 8 && 2 * s <= groups && tiles * s <= 2 * 512; ++s) {
+        int n = held[dev][s].load(std::memory_order_relaxed) - 1;
+        if (n < 0) {
+            cudaLaunchAttribute attr[2];
+            const cudaLaunchConfig_t cfg = config<BN, SWAP>((unsigned)s, s, nullptr, attr);
+            if (cudaOccupancyMaxActiveClusters(&n, gemm_kernel<BN, SWAP>, &cfg) != cudaSuccess) {
+                (void)cudaGetLastError();
+                n = 0;
+            }
+            held[dev][s].store(n + 1, std::memory_order_relaxed);
+        }
+        if (tiles <= n && (groups + s - 1) / s < (groups + best - 1) / best) best = s;
+    }
+    return best;
+}
+
+template <int BN, bool SWAP>
 int run(const Operand &x, const Operand &y, int k, GemmFp8Args a, int sms, cudaStream_t st) {
-    using L = Lay<BN>;
     CUtensorMap tmx, tmy;
     if (!tensor_map(&tmx, x.p, x.rows, k, x.stride, BM) || !tensor_map(&tmy, y.p, y.rows, k, y.stride, BN))
         return fail(HV_ERR_CUDA, "gemm_fp8: cannot encode the operands' tensor maps");
     a.xs = x.scale, a.xs_row = x.s_row, a.xs_group = x.s_group;
     a.ys = y.scale, a.ys_row = y.s_row, a.ys_group = y.s_group;
     a.x_rows = (int)x.rows, a.y_rows = (int)y.rows;
-    a.tiles_x = (int)((x.rows + BM - 1) / BM);
-    const int64_t tiles = (int64_t)a.tiles_x * ((y.rows + BN - 1) / BN);
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= sms && a.groups >= split * 2) split *= 2;
-    if (tiles * split > INT32_MAX) return fail(HV_ERR_VALUE, "gemm_fp8: too many tiles");
-    a.split = split;
-    auto kernel = gemm_kernel<BN, SWAP>;
+    a.tiles_x = (int)((x.rows + BM - 1) / BM), a.tiles_y = (int)((y.rows + BN - 1) / BN);
+    const int64_t tiles = (int64_t)a.tiles_x * a.tiles_y;
+    if (tiles > INT32_MAX / 16) return fail(HV_ERR_VALUE, "gemm_fp8: too many tiles");
+    const auto kernel = gemm_kernel<BN, SWAP>;
     static std::atomic<uint64_t> ready;
     cudaError_t e = allow_shared(kernel, ready);
     if (e == cudaSuccess) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(tiles * split));
-        cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = L::BYTES;
-        cfg.stream = st;
+        a.split = BN == 256 ? 1 : split_of<BN, SWAP>(tiles, a.groups);
+        const int64_t grid = a.split > 1 ? tiles * a.split : std::min<int64_t>(tiles, sms * Lay<BN, SWAP>::PER_SM);
         cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = (unsigned)split;
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 2;
+        const cudaLaunchConfig_t cfg = config<BN, SWAP>((unsigned)grid, a.split, st, attr);
         e = cudaLaunchKernelEx(&cfg, kernel, tmx, tmy, a);
     }
-    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "gemm_fp8: %s", cudaGetErrorString(e));
-    return HV_OK;
-}
-
-int run_wide(const Operand &x, const Operand &y, int k, GemmFp8Args a, int sms, cudaStream_t st) {
-    CUtensorMap tmx, tmy;
-    if (!tensor_map(&tmx, x.p, x.rows, k, x.stride, BM) || !tensor_map(&tmy, y.p, y.rows, k, y.stride, WIDE_BN))
-        return fail(HV_ERR_CUDA, "gemm_fp8: cannot encode the operands' tensor maps");
-    a.xs = x.scale, a.xs_row = x.s_row, a.xs_group = x.s_group;
-    a.ys = y.scale, a.ys_row = y.s_row, a.ys_group = y.s_group;
-    a.x_rows = (int)x.rows, a.y_rows = (int)y.rows;
-    a.tiles_x = (int)((x.rows + BM - 1) / BM);
-    const int64_t tiles = (int64_t)a.tiles_x * ((y.rows + WIDE_BN - 1) / WIDE_BN);
-    if (tiles > INT32_MAX / 2) return fail(HV_ERR_VALUE, "gemm_fp8: too many tiles");
-    static std::atomic<uint64_t> ready;
-    cudaError_t e = allow_shared(gemm_wide_kernel, ready);
-    if (e == cudaSuccess)
-        e = launch_pdl(gemm_wide_kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(WIDE_THREADS), WIDE_BYTES, st,
-                       tmx, tmy, a);
     if (e != cudaSuccess) return fail(HV_ERR_CUDA, "gemm_fp8: %s", cudaGetErrorString(e));
     return HV_OK;
 }
@@ -638,7 +597,9 @@ extern "C" int hv_gemm_fp8(const hv_gemm_fp8_args *p, void *stream) {
     if (!err || !sms) return fail(HV_ERR_CUDA, "cannot read the device's properties");
     GemmFp8Args g{};
     g.out = p->d_out, g.ldc = p->out_stride, g.out_dtype = p->out_dtype, g.groups = (int)((k + GK - 1) / GK), g.err = err;
-    g.vec = dec::aligned(p->d_out, 16) && (m == 1 || p->out_stride * dec::elem_size(p->out_dtype) % 16 == 0);
+    // 16-byte stores: rows start on 16 bytes and are whole groups of them
+    const int es = dec::elem_size(p->out_dtype);
+    g.vec = dec::aligned(p->d_out, 16) && n * es % 16 == 0 && (m == 1 || p->out_stride * es % 16 == 0);
     const Operand a{p->d_a, m, sa, p->d_a_scale, p->a_scale_strides[0], p->a_scale_strides[1]};
     const Operand b{p->d_b, n, sb, p->d_b_scale, p->b_scale_strides[0], p->b_scale_strides[1]};
     const cudaStream_t st = (cudaStream_t)stream;
@@ -646,7 +607,9 @@ extern "C" int hv_gemm_fp8(const hv_gemm_fp8_args *p, void *stream) {
     if (m <= 16) return run<16, true>(b, a, kk, g, sms, st);
     if (m <= 32) return run<32, true>(b, a, kk, g, sms, st);
     if (m <= 64) return run<64, true>(b, a, kk, g, sms, st);
-    // a 256-wide tile reads each operand byte for more products; a 128-wide one fills more SMs
-    if (((m + 127) / 128) * ((n + 255) / 256) >= sms) return run_wide(a, b, kk, g, sms, st);
+    // A 256-wide tile's group takes about the time of 1.5 of a 128-wide one's, which may split K.
+    const int64_t tm = (m + BM - 1) / BM, t128 = tm * ((n + 127) / 128), t256 = tm * ((n + 255) / 256);
+    const int64_t waves128 = (t128 + sms - 1) / sms, waves256 = (t256 + sms - 1) / sms;
+    if (3 * waves256 <= 2 * waves128) return run<256, false>(a, b, kk, g, sms, st);
     return run<128, false>(a, b, kk, g, sms, st);
 }
