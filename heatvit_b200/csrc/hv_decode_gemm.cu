@@ -467,6 +467,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
         cluster_sync();  // no CTA leaves while its sums may be read
     }
     if (tid == 0 && stop) atomicOr(a.err, HV_DECODE_STALLED);
+    __syncwarp();
     tc05::fence_before();
     __syncthreads();
     if (warp == 2) {
@@ -524,15 +525,17 @@ cudaLaunchConfig_t config(unsigned grid, int split, cudaStream_t st, cudaLaunchA
     return cfg;
 }
 
-// How many ways K is split: as many as leave every cluster resident at once and a CTA at least
-// two groups.  (A second wave of clusters costs more than it saves: 512 x 4096 x 4096 took 19 us
-// unsplit and 284 split eight ways.)  How many clusters a device holds is asked once.
+// How many ways K is split: the most of 2, 3, 4 and 8 that leaves every cluster resident at once
+// and a CTA two groups.  (A second wave of clusters costs more than it saves: 512 x 4096 x 4096
+// took 19 us unsplit and 284 split eight ways.  Five or six shares of 1 x 4096 x 4096 took 7.5
+// us, four 6.8; of 48 x 10240 x 4096 one took 20 us, two 17.6, three 15.8.)  How many clusters a device holds is asked once; the answer counts one
+// CTA an SM for kernels with tensor memory, of which PER_SM fit.
 template <int BN, bool SWAP>
 int split_of(int64_t tiles, int groups) {
     static std::atomic<int> held[64][9];  // clusters of each size, plus one
     int dev = 0, best = 1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 1;
-    for (int s = 2; s <= 8 && 2 * s <= groups && tiles * s <= 2 * 512; ++s) {
+    for (int s = 2; s <= 8 && 2 * s <= groups && tiles * s <= 2 * 512; s = s == 2 ? 3 : s == 3 ? 4 : 2 * s) {
         int n = held[dev][s].load(std::memory_order_relaxed) - 1;
         if (n < 0) {
             cudaLaunchAttribute attr[2];
@@ -543,7 +546,7 @@ int split_of(int64_t tiles, int groups) {
             }
             held[dev][s].store(n + 1, std::memory_order_relaxed);
         }
-        if (tiles <= n && (groups + s - 1) / s < (groups + best - 1) / best) best = s;
+        if (tiles <= n * Lay<BN, SWAP>::PER_SM) best = s;
     }
     return best;
 }
