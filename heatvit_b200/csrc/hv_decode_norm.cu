@@ -102,10 +102,11 @@ struct alignas(16) Group {
     }
 };
 
-__device__ __forceinline__ float reciprocal(float x) {  // within one unit in the last place
+// An approximate reciprocal and one Newton step: a block's 128 quotients share its error.
+__device__ __forceinline__ float reciprocal(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
+    return fmaf(y, fmaf(-x, y, 1.f), y);
 }
 
 // e4m3(y * f) of a group.
