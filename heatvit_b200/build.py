@@ -1,19 +1,26 @@
 """Build the CUDA library in-tree: heatvit_b200/_lib/libheatvit_b200.so.
 
 One nvcc invocation per translation unit (parallel), linked into a shared
-library with the CUDA runtime statically linked, for sm_100a only.
+library with the CUDA runtime statically linked, for sm_100a only.  Beside it
+_decode_native.so, the decode operators' calls from Python (a CPython module
+on the installed torch's headers, linked against the library).
 """
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "libheatvit_b200.so")
+NATIVE = os.path.join(LIBDIR, "_decode_native.so")
+NATIVE_SOURCE = os.path.join(CSRC, "hv_decode_torch.cpp")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+CXX = os.environ.get("CXX", "g++")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -37,8 +44,35 @@ def up_to_date():
     return all(os.path.getmtime(f) <= t for f in _deps())
 
 
+def native_up_to_date():
+    header = os.path.join(os.path.dirname(HERE), "include", "heatvit_b200.h")
+    return os.path.exists(NATIVE) and all(os.path.getmtime(f) <= os.path.getmtime(NATIVE)
+                                          for f in (NATIVE_SOURCE, header))
+
+
+def build_native(force=False):
+    """The decode operators' Python module, for the installed torch."""
+    if not force and native_up_to_date():
+        return NATIVE
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    tmp = NATIVE + ".tmp"
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", "-Wall", NATIVE_SOURCE, "-o", tmp,
+           "-isystem", os.path.join(torch, "include"),
+           "-isystem", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           "-isystem", cuda, "-I" + sysconfig.get_paths()["include"],
+           "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+           "-L" + LIBDIR, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for {NATIVE_SOURCE}:\n{r.stderr}")
+    os.replace(tmp, NATIVE)
+    return NATIVE
+
+
 def build(force=False, verbose=False, ptxas_info=False):
     if not force and up_to_date():
+        build_native()
         return LIB
     os.makedirs(os.path.join(LIBDIR, "obj"), exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas_info else []
@@ -64,6 +98,7 @@ def build(force=False, verbose=False, ptxas_info=False):
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
+    build_native(force)
     return LIB
 
 
