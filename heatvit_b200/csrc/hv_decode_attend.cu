@@ -58,16 +58,17 @@ struct Lay {
     static constexpr int HALVES = D > 128 ? 2 : 1, DH = D / HALVES;
     static constexpr int WARPS = SLICES * HALVES, THREADS = WARPS * 32;
     // 16-token blocks of a warp's step: a step costs about the same for 32 tokens of 64
-    // dimensions (16 heads of 64 over 64 x 4000 tokens: BEFORE -> AFTER us) as for 16 of 128
+    // dimensions (16 heads of 64 over 64 x 4000 tokens: 245 us with 16, 223 with 32) as for 16 of 128
     static constexpr int BLOCKS = D <= 64 ? 2 : 1, WTOK = BLOCKS * BLOCK, TILE = SLICES * WTOK;
     static constexpr int ROW = DH * 2 + 16;  // bytes: rows 16 bytes apart modulo 128 (ldmatrix without conflicts)
     static constexpr int STAGES = 3;
     static constexpr int STAGE = 2 * WTOK * ROW;
-    static constexpr int SUM_ROW = D + 4;
-    static constexpr int SUM = WARPS * STAGES * STAGE;  // [ROWS][SUM_ROW] float, at an item's end
-    static constexpr int EXCHANGE = HALVES == 1 ? 0 : 2 * WARPS * 32 * 8 * 4;  // halves of scores, before it
-    static constexpr int STAT = SUM + (ROWS * SUM_ROW * 4 > EXCHANGE ? ROWS * SUM_ROW * 4 : EXCHANGE);
-    static constexpr int MISC = STAT + SLICES * ROWS * 2 * 4;  // stat: [SLICES][ROWS][2] float
+    static constexpr int PART_ROW = DH + 4;  // a warp's sums at an item's end, where its last stage was
+    static constexpr int SUM = WARPS * STAGES * STAGE;  // weights of parts, or halves of scores before that
+    static constexpr int EXCHANGE = HALVES == 1 ? 0 : 2 * WARPS * 32 * 8 * 4, JOIN = 2 * FAN * ROWS * 4;
+    static constexpr int STAT = SUM + (JOIN > EXCHANGE ? JOIN : EXCHANGE);  // [SLICES + 1][ROWS][2] float
+    static constexpr int MISC = STAT + (SLICES + 1) * ROWS * 2 * 4;
+    static_assert(ROWS * PART_ROW * 4 <= STAGE, "a warp's sums fit in a stage");
     static constexpr int BYTES = MISC + 32;
     static constexpr int PER_SM = D <= 128 ? 2 : 1;
     static_assert(PER_SM * (BYTES + 1024) <= 228 * 1024, "the CTAs of a wave are resident together");
@@ -205,12 +206,12 @@ __device__ __forceinline__ void join_parts(float *parts, float *sum, float *stat
         if (tid < ROWS) {  // weights of the parts of row `tid`
             const float was = k0 ? stat[2 * tid] : -CUDART_INF_F;
             float M = was;
-            for (int k = 0; k < FAN; ++k) M = fmaxf(M, sum[k * ROWS + tid]);
+            for (int k = 0; k < m; ++k) M = fmaxf(M, sum[k * ROWS + tid]);
             const float f = k0 ? exp2_(was - M) : 0.f;
             float S = k0 ? stat[2 * tid + 1] * f : 0.f;
-            for (int k = 0; k < FAN; ++k) {
-                const float w = k < m ? exp2_(sum[k * ROWS + tid] - M) : 0.f;
-                if (k < m) S += w * sum[(FAN + k) * ROWS + tid];
+            for (int k = 0; k < m; ++k) {
+                const float w = exp2_(sum[k * ROWS + tid] - M);
+                S += w * sum[(FAN + k) * ROWS + tid];
                 sum[k * ROWS + tid] = w;
             }
             stat[2 * tid] = M;
@@ -253,16 +254,16 @@ __device__ __forceinline__ void join_parts(float *parts, float *sum, float *stat
 // Counts this CTA in; true in the one that comes last, for which the counter is zero again
 // and the others' stores are visible.
 __device__ __forceinline__ bool comes_last(uint32_t *counter, uint32_t of, long long *flag) {
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();  // the CTA's stores, which the barrier put before this
         const bool last = atomicAdd(counter, 1u) == of - 1;
         if (last) *counter = 0;
+        __threadfence();  // and the others', before what follows the next barrier
         *flag = last;
     }
     __syncthreads();
     const bool last = *flag;
-    if (last) __threadfence();
     __syncthreads();
     return last;
 }
@@ -577,45 +578,44 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 for (int w = 0; w < SLICES; ++w) top = fmaxf(top, stat[(w * ROWS + (lane >> 2) + 8 * i) * 2]);
                 f[i] = m[i] == -CUDART_INF_F ? 0.f : exp2_(m[i] - top);
             }
-            for (int w = 0; w < SLICES; ++w) {
-                if (slice == w) {
+            float *mine = (float *)(ring + (u % L::STAGES) * L::STAGE);  // read, and not yet refilled
 #pragma unroll
-                    for (int j = 0; j < DH / 8; ++j)
+            for (int j = 0; j < DH / 8; ++j)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            float2 *d = (float2 *)(sum + ((lane >> 2) + 8 * i) * L::SUM_ROW + half * DH + j * 8 +
-                                                   (lane & 3) * 2);
-                            float2 v = make_float2(o[j][2 * i] * f[i], o[j][2 * i + 1] * f[i]);
-                            if (w) {
-                                const float2 x = *d;
-                                v.x += x.x;
-                                v.y += x.y;
-                            }
-                            *d = v;
-                        }
-                }
-                __syncthreads();
-            }
+                for (int i = 0; i < 2; ++i)
+                    *(float2 *)(mine + ((lane >> 2) + 8 * i) * L::PART_ROW + j * 8 + (lane & 3) * 2) =
+                        make_float2(o[j][2 * i] * f[i], o[j][2 * i + 1] * f[i]);
             float M = -CUDART_INF_F, S = 0.f;
-            if (tid < ROWS) {  // a row's maximum and sum, into its first place
+            float *of_row = stat + SLICES * ROWS * 2;
+            if (tid < ROWS) {  // a row's maximum and sum
                 for (int w = 0; w < SLICES; ++w) M = fmaxf(M, stat[(w * ROWS + tid) * 2]);
                 for (int w = 0; w < SLICES; ++w) {
                     const float mw = stat[(w * ROWS + tid) * 2];
                     if (mw != -CUDART_INF_F) S += stat[(w * ROWS + tid) * 2 + 1] * exp2_(mw - M);
                 }
-                stat[tid * 2] = M;
-                stat[tid * 2 + 1] = S;
+                of_row[tid * 2 + 1] = S;
             }
+            __syncthreads();
+            // four columns of the item's sums
+            auto four = [&](int r, int c) {
+                const float *p = (const float *)(smem + (c / DH * SLICES * L::STAGES + u % L::STAGES) * L::STAGE) +
+                                 r * L::PART_ROW + c % DH;
+                float4 v = *(const float4 *)p;
+#pragma unroll
+                for (int w = 1; w < SLICES; ++w) {
+                    const float4 x = *(const float4 *)(p + w * (L::STAGES * L::STAGE / 4));
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                }
+                return v;
+            };
             const int nvec = nrows * (D / 4);
             T *out = (T *)a.out + cur.b * a.o_seq + h0 * a.o_head;
             float *lse = a.lse ? a.lse + cur.b * a.lse_seq + h0 * a.lse_head : nullptr;
             const int c_first = (int)(item_first / share), c_last = (int)((item_first + cur.tiles - 1) / share);
             if (c_first == c_last) {
-                __syncthreads();
                 for (int i = tid; i < nvec; i += THREADS) {
                     const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
-                    const float4 x = *(const float4 *)(sum + r * L::SUM_ROW + c);
-                    store4(out + r * a.o_head + c, a.o_vec, x, 1.f / stat[r * 2 + 1]);
+                    store4(out + r * a.o_head + c, a.o_vec, four(r, c), 1.f / of_row[r * 2 + 1]);
                 }
                 if (lse && tid < nrows) lse[tid * a.lse_head] = (M + log2f(S)) * 0.69314718055994531f;
             } else {
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 float4 *po = (float4 *)(a.parts + mine * (ROWS * D));
                 float2 *pst = (float2 *)(a.parts + 2ll * gridDim.x * (ROWS * D)) + mine * ROWS;
                 for (int i = tid; i < nvec; i += THREADS)
-                    __stcg(po + i, *(const float4 *)(sum + (i / (D / 4)) * L::SUM_ROW + i % (D / 4) * 4));
+                    __stcg(po + i, four(i / (D / 4), i % (D / 4) * 4));
                 if (tid < nrows) __stcg(pst + tid, make_float2(M, S));
                 const int n = c_last - c_first + 1;
                 if (n <= ONE_LEVEL) {
