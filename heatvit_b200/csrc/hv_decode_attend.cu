@@ -61,7 +61,9 @@ struct Lay {
     // dimensions (16 heads of 64 over 64 x 4000 tokens: 245 us with 16, 223 with 32) as for 16 of 128
     static constexpr int BLOCKS = D <= 64 ? 2 : 1, WTOK = BLOCKS * BLOCK, TILE = SLICES * WTOK;
     static constexpr int ROW = DH * 2 + 16;  // bytes: rows 16 bytes apart modulo 128 (ldmatrix without conflicts)
-    static constexpr int STAGES = 3;
+    // Three CTAs an SM of two stages where registers allow, else two of three: 16 heads of 64 took
+    // 223 us as two of three, 186 as three of two; heads of 128 spill at 168 registers (187, 381).
+    static constexpr int PER_SM = D <= 64 ? 3 : D <= 128 ? 2 : 1, STAGES = D <= 64 ? 2 : 3;
     static constexpr int STAGE = 2 * WTOK * ROW;
     static constexpr int PART_ROW = DH + 4;  // a warp's sums at an item's end, where its last stage was
     static constexpr int SUM = WARPS * STAGES * STAGE;  // weights of parts, or halves of scores before that
@@ -70,7 +72,6 @@ struct Lay {
     static constexpr int MISC = STAT + (SLICES + 1) * ROWS * 2 * 4;
     static_assert(ROWS * PART_ROW * 4 <= STAGE, "a warp's sums fit in a stage");
     static constexpr int BYTES = MISC + 32;
-    static constexpr int PER_SM = D <= 128 ? 2 : 1;
     static_assert(PER_SM * (BYTES + 1024) <= 228 * 1024, "the CTAs of a wave are resident together");
 };
 
@@ -665,7 +666,7 @@ constexpr int COUNT_BYTES = 3 * MAX_GRID * 4;
 // CTAs of one resident wave on the current device.
 int wave(int d) {
     const int sms = sm_count();
-    const int grid = sms * (d <= 128 ? Lay<128>::PER_SM : Lay<256>::PER_SM);
+    const int grid = sms * (d <= 64 ? Lay<64>::PER_SM : d <= 128 ? Lay<128>::PER_SM : Lay<256>::PER_SM);
     return grid < MAX_GRID ? grid : MAX_GRID;
 }
 
