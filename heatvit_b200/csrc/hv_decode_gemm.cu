@@ -147,11 +147,12 @@ __device__ __forceinline__ void split2(uint64_t pair, float &lo, float &hi) {
     asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(pair));
 }
 
-// A warp's 32 rows x 2 * N columns of sums to `out` (row `m0` + lane at column 0), through 2 KB of
-// shared memory in pieces of 64 bytes a row, so that a store writes eight rows' 64 bytes and
-// not 32 rows' 16.  Everything lies on 16 bytes, and whole groups of 16 bytes are in or out.
+// A warp's 32 rows x 2 * N columns of sums to `out` (row 0 of the 32, column 0), of which `rows`
+// and `cols` exist, through 2 KB of shared memory in pieces of 64 bytes a row: a store then
+// writes 64 neighbouring bytes of eight rows (vec: rows lie on 16 bytes and end with a whole 16)
+// or of one or two, and not 32 rows' 16 or 2.
 template <typename T, int N>
-__device__ __forceinline__ void store_rows(T *out, long long ldc, int rows, int cols, uint4 *stage,
+__device__ __forceinline__ void store_rows(T *out, long long ldc, int rows, int cols, bool vec, uint4 *stage,
                                            const uint64_t (&acc)[N]) {
     constexpr int PER = 16 / sizeof(T);  // elements of 16 bytes
     const int lane = threadIdx.x & 31;
@@ -170,10 +171,19 @@ __device__ __forceinline__ void store_rows(T *out, long long ldc, int rows, int 
             stage[lane * 4 + (u ^ (lane >> 1 & 3))] = *(const uint4 *)e;
         }
         __syncwarp();
+        if (vec) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2), u = lane & 3, c = (p * 4 + u) * PER;
-            if (r < rows && c < cols) *(uint4 *)(out + r * ldc + c) = stage[r * 4 + (u ^ (r >> 1 & 3))];
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 2), u = lane & 3, c = (p * 4 + u) * PER;
+                if (r < rows && c < cols) *(uint4 *)(out + r * ldc + c) = stage[r * 4 + (u ^ (r >> 1 & 3))];
+            }
+        } else {
+            constexpr int ROW = 4 * PER, AT_ONCE = 32 / ROW;  // elements of a piece, rows of a store
+            const int r0 = lane / ROW, e = lane % ROW, u = e / PER, c = p * ROW + e;
+#pragma unroll 8
+            for (int r = r0; r < 32; r += AT_ONCE)
+                if (r < rows && c < cols)
+                    out[r * ldc + c] = ((const T *)(stage + r * 4 + (u ^ (r >> 1 & 3))))[e % PER];
         }
         __syncwarp();
     }
@@ -415,22 +425,10 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
                 const int m0 = tx * BM + (warp & 3) * 32;
                 const long long at = (long long)m0 * a.ldc + col;
                 uint4 *stage = (uint4 *)(smem + L::OUT) + (warp - 4) * 128;
-                if (a.vec && a.out_dtype == HV_BF16) {
-                    store_rows((__nv_bfloat16 *)a.out + at, a.ldc, a.x_rows - m0, a.y_rows - col, stage, acc);
-                } else if (a.vec && a.out_dtype == HV_F16) {
-                    store_rows((__half *)a.out + at, a.ldc, a.x_rows - m0, a.y_rows - col, stage, acc);
-                } else if (a.vec) {
-                    store_rows((float *)a.out + at, a.ldc, a.x_rows - m0, a.y_rows - col, stage, acc);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < HC / 2; ++j) {
-                        float v[2];
-                        split2(acc[j], v[0], v[1]);
-                        for (int e = 0; e < 2; ++e)
-                            if (m < a.x_rows && col + 2 * j + e < a.y_rows)
-                                put_any(a.out, a.out_dtype, (long long)m * a.ldc + col + 2 * j + e, v[e]);
-                    }
-                }
+                const int rows = a.x_rows - m0, cols = a.y_rows - col;
+                if (a.out_dtype == HV_BF16) store_rows((__nv_bfloat16 *)a.out + at, a.ldc, rows, cols, a.vec, stage, acc);
+                else if (a.out_dtype == HV_F16) store_rows((__half *)a.out + at, a.ldc, rows, cols, a.vec, stage, acc);
+                else store_rows((float *)a.out + at, a.ldc, rows, cols, a.vec, stage, acc);
 #pragma unroll
                 for (int j = 0; j < HC / 2; ++j) acc[j] = 0;
             }
