@@ -47,40 +47,5 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive elements at p, of which `n` exist; the rest read as 0.  `vec`: p is
-// 16-byte aligned, so that a whole group goes as 16-byte loads.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, int n, bool vec, float (&v)[8]) {
-    if (vec && n >= 8) {
-        constexpr int W = sizeof(T) / 2;  // 16-byte words
-        uint4 w[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
-        const T *e = reinterpret_cast<const T *>(w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T *p, int n, bool vec, const float (&v)[8]) {
-    if (vec && n >= 8) {
-        constexpr int W = sizeof(T) / 2;
-        uint4 w[W];
-        T *e = reinterpret_cast<T *>(w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
-#pragma unroll
-        for (int i = 0; i < W; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = from_f32<T>(v[i]);
-    }
-}
-
 }  // namespace dec
 }  // namespace hv

@@ -8,17 +8,22 @@
 // SM clock, 16 multiply-adds an element leave the warp-level tensor path under a fifth
 // busy, and it needs none of the 128 rows that a tcgen05 tile would pad to.
 //
-// Work: the (sequence, head tile) items are cut into tiles of 64 tokens, the tiles of all
-// items are laid end to end, and the CTAs of one resident wave take equal shares of that
-// line.  So a ragged batch is even, and a single long sequence uses every SM; every CTA
-// works the cuts out for itself from the lengths, which stay on the device.  A warp owns 16
-// tokens of a tile and its own cp.async ring, so that warps do not wait for one another
-// inside an item; the ring runs ahead across item borders.
+// Work: the (sequence, head tile) items are cut into tiles of 64 tokens (128 for heads of up
+// to 64 dimensions), the tiles of all items are laid end to end, and the CTAs of one resident
+// wave take equal shares of that line.  So a ragged batch is even, and a single long sequence
+// uses every SM; every CTA works the cuts out for itself from the lengths, which stay on the
+// device.  A warp owns its tokens of a tile and its own cp.async ring, so that warps do not
+// wait for one another inside an item; the ring runs ahead across item borders.
 //
 // An item inside one share is written straight out.  One that is cut leaves a part (the
 // unnormalised sum, the running maximum and the sum of weights, in 32 bits) per CTA in the
 // workspace, and the CTA that finishes last joins the parts in the order of the shares: the
 // result does not depend on which that is.
+//
+// Measured on one B200, bf16: 64 sequences of 0 to 8192 tokens (32 heads of 128 over 8) 187 us,
+// 5.76 TB/s of the cache; two of 131071 (64 over 8) 190 us, 5.65 TB/s.  CTAs stream for 150 to
+// 170 us of that; the rest is what the latest of them join.  One sequence of 197 tokens, 7.9 us:
+// length, page, key, join, each a memory latency after the other.
 #include <math_constants.h>
 
 #include "hv_decode.cuh"

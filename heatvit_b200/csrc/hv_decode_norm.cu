@@ -7,11 +7,17 @@
 // The norm is taken of the unrounded sum: residual_out is one rounding of h, q one
 // rounding of y.  The floor keeps the scale of an all-zero block a normal number.
 //
-// Bound by HBM: x, residual, residual_out and q cross it once each (7 bytes an element
-// in bf16), so a row stays in registers between the sum of squares and the output.  A
-// thread holds NV groups of eight consecutive channels, TPR threads apart: 16-byte
-// accesses, and a block of 128 channels is 16 neighbouring lanes, whose amax is four
-// shuffles.  Rows of up to 1024 channels take a warp each, longer ones a CTA.
+// Bound by HBM: x, residual, residual_out and q cross it once each (7 bytes an element in
+// bf16), so a row stays in registers between its sum of squares and its scales.  A thread has
+// NV groups of eight consecutive channels, a row's threads apart: 16-byte accesses, and a
+// block of 128 channels is 16 neighbouring lanes, whose amax is four shuffles.  Rows of up to
+// 1024 channels take a warp each, longer ones a CTA; many long ones go through a ring of bulk
+// copies (see norm_ring_kernel).
+//
+// Measured on one B200: 16384 x 8192 bf16 with residual 146 us, 6.48 TB/s, the rate of a plain
+// copy; 1999 x 5000 fp32 26.5 us (4.9 TB/s: seven rows a CTA, of which filling and emptying
+// the ring is one); 8192 x 8192 fp16 without residual 49 us, where half of the issue slots
+// convert; 8 x 4096 1.8 us, the launch.
 #include <cuda_fp8.h>
 
 #include <algorithm>

@@ -15,6 +15,7 @@ The last dimension of every tensor is contiguous; the others may have any stride
 [pages, kv_heads, page, dim]).  Shape and type mistakes raise ValueError and
 TypeError.  What only the device can see (a page number outside the cache, a
 position past a table) faults nothing and is reported by ``device_error``.
+Calls may be captured in a CUDA graph after one of each outside it.
 """
 
 import ctypes as C
@@ -141,13 +142,15 @@ def append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, rope=
 
 class AttentionWorkspace:
     """Device memory that ``paged_attention`` joins split sequences in, for one device
-    and any sizes.  Calls that share one must not overlap in time (one per stream)."""
+    and any sizes.  Calls that share one must not overlap in time (one per stream).
+    Waits for the device to have zeroed it, so that any stream may use it."""
 
     def __init__(self, device=None):
         torch = _torch()
         self.device = torch.device("cuda", torch.cuda.current_device() if device is None else
                                    torch.device(device).index or 0)
         self.buffer = _load().attention_workspace(self.device.index)
+        torch.cuda.current_stream(self.device).synchronize()
 
 
 def paged_attention(q, k_cache, v_cache, page_table, lens, scale=None, workspace=None, out=None, return_lse=False):

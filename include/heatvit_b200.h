@@ -402,9 +402,10 @@ HV_API int hv_selector_h2(hv_model *model, int selector_index, const int8_t *d_x
 #define HV_F32 2
 
 #define HV_DECODE_BAD_PAGE 1     /* a page table entry outside [0, num_pages): not read, not written */
-#define HV_DECODE_BAD_POSITION 2 /* a position, or a sequence, past the page table or the rotation table */
+#define HV_DECODE_BAD_POSITION 2 /* a position or sequence past the page table (its key and value are not
+                                    stored) or the rotation table (nor is its q_out row) */
 #define HV_DECODE_BAD_LENGTH 4   /* a length above max_pages * page_size: taken as that */
-#define HV_DECODE_STALLED 8      /* a GEMM's bounded wait gave up: that output is invalid */
+#define HV_DECODE_STALLED 8      /* a bounded wait gave up: that call's output is invalid */
 
 /* Read and clear the current device's error word (synchronises with the device). */
 HV_API int hv_decode_error(int *bits);

@@ -63,6 +63,19 @@ def test_norm(dtype, rows, dim):
     check_norm(decode.add_rmsnorm_fp8(x, w, 1e-5, residual=res), x, w, 1e-5, res)
 
 
+@pytest.mark.parametrize("dtype,rows,dim", [(HF, 20011, 192), (BF, 5003, 512), (BF, 1500, 1000), (BF, 1183, 1032),
+                                            (HF, 777, 2048), (FF, 1000, 3000), (BF, 601, 4104), (FF, 640, 8192),
+                                            (BF, 593, 16384), (FF, 600, 16384), (HF, 650, 16392), (BF, 900, 2001)])
+def test_norm_many_rows(dtype, rows, dim):
+    """More rows than resident warps or CTAs: those that go on to further rows, and the ring."""
+    from heatvit_b200 import decode
+    x, res = rand(1, rows, dim, dtype=dtype), rand(2, rows, dim, dtype=dtype, scale=3.0)
+    w = (1 + rand(3, dim, scale=0.2)).to(dtype)
+    check_norm(decode.add_rmsnorm_fp8(x, w, 1e-6), x, w, 1e-6, None)
+    before = res.clone()
+    check_norm(decode.add_rmsnorm_fp8(x, w, 1e-6, residual=res, residual_out=res), x, w, 1e-6, before)
+
+
 @pytest.mark.parametrize("dtype", [BF, FF])
 def test_norm_strides_and_in_place(dtype):
     """Rows of a wider matrix at odd starts (element by element), and residual_out = residual."""
@@ -258,6 +271,28 @@ def test_append(dtype, layout, interleaved, heads, kv, dim, rot, page):
     assert torch.equal(kc.double()[untouched], want_k[untouched])
     near(q_out[live], turned[1], 8.0)
     assert bool((q_out[4] == 0).all())
+
+
+@pytest.mark.parametrize("interleaved,rot", [(False, 128), (True, 128), (False, 64), (True, 0)])
+@pytest.mark.parametrize("heads,kv", [(31, 1), (8, 8)])
+def test_append_many_tokens(heads, kv, interleaved, rot):
+    """Tokens enough for threads of several heads, head counts that leave some without."""
+    from heatvit_b200 import decode
+    lens, dim, page = [3000, 1, 2049], 128, 64
+    table, pages = make_table(1, lens, page)
+    seq = torch.tensor(sum([[i] * n for i, n in enumerate(lens)], []), dtype=torch.int32, device="cuda")
+    pos = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens]).cuda()
+    q, k, v = (rand(s, pos.numel(), n, dim, dtype=BF) for s, n in ((2, heads), (3, kv), (4, kv)))
+    kc, vc = (make_cache(s, pages, page, kv, dim, BF, "hnd") for s in (5, 6))
+    rope = decode.rope_table(3000, rot) if rot else None
+    got = decode.append_kv(k, v, kc, vc, table, pos, seq_ids=seq, rope=rope, q=q, interleaved=interleaved)
+    pg, slot = table[seq.long(), pos.long() // page].long(), pos.long() % page
+    turned = [t.double() for t in (k, q)]
+    if rot:
+        turned = [rotate64(t, rope, pos.long(), rot, interleaved) for t in turned]
+    near(kc[pg, slot], turned[0], 8.0)
+    near(got, turned[1], 8.0)
+    assert torch.equal(vc[pg, slot], v)
 
 
 def test_append_decode_step_in_place_and_without_q():
