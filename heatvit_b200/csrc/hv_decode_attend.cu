@@ -38,6 +38,10 @@ constexpr int ROWS = 16, BLOCK = 16, SLICES = 4;
 // Tiles: a part costs more than the loads of fewer.  One sequence of 1000 tokens, heads of 128: 10.3
 // us with one, 10.7 with two, 13.0 with four; one of 197, heads of 64: 9.1, 8.2, 11.8.
 constexpr int MIN_SHARE = 2;
+// Tiles that a share may grow by so that items of one length end where shares do and none is cut.
+// 32 sequences of 512 tokens (32 heads of 128 over 8; shares of 7, items of 8) 24.8 -> 20.8 us, 64
+// of 512 (14, 16) 38.5 -> 34.0.  By four, 16 of 512 (4, 8) would go from 16.0 to 18.9.
+constexpr int SLACK = 2;
 constexpr int FAN = 16;       // parts whose loads a joining CTA has in flight together
 // A further FAN parts cost a joining CTA about 1.5 us, a second level about 7.
 constexpr int ONE_LEVEL = 4 * FAN, GROUP = FAN;
@@ -305,14 +309,26 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
     if (warp == 0) {
         long long total = 0;
         int held = 0;  // this lane's sequence of the last 32
+        int most = 0, live = 0;  // the longest of this lane's sequences, and how many have tokens
         for (int b0 = 0; b0 < a.seqs; b0 += 32) {
             const int b = b0 + lane;
             held = b < a.seqs ? (length_of(a, b) + TILE - 1) / TILE : 0;
             total += __reduce_add_sync(~0u, held);
+            most = max(most, held);
+            live += held > 0;
         }
+        const long long tiles = total;
         total *= items;
         long long share = (total + gridDim.x - 1) / gridDim.x;
-        if (share < MIN_SHARE) share = MIN_SHARE;
+        if (share <= MIN_SHARE) {
+            share = MIN_SHARE;
+        } else {
+            most = __reduce_max_sync(~0u, most);
+            if (tiles == (long long)most * __reduce_add_sync(~0u, live)) {
+                const long long whole = share <= most ? most : (share + most - 1) / most * most;
+                if (whole - share <= SLACK) share = whole;
+            }
+        }
         const long long first = share * blockIdx.x;
         long long before = 0;  // tiles of the sequences ahead of b0
         int found = -1;

@@ -406,6 +406,14 @@ def test_attention_lengths(lens):
     check_attention(q, kc, vc, table, lens)
 
 
+@pytest.mark.parametrize("lens", [[512] * 32, [470, 0, 512, 449] * 11, [1024] * 40 + [0] * 5, [150] * 75 + [600]])
+def test_attention_lengths_of_as_many_tiles(lens):
+    """Items of one size, whose borders the cuts are moved to, among empty rows; one that differs."""
+    q, kc, vc, table = attend_case(5, lens, 32, 8, 128, 16, BF, "nhd")
+    out = check_attention(q, kc, vc, table, lens)
+    assert bool((out[torch.tensor(lens, device="cuda") == 0] == 0).all())
+
+
 def test_attention_scale_and_wide_scores():
     """Scores over hundreds: the running maximum moves, and weights underflow to zero."""
     lens = [777, 64]
