@@ -138,14 +138,20 @@ __device__ __forceinline__ void put_q(const NormArgs &a, long long row, int c, i
             if (j < n) q[j] = (uint8_t)(b[j >> 2] >> (8 * (j & 3)));
     }
 }
+// The larger, or a NaN where either is one (fmaxf would drop it): the NaN then reaches the scale.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
 // A block's amax: 16 neighbouring lanes hold its 128 channels, and every lane of the warp
 // takes part.
 __device__ __forceinline__ float block_amax(const float (&y)[8]) {
     float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(y[j]));
+    for (int j = 0; j < 8; ++j) m = max_or_nan(m, fabsf(y[j]));
 #pragma unroll
-    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    for (int o = 8; o; o >>= 1) m = max_or_nan(m, __shfl_xor_sync(~0u, m, o));
     return m;
 }
 // A row's 1 / rms cancels in y / scale, so q goes out before the row's sum is known:
@@ -187,7 +193,7 @@ __device__ __forceinline__ void put_scales(const NormArgs &a, long long row, int
             if (k == i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] = h[k][j] * rstd * to_f32(w[k].e[j]);
-        const float top = fmaxf(block_amax(y), kAmaxFloor);
+        const float top = max_or_nan(block_amax(y), kAmaxFloor);
         put_q<FULL>(a, row, c, a.dim - c, y, kE4m3Max / top);
         if ((t & 15) == 0 && c < a.dim) a.scale[row * a.scale_row + (c >> 7) * a.scale_group] = top * (1.f / kE4m3Max);
     }

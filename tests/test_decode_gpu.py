@@ -110,6 +110,21 @@ def test_norm_extreme_rows():
         assert torch.equal(r.scale[i], clean_rows.scale[i])
 
 
+@pytest.mark.parametrize("rows,dim", [(6, 384), (5, 1500), (700, 2048)])
+def test_norm_nan_reaches_scale(rows, dim):
+    """As in the formula, a NaN makes its block's scale and every q of the block a NaN, and no other block's."""
+    from heatvit_b200 import decode
+    x, w = rand(1, rows, dim), torch.ones(dim, device="cuda")
+    x[3, 5], x[4, 6] = math.nan, math.inf
+    w[300] = math.nan
+    r = decode.add_rmsnorm_fp8(x, w, 1e-6)
+    y = x.double() * torch.rsqrt((x.double() ** 2).mean(1, keepdim=True) + 1e-6) * w.double()
+    g = -(-dim // 128)
+    amax = torch.nn.functional.pad(y, (0, g * 128 - dim)).view(rows, g, 128).abs().amax(2)
+    assert torch.equal(r.scale.isnan(), amax.isnan())
+    assert torch.equal(r.q.float().isnan(), amax.isnan().repeat_interleave(128, 1)[:, :dim])
+
+
 # ---- GEMM ---------------------------------------------------------------------------
 
 def e4m3(seed, rows, k, pad=0):
