@@ -35,6 +35,9 @@ namespace {
 using namespace dec;
 
 constexpr int ROWS = 16, BLOCK = 16, SLICES = 4;
+// A running maximum before the first score.  Finite, so that a score of -inf (a product out of
+// range) weighs exp2(-inf) = 0 and not NaN; a NaN passes every maximum and shows in the sums.
+constexpr float LOWEST = -3.402823466e38f;
 // Tiles: a part costs more than the loads of fewer.  One sequence of 1000 tokens, heads of 128: 10.3
 // us with one, 10.7 with two, 13.0 with four; one of 197, heads of 64: 9.1, 8.2, 11.8.
 constexpr int MIN_SHARE = 2;
@@ -199,7 +202,7 @@ __device__ __forceinline__ void join_parts(float *parts, float *sum, float *stat
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const int k = (tid + e * THREADS) / ROWS, r = tid % ROWS;
-            v[e] = k < m && r < nrows ? __ldcg(pst + slot(k0 + k) * ROWS + r) : make_float2(-CUDART_INF_F, 0.f);
+            v[e] = k < m && r < nrows ? __ldcg(pst + slot(k0 + k) * ROWS + r) : make_float2(LOWEST, 0.f);
         }
         float4 x[FAN];
         auto fetch = [&](int t) {
@@ -216,7 +219,7 @@ __device__ __forceinline__ void join_parts(float *parts, float *sum, float *stat
         }
         __syncthreads();
         if (tid < ROWS) {  // weights of the parts of row `tid`
-            const float was = k0 ? stat[2 * tid] : -CUDART_INF_F;
+            const float was = k0 ? stat[2 * tid] : LOWEST;
             float M = was;
             for (int k = 0; k < m; ++k) M = fmaxf(M, sum[k * ROWS + tid]);
             const float f = k0 ? exp2_(was - M) : 0.f;
@@ -482,7 +485,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 }
 #pragma unroll
             for (int j = 0; j < DH / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-            m[0] = m[1] = -CUDART_INF_F;
+            m[0] = m[1] = LOWEST;
             l[0] = l[1] = 0.f;
             fresh = false;
         }
@@ -598,9 +601,9 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
             float f[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float top = -CUDART_INF_F;
+                float top = LOWEST;
                 for (int w = 0; w < SLICES; ++w) top = fmaxf(top, stat[(w * ROWS + (lane >> 2) + 8 * i) * 2]);
-                f[i] = m[i] == -CUDART_INF_F ? 0.f : exp2_(m[i] - top);
+                f[i] = exp2_(m[i] - top);
             }
             float *mine = (float *)(ring + (u % L::STAGES) * L::STAGE);  // read, and not yet refilled
 #pragma unroll
@@ -609,14 +612,12 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 for (int i = 0; i < 2; ++i)
                     *(float2 *)(mine + ((lane >> 2) + 8 * i) * L::PART_ROW + j * 8 + (lane & 3) * 2) =
                         make_float2(o[j][2 * i] * f[i], o[j][2 * i + 1] * f[i]);
-            float M = -CUDART_INF_F, S = 0.f;
+            float M = LOWEST, S = 0.f;
             float *of_row = stat + SLICES * ROWS * 2;
             if (tid < ROWS) {  // a row's maximum and sum
                 for (int w = 0; w < SLICES; ++w) M = fmaxf(M, stat[(w * ROWS + tid) * 2]);
-                for (int w = 0; w < SLICES; ++w) {
-                    const float mw = stat[(w * ROWS + tid) * 2];
-                    if (mw != -CUDART_INF_F) S += stat[(w * ROWS + tid) * 2 + 1] * exp2_(mw - M);
-                }
+                for (int w = 0; w < SLICES; ++w)
+                    S += stat[(w * ROWS + tid) * 2 + 1] * exp2_(stat[(w * ROWS + tid) * 2] - M);
                 of_row[tid * 2 + 1] = S;
             }
             __syncthreads();

@@ -438,6 +438,34 @@ def test_attention_scale_and_wide_scores():
     check_attention(q, kc, vc, table, lens, scale=0.0)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,dead", [(40, 33), (700, 640), (30000, 12000)])
+def test_attention_scores_out_of_range(dim, n, dead):
+    """Leading tokens whose scores are -inf weigh nothing, as in the formula; all of them: a NaN, and lse -inf.
+    A NaN in q is its head's alone, in the output and lse."""
+    from heatvit_b200 import decode
+    lens = [n, n, n]
+    q, kc, vc, table = attend_case(6, lens, 4, 2, dim, 16, BF, "nhd")
+    t = torch.arange(n, device="cuda")
+    for b, stop in ((0, dead), (1, n)):
+        at = t[:stop]
+        kc[table[b, at // 16].long(), at % 16] = -1e30
+    q[:2], q[2, 1, 3] = 1e30, math.nan
+    rest = torch.arange(dead, n, device="cuda")
+    kc[table[0, rest // 16].long(), rest % 16] = 0.0  # scores of 0: the mean of the values
+    out, lse = decode.paged_attention(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                                      return_lse=True)
+    v = vc[table[0, rest // 16].long(), rest % 16].double().repeat_interleave(2, 1)  # [tokens, heads, dim]
+    want, size = v.mean(0), v.abs().mean(0)
+    # equal weights of one are exact, their sum too; the product's sum and the one rounding are not
+    assert bool(((out[0].double() - want).abs() <= want.abs() * 2.0 ** -8 + size * 2.0 ** -14).all())
+    assert bool(((lse[0].double() - math.log(n - dead)).abs() <= 1e-5).all())
+    assert bool(out[1].isnan().all()) and bool((lse[1] == -math.inf).all())
+    assert bool(out[2, 1].isnan().all()) and bool(lse[2, 1].isnan())
+    others = [0, 2, 3]
+    assert bool(out[2, others].isfinite().all()) and bool(lse[2, others].isfinite().all())
+
+
 def test_attention_strided_q_and_out():
     """q as a slice of a projection at an odd place, out as every other row of a larger buffer."""
     from heatvit_b200 import decode
