@@ -102,6 +102,14 @@ Tensor padded_rows(int64_t rows, int64_t dim, int64_t by, at::ScalarType type, c
     return empty({rows, wide}, type, like).narrow(1, 0, dim);
 }
 
+// A tensor of `size` and `strides` in the storage of `bytes`, from byte `at` (a multiple of an element).
+Tensor within(const Tensor &bytes, int64_t at, c10::IntArrayRef size, c10::IntArrayRef strides, at::ScalarType type) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(),
+                                                        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(size, strides, at / (int64_t)c10::elementSize(type));
+    return t;
+}
+
 // Around a function's body: no C++ exception passes into Python.
 #define BEGIN        \
     HANDLE_TH_ERRORS \
@@ -150,8 +158,12 @@ PyObject *add_rmsnorm_fp8(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
         throw ValueError("residual_out without a residual");
     }
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-    Tensor q = padded_rows(rows, dim, 16, at::kFloat8_e4m3fn, x);
-    Tensor scale = at::detail::empty_strided_cuda({rows, groups}, {1, rows}, at::kFloat, x.device());
+    // q and its scales are used together, so they share a storage: an allocation less is 0.5 us
+    // of a call of 6.
+    const int64_t wide = (dim + 15) / 16 * 16, scale_at = (rows * wide + 255) / 256 * 256;
+    const Tensor both = empty({scale_at + rows * groups * 4}, at::kByte, x);
+    Tensor q = within(both, 0, {rows, dim}, {wide, 1}, at::kFloat8_e4m3fn);
+    Tensor scale = within(both, scale_at, {rows, groups}, {1, rows}, at::kFloat);
     hv_norm_args a{};
     a.d_x = x.data_ptr(), a.d_weight = w.data_ptr(), a.d_q = q.data_ptr(), a.d_scale = scale.data_ptr<float>();
     a.rows = rows, a.x_stride = x.stride(0), a.q_stride = q.stride(0);

@@ -78,8 +78,9 @@ def add_rmsnorm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None):
     ``q = e4m3(y / scale)``.  x and residual [rows, dim] and weight [dim] share one of
     bfloat16, float16, float32; ``residual_out`` (a new tensor unless given, and it may
     be ``residual``) receives h rounded to that type.  q's row stride is a multiple of 16 and
-    scale is stored group by group, both as ``gemm_fp8`` reads them best; a new residual's
-    row stride is a multiple of 8, since rows that start on 16 bytes go faster."""
+    scale is stored group by group, both as ``gemm_fp8`` reads them best, and they share a
+    storage; a new residual's row stride is a multiple of 8, since rows that start on 16
+    bytes go faster."""
     q, scale, out = _done((_native or _load()).add_rmsnorm_fp8(x, weight, eps, residual, residual_out))
     return Fp8Rows(q, scale, out)
 
