@@ -23,8 +23,8 @@
 // takes 455 us, with one MMA in four 325: its operands come at 70 bytes an SM clock.  Tiles of
 // 256 x 256 over CTA pairs (cta_group::2) move a third less and took as long (536 us, 648 at the
 // power limit), an accumulator's way to the other CTA and back being longer.  48 x 10240 x 4096
-// 15.4 us (2.8 TB/s of weights: five to the first sums, six to stream, four to join), 1 x 4096 x
-// 4096 7.4 us, 1576 x 768 x 192 4.6 us.
+// 15.0 us (2.9 TB/s of weights: five to the first sums, six to stream, four to join), 1 x 4096 x
+// 4096 6.9 us, 1576 x 768 x 192 4.6 us.
 //
 // Every mbarrier wait is bounded: after a timeout the CTA waits for what it has in flight,
 // releases its TMEM and sets the device's error word.
@@ -60,7 +60,7 @@ template <int BN, bool SWAP>
 struct Lay {
     static constexpr int A_ST = BM * GK, B_ST = BN * GK, STAGE = A_ST + B_ST;
     static constexpr int PER_SM = SWAP ? 2 : 1;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : BN == 64 ? 4 : BN == 32 ? 5 : 6;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : BN == 64 ? 3 : BN == 32 ? 4 : 5;
     static constexpr int BUFS = BN == 256 ? 2 : 4;  // TMEM accumulators
     static constexpr int COLS = BN < 32 ? 32 : BN;  // TMEM columns of one
     static constexpr int TMEM = BUFS * COLS;
@@ -68,7 +68,8 @@ struct Lay {
     static constexpr int SCALES = SWAP ? BN : 2 * BM;
     static constexpr int SC = STAGES * STAGE;  // [2][SB][SCALES] float
     static constexpr int OUT = SC + 2 * SB * SCALES * 4;  // 2 KB an adding warp (see store_rows)
-    static constexpr int BARS = OUT + (SWAP ? 0 : EPI_WARPS * 2048);
+    // SWAP: the cluster's sums of this CTA's share of the output's rows (a third of BN rounds up to two more in all)
+    static constexpr int BARS = OUT + (SWAP ? (BN + 2) * BM * 4 : EPI_WARPS * 2048);
     static constexpr int BYTES = BARS + 256 + 1024;  // and room to align the ring to 1024
     static_assert(PER_SM * TMEM <= 512 && PER_SM * (BYTES + 1024) <= 228 * 1024, "resident CTAs");
 };
@@ -138,8 +139,16 @@ __device__ __forceinline__ void put4_any(const GemmFp8Args &a, long long i, int 
     else if (a.out_dtype == HV_F16) put4((__half *)a.out + i, a.vec, n, v);
     else put4((float *)a.out + i, a.vec, n, v);
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
+}
+__device__ __forceinline__ void st_peer(uint32_t saddr, uint32_t rank, float v) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(saddr), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(a), "f"(v) : "memory");
 }
 __device__ __forceinline__ float4 ld_peer(uint32_t saddr, uint32_t rank) {
     uint32_t a;
@@ -266,6 +275,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
     tc05::fence_before();
     __syncthreads();
     tc05::fence_after();
+    if (SWAP && split > 1) cluster_arrive();  // the others may write to this CTA's memory from now on
     griddep_wait();
     griddep_launch();
     const uint32_t tmem = tslot;
@@ -443,11 +453,46 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
         }
     }
 
-    if (BN < 256 && split > 1) {
+    if (SWAP && split > 1) {
+        // Each rank has a share of the output's rows (the tokens), and the others send it their sums
+        // of those as they finish: one cluster barrier and no remote reads (1 x 4096 x 4096 7.3 ->
+        // 6.9 us, 8 x 1024 x 16384 10.7 -> 10.2).
+        int tx, ty;
+        tile_at(first, a.tiles_x, a.tiles_y, tx, ty);
+        const int cols = min(BN, a.y_rows - ty * BN), per = (cols + split - 1) / split;
+        float *sums = (float *)(smem + L::OUT);  // [split][per][BM]
+        __syncwarp();
+        cluster_wait();  // every CTA has begun
+        if (warp >= 4) {
+            int owner = c0 / per, in = c0 - owner * per;
+#pragma unroll
+            for (int j = 0; j < HC / 2; ++j) {
+                float v[2];
+                split2(acc[j], v[0], v[1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (c0 + 2 * j + e < cols)
+                        st_peer(tc05::smem_u32(sums + (rank * per + in) * BM + row), owner, v[e]);
+                    if (++in == per) in = 0, ++owner;
+                }
+            }
+        }
+        cluster_sync();
+        const int from = rank * per, share = min(per, cols - from);
+        for (int i = tid; i < share * (BM / 4); i += THREADS) {
+            const int p = i / (BM / 4), q = i % (BM / 4) * 4;
+            float4 v = *(const float4 *)(sums + p * BM + q);
+            for (int k = 1; k < split; ++k) {
+                const float4 x = *(const float4 *)(sums + (k * per + p) * BM + q);
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+            }
+            put4_any(a, (ty * BN + from + p) * a.ldc + tx * BM + q, a.x_rows - tx * BM - q, v);
+        }
+    } else if (BN < 256 && split > 1) {
         // Every copy and product of this CTA has completed (or its waits gave up and were
-        // drained): the ring's memory takes the sums, along the output's rows.
-        constexpr int ALONG = SWAP ? BM : BN, ACROSS = SWAP ? BN : BM, LD = ALONG + 4;
-        static_assert(BN == 256 || ACROSS * LD * 4 <= L::SC, "the sums fit where the ring was");
+        // drained): the ring's memory takes the sums.
+        constexpr int LD = BN + 4;
+        static_assert(BN == 256 || BM * LD * 4 <= L::SC, "the sums fit where the ring was");
         float *part = (float *)smem;
         __syncthreads();
         if (warp >= 4)
@@ -456,33 +501,24 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
                 float4 v;
                 split2(acc[j], v.x, v.y);
                 split2(acc[j + 1], v.z, v.w);
-                const int c = c0 + 2 * j;
-                if (SWAP) {
-                    part[c * LD + row] = v.x;
-                    part[(c + 1) * LD + row] = v.y;
-                    part[(c + 2) * LD + row] = v.z;
-                    part[(c + 3) * LD + row] = v.w;
-                } else {
-                    *(float4 *)(part + row * LD + c) = v;
-                }
+                *(float4 *)(part + row * LD + c0 + 2 * j) = v;
             }
         cluster_sync();
         int tx, ty;
         tile_at(first, a.tiles_x, a.tiles_y, tx, ty);
         // Each rank has a share of the output's rows, four neighbouring elements a thread.
-        const int per = (ACROSS + split - 1) / split, from = rank * per, share = min(per, ACROSS - from);
-        const int p0 = SWAP ? ty * BN : tx * BM, q0 = SWAP ? tx * BM : ty * BN;
-        const int p_end = SWAP ? a.y_rows : a.x_rows, q_end = SWAP ? a.x_rows : a.y_rows;
+        const int per = (BM + split - 1) / split, from = rank * per, share = min(per, BM - from);
 #pragma unroll 2
-        for (int i = tid; i < share * (ALONG / 4); i += THREADS) {
-            const int p = from + i / (ALONG / 4), q = i % (ALONG / 4) * 4;
+        for (int i = tid; i < share * (BN / 4); i += THREADS) {
+            const int p = from + i / (BN / 4), q = i % (BN / 4) * 4;
             const uint32_t at = tc05::smem_u32(part + p * LD + q);
             float4 v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = k < split ? ld_peer(at, k) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 1; k < 8; ++k) v[0].x += v[k].x, v[0].y += v[k].y, v[0].z += v[k].z, v[0].w += v[k].w;
-            if (p0 + p < p_end) put4_any(a, (p0 + p) * a.ldc + q0 + q, q_end - q0 - q, v[0]);
+            if (tx * BM + p < a.x_rows)
+                put4_any(a, (tx * BM + p) * a.ldc + ty * BN + q, a.y_rows - ty * BN - q, v[0]);
         }
         cluster_sync();  // no CTA leaves while its sums may be read
     }
@@ -548,8 +584,9 @@ cudaLaunchConfig_t config(unsigned grid, int split, cudaStream_t st, cudaLaunchA
 // How many ways K is split: the most of 2, 3, 4 and 8 that leaves every cluster resident at once
 // and a CTA two groups.  (A second wave of clusters costs more than it saves: 512 x 4096 x 4096
 // took 19 us unsplit and 284 split eight ways.  Five or six shares of 1 x 4096 x 4096 took 7.5
-// us, four 6.8; of 48 x 10240 x 4096 one took 20 us, two 17.6, three 15.8.)  How many clusters a device holds is asked once; the answer counts one
-// CTA an SM for kernels with tensor memory, of which PER_SM fit.
+// us, four 6.8; of 48 x 10240 x 4096 one took 20 us, two 17.6, three 15.8.)  How many clusters a
+// device holds is asked once; the answer counts one CTA an SM for kernels with tensor memory, of
+// which PER_SM fit.
 template <int BN, bool SWAP>
 int split_of(int64_t tiles, int groups) {
     static std::atomic<int> held[64][9];  // clusters of each size, plus one
