@@ -275,7 +275,8 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
     tc05::fence_before();
     __syncthreads();
     tc05::fence_after();
-    if (SWAP && split > 1) cluster_arrive();  // the others may write to this CTA's memory from now on
+    if (SWAP && split > 1)  // the others may write to this CTA's memory from now on
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n");
     griddep_wait();
     griddep_launch();
     const uint32_t tmem = tslot;
