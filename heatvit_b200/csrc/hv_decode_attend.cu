@@ -45,6 +45,16 @@ constexpr int MIN_SHARE = 2;
 // 32 sequences of 512 tokens (32 heads of 128 over 8; shares of 7, items of 8) 24.8 -> 20.8 us, 64
 // of 512 (14, 16) 38.5 -> 34.0.  By four, 16 of 512 (4, 8) would go from 16.0 to 18.9.
 constexpr int SLACK = 2;
+// A row's weights are taken beside a reference that makes its largest 2^TOP when it is set, and that moves
+// when one passes it by more than 2^SOFT.  fp16 has normal numbers from 2^-14 to 2^15 and none under 2^-24: its
+// weights begin at 2^9, so that those of a long tail, each 2^-23 of one large weight, keep their bits, and those
+// under 2^-34 of it are lost (with TOP = 0, weights 16 nats under one had a single bit left).  bf16 has the
+// range of the 32-bit weights.
+template <typename T>
+constexpr float TOP = 0.f;
+template <>
+constexpr float TOP<__half> = 9.f;
+constexpr float SOFT = 6.f;
 constexpr int FAN = 16;       // parts whose loads a joining CTA has in flight together
 // A further FAN parts cost a joining CTA about 1.5 us, a second level about 7.
 constexpr int ONE_LEVEL = 4 * FAN, GROUP = FAN;
@@ -137,6 +147,16 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
 __device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *(uint32_t *)&v;
+}
+
+// What a rounded pair of weights leaves of (lo, hi), rounded in turn: the two together are
+// within 2^-16 of a weight (bf16; fp16 2^-22).
+__device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t p, __nv_bfloat16 t) {
+    return pack(lo - __uint_as_float(p << 16), hi - __uint_as_float(p & 0xffff0000u), t);
+}
+__device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t p, __half t) {
+    const float2 v = __half22float2(*(const __half2 *)&p);
+    return pack(lo - v.x, hi - v.y, t);
 }
 
 // Live tokens of sequence b: never beyond what its page table row can name.
@@ -283,12 +303,15 @@ __device__ __forceinline__ bool comes_last(uint32_t *counter, uint32_t of, long 
     return last;
 }
 
-template <typename T, int D>
+// HALF: items of up to eight heads.  Their weights take eight rows of the second product, and
+// the other eight take what rounding left of those (see there).
+template <typename T, int D, bool HALF>
 __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
     attend_kernel(const __grid_constant__ AttendArgs a) {
     griddep_wait();
     griddep_launch();
     using L = Lay<D>;
+    constexpr int NR = HALF ? 1 : 2;  // rows of a thread: lane / 4 + 8 i
     constexpr int DH = L::DH, THREADS = L::THREADS, BLOCKS = L::BLOCKS, WTOK = L::WTOK, TILE = L::TILE;
     using Place = Place<L::TILE>;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -468,7 +491,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
 
     uint32_t qf[DH / 16][4];
     float o[DH / 8][4];
-    float m[2], l[2];
+    float m[NR], l[NR];
     bool fresh = true;
     for (int u = 0; u < count; ++u) {
         const int head = cur.h / a.head_tiles, ht = cur.h - head * a.head_tiles;
@@ -481,12 +504,12 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = (lane >> 2) + (i & 1) * 8, c = half * DH + j * 16 + (lane & 3) * 2 + (i >> 1) * 8;
-                    qf[j][i] = r < nrows ? load_pair(q + r * a.q_head + c, a.q_pairs) : 0;
+                    qf[j][i] = (i & 1) < NR && r < nrows ? load_pair(q + r * a.q_head + c, a.q_pairs) : 0;
                 }
 #pragma unroll
             for (int j = 0; j < DH / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-            m[0] = m[1] = LOWEST;
-            l[0] = l[1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NR; ++i) m[i] = LOWEST, l[i] = 0.f;
             fresh = false;
         }
         asm volatile("cp.async.wait_group %0;\n" ::"n"(L::STAGES - 2) : "memory");
@@ -521,29 +544,29 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
 #pragma unroll
             for (int n = 0; n < 2 * BLOCKS; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] *= a.scale_log2;
+                for (int e = 0; e < 2 * NR; ++e) s[n][e] *= a.scale_log2;
             if (t0 + WTOK > cur.len)
 #pragma unroll
                 for (int n = 0; n < 2 * BLOCKS; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
+                    for (int e = 0; e < 2 * NR; ++e)
                         if (t0 + n * 8 + (lane & 3) * 2 + (e & 1) >= cur.len) s[n][e] = -CUDART_INF_F;
-            // The reference of the weights moves only when a maximum passes it by more than 2^6:
-            // until then weights are at most 64, exact powers apart from what they would be.
-            float x[2];
+            float x[NR];
+            bool moves = false;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < NR; ++i) {
                 x[i] = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
 #pragma unroll
                 for (int n = 1; n < 2 * BLOCKS; ++n) x[i] = fmaxf(x[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
                 x[i] = fmaxf(x[i], __shfl_xor_sync(~0u, x[i], 1));
                 x[i] = fmaxf(x[i], __shfl_xor_sync(~0u, x[i], 2));
+                moves |= x[i] > m[i] + (TOP<T> + SOFT);
             }
-            if (__any_sync(~0u, x[0] > m[0] + 6.f || x[1] > m[1] + 6.f)) {
-                float f[2];
+            if (__any_sync(~0u, moves)) {
+                float f[NR];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    x[i] = fmaxf(x[i], m[i]);
+                for (int i = 0; i < NR; ++i) {
+                    x[i] = fmaxf(x[i] - TOP<T>, m[i]);
                     f[i] = exp2_(m[i] - x[i]);
                     m[i] = x[i];
                     l[i] *= f[i];
@@ -552,24 +575,29 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 for (int j = 0; j < DH / 8; ++j) {
                     o[j][0] *= f[0];
                     o[j][1] *= f[0];
-                    o[j][2] *= f[1];
-                    o[j][3] *= f[1];
+                    o[j][2] *= f[NR - 1];
+                    o[j][3] *= f[NR - 1];
                 }
             }
 #pragma unroll
             for (int n = 0; n < 2 * BLOCKS; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 2 * NR; ++e) {
                     s[n][e] = exp2_(s[n][e] - m[e >> 1]);
                     l[e >> 1] += s[n][e];
                 }
-            // weights in T for the product: each is within 2^-9 (bf16) of its 32-bit value,
-            // as the values that it multiplies are of theirs; the sums stay in 32 bits
+            // A weight goes into the product as two numbers of type T, the rounded one and what that
+            // leaves: rounded alone, weights that are alike would all be off the same way, by up to 2^-8
+            // (bf16), against a sum that is not.  With up to eight heads the second ones take the rows
+            // that no head has, with more a product of their own (64 heads over 4, 64 x 4000 tokens: 99 us
+            // without it, 103 with).
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
                 const float(&x)[4] = s[2 * b], (&y)[4] = s[2 * b + 1];
-                const uint32_t p[4] = {pack(x[0], x[1], T()), pack(x[2], x[3], T()), pack(y[0], y[1], T()),
-                                       pack(y[2], y[3], T())};
+                const uint32_t x0 = pack(x[0], x[1], T()), y0 = pack(y[0], y[1], T());
+                const uint32_t x0r = pack_rest(x[0], x[1], x0, T()), y0r = pack_rest(y[0], y[1], y0, T());
+                const uint32_t x1 = HALF ? x0r : pack(x[2], x[3], T()), y1 = HALF ? y0r : pack(y[2], y[3], T());
+                const uint32_t p[4] = {x0, x1, y0, y1};
                 const uint32_t va = vb + (b * BLOCK + (lane & 15)) * L::ROW + (lane >> 4) * 16;
 #pragma unroll
                 for (int j = 0; j < DH / 16; ++j) {
@@ -577,6 +605,11 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                     ldsm4t(va + j * 32, r);
                     mma<T>(o[2 * j], p, r[0], r[1]);
                     mma<T>(o[2 * j + 1], p, r[2], r[3]);
+                    if constexpr (!HALF) {
+                        const uint32_t d[4] = {x0r, pack_rest(x[2], x[3], x1, T()), y0r, pack_rest(y[2], y[3], y1, T())};
+                        mma<T>(o[2 * j], d, r[0], r[1]);
+                        mma<T>(o[2 * j + 1], d, r[2], r[3]);
+                    }
                 }
             }
         }
@@ -588,7 +621,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
             // Join the slices of tokens: rows' maxima, then the sums in the order of the slices.
             if (L::HALVES == 2) __syncthreads();  // the scores that were exchanged last have been read
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < NR; ++i) {
                 l[i] += __shfl_xor_sync(~0u, l[i], 1);
                 l[i] += __shfl_xor_sync(~0u, l[i], 2);
                 if ((lane & 3) == 0 && half == 0) {
@@ -598,23 +631,25 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
                 }
             }
             __syncthreads();
-            float f[2];
+            float f[NR];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < NR; ++i) {
                 float top = LOWEST;
                 for (int w = 0; w < SLICES; ++w) top = fmaxf(top, stat[(w * ROWS + (lane >> 2) + 8 * i) * 2]);
                 f[i] = exp2_(m[i] - top);
             }
             float *mine = (float *)(ring + (u % L::STAGES) * L::STAGE);  // read, and not yet refilled
 #pragma unroll
-            for (int j = 0; j < DH / 8; ++j)
+            for (int j = 0; j < DH / 8; ++j) {
+                if (HALF) o[j][0] += o[j][2], o[j][1] += o[j][3];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < NR; ++i)
                     *(float2 *)(mine + ((lane >> 2) + 8 * i) * L::PART_ROW + j * 8 + (lane & 3) * 2) =
                         make_float2(o[j][2 * i] * f[i], o[j][2 * i + 1] * f[i]);
+            }
             float M = LOWEST, S = 0.f;
             float *of_row = stat + SLICES * ROWS * 2;
-            if (tid < ROWS) {  // a row's maximum and sum
+            if (tid < 8 * NR) {  // a row's maximum and sum
                 for (int w = 0; w < SLICES; ++w) M = fmaxf(M, stat[(w * ROWS + tid) * 2]);
                 for (int w = 0; w < SLICES; ++w)
                     S += stat[(w * ROWS + tid) * 2 + 1] * exp2_(stat[(w * ROWS + tid) * 2] - M);
@@ -694,23 +729,27 @@ int wave(int d) {
     return grid < MAX_GRID ? grid : MAX_GRID;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool HALF>
 cudaError_t launch(const AttendArgs &a, int grid, cudaStream_t st) {
     static std::atomic<uint64_t> ready;
-    const cudaError_t e = allow_shared(attend_kernel<T, D>, ready);
+    const cudaError_t e = allow_shared(attend_kernel<T, D, HALF>, ready);
     if (e != cudaSuccess) return e;
-    return launch_pdl(attend_kernel<T, D>, dim3((unsigned)grid), dim3(Lay<D>::THREADS), Lay<D>::BYTES, st, a);
+    return launch_pdl(attend_kernel<T, D, HALF>, dim3((unsigned)grid), dim3(Lay<D>::THREADS), Lay<D>::BYTES, st, a);
+}
+template <typename T, int D>
+cudaError_t by_group(const AttendArgs &a, int grid, cudaStream_t st) {
+    return a.group <= ROWS / 2 ? launch<T, D, true>(a, grid, st) : launch<T, D, false>(a, grid, st);
 }
 
 template <typename T>
 cudaError_t by_dim(const AttendArgs &a, int dim, int grid, cudaStream_t st) {
     switch (dim) {
-        case 32: return launch<T, 32>(a, grid, st);
-        case 64: return launch<T, 64>(a, grid, st);
-        case 96: return launch<T, 96>(a, grid, st);
-        case 128: return launch<T, 128>(a, grid, st);
-        case 192: return launch<T, 192>(a, grid, st);
-        default: return launch<T, 256>(a, grid, st);
+        case 32: return by_group<T, 32>(a, grid, st);
+        case 64: return by_group<T, 64>(a, grid, st);
+        case 96: return by_group<T, 96>(a, grid, st);
+        case 128: return by_group<T, 128>(a, grid, st);
+        case 192: return by_group<T, 192>(a, grid, st);
+        default: return by_group<T, 256>(a, grid, st);
     }
 }
 

@@ -1,0 +1,81 @@
+"""Decode operators on the GPU where they can go quietly wrong: small weights, equal weights, workspaces.
+
+Bounds are derived as in test_decode_gpu, whose helpers are used."""
+
+import math
+import os
+import sys
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+
+import test_decode_gpu as G  # noqa: E402
+from test_decode_gpu import BF, FF, HF, clean, rand  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- attention: weights -------------------------------------------------------------
+
+def scored(scores, v, dtype, heads, kv, dim, seqs, scale=1.0):
+    """Attention over tokens of the given scores (before `scale`) and values [tokens, dim], the same for every
+    head and sequence: enough items that none is cut, over one set of pages.  -> out, lse, 64-bit out, lse, bound."""
+    from heatvit_b200 import decode
+    n = len(scores)
+    page = 16
+    kc, vc = (torch.zeros(-(-n // page), page, kv, dim, dtype=dtype, device="cuda") for _ in range(2))
+    kc.view(-1, kv, dim)[:n, :, 0] = scores.to(dtype)[:, None]
+    vc.view(-1, kv, dim)[:n] = v.to(dtype)[:, None]
+    q = torch.zeros(seqs, heads, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    table = torch.arange(kc.shape[0], dtype=torch.int32, device="cuda").expand(seqs, -1)
+    out, lse = decode.paged_attention(q, kc, vc, table, torch.full((seqs,), n, dtype=torch.int32, device="cuda"),
+                                      scale=scale, return_lse=True)
+    s, x = kc.view(-1, kv, dim)[:n, 0, 0].double() * scale, vc.view(-1, kv, dim)[:n, 0].double()
+    p = torch.softmax(s, 0)
+    want = p @ x
+    # A score is one exact product, scaled in 32 bits, and its exponential within 2^-21 (2^-20 of a score); a
+    # weight is held in two numbers of the cache's type, within 2^-16, in fp16 also to 2^-34 of the largest weight
+    # (2^-25 beside a reference of 2^9); a warp adds n / 32 products in a chain of 2^-23 each.
+    rel = float(s.abs().max()) * 2.0 ** -20 + 2.0 ** -16 + 2.0 ** -21 + n / 32 * 2.0 ** -23
+    error = p @ x.abs() * 2 * rel
+    if dtype == HF:
+        error = error + 2.0 ** -34 * p.max() * x.abs().sum(0)
+    # One rounding to nearest of what is within `error` of `want`: no farther from that than the number of the
+    # type nearest to `want` is, so no farther from `want` than that number's distance and twice `error`.
+    bound = (want.to(dtype).double() - want).abs() + 2 * error
+    return out, lse, want, torch.logsumexp(s, 0), bound
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (8, 4, 128), (4, 4, 256), (64, 4, 64), (36, 4, 128)])
+@pytest.mark.parametrize("nats", [11.5755, 12.0, 14.0, 16.0])
+def test_attention_long_tail_under_one_weight(dtype, heads, kv, dim, nats):
+    """One early token takes nearly all the weight and has a value of zero: the output is the tail's, whose weights
+    are 12 to 16 nats smaller each (11.5755: all of them exactly 16.7 bits)."""
+    n = 8192
+    tail = torch.zeros(n, device="cuda") if nats == 11.5755 else rand(1, n, scale=0.3)
+    tail[0] = nats
+    v = 1 + rand(2, n, dim)
+    v[0] = 0
+    out, lse, want, want_lse, bound = scored(tail, v, dtype, heads, kv, dim, 112)
+    assert bool(((out.double() - want).abs() <= bound).all()), float(((out.double() - want).abs() / bound).max())
+    assert bool(((lse.double() - want_lse).abs() <= 1e-4 + 2.0 ** -18 * want_lse.abs()).all())
+
+
+@pytest.mark.parametrize("dtype,step", [(BF, 2.0 ** -8), (HF, 2.0 ** -11)])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (8, 4, 128), (4, 4, 256), (64, 4, 64), (36, 4, 128)])
+def test_attention_equal_weights_between_two_numbers(dtype, step, heads, kv, dim):
+    """Weights of 1 + half a step of the cache's type, after a tile of ones: were each rounded alone, the output
+    would be half a step off as a whole."""
+    n = 4096
+    scores = torch.ones(n, device="cuda")
+    scores[:128] = 0
+    v = torch.ones(n, dim, device="cuda")
+    v[:, 1] = rand(3, n)
+    out, lse, want, want_lse, bound = scored(scores, v, dtype, heads, kv, dim, 112, scale=math.log1p(step))
+    assert bool(((out.double() - want).abs() <= bound).all()), float(((out.double() - want).abs() / bound).max())
+    assert bool(((lse.double() - want_lse).abs() <= 1e-4 + 2.0 ** -18 * want_lse.abs()).all())
