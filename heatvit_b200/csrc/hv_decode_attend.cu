@@ -721,6 +721,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
 // The counters come first and take the same room for every call, so that calls of other
 // sizes with the same workspace never find a part where a zero belongs.
 constexpr int COUNT_BYTES = 3 * MAX_GRID * 4;
+static_assert(COUNT_BYTES == HV_ATTENTION_COUNTER_BYTES, "what the caller zeroes");
 
 // CTAs of one resident wave on the current device.
 int wave(int d) {

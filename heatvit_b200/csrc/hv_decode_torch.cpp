@@ -315,14 +315,16 @@ int64_t workspace_bytes() {
     return most;
 }
 
+// Only the counters have to be zero: a fill of the whole 5 MB took 2.3 us of every captured call.
 Tensor new_workspace(int dev) {
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
     Tensor t = at::detail::empty_cuda({workspace_bytes()}, at::kByte, at::Device(at::kCUDA, (c10::DeviceIndex)dev),
                                       std::nullopt);
-    return t.zero_();
+    t.narrow(0, 0, HV_ATTENTION_COUNTER_BYTES).zero_();
+    return t;
 }
 
-// (device index) -> a zeroed workspace tensor
+// (device index) -> a workspace tensor, its counters zeroed
 PyObject *attention_workspace(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     BEGIN
     ARGUMENTS(1)

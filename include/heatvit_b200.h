@@ -469,8 +469,10 @@ HV_API int hv_append_kv(const hv_append_args *args, void *stream);
  * first d_lens[seq] cached tokens, `heads / kv_heads` query heads sharing a key head.  A length
  * of zero (or less) gives zeros, and -inf in d_lse.
  * dim one of 32, 64, 96, 128, 192, 256; cache rows start on 16 bytes.
- * d_workspace: hv_paged_attention_workspace bytes, 256-byte aligned, zeroed once after it is
- * allocated; calls of any sizes may share it one after another, calls that overlap in time not. */
+ * d_workspace: hv_paged_attention_workspace bytes, 256-byte aligned, the first
+ * HV_ATTENTION_COUNTER_BYTES of them zeroed once after it is allocated (every call leaves zeros
+ * there); calls of any sizes may share it one after another, calls that overlap in time not. */
+#define HV_ATTENTION_COUNTER_BYTES 12288
 typedef struct hv_attention_args {
     const void *d_q;                   /* [seqs][heads][dim] */
     void *d_out;                       /* [seqs][heads][dim] */

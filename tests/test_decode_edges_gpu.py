@@ -79,3 +79,24 @@ def test_attention_equal_weights_between_two_numbers(dtype, step, heads, kv, dim
     out, lse, want, want_lse, bound = scored(scores, v, dtype, heads, kv, dim, 112, scale=math.log1p(step))
     assert bool(((out.double() - want).abs() <= bound).all()), float(((out.double() - want).abs() / bound).max())
     assert bool(((lse.double() - want_lse).abs() <= 1e-4 + 2.0 ** -18 * want_lse.abs()).all())
+
+
+# ---- attention: workspaces ----------------------------------------------------------
+
+def test_new_workspace_zeroes_its_counters_alone():
+    """The rest of the 5 MB is written before it is read: a captured call makes a workspace of its own, and a
+    graph would fill it at every replay."""
+    from heatvit_b200 import decode
+    size = decode.AttentionWorkspace().buffer.numel()
+    torch.cuda.empty_cache()
+    block = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    at = block.data_ptr()
+    del block
+    ws = decode.AttentionWorkspace()  # the allocator gives the block that has just come free
+    assert ws.buffer.data_ptr() == at
+    counters = 12288  # HV_ATTENTION_COUNTER_BYTES
+    assert bool((ws.buffer[:counters] == 0).all()) and bool((ws.buffer[counters:] == 255).all())
+    case = G.attend_case(6, [50000, 7, 30000], 8, 1, 128, 16, BF, "nhd", poison=False)
+    for _ in range(2):  # parts are joined, and nothing of what was there before (NaN) is in them
+        G.check_attention(*case, [50000, 7, 30000], workspace=ws)
+    assert bool((ws.buffer[:counters] == 0).all())
