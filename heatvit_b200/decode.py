@@ -143,13 +143,16 @@ def append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, rope=
 
 class AttentionWorkspace:
     """Device memory that ``paged_attention`` joins split sequences in, for one device
-    and any sizes.  Calls that share one must not overlap in time (one per stream).
-    Waits for the device to have zeroed its counters, so that any stream may use it."""
+    (the current one unless named) and any sizes.  Calls that share one must not overlap
+    in time (one per stream).  Waits for the device to have zeroed its counters, so that
+    any stream may use it."""
 
     def __init__(self, device=None):
         torch = _torch()
-        self.device = torch.device("cuda", torch.cuda.current_device() if device is None else
-                                   torch.device(device).index or 0)
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError("an attention workspace lives on a CUDA device")
+        self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
         self.buffer = _load().attention_workspace(self.device.index)
         torch.cuda.current_stream(self.device).synchronize()
 

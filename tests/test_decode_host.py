@@ -1,0 +1,35 @@
+"""Host side of the decode operators, without a GPU: devices and builds."""
+
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture
+def device_three(monkeypatch):
+    """A process whose current CUDA device is 3 (of which only the index is asked); the devices of the workspaces made."""
+    from heatvit_b200 import decode
+    made = []
+    stream = types.SimpleNamespace(synchronize=lambda: None)
+    cuda = types.SimpleNamespace(current_device=lambda: 3, current_stream=lambda device: stream)
+    monkeypatch.setattr(decode, "_torch", lambda: types.SimpleNamespace(cuda=cuda, device=torch.device))
+    monkeypatch.setattr(decode, "_load", lambda: types.SimpleNamespace(attention_workspace=made.append))
+    return made
+
+
+@pytest.mark.parametrize("device,index", [(None, 3), ("cuda", 3), (torch.device("cuda"), 3), ("cuda:0", 0),
+                                          (torch.device("cuda", 5), 5)])
+def test_workspace_lives_on_the_device_that_was_meant(device_three, device, index):
+    """A device without an index is the current one, as everywhere in torch."""
+    from heatvit_b200 import decode
+    ws = decode.AttentionWorkspace(device)
+    assert device_three == [index] and ws.device == torch.device("cuda", index)
+
+
+def test_workspace_refuses_what_is_no_cuda_device(device_three):
+    from heatvit_b200 import decode
+    with pytest.raises(ValueError, match="CUDA"):
+        decode.AttentionWorkspace("cpu")
+    assert device_three == []
