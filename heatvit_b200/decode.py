@@ -95,7 +95,7 @@ def quantize_weight_fp8(weight):
     n, k = weight.shape
     nb, kb = -(-n // GROUP), -(-k // GROUP)
     w = torch.zeros((nb * GROUP, kb * GROUP), dtype=torch.float32, device=weight.device)
-    w[:n, :k] = weight
+    w[:n, :k] = weight.detach()
     blocks = w.view(nb, GROUP, kb, GROUP)
     scale = blocks.abs().amax((1, 3)).clamp_(min=2.0 ** -100) / E4M3_MAX
     q = torch.empty((n, -(-k // 16) * 16), dtype=torch.float8_e4m3fn, device=weight.device)[:, :k]

@@ -33,3 +33,15 @@ def test_workspace_refuses_what_is_no_cuda_device(device_three):
     with pytest.raises(ValueError, match="CUDA"):
         decode.AttentionWorkspace("cpu")
     assert device_three == []
+
+
+def test_quantized_weight_keeps_no_graph(monkeypatch):
+    """A parameter's e4m3 form is a plain tensor: it neither asks for gradients nor holds the float32 copies."""
+    from heatvit_b200 import decode
+    monkeypatch.setattr(decode, "_torch", lambda: torch)
+    weight = torch.nn.Parameter(torch.randn(200, 150))
+    q, scale = decode.quantize_weight_fp8(weight)
+    assert not q.requires_grad and q.grad_fn is None and q._base.grad_fn is None
+    assert not scale.requires_grad and scale.grad_fn is None
+    plain, its_scale = decode.quantize_weight_fp8(weight.detach())
+    assert torch.equal(q.view(torch.uint8), plain.view(torch.uint8)) and torch.equal(scale, its_scale)
