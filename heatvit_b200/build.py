@@ -3,7 +3,8 @@
 One nvcc invocation per translation unit (parallel), linked into a shared
 library with the CUDA runtime statically linked, for sm_100a only.  Beside it
 _decode_native.so, the decode operators' calls from Python (a CPython module
-on the installed torch's headers, linked against the library).
+on the installed torch's headers, linked against the library; left out where
+there is no torch, which the library does not need).
 """
 
 import importlib.util
@@ -51,10 +52,15 @@ def native_up_to_date():
 
 
 def build_native(force=False):
-    """The decode operators' Python module, for the installed torch."""
+    """The decode operators' Python module, for the installed torch; None without one."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        print(f"heatvit_b200: torch is not installed, {os.path.basename(NATIVE)} (heatvit_b200.decode) is not built",
+              file=sys.stderr)
+        return None
     if not force and native_up_to_date():
         return NATIVE
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    torch = spec.submodule_search_locations[0]
     cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
     tmp = NATIVE + ".tmp"
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", "-Wall", NATIVE_SOURCE, "-o", tmp,

@@ -45,3 +45,19 @@ def test_quantized_weight_keeps_no_graph(monkeypatch):
     assert not scale.requires_grad and scale.grad_fn is None
     plain, its_scale = decode.quantize_weight_fp8(weight.detach())
     assert torch.equal(q.view(torch.uint8), plain.view(torch.uint8)) and torch.equal(scale, its_scale)
+
+
+# ---- builds -------------------------------------------------------------------------
+
+def test_library_builds_without_torch(monkeypatch, tmp_path, capsys):
+    """The C library needs nvcc alone: without torch the Python module is left out, and that is said."""
+    import importlib.util
+    from heatvit_b200 import build
+    build.build()
+    find = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else find(name, *a))
+    monkeypatch.setattr(build, "NATIVE", str(tmp_path / "_decode_native.so"))
+    assert build.build() == build.LIB
+    assert not (tmp_path / "_decode_native.so").exists()
+    assert "torch" in capsys.readouterr().err
+    assert build.build_native(force=True) is None
