@@ -45,10 +45,22 @@ def up_to_date():
     return all(os.path.getmtime(f) <= t for f in _deps())
 
 
+def native_made_for():
+    """What the Python module is bound to beside its source: torch's version file and Python's ABI."""
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    with open(os.path.join(torch, "version.py")) as f:
+        return sysconfig.get_config_var("EXT_SUFFIX") + "\n" + f.read()
+
+
 def native_up_to_date():
     header = os.path.join(os.path.dirname(HERE), "include", "heatvit_b200.h")
-    return os.path.exists(NATIVE) and all(os.path.getmtime(f) <= os.path.getmtime(NATIVE)
-                                          for f in (NATIVE_SOURCE, header))
+    stamp = NATIVE + ".made_for"
+    if not os.path.exists(NATIVE) or not os.path.exists(stamp):
+        return False
+    with open(stamp) as f:
+        if f.read() != native_made_for():
+            return False
+    return all(os.path.getmtime(f) <= os.path.getmtime(NATIVE) for f in (NATIVE_SOURCE, header))
 
 
 def build_native(force=False):
@@ -73,6 +85,8 @@ def build_native(force=False):
     if r.returncode != 0:
         raise RuntimeError(f"{CXX} failed for {NATIVE_SOURCE}:\n{r.stderr}")
     os.replace(tmp, NATIVE)
+    with open(NATIVE + ".made_for", "w") as f:
+        f.write(native_made_for())
     return NATIVE
 
 

@@ -61,3 +61,16 @@ def test_library_builds_without_torch(monkeypatch, tmp_path, capsys):
     assert not (tmp_path / "_decode_native.so").exists()
     assert "torch" in capsys.readouterr().err
     assert build.build_native(force=True) is None
+
+
+def test_module_is_stale_beside_another_torch(monkeypatch, tmp_path):
+    """The module uses torch's C++ interfaces, which other versions of torch or Python do not keep."""
+    from heatvit_b200 import build
+    build.build()
+    assert build.native_up_to_date()
+    with monkeypatch.context() as m:
+        m.setattr(build, "native_made_for", lambda: "another torch")
+        assert not build.native_up_to_date()
+    assert build.native_up_to_date()
+    made_for = build.native_made_for()
+    assert torch.__version__ in made_for and build.sysconfig.get_config_var("EXT_SUFFIX") in made_for
