@@ -162,25 +162,27 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__
 }
 
 template <typename T, int W, bool INTER, int NH>
-cudaError_t launch(AppendArgs &a, int tokens, int dim, cudaStream_t st) {
+int launch(AppendArgs &a, int tokens, int dim, cudaStream_t st) {
     uint32_t blocks = 0;
     for (int i = 0; i < 3; ++i) {
         Tensor &t = a.t[i];
         const int rotated = !INTER || W == 1 ? t.rot / 2 / W : t.rot / W, places = rotated + (dim - t.rot) / W;
         t.strips = (t.heads + NH - 1) / NH;
         const double total = (double)tokens * t.strips * places;
-        if (total > 2147483392.0) return cudaErrorInvalidValue;
+        if (total > 2147483392.0) return fail(HV_ERR_VALUE, "too many elements for one call");
         t.total = (uint32_t)total;
         t.by_token = Divider(std::max(1u, t.strips * places));
         t.by_place = Divider(places);
         a.first[i] = blocks;
         blocks += (t.total + THREADS - 1) / THREADS;
     }
-    return launch_pdl(append_kernel<T, W, INTER, NH>, dim3(blocks), dim3(THREADS), 0, st, a);
+    const cudaError_t e = launch_pdl(append_kernel<T, W, INTER, NH>, dim3(blocks), dim3(THREADS), 0, st, a);
+    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "append_kv: %s", cudaGetErrorString(e));
+    return HV_OK;
 }
 
 template <typename T>
-cudaError_t launch(AppendArgs &a, int tokens, int dim, bool wide, bool inter, int sms, cudaStream_t st) {
+int launch(AppendArgs &a, int tokens, int dim, bool wide, bool inter, int sms, cudaStream_t st) {
     if (!wide) return inter ? launch<T, 1, true, 1>(a, tokens, dim, st) : launch<T, 1, false, 1>(a, tokens, dim, st);
     // One head a thread until that fills the SMs' threads twice, then two: 24 ragged prompts of 36
     // heads of 64 (interleaved) took 70 us with one, 59 with two, 62 with four, 8 x 1024 tokens of
@@ -239,9 +241,6 @@ extern "C" int hv_append_kv(const hv_append_args *p, void *stream) {
     rows(p->d_k_cache, p->k_cache_strides, 3), rows(p->d_v_cache, p->v_cache_strides, 3);
     if (p->heads) rows(p->d_q, p->q_strides, 2), rows(p->d_q_out, p->q_out_strides, 2);
     const cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e =
-        p->dtype == HV_BF16 ? launch<__nv_bfloat16>(a, p->tokens, p->dim, wide, p->interleaved != 0, sms, st)
-                            : launch<__half>(a, p->tokens, p->dim, wide, p->interleaved != 0, sms, st);
-    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "append_kv: %s", cudaGetErrorString(e));
-    return HV_OK;
+    return p->dtype == HV_BF16 ? launch<__nv_bfloat16>(a, p->tokens, p->dim, wide, p->interleaved != 0, sms, st)
+                               : launch<__half>(a, p->tokens, p->dim, wide, p->interleaved != 0, sms, st);
 }

@@ -100,3 +100,17 @@ def test_new_workspace_zeroes_its_counters_alone():
     for _ in range(2):  # parts are joined, and nothing of what was there before (NaN) is in them
         G.check_attention(*case, [50000, 7, 30000], workspace=ws)
     assert bool((ws.buffer[:counters] == 0).all())
+
+
+# ---- append -------------------------------------------------------------------------
+
+def test_append_refuses_more_elements_than_threads():
+    """Rows off 16 bytes take a thread an element: too many are a ValueError, as with aligned rows, and not a CUDA error."""
+    from heatvit_b200 import decode
+    tokens, dim = 1 << 20, 4096
+    k = torch.zeros(dim + 1, dtype=BF, device="cuda")[1:].view(1, 1, dim).expand(tokens, 1, dim)
+    cache = torch.zeros(1, 1, 1, dim, dtype=BF, device="cuda")
+    nowhere = torch.full((tokens,), -1, dtype=torch.int32, device="cuda")  # padding tokens
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="too many elements"):
+        decode.append_kv(k, k, cache, cache.clone(), table, nowhere, seq_ids=nowhere)
