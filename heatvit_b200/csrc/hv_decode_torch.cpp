@@ -78,6 +78,12 @@ void need_like(const Tensor &t, const char *name, const Tensor &other, const cha
     if (t.scalar_type() != other.scalar_type()) throw TypeError("%s must have %s's type", name, its_name);
 }
 
+// A caller's tensor has been written: autograd's check of saved tensors goes by this.  (Tensors
+// made in inference mode have no versions.)
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int type_code(at::ScalarType t) {
     return t == at::kBFloat16 ? HV_BF16 : t == at::kHalf ? HV_F16 : t == at::kFloat ? HV_F32 : -1;
 }
@@ -174,6 +180,7 @@ PyObject *add_rmsnorm_fp8(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     a.scale_strides[0] = 1, a.scale_strides[1] = rows;
     a.dim = int_of(dim, "dim"), a.dtype = code, a.eps = (float)eps;
     if (const int rc = hv_add_rmsnorm_fp8(&a, stream_of(dev))) return PyLong_FromLong(rc);
+    if (o[4] != Py_None) written(out);
     PyObject *r = PyTuple_New(3);
     if (!r) return nullptr;
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(q)));
@@ -228,6 +235,7 @@ PyObject *gemm_fp8(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     for (int i = 0; i < 2; ++i) g.a_scale_strides[i] = as.stride(i), g.b_scale_strides[i] = bs.stride(i);
     g.out_dtype = code;
     if (const int rc = hv_gemm_fp8(&g, stream_of(dev))) return PyLong_FromLong(rc);
+    if (o[5] != Py_None) written(out);
     return THPVariable_Wrap(std::move(out));
     END
 }
@@ -302,6 +310,9 @@ PyObject *append_kv(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     a.num_pages = int_of(kc.size(0), "pages"), a.page_size = int_of(kc.size(1), "page size");
     a.seqs = int_of(table.size(0), "page_table"), a.max_pages = int_of(table.size(1), "page_table");
     if (const int rc = hv_append_kv(&a, stream_of(dev))) return PyLong_FromLong(rc);
+    written(kc);
+    written(vc);
+    if (o[10] != Py_None) written(out);
     return out.defined() ? THPVariable_Wrap(std::move(out)) : none();
     END
 }
@@ -407,6 +418,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     a.num_pages = int_of(kc.size(0), "pages"), a.page_size = int_of(kc.size(1), "page size");
     a.max_pages = int_of(table.size(1), "page_table"), a.scale = (float)scale;
     if (const int rc = hv_paged_attention(&a, stream)) return PyLong_FromLong(rc);
+    if (o[7] != Py_None) written(out);
     if (!with_lse) return THPVariable_Wrap(std::move(out));
     PyObject *r = PyTuple_New(2);
     if (!r) return nullptr;

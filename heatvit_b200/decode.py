@@ -15,7 +15,8 @@ The last dimension of every tensor is contiguous; the others may have any stride
 [pages, kv_heads, page, dim]).  Shape and type mistakes raise ValueError and
 TypeError.  What only the device can see (a page number outside the cache, a
 position past a table) faults nothing and is reported by ``device_error``.
-Calls may be captured in a CUDA graph after one of each outside it.
+Calls may be captured in a CUDA graph after one of each outside it.  There are no
+gradients: an input that asks for them is read as its values, a result never does.
 """
 
 import ctypes as C

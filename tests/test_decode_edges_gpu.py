@@ -114,3 +114,51 @@ def test_append_refuses_more_elements_than_threads():
     table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="too many elements"):
         decode.append_kv(k, k, cache, cache.clone(), table, nowhere, seq_ids=nowhere)
+
+
+# ---- autograd -----------------------------------------------------------------------
+
+def a_step(make):
+    """One call of each operator into the caller's tensors, which `make` allocates -> those tensors."""
+    from heatvit_b200 import decode
+    x, w = rand(1, 5, 512, dtype=BF), rand(3, 512, dtype=BF)
+    residual, out = make(5, 512, dtype=BF), make(5, 256, dtype=BF)
+    rows = decode.add_rmsnorm_fp8(x, w, residual=residual, residual_out=residual)
+    wq, ws = decode.quantize_weight_fp8(rand(4, 256, 512, scale=0.05))
+    decode.gemm_fp8(rows.q, rows.scale, wq, ws, out=out)
+    kc, vc, q, attended = (make(*size, dtype=BF) for size in ((5, 16, 1, 64), (5, 16, 1, 64), (5, 2, 64), (5, 2, 64)))
+    h = out.view(5, 4, 64)
+    table = torch.arange(5, dtype=torch.int32, device="cuda")[:, None]
+    pos = torch.zeros(5, dtype=torch.int32, device="cuda")
+    decode.append_kv(h[:, 2:3], h[:, 3:], kc, vc, table, pos, q=h[:, :2], q_out=q)
+    decode.paged_attention(q, kc, vc, table, pos + 1, out=attended)
+    return residual, out, kc, vc, q, attended
+
+
+def test_written_tensors_count_their_versions():
+    """What a call writes of the caller's, and nothing else, is newer to autograd than what it saved before."""
+    made = {}
+
+    def make(*size, dtype):
+        t = torch.zeros(*size, dtype=dtype, device="cuda")
+        made[t] = t._version
+        return t
+    for t in a_step(make):
+        assert t._version == made[t] + 1
+    with torch.inference_mode():
+        frozen = []
+
+        def make_frozen(*size, dtype):
+            frozen.append(torch.zeros(*size, dtype=dtype, device="cuda"))
+            return frozen[-1]
+        a_step(make_frozen)
+    a_step(lambda *size, dtype, held=iter(frozen): next(held))  # inference tensors outside that mode are taken too
+
+
+def test_inputs_that_ask_for_gradients_are_read_as_values():
+    from heatvit_b200 import decode
+    x, w = rand(1, 5, 512, dtype=BF), rand(3, 512, dtype=BF)
+    plain = decode.add_rmsnorm_fp8(x, w, residual=x)
+    r = decode.add_rmsnorm_fp8(x, torch.nn.Parameter(w), residual=x.clone().requires_grad_())
+    assert torch.equal(r.residual, plain.residual) and torch.equal(r.scale, plain.scale)
+    assert not (r.residual.requires_grad or r.scale.requires_grad or r.q.requires_grad)
