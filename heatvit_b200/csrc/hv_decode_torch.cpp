@@ -66,6 +66,12 @@ void need(const Tensor &t, const char *name, int64_t dims, int dev) {
         throw ValueError("%s's last dimension must be contiguous", name);
 }
 
+// An operand that is written: elements that share memory (an expanded tensor) would be a race.
+void need_apart(const Tensor &t, const char *name) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) == 0) throw ValueError("%s is written, so its elements may not share memory", name);
+}
+
 void need_ints(const Tensor &t, const char *name, int64_t dims, int dev) {
     if (t.scalar_type() != at::kInt) throw TypeError("%s must be int32", name);
     need(t, name, dims, dev);
@@ -157,6 +163,7 @@ PyObject *add_rmsnorm_fp8(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
         if (o[4] != Py_None) {
             out = tensor(o[4], "residual_out");
             need_like(out, "residual_out", x, "x", dev);
+            need_apart(out, "residual_out");
         } else {
             out = padded_rows(rows, dim, 8, x.scalar_type(), x);
         }
@@ -220,6 +227,7 @@ PyObject *gemm_fp8(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     if (o[5] != Py_None) {
         out = tensor(o[5], "out");
         need(out, "out", 2, dev);
+        need_apart(out, "out");
         if (out.size(0) != m || out.size(1) != n) throw ValueError("out must be [%lld, %lld]", (long long)m, (long long)n);
         if (o[4] != Py_None && out.scalar_type() != type) throw TypeError("out has another type than out_dtype");
         type = out.scalar_type();
@@ -255,6 +263,8 @@ PyObject *append_kv(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     need(k, "k", 3, dev);
     need_like(v, "v", k, "k", dev);
     need_caches(kc, vc, dev);
+    need_apart(kc, "k_cache");
+    need_apart(vc, "v_cache");
     need_ints(table, "page_table", 2, dev);
     need_ints(pos, "positions", 1, dev);
     const int code = type_code(k.scalar_type());
@@ -292,6 +302,7 @@ PyObject *append_kv(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
         if (o[10] != Py_None) {
             out = tensor(o[10], "q_out");
             need_like(out, "q_out", q, "q", dev);
+            need_apart(out, "q_out");
         } else {
             out = empty(q.sizes(), q.scalar_type(), q);
         }
@@ -391,6 +402,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     if (o[7] != Py_None) {
         out = tensor(o[7], "out");
         need_like(out, "out", q, "q", dev);
+        need_apart(out, "out");
     } else {
         out = empty(q.sizes(), q.scalar_type(), q);
     }

@@ -12,7 +12,8 @@ cache.  Floating point, inference only, with no counterpart in the reference.
 
 The last dimension of every tensor is contiguous; the others may have any stride
 (a cache may be [pages, page, kv_heads, dim] in memory or a transposed view of
-[pages, kv_heads, page, dim]).  Shape and type mistakes raise ValueError and
+[pages, kv_heads, page, dim]), but a tensor that is written may not be an expanded one,
+and rows of an e4m3 operand do not overlap.  Shape and type mistakes raise ValueError and
 TypeError.  What only the device can see (a page number outside the cache, a
 position past a table) faults nothing and is reported by ``device_error``.
 Calls may be captured in a CUDA graph after one of each outside it.  There are no

@@ -162,3 +162,31 @@ def test_inputs_that_ask_for_gradients_are_read_as_values():
     r = decode.add_rmsnorm_fp8(x, torch.nn.Parameter(w), residual=x.clone().requires_grad_())
     assert torch.equal(r.residual, plain.residual) and torch.equal(r.scale, plain.scale)
     assert not (r.residual.requires_grad or r.scale.requires_grad or r.q.requires_grad)
+
+
+# ---- refusals -----------------------------------------------------------------------
+
+def test_written_tensors_do_not_share_memory():
+    """An expanded tensor is read where it is an input, and refused where rows would race to write it."""
+    from heatvit_b200 import decode
+    x, w = rand(1, 5, 512, dtype=BF), rand(3, 512, dtype=BF)
+    one = rand(2, 1, 512, dtype=BF)
+    many = one.expand(5, 512)
+    r = decode.add_rmsnorm_fp8(x, w, residual=many)
+    assert torch.equal(r.residual, decode.add_rmsnorm_fp8(x, w, residual=many.clone()).residual)
+    wq, ws = decode.quantize_weight_fp8(rand(4, 256, 512, scale=0.05))
+    kc, vc = (torch.zeros(5, 16, 1, 64, dtype=BF, device="cuda") for _ in range(2))
+    table = torch.arange(5, dtype=torch.int32, device="cuda")[:, None]
+    pos = torch.zeros(5, dtype=torch.int32, device="cuda")
+    h = rand(5, 5, 1, 64, dtype=BF)
+    for call in (lambda: decode.add_rmsnorm_fp8(x, w, residual=x, residual_out=many),
+                 lambda: decode.gemm_fp8(r.q, r.scale, wq, ws, out=one[:, :256].expand(5, 256)),
+                 lambda: decode.append_kv(h, h, kc[:1].expand(5, 16, 1, 64), vc, table, pos),
+                 lambda: decode.append_kv(h, h, kc, vc[:, :1].expand(5, 16, 1, 64), table, pos),
+                 lambda: decode.append_kv(h, h, kc, vc, table, pos, q=h, q_out=h[:1].expand(5, 1, 64)),
+                 lambda: decode.paged_attention(h, kc, vc, table, pos, out=h[:1].expand(5, 1, 64))):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    # one page read by every sequence is no such thing
+    shared = decode.paged_attention(h, kc[:1].expand(5, 16, 1, 64), vc[:1].expand(5, 16, 1, 64), table, pos + 1)
+    assert torch.equal(shared, torch.zeros_like(shared))
