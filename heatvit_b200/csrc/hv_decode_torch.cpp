@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -397,7 +398,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     const int with_lse = PyObject_IsTrue(o[8]);
     if (with_lse < 0) return nullptr;
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-    const auto stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+    const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev);
+    const cudaStream_t stream = current.stream();
     Tensor out;
     if (o[7] != Py_None) {
         out = tensor(o[7], "out");
@@ -411,6 +413,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
         ws = tensor(o[6], "workspace");
         on(ws, "workspace", dev);
         if (ws.scalar_type() != at::kByte || !ws.is_contiguous()) throw TypeError("workspace must be contiguous bytes");
+        // made on another stream perhaps: its memory is not handed on before this call is through
+        c10::cuda::CUDACachingAllocator::recordStream(ws.storage().data_ptr(), current);
     } else {
         ws = workspace_of(dev, stream);
     }

@@ -102,6 +102,63 @@ def test_new_workspace_zeroes_its_counters_alone():
     assert bool((ws.buffer[:counters] == 0).all())
 
 
+def test_workspace_dropped_while_another_stream_uses_it():
+    """Its memory goes to nobody before the call on the other stream is through."""
+    from heatvit_b200 import decode
+    lens = [9000, 300]
+    q, kc, vc, table = G.attend_case(6, lens, 8, 1, 128, 16, BF, "nhd")
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = decode.paged_attention(q, kc, vc, table, n)
+    ws = decode.AttentionWorkspace()
+    at, size = ws.buffer.data_ptr(), ws.buffer.numel()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # the call is still ahead of the device when the workspace goes
+        got = decode.paged_attention(q, kc, vc, table, n, workspace=ws)
+    del ws
+    other = torch.empty(size, dtype=torch.uint8, device="cuda")
+    assert other.data_ptr() != at
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_workspace_in_a_graph():
+    """One workspace through a captured step of several calls, replayed on another stream, and then dropped."""
+    from heatvit_b200 import decode
+    ws = decode.AttentionWorkspace()
+    cases = [(*G.attend_case(seed, lens, 8, 1, 128, 16, BF, "nhd"), torch.tensor(lens, dtype=torch.int32, device="cuda"))
+             for seed, lens in ((6, [9000, 300]), (7, [40, 0, 20000]))]
+    want = [decode.paged_attention(*c) for c in cases]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [decode.paged_attention(*c, workspace=ws) for c in cases * 2]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            graph.replay()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want * 2))
+    del graph, ws
+    torch.cuda.empty_cache()
+
+
+def test_workspace_refusals():
+    """One that is too small, not on 256 bytes, not contiguous bytes, or not on a device at all."""
+    from types import SimpleNamespace
+    from heatvit_b200 import decode
+    q, kc, vc, table = G.attend_case(1, [20, 5], 4, 2, 64, 16, BF, "nhd")
+    n = torch.tensor([20, 5], dtype=torch.int32, device="cuda")
+    size = decode.AttentionWorkspace().buffer.numel()
+    room = torch.zeros(2 * size, dtype=torch.uint8, device="cuda")
+    for kind, buffer in ((ValueError, room[:4096]), (ValueError, room[16:16 + size]), (TypeError, room[::2]),
+                         (TypeError, room.view(torch.int32)), (ValueError, room.cpu()), (TypeError, "workspace")):
+        with pytest.raises(kind):
+            decode.paged_attention(q, kc, vc, table, n, workspace=SimpleNamespace(buffer=buffer))
+    assert bool((room == 0).all())
+
+
 # ---- append -------------------------------------------------------------------------
 
 def test_append_refuses_more_elements_than_threads():
