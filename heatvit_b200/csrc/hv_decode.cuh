@@ -20,6 +20,14 @@ int *error_word();
 // SMs of the current device; 0 when that cannot be read.
 int sm_count();
 
+constexpr uint32_t WAIT_ITERS = 1u << 22;  // polls of an mbarrier before a wait gives up
+// What a launch is given of that: the limit, and a copy that each CTA leaves out (none unless
+// hv_test_decode_stall asks for one).
+struct Waits {
+    uint32_t iters, skip;
+};
+Waits waits();
+
 // Lets `kernel` have all of an SM's shared memory, once a device: `ready` has a bit for each.
 template <typename K>
 cudaError_t allow_shared(K kernel, std::atomic<uint64_t> &ready) {

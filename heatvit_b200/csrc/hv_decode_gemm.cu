@@ -27,7 +27,7 @@
 // 4096 6.9 us, 1576 x 768 x 192 4.6 us.
 //
 // Every mbarrier wait is bounded: after a timeout the CTA waits for what it has in flight,
-// releases its TMEM and sets the device's error word.
+// releases its TMEM and, when all of its roles are through, sets the device's error word.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -42,7 +42,6 @@ using namespace dec;
 
 constexpr int BM = 128, GK = 128;  // rows of a tile; a group of K, in elements and bytes
 constexpr int EPI_WARPS = 8, THREADS = 128 + EPI_WARPS * 32;
-constexpr uint32_t WAIT_ITERS = 1u << 22;
 constexpr int SB = 8;      // groups whose scales are fetched together
 constexpr int BAND = 16;   // tile rows of a band
 constexpr int AHEAD = 16;  // groups that are prefetched into L2
@@ -53,6 +52,7 @@ struct GemmFp8Args {
     void *out;
     long long ldc;
     int x_rows, y_rows, groups, tiles_x, tiles_y, split, out_dtype, vec;
+    Waits waits;
     int *err;
 };
 
@@ -103,13 +103,17 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-// Bounded wait that also ends when another role of the CTA has given up.
+constexpr int POLLS = 64;
+// Bounded wait that also ends when another role of the CTA has given up.  stop: that, and the limit in
+// POLLS polls, both in shared memory and read when the first POLLS have not done (a limit from the
+// arguments in the loop cost 4096^3 3% and 256 x 8192 x 8192 8%).
 __device__ __forceinline__ bool wait_or_stop(uint64_t *bar, uint32_t parity, volatile int *stop) {
-    for (uint32_t i = 0; i < WAIT_ITERS / 64; ++i) {
-        if (tc05::mbar_wait(bar, parity, 64)) return true;
-        if (*stop) return false;
-    }
-    *stop = 1;
+    int i = 0;
+    do {
+        if (tc05::mbar_wait(bar, parity, POLLS)) return true;
+        if (stop[0]) return false;
+    } while (++i < stop[1]);
+    stop[0] = 1;
     return false;
 }
 
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
     using L = Lay<BN, SWAP>;
     extern __shared__ uint8_t raw[];
     __shared__ uint32_t tslot;
-    __shared__ volatile int stop;
+    __shared__ volatile int stop[2];  // a role has given up; POLLS polls that a wait may take
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     float(*sc)[SB][L::SCALES] = (float(*)[SB][L::SCALES])(smem + L::SC);
     uint64_t *full = (uint64_t *)(smem + L::BARS), *empty = full + L::STAGES;
@@ -243,7 +247,8 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
         tc05::tmem_relinquish();
     }
     if (tid == 0) {
-        stop = 0;
+        stop[0] = 0;
+        stop[1] = (int)(a.waits.iters / POLLS);
         for (int i = 0; i < L::STAGES; ++i) {
             tc05::mbar_init(&full[i], 1);
             tc05::mbar_init(&empty[i], 1);
@@ -296,19 +301,20 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
                 tile_at(t, a.tiles_x, a.tiles_y, tx, ty);
                 for (int g = g0; g < g1; ++g, ++n) {
                     const uint32_t s = n % L::STAGES;
-                    if (n >= L::STAGES && !wait_or_stop(&empty[s], (n / L::STAGES - 1) & 1, &stop)) {
+                    if (n >= L::STAGES && !wait_or_stop(&empty[s], (n / L::STAGES - 1) & 1, stop)) {
                         ok = false;
                         break;
                     }
+                    if (n == a.waits.skip) continue;
                     const uint32_t dst = tc05::smem_u32(smem + s * L::STAGE);
                     expect_tx(&full[s], L::STAGE);
                     tma_box(dst, &tmx, g * GK, tx * BM, &full[s]);
                     tma_box(dst + L::A_ST, &tmy, g * GK, ty * BN, &full[s]);
                 }
             }
-            if (!ok)  // what was issued has to land before shared memory goes
-                for (uint32_t k = n > L::STAGES ? n - L::STAGES : 0; k < n; ++k)
-                    tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, WAIT_ITERS);
+            // What was issued has landed before shared memory goes, whichever role gives up.
+            for (uint32_t k = n > L::STAGES ? n - L::STAGES : 0; k < n; ++k)
+                if (k != a.waits.skip) tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, WAIT_ITERS);
         } else if (warp == 1 && lane == 0) {  // products
             constexpr uint32_t idesc = idesc_e4m3(BM, BN);
             uint32_t n = 0;
@@ -316,8 +322,8 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
             for (int t = first; t < tiles && ok; t += step)
                 for (int g = g0; g < g1; ++g, ++n) {
                     const uint32_t s = n % L::STAGES, b = n % L::BUFS;
-                    ok = (n < L::BUFS || wait_or_stop(&tempty[b], (n / L::BUFS - 1) & 1, &stop)) &&
-                         wait_or_stop(&full[s], (n / L::STAGES) & 1, &stop);
+                    ok = (n < L::BUFS || wait_or_stop(&tempty[b], (n / L::BUFS - 1) & 1, stop)) &&
+                         wait_or_stop(&full[s], (n / L::STAGES) & 1, stop);
                     if (!ok) break;
                     tc05::fence_after();
                     const uint32_t at = tc05::smem_u32(smem + s * L::STAGE);
@@ -327,17 +333,15 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
                     tc05::commit(&empty[s]);
                     tc05::commit(&tfull[b]);
                 }
-            if (!ok) {
-                tc05::commit(drain);
-                tc05::mbar_wait(drain, 0, WAIT_ITERS);
-            }
+            tc05::commit(drain);  // and what was issued has read it, and written tensor memory
+            tc05::mbar_wait(drain, 0, WAIT_ITERS);
         } else if (warp >= 2) {  // scales (their loads in the adding warps made those wait: 711 us, 8192^3)
             const int r = tid - 64;  // row r and r + 64, or column r
             int t = first, g = g0;
             const float *x0 = nullptr, *x1 = nullptr, *y0 = nullptr, *y1 = nullptr;
             for (uint32_t q = 0; t < tiles; ++q) {
                 const int b = q & 1;
-                if (q >= 2 && !wait_or_stop(&sempty[b], (q / 2 - 1) & 1, &stop)) break;
+                if (q >= 2 && !wait_or_stop(&sempty[b], (q / 2 - 1) & 1, stop)) break;
 #pragma unroll
                 for (int e0 = 0; e0 < SB; e0 += 4) {
                     float vx0[4], vx1[4], vy0[4], vy1[4];
@@ -395,11 +399,11 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
         for (int t = first; t < tiles && ok; t += step) {
             for (int g = g0; g < g1; ++g, ++n) {
                 const uint32_t b = n % L::BUFS, sb = n / SB;
-                ok = n % SB || wait_or_stop(&sfull[sb & 1], (sb / 2) & 1, &stop);
+                ok = n % SB || wait_or_stop(&sfull[sb & 1], (sb / 2) & 1, stop);
                 const float *f = sc[sb & 1][n % SB] + (SWAP ? c0 : half * BM + row);
                 uint64_t s2 = 0;
                 if (!SWAP) asm("mov.b64 %0, {%1, %1};\n" : "=l"(s2) : "f"(*f));
-                ok = ok && wait_or_stop(&tfull[b], (n / L::BUFS) & 1, &stop);
+                ok = ok && wait_or_stop(&tfull[b], (n / L::BUFS) & 1, stop);
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
                 tc05::fence_after();
@@ -523,10 +527,10 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
         }
         cluster_sync();  // no CTA leaves while its sums may be read
     }
-    if (tid == 0 && stop) atomicOr(a.err, HV_DECODE_STALLED);
     __syncwarp();
     tc05::fence_before();
     __syncthreads();
+    if (tid == 0 && stop[0]) atomicOr(a.err, HV_DECODE_STALLED);  // every role has been through
     if (warp == 2) {
         tc05::fence_after();
         tc05::tmem_dealloc(tmem, L::TMEM);
@@ -658,6 +662,7 @@ extern "C" int hv_gemm_fp8(const hv_gemm_fp8_args *p, void *stream) {
     if (!err || !sms) return fail(HV_ERR_CUDA, "cannot read the device's properties");
     GemmFp8Args g{};
     g.out = p->d_out, g.ldc = p->out_stride, g.out_dtype = p->out_dtype, g.groups = (int)((k + GK - 1) / GK), g.err = err;
+    g.waits = dec::waits();
     // 16-byte stores: rows start on 16 bytes and are whole groups of them
     const int es = dec::elem_size(p->out_dtype);
     g.vec = dec::aligned(p->d_out, 16) && n * es % 16 == 0 && (m == 1 || p->out_stride * es % 16 == 0);
