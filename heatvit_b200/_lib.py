@@ -52,7 +52,7 @@ _SIGNATURES = {
     "hv_selector_h2": (I, [P, I, P, P, I, P, P]),
     "hv_align_add_i8": (I, [P, I, P, I, I, I64, P, P]),
     "hv_decode_error": (I, [C.POINTER(C.c_int)]),
-    "hv_test_decode_stall": (I, [C.c_uint, I]),
+    "hv_test_decode_stall": (I, [I]),
     "hv_add_rmsnorm_fp8": (I, [P, P]),
     "hv_gemm_fp8": (I, [P, P]),
     "hv_append_kv": (I, [P, P]),

@@ -11,7 +11,7 @@ __device__ int g_decode_error;
 constexpr int MAX_DEVICES = 64;
 std::atomic<int *> g_address[MAX_DEVICES];
 std::atomic<int> g_sms[MAX_DEVICES];
-std::atomic<uint32_t> g_wait_iters{dec::WAIT_ITERS}, g_skip{UINT32_MAX};
+std::atomic<uint32_t> g_skip{dec::NO_COPY};
 
 }  // namespace
 
@@ -41,16 +41,15 @@ int sm_count() {
     return n;
 }
 
-Waits waits() { return {g_wait_iters.load(std::memory_order_relaxed), g_skip.load(std::memory_order_relaxed)}; }
+uint32_t skipped_copy() { return g_skip.load(std::memory_order_relaxed); }
 
 }  // namespace dec
 }  // namespace hv
 
-extern "C" int hv_test_decode_stall(unsigned wait_iters, int skip_copy) {
+extern "C" int hv_test_decode_stall(int skip_copy) {
     using namespace hv;
     if (skip_copy < -1) return fail(HV_ERR_VALUE, "skip_copy must be -1 (none) or a copy's number");
-    g_wait_iters.store(wait_iters ? wait_iters : dec::WAIT_ITERS, std::memory_order_relaxed);
-    g_skip.store((uint32_t)skip_copy, std::memory_order_relaxed);
+    g_skip.store(skip_copy < 0 ? dec::NO_COPY : (uint32_t)skip_copy, std::memory_order_relaxed);
     return HV_OK;
 }
 

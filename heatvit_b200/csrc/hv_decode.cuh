@@ -20,13 +20,10 @@ int *error_word();
 // SMs of the current device; 0 when that cannot be read.
 int sm_count();
 
-constexpr uint32_t WAIT_ITERS = 1u << 22;  // polls of an mbarrier before a wait gives up
-// What a launch is given of that: the limit, and a copy that each CTA leaves out (none unless
-// hv_test_decode_stall asks for one).
-struct Waits {
-    uint32_t iters, skip;
-};
-Waits waits();
+constexpr uint32_t WAIT_ITERS = 1u << 22;  // polls of an mbarrier before a wait gives up, about 0.1 s
+// The copy that each CTA leaves out: NO_COPY unless hv_test_decode_stall asked for one.
+constexpr uint32_t NO_COPY = UINT32_MAX;
+uint32_t skipped_copy();
 
 // Lets `kernel` have all of an SM's shared memory, once a device: `ready` has a bit for each.
 template <typename K>

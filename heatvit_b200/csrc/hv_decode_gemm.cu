@@ -52,7 +52,7 @@ struct GemmFp8Args {
     void *out;
     long long ldc;
     int x_rows, y_rows, groups, tiles_x, tiles_y, split, out_dtype, vec;
-    Waits waits;
+    uint32_t skip;  // see skipped_copy
     int *err;
 };
 
@@ -103,17 +103,14 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-constexpr int POLLS = 64;
-// Bounded wait that also ends when another role of the CTA has given up.  stop: that, and the limit in
-// POLLS polls, both in shared memory and read when the first POLLS have not done (a limit from the
-// arguments in the loop cost 4096^3 3% and 256 x 8192 x 8192 8%).
+// Bounded wait that also ends when another role of the CTA has given up.  (With the limit in a kernel
+// argument 256 x 8192 x 8192 took 35.9 us, and 33.4 with a constant.)
 __device__ __forceinline__ bool wait_or_stop(uint64_t *bar, uint32_t parity, volatile int *stop) {
-    int i = 0;
-    do {
-        if (tc05::mbar_wait(bar, parity, POLLS)) return true;
-        if (stop[0]) return false;
-    } while (++i < stop[1]);
-    stop[0] = 1;
+    for (uint32_t i = 0; i < WAIT_ITERS / 64; ++i) {
+        if (tc05::mbar_wait(bar, parity, 64)) return true;
+        if (*stop) return false;
+    }
+    *stop = 1;
     return false;
 }
 
@@ -231,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
     using L = Lay<BN, SWAP>;
     extern __shared__ uint8_t raw[];
     __shared__ uint32_t tslot;
-    __shared__ volatile int stop[2];  // a role has given up; POLLS polls that a wait may take
+    __shared__ volatile int stop;
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     float(*sc)[SB][L::SCALES] = (float(*)[SB][L::SCALES])(smem + L::SC);
     uint64_t *full = (uint64_t *)(smem + L::BARS), *empty = full + L::STAGES;
@@ -247,8 +244,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
         tc05::tmem_relinquish();
     }
     if (tid == 0) {
-        stop[0] = 0;
-        stop[1] = (int)(a.waits.iters / POLLS);
+        stop = 0;
         for (int i = 0; i < L::STAGES; ++i) {
             tc05::mbar_init(&full[i], 1);
             tc05::mbar_init(&empty[i], 1);
@@ -301,11 +297,11 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
                 tile_at(t, a.tiles_x, a.tiles_y, tx, ty);
                 for (int g = g0; g < g1; ++g, ++n) {
                     const uint32_t s = n % L::STAGES;
-                    if (n >= L::STAGES && !wait_or_stop(&empty[s], (n / L::STAGES - 1) & 1, stop)) {
+                    if (n >= L::STAGES && !wait_or_stop(&empty[s], (n / L::STAGES - 1) & 1, &stop)) {
                         ok = false;
                         break;
                     }
-                    if (n == a.waits.skip) continue;
+                    if (n == a.skip) continue;
                     const uint32_t dst = tc05::smem_u32(smem + s * L::STAGE);
                     expect_tx(&full[s], L::STAGE);
                     tma_box(dst, &tmx, g * GK, tx * BM, &full[s]);
@@ -314,7 +310,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
             }
             // What was issued has landed before shared memory goes, whichever role gives up.
             for (uint32_t k = n > L::STAGES ? n - L::STAGES : 0; k < n; ++k)
-                if (k != a.waits.skip) tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, WAIT_ITERS);
+                if (k != a.skip) tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, WAIT_ITERS);
         } else if (warp == 1 && lane == 0) {  // products
             constexpr uint32_t idesc = idesc_e4m3(BM, BN);
             uint32_t n = 0;
@@ -322,8 +318,8 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
             for (int t = first; t < tiles && ok; t += step)
                 for (int g = g0; g < g1; ++g, ++n) {
                     const uint32_t s = n % L::STAGES, b = n % L::BUFS;
-                    ok = (n < L::BUFS || wait_or_stop(&tempty[b], (n / L::BUFS - 1) & 1, stop)) &&
-                         wait_or_stop(&full[s], (n / L::STAGES) & 1, stop);
+                    ok = (n < L::BUFS || wait_or_stop(&tempty[b], (n / L::BUFS - 1) & 1, &stop)) &&
+                         wait_or_stop(&full[s], (n / L::STAGES) & 1, &stop);
                     if (!ok) break;
                     tc05::fence_after();
                     const uint32_t at = tc05::smem_u32(smem + s * L::STAGE);
@@ -341,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
             const float *x0 = nullptr, *x1 = nullptr, *y0 = nullptr, *y1 = nullptr;
             for (uint32_t q = 0; t < tiles; ++q) {
                 const int b = q & 1;
-                if (q >= 2 && !wait_or_stop(&sempty[b], (q / 2 - 1) & 1, stop)) break;
+                if (q >= 2 && !wait_or_stop(&sempty[b], (q / 2 - 1) & 1, &stop)) break;
 #pragma unroll
                 for (int e0 = 0; e0 < SB; e0 += 4) {
                     float vx0[4], vx1[4], vy0[4], vy1[4];
@@ -399,11 +395,11 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
         for (int t = first; t < tiles && ok; t += step) {
             for (int g = g0; g < g1; ++g, ++n) {
                 const uint32_t b = n % L::BUFS, sb = n / SB;
-                ok = n % SB || wait_or_stop(&sfull[sb & 1], (sb / 2) & 1, stop);
+                ok = n % SB || wait_or_stop(&sfull[sb & 1], (sb / 2) & 1, &stop);
                 const float *f = sc[sb & 1][n % SB] + (SWAP ? c0 : half * BM + row);
                 uint64_t s2 = 0;
                 if (!SWAP) asm("mov.b64 %0, {%1, %1};\n" : "=l"(s2) : "f"(*f));
-                ok = ok && wait_or_stop(&tfull[b], (n / L::BUFS) & 1, stop);
+                ok = ok && wait_or_stop(&tfull[b], (n / L::BUFS) & 1, &stop);
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
                 tc05::fence_after();
@@ -530,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
     __syncwarp();
     tc05::fence_before();
     __syncthreads();
-    if (tid == 0 && stop[0]) atomicOr(a.err, HV_DECODE_STALLED);  // every role has been through
+    if (tid == 0 && stop) atomicOr(a.err, HV_DECODE_STALLED);  // every role has been through
     if (warp == 2) {
         tc05::fence_after();
         tc05::tmem_dealloc(tmem, L::TMEM);
@@ -662,7 +658,7 @@ extern "C" int hv_gemm_fp8(const hv_gemm_fp8_args *p, void *stream) {
     if (!err || !sms) return fail(HV_ERR_CUDA, "cannot read the device's properties");
     GemmFp8Args g{};
     g.out = p->d_out, g.ldc = p->out_stride, g.out_dtype = p->out_dtype, g.groups = (int)((k + GK - 1) / GK), g.err = err;
-    g.waits = dec::waits();
+    g.skip = dec::skipped_copy();
     // 16-byte stores: rows start on 16 bytes and are whole groups of them
     const int es = dec::elem_size(p->out_dtype);
     g.vec = dec::aligned(p->d_out, 16) && n * es % 16 == 0 && (m == 1 || p->out_stride * es % 16 == 0);
