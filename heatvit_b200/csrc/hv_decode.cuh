@@ -20,7 +20,10 @@ int *error_word();
 // SMs of the current device; 0 when that cannot be read.
 int sm_count();
 
-constexpr uint32_t WAIT_ITERS = 1u << 22;  // polls of an mbarrier before a wait gives up, about 0.1 s
+// Polls of an mbarrier before a wait gives up: a poll takes 4 us where bytes of a copy are missing and 24 ns
+// where nobody has arrived, so 1 s and 6 ms (2^22 polls held the GPU for 17 s).  Then, before memory goes,
+// for what is under way, which has had that long already.
+constexpr uint32_t WAIT_ITERS = 1u << 18, DRAIN_ITERS = 1u << 14;
 // The copy that each CTA leaves out: NO_COPY unless hv_test_decode_stall asked for one.
 constexpr uint32_t NO_COPY = UINT32_MAX;
 uint32_t skipped_copy();

@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
             }
             // What was issued has landed before shared memory goes, whichever role gives up.
             for (uint32_t k = n > L::STAGES ? n - L::STAGES : 0; k < n; ++k)
-                if (k != a.skip) tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, WAIT_ITERS);
+                if (k != a.skip) tc05::mbar_wait(&full[k % L::STAGES], (k / L::STAGES) & 1, DRAIN_ITERS);
         } else if (warp == 1 && lane == 0) {  // products
             constexpr uint32_t idesc = idesc_e4m3(BM, BN);
             uint32_t n = 0;
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, Lay<BN, SWAP>::PER_SM)
                     tc05::commit(&tfull[b]);
                 }
             tc05::commit(drain);  // and what was issued has read it, and written tensor memory
-            tc05::mbar_wait(drain, 0, WAIT_ITERS);
+            tc05::mbar_wait(drain, 0, DRAIN_ITERS);
         } else if (warp >= 2) {  // scales (their loads in the adding warps made those wait: 711 us, 8192^3)
             const int r = tid - 64;  // row r and r + 64, or column r
             int t = first, g = g0;

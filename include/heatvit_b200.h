@@ -410,11 +410,12 @@ HV_API int hv_selector_h2(hv_model *model, int selector_index, const int8_t *d_x
 /* Read and clear the current device's error word (synchronises with the device). */
 HV_API int hv_decode_error(int *bits);
 
-/* Test hook: in GEMM calls made from now on, by any thread, every CTA leaves its copy number
- * `skip_copy` (of those it makes one after another) out, so that the waits on it run out (after about
- * 0.1 s).  The launch stops issuing work, waits for the copies and tensor-core operations under way,
- * releases its TMEM and sets HV_DECODE_STALLED.  Nothing faults and the context stays usable.
- * skip_copy = -1 restores normal operation. */
+/* Test hook: in calls made from now on, by any thread, every CTA of the GEMM leaves its copy number
+ * `skip_copy` (of those it makes one after another) out, and the norm of many long rows waits for 16
+ * bytes that do not come, so that waits run out (within about 1 s).  The launch stops issuing work,
+ * waits for the copies and tensor-core operations under way, releases its TMEM and sets
+ * HV_DECODE_STALLED.  Nothing faults and the context stays usable.  skip_copy = -1 restores normal
+ * operation. */
 HV_API int hv_test_decode_stall(int skip_copy);
 
 /* h = x + residual; residual_out = h; y = h * rsqrt(mean(h^2) + eps) * weight, and y in e4m3

@@ -5,6 +5,7 @@ Bounds are derived as in test_decode_gpu, whose helpers are used."""
 import math
 import os
 import sys
+import time
 
 import pytest
 
@@ -271,12 +272,36 @@ def test_gemm_wait_runs_out_reports_and_recovers(stall, m, n, k, copy):
     good = decode.gemm_fp8(a, sa, b, sb)
     assert decode.device_error() == 0
     stall(copy)
+    start = time.monotonic()
     decode.gemm_fp8(a, sa, b, sb)
     assert decode.device_error() == abi.HV_DECODE_STALLED
+    assert time.monotonic() - start < 5
     assert decode.device_error() == 0  # reading clears the word
     stall(-1)
     for _ in range(2):
         assert torch.equal(decode.gemm_fp8(a, sa, b, sb), good)
+        assert decode.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,rows,dim,residual", [(BF, 1300, 2048, True), (FF, 700, 5000, True), (HF, 1300, 8192, False),
+                                                     (BF, 600, 16384, True)])
+def test_norm_wait_runs_out_reports_and_recovers(stall, dtype, rows, dim, residual):
+    """Rows that never come into the ring whole: the call returns and says so, and the next one is as it was."""
+    from heatvit_b200 import abi, decode
+    x, w = rand(1, rows, dim, dtype=dtype), rand(3, dim, dtype=dtype)
+    res = rand(2, rows, dim, dtype=dtype) if residual else None
+    good = decode.add_rmsnorm_fp8(x, w, residual=res)
+    assert decode.device_error() == 0
+    stall(0)
+    start = time.monotonic()
+    decode.add_rmsnorm_fp8(x, w, residual=res)
+    assert decode.device_error() == abi.HV_DECODE_STALLED
+    assert time.monotonic() - start < 5
+    stall(-1)
+    for _ in range(2):
+        r = decode.add_rmsnorm_fp8(x, w, residual=res)
+        assert torch.equal(r.q.view(torch.uint8), good.q.view(torch.uint8)) and torch.equal(r.scale, good.scale)
+        assert not residual or torch.equal(r.residual, good.residual)
         assert decode.device_error() == 0
 
 
