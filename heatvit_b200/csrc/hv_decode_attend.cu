@@ -159,10 +159,11 @@ __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t p, __
     return pack(lo - v.x, hi - v.y, t);
 }
 
-// Live tokens of sequence b: never beyond what its page table row can name.
+// Live tokens of sequence b: never beyond what its page table row can name, and so few that
+// the end of their last tile is an int as well.
 __device__ __forceinline__ int length_of(const AttendArgs &a, int b) {
     const int n = max(a.lens[b], 0);
-    const long long cap = (long long)a.max_pages * a.page;
+    const long long cap = min((long long)a.max_pages * a.page, (long long)HV_ATTENTION_MAX_LENGTH);
     if (n > cap) {
         atomicOr(a.err, HV_DECODE_BAD_LENGTH);
         return (int)cap;
@@ -721,6 +722,8 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
 // The counters come first and take the same room for every call, so that calls of other
 // sizes with the same workspace never find a part where a zero belongs.
 constexpr int COUNT_BYTES = 3 * MAX_GRID * 4;
+static_assert(HV_ATTENTION_MAX_LENGTH + (long long)Lay<64>::TILE + ROWS <= INT32_MAX && Lay<64>::TILE >= Lay<128>::TILE,
+              "token numbers of a last tile are ints");
 static_assert(COUNT_BYTES == HV_ATTENTION_COUNTER_BYTES, "what the caller zeroes");
 
 // CTAs of one resident wave on the current device.

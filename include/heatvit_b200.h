@@ -404,7 +404,7 @@ HV_API int hv_selector_h2(hv_model *model, int selector_index, const int8_t *d_x
 #define HV_DECODE_BAD_PAGE 1     /* a page table entry outside [0, num_pages): not read, not written */
 #define HV_DECODE_BAD_POSITION 2 /* a position or sequence past the page table (its key and value are not
                                     stored) or the rotation table (nor is its q_out row) */
-#define HV_DECODE_BAD_LENGTH 4   /* a length above max_pages * page_size: taken as that */
+#define HV_DECODE_BAD_LENGTH 4   /* a length above max_pages * page_size or HV_ATTENTION_MAX_LENGTH: taken as that */
 #define HV_DECODE_STALLED 8      /* a bounded wait gave up: that call's output is invalid */
 
 /* Read and clear the current device's error word (synchronises with the device). */
@@ -481,6 +481,7 @@ HV_API int hv_append_kv(const hv_append_args *args, void *stream);
  * HV_ATTENTION_COUNTER_BYTES of them zeroed once after it is allocated (every call leaves zeros
  * there); calls of any sizes may share it one after another, calls that overlap in time not. */
 #define HV_ATTENTION_COUNTER_BYTES 12288
+#define HV_ATTENTION_MAX_LENGTH 2147483392 /* 2^31 - 256 */
 typedef struct hv_attention_args {
     const void *d_q;                   /* [seqs][heads][dim] */
     void *d_out;                       /* [seqs][heads][dim] */

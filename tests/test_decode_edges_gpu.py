@@ -82,6 +82,26 @@ def test_attention_equal_weights_between_two_numbers(dtype, step, heads, kv, dim
     assert bool(((lse.double() - want_lse).abs() <= 1e-4 + 2.0 ** -18 * want_lse.abs()).all())
 
 
+@pytest.mark.parametrize("n", [(1 << 31) - 256, (1 << 31) - 1])
+def test_attention_length_at_the_end_of_its_type(n):
+    """The longest cache that lengths can name, on one page that the table repeats; above 2^31 - 256, that, reported."""
+    from heatvit_b200 import abi, decode
+    page, dim, most = 1 << 16, 32, (1 << 31) - 256
+    kc = rand(1, 1, page, 1, dim, dtype=BF)
+    vc = torch.randint(-1, 3, (1, page, 1, dim), generator=torch.Generator().manual_seed(2)).cuda().to(BF)
+    table = torch.zeros(1, 1 << 15, dtype=torch.int32, device="cuda")
+    q = torch.zeros(1, 2, dim, dtype=BF, device="cuda")  # equal weights: every warp's sums are whole numbers under 2^24
+    out, lse = decode.paged_attention(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                      return_lse=True)
+    assert decode.device_error() == (abi.HV_DECODE_BAD_LENGTH if n > most else 0)
+    v = vc.view(page, dim).double()
+    want = (v.sum(0) * (most // page) + v[:most % page].sum(0)) / most
+    # warps' sums joined in 32 bits (a few hundred additions), then one rounding
+    error = 2.0 ** -14 * 2
+    assert bool(((out[0].double() - want).abs() <= (want.to(BF).double() - want).abs() + 2 * error).all())
+    assert bool(((lse.double() - math.log(most)).abs() <= 1e-4).all())
+
+
 # ---- attention: workspaces ----------------------------------------------------------
 
 def test_new_workspace_zeroes_its_counters_alone():
