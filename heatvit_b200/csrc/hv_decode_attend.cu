@@ -149,14 +149,29 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
     return *(uint32_t *)&v;
 }
 
-// What a rounded pair of weights leaves of (lo, hi), rounded in turn: the two together are
-// within 2^-16 of a weight (bf16; fp16 2^-22).
+// What a number of T that stands for a weight leaves of it, rounded in turn, for a pair: the two
+// together are within 2^-16 of a weight (bf16; fp16 2^-22, and 2^-25).
 __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t p, __nv_bfloat16 t) {
     return pack(lo - __uint_as_float(p << 16), hi - __uint_as_float(p & 0xffff0000u), t);
 }
 __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t p, __half t) {
     const float2 v = __half22float2(*(const __half2 *)&p);
     return pack(lo - v.x, hi - v.y, t);
+}
+// A number of T a little under a weight, for a pair, so that what it leaves is above zero and not
+// rounded to it: both times infinity are then that infinity, and not 0 * inf or inf - inf.  (fp16
+// weights under 2^-24 are zeros either way.)
+__device__ __forceinline__ uint32_t pack_under(float lo, float hi, __nv_bfloat16) {
+    constexpr float F = 1.f - 0x1p-20f;
+    uint32_t p;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;\n" : "=r"(p) : "f"(hi * F), "f"(lo * F));
+    return p;
+}
+__device__ __forceinline__ uint32_t pack_under(float lo, float hi, __half) {
+    constexpr float F = 1.f - 0x1p-22f, D = 0x1.01p-25f;
+    uint32_t p;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;\n" : "=r"(p) : "f"(fmaf(hi, F, -D)), "f"(fmaf(lo, F, -D)));
+    return p;
 }
 
 // Live tokens of sequence b: never beyond what its page table row can name, and so few that
@@ -595,9 +610,11 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
                 const float(&x)[4] = s[2 * b], (&y)[4] = s[2 * b + 1];
-                const uint32_t x0 = pack(x[0], x[1], T()), y0 = pack(y[0], y[1], T());
+                const uint32_t x0 = HALF ? pack(x[0], x[1], T()) : pack_under(x[0], x[1], T());
+                const uint32_t y0 = HALF ? pack(y[0], y[1], T()) : pack_under(y[0], y[1], T());
                 const uint32_t x0r = pack_rest(x[0], x[1], x0, T()), y0r = pack_rest(y[0], y[1], y0, T());
-                const uint32_t x1 = HALF ? x0r : pack(x[2], x[3], T()), y1 = HALF ? y0r : pack(y[2], y[3], T());
+                const uint32_t x1 = HALF ? x0r : pack_under(x[2], x[3], T());
+                const uint32_t y1 = HALF ? y0r : pack_under(y[2], y[3], T());
                 const uint32_t p[4] = {x0, x1, y0, y1};
                 const uint32_t va = vb + (b * BLOCK + (lane & 15)) * L::ROW + (lane >> 4) * 16;
 #pragma unroll
@@ -642,7 +659,10 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, Lay<D>::PER_SM)
             float *mine = (float *)(ring + (u % L::STAGES) * L::STAGE);  // read, and not yet refilled
 #pragma unroll
             for (int j = 0; j < DH / 8; ++j) {
-                if (HALF) o[j][0] += o[j][2], o[j][1] += o[j][3];
+                if (HALF) {  // an infinity stays: the rest may have had a zero or another sign for it
+                    if (!isinf(o[j][0])) o[j][0] += o[j][2];
+                    if (!isinf(o[j][1])) o[j][1] += o[j][3];
+                }
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
                     *(float2 *)(mine + ((lane >> 2) + 8 * i) * L::PART_ROW + j * 8 + (lane & 3) * 2) =

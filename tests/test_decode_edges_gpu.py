@@ -82,6 +82,28 @@ def test_attention_equal_weights_between_two_numbers(dtype, step, heads, kv, dim
     assert bool(((lse.double() - want_lse).abs() <= 1e-4 + 2.0 ** -18 * want_lse.abs()).all())
 
 
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 1, 128), (2, 2, 256), (9, 1, 64), (32, 2, 128), (20, 1, 256)])
+@pytest.mark.parametrize("n,equal", [(1, True), (70, True), (70, False), (3000, False)])
+def test_attention_infinite_values(dtype, heads, kv, dim, n, equal):
+    """An infinity among the values of live tokens is the output's, as in the formula, whatever its weight rounds
+    to (one and halves among them); two of either sign, or a NaN, make a NaN."""
+    from heatvit_b200 import decode
+    q, kc, vc, table = G.attend_case(9, [n] * 4, heads, kv, dim, 16, dtype, "nhd")
+    if equal:
+        q.zero_()
+    q[:, :, :8] *= 0.25
+    at = lambda b, t: (table[b, t // 16].long(), t % 16)  # noqa: E731
+    vc[at(0, n // 2)] = math.inf
+    vc[at(1, n - 1)] = -math.inf
+    vc[at(2, 0)], vc[at(2, n - 1)] = math.inf, -math.inf
+    if n == 1:
+        vc[at(2, 0)] = math.nan
+    out = decode.paged_attention(q, kc, vc, table, torch.full((4,), n, dtype=torch.int32, device="cuda"), scale=0.02)
+    assert bool((out[0] == math.inf).all()) and bool((out[1] == -math.inf).all()) and bool(out[2].isnan().all())
+    assert bool(out[3].isfinite().all())
+
+
 @pytest.mark.parametrize("n", [(1 << 31) - 256, (1 << 31) - 1])
 def test_attention_length_at_the_end_of_its_type(n):
     """The longest cache that lengths can name, on one page that the table repeats; above 2^31 - 256, that, reported."""
