@@ -6,7 +6,9 @@ its pruned tokens, one new token a step.
 The encoder is the benchmark model with its selectors, so that each image keeps another number
 of tokens.  Those, as the last block leaves them, become the first entries of a paged cache of
 keys and values in every decoder layer; a step then runs each layer with the operators of
-heatvit_b200.decode.  The decoder's weights are random: it shows the calls, not a caption.
+heatvit_b200.decode.  The decoder's weights are random: it shows the calls, not a caption.  The
+image's tokens do not see one another in the decoder: every layer's entries are projections of
+what the first layer is given, since the operators have no attention over a prompt's own tokens.
 """
 
 import argparse
@@ -63,6 +65,7 @@ class Decoder:
         first = torch.cumsum(counts, 0) - counts
         ids = torch.repeat_interleave(torch.arange(len(counts), device="cuda"), counts.long())
         positions = (torch.arange(len(ids), device="cuda") - first[ids]).int()
+        # the codes as plain numbers: the power of two that they all share goes out in the norm
         x = self.image(decode.add_rmsnorm_fp8(tokens.bfloat16(), self.image_one))
         rows = decode.add_rmsnorm_fp8(x, self.one)
         for i in range(self.layers):

@@ -6,7 +6,8 @@
 // Bound by HBM: each live key and value is read once, for up to 16 query heads that share
 // it.  Those heads are the 16 rows of an m16n8k16 matrix product: at 23 bytes of cache an
 // SM clock, 16 multiply-adds an element leave the warp-level tensor path under a fifth
-// busy, and it needs none of the 128 rows that a tcgen05 tile would pad to.
+// busy, and it needs none of the 128 rows that a tcgen05 tile would pad to.  (More heads read
+// the cache again for every 16: 32 x 4000 tokens, 16 heads over one 23 us, 32 over one 35.)
 //
 // Work: the (sequence, head tile) items are cut into tiles of 64 tokens (128 for heads of up
 // to 64 dimensions), the tiles of all items are laid end to end, and the CTAs of one resident
@@ -20,10 +21,11 @@
 // workspace, and the CTA that finishes last joins the parts in the order of the shares: the
 // result does not depend on which that is.
 //
-// Measured on one B200, bf16: 64 sequences of 0 to 8192 tokens (32 heads of 128 over 8) 187 us,
-// 5.76 TB/s of the cache; two of 131071 (64 over 8) 190 us, 5.65 TB/s.  CTAs stream for 150 to
-// 170 us of that; the rest is what the latest of them join.  One sequence of 197 tokens, 7.9 us:
-// length, page, key, join, each a memory latency after the other.
+// Measured on one B200, bf16, in bursts: 64 sequences of 0 to 8192 tokens (32 heads of 128 over 8)
+// 182 us, 5.9 TB/s of the cache (201 when calls follow one another for long); two of 131071 (64 over
+// 8) 187 us, 5.7 TB/s.  CTAs stream for 150 to 170 us of that; the rest is what the latest of them
+// join.  One sequence of 197 tokens, 5.7 us: length, page, key, join, each a memory latency after the
+// other.  (A workspace made outside the graph; a captured call that makes its own takes 1 us more.)
 #include <math_constants.h>
 
 #include "hv_decode.cuh"
@@ -42,8 +44,9 @@ constexpr float LOWEST = -3.402823466e38f;
 // us with one, 10.7 with two, 13.0 with four; one of 197, heads of 64: 9.1, 8.2, 11.8.
 constexpr int MIN_SHARE = 2;
 // Tiles that a share may grow by so that items of one length end where shares do and none is cut.
-// 32 sequences of 512 tokens (32 heads of 128 over 8; shares of 7, items of 8) 24.8 -> 20.8 us, 64
-// of 512 (14, 16) 38.5 -> 34.0.  By four, 16 of 512 (4, 8) would go from 16.0 to 18.9.
+// Sequences of one length, 32 heads of 128 over 8, without and with it: 32 of 512 tokens (shares of 7,
+// items of 8) 22.1 and 18.0 us, 64 of 512 (14, 16) 35.6 and 31.8, 24 of 384 (4, 6) 17.1 and 14.3, 22 of
+// 320 (3, 5) 15.4 and 12.3.  By four, 16 of 512 (4, 8) took 18.9 instead of 16.0.
 constexpr int SLACK = 2;
 // A row's weights are taken beside a reference that makes its largest 2^TOP when it is set, and that moves
 // when one passes it by more than 2^SOFT.  fp16 has normal numbers from 2^-14 to 2^15 and none under 2^-24: its
@@ -87,6 +90,7 @@ struct Lay {
     static constexpr int ROW = DH * 2 + 16;  // bytes: rows 16 bytes apart modulo 128 (ldmatrix without conflicts)
     // Three CTAs an SM of two stages where registers allow, else two of three: 16 heads of 64 took
     // 223 us as two of three, 186 as three of two; heads of 128 spill at 168 registers (187, 381).
+    // (So do 64 bytes of heads of 64 in groups of over eight.)
     static constexpr int PER_SM = D <= 64 ? 3 : D <= 128 ? 2 : 1, STAGES = D <= 64 ? 2 : 3;
     static constexpr int STAGE = 2 * WTOK * ROW;
     static constexpr int PART_ROW = DH + 4;  // a warp's sums at an item's end, where its last stage was

@@ -18,13 +18,13 @@
 // Y = A, so that the 128 rows that an MMA has anyway are weights; split as well, two CTAs an SM;
 // the time is that of reading the weights once.
 //
-// Measured on one B200: 8192^3 542 to 590 us in bursts (up to 2.03 PFLOP/s; 630 to 660 us, at
-// 1.5 GHz, when it runs on at the power limit), 4096^3 81 us.  Without the adds the wide form
+// Measured on one B200: 8192^3 550 to 590 us in bursts (up to 2.0 PFLOP/s; 630 to 665 us, at
+// 1.5 GHz, when it runs on at the power limit), 4096^3 83 us.  Without the adds the wide form
 // takes 455 us, with one MMA in four 325: its operands come at 70 bytes an SM clock.  Tiles of
 // 256 x 256 over CTA pairs (cta_group::2) move a third less and took as long (536 us, 648 at the
 // power limit), an accumulator's way to the other CTA and back being longer.  48 x 10240 x 4096
-// 15.0 us (2.9 TB/s of weights: five to the first sums, six to stream, four to join), 1 x 4096 x
-// 4096 6.9 us, 1576 x 768 x 192 4.6 us.
+// 15.1 us (2.9 TB/s of weights: five to the first sums, six to stream, four to join; 16 bytes of its 80
+// registers spill), 1 x 4096 x 4096 6.7 us, 1576 x 768 x 192 4.6 us.
 //
 // Every mbarrier wait is bounded: after a timeout the CTA waits for what it has in flight,
 // releases its TMEM and, when all of its roles are through, sets the device's error word.

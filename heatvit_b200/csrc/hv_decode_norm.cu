@@ -14,10 +14,12 @@
 // 1024 channels take a warp each, longer ones a CTA; many long ones go through a ring of bulk
 // copies (see norm_ring_kernel).
 //
-// Measured on one B200: 16384 x 8192 bf16 with residual 146 us, 6.48 TB/s, the rate of a plain
-// copy; 1999 x 5000 fp32 26.5 us (4.9 TB/s: seven rows a CTA, of which filling and emptying
-// the ring is one); 8192 x 8192 fp16 without residual 49 us, where half of the issue slots
-// convert; 8 x 4096 1.8 us, the launch.
+// Measured on one B200, in bursts: 16384 x 8192 bf16 with residual 146 us, 6.48 TB/s, the rate of a
+// plain copy (164 us, 5.7 TB/s, when calls follow one another for long and the memory slows down);
+// 1999 x 5000 fp32 26.6 us (4.9 TB/s: 13 or 14 rows a CTA, and filling and emptying the ring);
+// 8192 x 8192 fp16 without residual 49 us, where half of the issue slots convert; 4096 x 32768 bf16
+// 207 us (4.5 TB/s: rows over 16384 channels take 1024 threads of 64 registers, which spill 112 to
+// 756 bytes); 8 x 4096 1.8 us, the launch.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -357,8 +359,8 @@ cudaError_t launch(const NormArgs &a, int sms, cudaStream_t st) {
 }
 
 // CTAs of an SM and stages of a ring: enough threads to keep up (16-bit rows with a residual
-// 512 an SM, without one twice as many, float32 half), and 64 KB ahead an SM (128 where one CTA
-// has it): 32768 x 2048 bf16 took 72 us with 64 KB, 83 with 96 and 94 with 128.
+// 512 an SM, without one twice as many, float32 half of those, but one CTA at least: float32 rows of
+// over 4096 channels have 512), and 64 KB ahead an SM (128 where one CTA has it): 32768 x 2048 bf16 took 72 us with 64 KB, 83 with 96 and 94 with 128.
 template <typename T, int THREADS, int NV>
 cudaError_t launch_ring(const NormArgs &a, int sms, int row_bytes, int *err, cudaStream_t st) {
     const auto kernel = a.res ? norm_ring_kernel<T, THREADS, NV, true> : norm_ring_kernel<T, THREADS, NV, false>;
@@ -366,7 +368,8 @@ cudaError_t launch_ring(const NormArgs &a, int sms, int row_bytes, int *err, cud
     const int per_sm = std::max(1, (a.res ? 512 : 1024) * 2 / (int)sizeof(T) / THREADS);
     const int ahead = (per_sm > 1 ? 64 : 128) * 1024 / (per_sm * stage);
     const int stages = std::max(2, std::min(MAX_STAGES, ahead)), smem = stages * stage;
-    // with hv_test_decode_stall 16 bytes more, which do not come (a row left out by the kernel costs 16384 x 8192 1.5%)
+    // with hv_test_decode_stall 16 bytes more, which do not come (a test in the kernel for a row to leave
+    // out took 1.5% of 16384 x 8192)
     const uint32_t expect = row_bytes * (a.res ? 2 : 1) + (skipped_copy() == NO_COPY ? 0 : 16);
     static std::atomic<uint64_t> ready[2];
     const cudaError_t e = allow_shared(kernel, ready[a.res != nullptr]);
