@@ -83,6 +83,30 @@ def test_attention_equal_weights_between_two_numbers(dtype, step, heads, kv, dim
 
 
 @pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (12, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("where", ["first", "middle", "none"])
+def test_attention_long_tail_over_many_parts(dtype, heads, kv, dim, where):
+    """One sequence over every SM: the parts, one of which holds a token that outweighs its tail 1000 times, have
+    references of their own."""
+    n = 100000
+    scores = rand(1, n, scale=0.5)
+    v = 1 + rand(2, n, dim)
+    if where != "none":
+        at = 0 if where == "first" else n // 2 + 5
+        scores[at] = math.log(n) + math.log(1000.0)
+        v[at] = 0
+    out, lse, want, want_lse, bound = scored(scores, v, dtype, heads, kv, dim, 1)
+    assert bool(((out.double() - want).abs() <= bound).all()), float(((out.double() - want).abs() / bound).max())
+    assert bool(((lse.double() - want_lse).abs() <= 1e-4 + 2.0 ** -18 * want_lse.abs()).all())
+
+
+@pytest.mark.parametrize("lens", [[100000, 3], [40000, 0, 777, 12345]])
+def test_attention_long_fp16(lens):
+    q, kc, vc, table = G.attend_case(3, lens, 4, 1, 128, 32, HF, "hnd", poison=False)
+    G.check_attention(q, kc, vc, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
 @pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 1, 128), (2, 2, 256), (9, 1, 64), (32, 2, 128), (20, 1, 256)])
 @pytest.mark.parametrize("n,equal", [(1, True), (70, True), (70, False), (3000, False)])
 def test_attention_infinite_values(dtype, heads, kv, dim, n, equal):
