@@ -58,6 +58,10 @@ _SIGNATURES = {
     "hv_append_kv": (I, [P, P]),
     "hv_paged_attention_workspace": (I, [I, C.POINTER(I64)]),
     "hv_paged_attention": (I, [P, P]),
+    "hv_norm_append_kv": (I, [P, P]),
+    "hv_paged_chunk_attention_workspace": (I, [I, C.POINTER(I64)]),
+    "hv_paged_chunk_attention": (I, [P, P]),
+    "hv_sample_tokens": (I, [P, P]),
 }
 
 

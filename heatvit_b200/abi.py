@@ -43,6 +43,8 @@ HV_DECODE_BAD_PAGE = 1
 HV_DECODE_BAD_POSITION = 2
 HV_DECODE_BAD_LENGTH = 4
 HV_DECODE_STALLED = 8
+HV_DECODE_BAD_LOGITS = 16
+HV_DECODE_BAD_START = 32
 
 WARN_HEAD_DEN_ZERO = 1
 WARN_PACKAGE_DEN_ZERO = 2

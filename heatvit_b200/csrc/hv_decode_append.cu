@@ -46,6 +46,7 @@ struct Tensor {
     int head, to_head, heads, rot, cached;
     uint32_t strips, total;  // threads: tokens * strips * places
     Divider by_token, by_place;
+    int lanes;  // of a head, where a norm adds up its squares
 };
 
 struct AppendArgs {
@@ -58,6 +59,9 @@ struct AppendArgs {
     int num_pages, seqs, max_pages, table_rows, rot;
     Divider by_page;
     int *err;
+    const void *weight[3];  // of the norms ahead of the rotation; null: none
+    float eps;
+    int dim;
 };
 
 constexpr int THREADS = 256;
@@ -163,6 +167,236 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__
     }
 }
 
+// Where a cached head of this token goes: its page and slot, -1 after a mistake, which is reported.
+__device__ __forceinline__ long long cached_at(const AppendArgs &a, const Tensor &t, unsigned tok, int pos) {
+    const int s = a.seq_ids ? a.seq_ids[tok] : (int)tok;
+    const int col = a.by_page(pos), slot = pos - col * a.by_page.d;
+    if (s < 0 || s >= a.seqs || col >= a.max_pages) {
+        atomicOr(a.err, HV_DECODE_BAD_POSITION);
+        return -1;
+    }
+    const int pg = a.pages[s * a.pages_stride + col];
+    if (pg < 0 || pg >= a.num_pages) {
+        atomicOr(a.err, HV_DECODE_BAD_PAGE);
+        return -1;
+    }
+    return pg * t.page + slot * t.slot;
+}
+
+// With a norm of each head ahead of the rotation: y = x * rsqrt(mean(x^2) + eps) * weight.  The
+// lanes of a head, a power of two of them, add up their squares; places as in append_kernel, one to a lane.
+template <typename T, bool INTER, int NH>
+__global__ void __launch_bounds__(THREADS) norm_append_kernel(const __grid_constant__ AppendArgs a) {
+    griddep_wait();
+    griddep_launch();
+    constexpr int W = 8;
+    const int which = (blockIdx.x >= a.first[1]) + (blockIdx.x >= a.first[2]);
+    const Tensor &t = a.t[which];
+    const unsigned id = (blockIdx.x - a.first[which]) * THREADS + threadIdx.x;
+    const bool exists = id < t.total;
+    const unsigned tok = exists ? t.by_token(id) : 0, in = exists ? id - tok * t.by_token.d : 0;
+    const int lanes = t.lanes, strip = in / lanes, u = in & (lanes - 1);
+    const int half = t.rot / 2;
+    constexpr bool PAIRED = !INTER;
+    const int rotated = PAIRED ? half / W : t.rot / W;
+    const bool works = exists && u < rotated + (a.dim - t.rot) / W;
+    const bool turned = works && u < rotated, two = PAIRED && turned;
+    const int c0 = !works ? 0 : !turned && PAIRED ? t.rot + (u - rotated) * W : u * W;
+    const int n = works ? min((t.heads - strip + (int)t.strips - 1) / (int)t.strips, NH) : 0;
+
+    const T *src = (const T *)t.from + (tok * t.tok + (long long)strip * t.head + c0);
+    Elems<T, W> x[NH], y[NH], wx, wy;
+#pragma unroll
+    for (int j = 0; j < NH; ++j)
+        if (j < n) {
+            const T *p = src + (long long)(j * (int)t.strips) * t.head;
+            x[j].load(p);
+            if (two) y[j].load(p + half);
+        }
+    const T *weight = (const T *)a.weight[which];
+    const int pos = works ? a.positions[tok] : -1;
+    float inv[NH];
+    if (weight) {
+        if (works) {
+            wx.load(weight + c0);
+            if (two) wy.load(weight + c0 + half);
+        }
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+            float s = 0.f;
+            if (j < n) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) s += to_f32(x[j].e[i]) * to_f32(x[j].e[i]);
+                if (two)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) s += to_f32(y[j].e[i]) * to_f32(y[j].e[i]);
+            }
+            for (int o = lanes / 2; o; o /= 2) s += __shfl_xor_sync(~0u, s, o);
+            inv[j] = rsqrtf(s / (float)a.dim + a.eps);
+        }
+    }
+    if (!works) return;
+    const bool live = pos >= 0;
+    if (a.rot && pos >= a.table_rows) {
+        atomicOr(a.err, HV_DECODE_BAD_POSITION);
+        return;
+    }
+    constexpr int NA = INTER ? 4 : W;
+    alignas(16) float cs[NA], sn[NA];
+    if (turned && live) {
+        const float *tab = a.table + pos * a.table_stride + (INTER ? c0 / 2 : c0);
+#pragma unroll
+        for (int i = 0; i < NA; i += 4) {
+            *(float4 *)(cs + i) = *(const float4 *)(tab + i);
+            *(float4 *)(sn + i) = *(const float4 *)(tab + half + i);
+        }
+    }
+    T *dst = (T *)t.to + ((long long)strip * t.to_head + c0);
+    if (t.cached) {
+        if (!live) return;
+        const long long at = cached_at(a, t, tok, pos);
+        if (at == -1) return;
+        dst += at;
+    } else {
+        dst += tok * t.to_tok;
+    }
+#pragma unroll
+    for (int j = 0; j < NH; ++j) {
+        if (j >= n) break;
+        if (!live) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) x[j].e[i] = y[j].e[i] = from_f32<T>(0.f);
+        } else if (weight || turned) {
+            float fx[W], fy[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                fx[i] = to_f32(x[j].e[i]);
+                if (weight) fx[i] = fx[i] * inv[j] * to_f32(wx.e[i]);
+                if (two) {
+                    fy[i] = to_f32(y[j].e[i]);
+                    if (weight) fy[i] = fy[i] * inv[j] * to_f32(wy.e[i]);
+                }
+            }
+            if (turned) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    float &p = PAIRED ? fx[i] : fx[(2 * i) % W], &w = PAIRED ? fy[i] : fx[(2 * i + 1) % W];
+                    const float fp = p, fw = w;
+                    p = fp * cs[i] - fw * sn[i];
+                    w = fp * sn[i] + fw * cs[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                x[j].e[i] = from_f32<T>(fx[i]);
+                if (two) y[j].e[i] = from_f32<T>(fy[i]);
+            }
+        }
+        T *p = dst + (long long)(j * (int)t.strips) * t.to_head;
+        x[j].store(p);
+        if (two) y[j].store(p + half);
+    }
+}
+
+// The same for sizes and alignments that 16-byte accesses or 32 lanes of them do not cover: a
+// warp a head, an element or a pair a lane, the head read again (from L1) for the result.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) norm_append_any_kernel(const __grid_constant__ AppendArgs a, int inter) {
+    griddep_wait();
+    griddep_launch();
+    const int which = (blockIdx.x >= a.first[1]) + (blockIdx.x >= a.first[2]);
+    const Tensor &t = a.t[which];
+    const unsigned id = ((blockIdx.x - a.first[which]) * THREADS + threadIdx.x) / 32, lane = threadIdx.x % 32;
+    if (id >= t.total) return;  // of warps
+    const unsigned tok = t.by_token(id);
+    const int head = id - tok * t.by_token.d, half = t.rot / 2;
+    const T *src = (const T *)t.from + (tok * t.tok + (long long)head * t.head);
+    const T *weight = (const T *)a.weight[which];
+    float inv = 1.f;
+    if (weight) {
+        float s = 0.f;
+        for (int i = lane; i < a.dim; i += 32) s += to_f32(src[i]) * to_f32(src[i]);
+        for (int o = 16; o; o /= 2) s += __shfl_xor_sync(~0u, s, o);
+        inv = rsqrtf(s / (float)a.dim + a.eps);
+    }
+    const int pos = a.positions[tok];
+    const bool live = pos >= 0;
+    if (a.rot && pos >= a.table_rows) {
+        if (lane == 0) atomicOr(a.err, HV_DECODE_BAD_POSITION);
+        return;
+    }
+    T *dst = (T *)t.to + (long long)head * t.to_head;
+    if (t.cached) {
+        if (!live) return;
+        const long long at = cached_at(a, t, tok, pos);
+        if (at == -1) return;
+        dst += at;
+    } else {
+        dst += tok * t.to_tok;
+    }
+    const float *tab = a.table + (live ? pos : 0) * a.table_stride;
+    auto normed = [&](int i) {
+        const float v = to_f32(src[i]);
+        return weight ? v * inv * to_f32(weight[i]) : v;
+    };
+    for (int i = lane; i < half; i += 32) {
+        const int c0 = inter ? 2 * i : i, c1 = inter ? 2 * i + 1 : i + half;
+        float p = 0.f, w = 0.f;
+        if (live) {
+            const float fp = normed(c0), fw = normed(c1), cs = tab[i], sn = tab[half + i];
+            p = fp * cs - fw * sn;
+            w = fp * sn + fw * cs;
+        }
+        dst[c0] = from_f32<T>(p);
+        dst[c1] = from_f32<T>(w);
+    }
+    for (int i = t.rot + lane; i < a.dim; i += 32) dst[i] = !live ? from_f32<T>(0.f) : weight ? from_f32<T>(normed(i)) : src[i];
+}
+
+template <typename T, bool INTER, int NH>
+int launch_norm(AppendArgs &a, int tokens, cudaStream_t st) {
+    uint32_t blocks = 0;
+    for (int i = 0; i < 3; ++i) {
+        Tensor &t = a.t[i];
+        const int places = (INTER ? t.rot : t.rot / 2) / 8 + (a.dim - t.rot) / 8;
+        for (t.lanes = 1; t.lanes < places;) t.lanes *= 2;
+        t.strips = (t.heads + NH - 1) / NH;
+        const double total = (double)tokens * t.strips * t.lanes;
+        if (total > 2147483392.0) return fail(HV_ERR_VALUE, "too many elements for one call");
+        t.total = (uint32_t)total;
+        t.by_token = Divider(std::max(1u, t.strips * t.lanes));
+        a.first[i] = blocks;
+        blocks += (t.total + THREADS - 1) / THREADS;
+    }
+    const cudaError_t e = launch_pdl(norm_append_kernel<T, INTER, NH>, dim3(blocks), dim3(THREADS), 0, st, a);
+    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "append_kv: %s", cudaGetErrorString(e));
+    return HV_OK;
+}
+
+template <typename T>
+int launch_norm_any(AppendArgs &a, int tokens, bool inter, cudaStream_t st) {
+    uint32_t blocks = 0;
+    for (int i = 0; i < 3; ++i) {
+        Tensor &t = a.t[i];
+        const double total = (double)tokens * t.heads;
+        if (total * 32 > 2147483392.0) return fail(HV_ERR_VALUE, "too many elements for one call");
+        t.total = (uint32_t)total;
+        t.by_token = Divider(std::max(1, t.heads));
+        a.first[i] = blocks;
+        blocks += (t.total * 32 + THREADS - 1) / THREADS;
+    }
+    const cudaError_t e = launch_pdl(norm_append_any_kernel<T>, dim3(blocks), dim3(THREADS), 0, st, a, (int)inter);
+    if (e != cudaSuccess) return fail(HV_ERR_CUDA, "append_kv: %s", cudaGetErrorString(e));
+    return HV_OK;
+}
+
+template <typename T>
+int launch_norm(AppendArgs &a, int tokens, bool wide, bool inter, cudaStream_t st) {
+    // 32 lanes hold 256 elements of a head that is not rotated, or in neighbouring pairs; all three share a layout
+    if (!wide || a.dim > 256) return launch_norm_any<T>(a, tokens, inter, st);
+    return inter ? launch_norm<T, true, 1>(a, tokens, st) : launch_norm<T, false, 1>(a, tokens, st);
+}
+
 template <typename T, int W, bool INTER, int NH>
 int launch(AppendArgs &a, int tokens, int dim, cudaStream_t st) {
     uint32_t blocks = 0;
@@ -199,8 +433,8 @@ int launch(AppendArgs &a, int tokens, int dim, bool wide, bool inter, int sms, c
 
 using namespace hv;
 
-extern "C" int hv_append_kv(const hv_append_args *p, void *stream) {
-    if (!p) return fail(HV_ERR_VALUE, "null argument");
+static int append(const hv_append_args *p, const void *q_weight, const void *k_weight, float eps, void *stream) {
+    const bool norm = q_weight || k_weight;
     if (p->dtype != HV_BF16 && p->dtype != HV_F16) return fail(HV_ERR_TYPE, "dtype must be HV_BF16 or HV_F16");
     if (p->tokens < 0 || p->heads < 0) return fail(HV_ERR_VALUE, "negative token or head count");
     if (p->kv_heads < 1 || p->dim < 1) return fail(HV_ERR_VALUE, "kv_heads and dim must be positive");
@@ -218,6 +452,7 @@ extern "C" int hv_append_kv(const hv_append_args *p, void *stream) {
     const int sms = dec::sm_count();
     if (!err || !sms) return fail(HV_ERR_CUDA, "cannot read the device's properties");
     AppendArgs a;
+    a.weight[0] = q_weight, a.weight[1] = k_weight, a.weight[2] = nullptr, a.eps = eps, a.dim = p->dim;
     a.t[0] = {p->d_q, p->d_q_out, p->q_strides[0], p->q_out_strides[0], 0, 0, (int)p->q_strides[1],
               (int)p->q_out_strides[1], p->heads, p->rot, 0};
     a.t[1] = {p->d_k, p->d_k_cache, p->k_strides[0], 0, p->k_cache_strides[0], p->k_cache_strides[1],
@@ -243,6 +478,23 @@ extern "C" int hv_append_kv(const hv_append_args *p, void *stream) {
     rows(p->d_k_cache, p->k_cache_strides, 3), rows(p->d_v_cache, p->v_cache_strides, 3);
     if (p->heads) rows(p->d_q, p->q_strides, 2), rows(p->d_q_out, p->q_out_strides, 2);
     const cudaStream_t st = (cudaStream_t)stream;
+    if (norm) {
+        wide = wide && dec::aligned(q_weight, 16) && dec::aligned(k_weight, 16);
+        return p->dtype == HV_BF16 ? launch_norm<__nv_bfloat16>(a, p->tokens, wide, p->interleaved != 0, st)
+                                   : launch_norm<__half>(a, p->tokens, wide, p->interleaved != 0, st);
+    }
     return p->dtype == HV_BF16 ? launch<__nv_bfloat16>(a, p->tokens, p->dim, wide, p->interleaved != 0, sms, st)
                                : launch<__half>(a, p->tokens, p->dim, wide, p->interleaved != 0, sms, st);
+}
+
+extern "C" int hv_append_kv(const hv_append_args *p, void *stream) {
+    if (!p) return fail(HV_ERR_VALUE, "null argument");
+    return append(p, nullptr, nullptr, 0.f, stream);
+}
+
+extern "C" int hv_norm_append_kv(const hv_norm_append_args *p, void *stream) {
+    if (!p) return fail(HV_ERR_VALUE, "null argument");
+    if (!(p->eps >= 0.f)) return fail(HV_ERR_VALUE, "eps must not be negative");
+    if (p->d_q_weight && !p->append.heads) return fail(HV_ERR_VALUE, "a weight for q without q heads");
+    return append(&p->append, p->d_q_weight, p->d_k_weight, p->eps, stream);
 }

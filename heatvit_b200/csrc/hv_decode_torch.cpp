@@ -254,10 +254,20 @@ void need_caches(const Tensor &kc, const Tensor &vc, int dev) {
     need_like(vc, "v_cache", kc, "k_cache", dev);
 }
 
-// (k, v, k_cache, v_cache, page_table, positions, seq_ids, rope, q, interleaved, q_out) -> q_out
-PyObject *append_kv(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
+// The weight of a norm of heads of `dim`, or null.
+const void *head_weight(PyObject *o, const char *name, int64_t dim, at::ScalarType type, int dev) {
+    if (o == Py_None) return nullptr;
+    const Tensor &w = tensor(o, name);
+    need(w, name, 1, dev);
+    if (w.size(0) != dim) throw ValueError("%s has %lld channels, a head %lld", name, (long long)w.size(0), (long long)dim);
+    if (w.scalar_type() != type) throw TypeError("%s must have k's type", name);
+    return w.data_ptr();
+}
+
+// (k, v, k_cache, v_cache, page_table, positions, seq_ids, rope, q, interleaved, q_out) -> q_out; with the norms'
+// (q_weight, k_weight, eps) behind them where `norm`
+PyObject *append(PyObject *const *o, bool norm) {
     BEGIN
-    ARGUMENTS(11)
     const Tensor &k = tensor(o[0], "k"), &v = tensor(o[1], "v"), &kc = tensor(o[2], "k_cache"), &vc = tensor(o[3], "v_cache");
     const Tensor &table = tensor(o[4], "page_table"), &pos = tensor(o[5], "positions");
     const int dev = device_of(k, "k");
@@ -321,27 +331,51 @@ PyObject *append_kv(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     a.interleaved = interleaved, a.dtype = code;
     a.num_pages = int_of(kc.size(0), "pages"), a.page_size = int_of(kc.size(1), "page size");
     a.seqs = int_of(table.size(0), "page_table"), a.max_pages = int_of(table.size(1), "page_table");
-    if (const int rc = hv_append_kv(&a, stream_of(dev))) return PyLong_FromLong(rc);
+    int rc;
+    if (norm) {
+        hv_norm_append_args n{a, nullptr, nullptr, 0.f};
+        if (o[11] != Py_None && o[8] == Py_None) throw ValueError("q_weight without q");
+        n.d_q_weight = head_weight(o[11], "q_weight", dim, k.scalar_type(), dev);
+        n.d_k_weight = head_weight(o[12], "k_weight", dim, k.scalar_type(), dev);
+        const double eps = PyFloat_AsDouble(o[13]);
+        if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+        n.eps = (float)eps;
+        rc = hv_norm_append_kv(&n, stream_of(dev));
+    } else {
+        rc = hv_append_kv(&a, stream_of(dev));
+    }
+    if (rc) return PyLong_FromLong(rc);
     written(kc);
     written(vc);
     if (o[10] != Py_None) written(out);
     return out.defined() ? THPVariable_Wrap(std::move(out)) : none();
     END
 }
+PyObject *append_kv(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
+    ARGUMENTS(11)
+    return append(o, false);
+}
+PyObject *norm_append_kv(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
+    ARGUMENTS(14)
+    return append(o, true);
+}
 
-int64_t workspace_bytes() {
+int64_t workspace_bytes(bool chunks) {
     int64_t most = 0, need = 0;
     for (const int dim : {32, 64, 96, 128, 192, 256}) {
         TORCH_CHECK(hv_paged_attention_workspace(dim, &need) == HV_OK, hv_last_error());
+        most = std::max(most, need);
+        if (!chunks) continue;
+        TORCH_CHECK(hv_paged_chunk_attention_workspace(dim, &need) == HV_OK, hv_last_error());
         most = std::max(most, need);
     }
     return most;
 }
 
 // Only the counters have to be zero: a fill of the whole 5 MB took 2.3 us of every captured call.
-Tensor new_workspace(int dev) {
+Tensor new_workspace(int dev, bool chunks) {
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-    Tensor t = at::detail::empty_cuda({workspace_bytes()}, at::kByte, at::Device(at::kCUDA, (c10::DeviceIndex)dev),
+    Tensor t = at::detail::empty_cuda({workspace_bytes(chunks)}, at::kByte, at::Device(at::kCUDA, (c10::DeviceIndex)dev),
                                       std::nullopt);
     t.narrow(0, 0, HV_ATTENTION_COUNTER_BYTES).zero_();
     return t;
@@ -353,21 +387,57 @@ PyObject *attention_workspace(PyObject *, PyObject *const *o, Py_ssize_t nargs) 
     ARGUMENTS(1)
     const long dev = PyLong_AsLong(o[0]);
     if (dev == -1 && PyErr_Occurred()) return nullptr;
-    return THPVariable_Wrap(new_workspace((int)dev));
+    return THPVariable_Wrap(new_workspace((int)dev, false));
+    END
+}
+// (device index) -> one that paged_chunk_attention can use as well
+PyObject *chunk_attention_workspace(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
+    BEGIN
+    ARGUMENTS(1)
+    const long dev = PyLong_AsLong(o[0]);
+    if (dev == -1 && PyErr_Occurred()) return nullptr;
+    return THPVariable_Wrap(new_workspace((int)dev, true));
     END
 }
 
 // The current stream's own workspace, made at its first call; a fresh one while the stream is
 // being captured, since a graph may be replayed on any stream.
-Tensor workspace_of(int dev, cudaStream_t stream) {
+Tensor workspace_of(int dev, cudaStream_t stream, bool chunks) {
     // never destroyed: the CUDA context may be gone before a static would be
-    static auto *held = new std::map<std::pair<int, cudaStream_t>, Tensor>;
+    static auto *held = new std::map<std::pair<int, cudaStream_t>, Tensor>[2];
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &status));
-    if (status != cudaStreamCaptureStatusNone) return new_workspace(dev);
-    Tensor &t = (*held)[{dev, stream}];
-    if (!t.defined()) t = new_workspace(dev);
+    if (status != cudaStreamCaptureStatusNone) return new_workspace(dev, chunks);
+    Tensor &t = held[chunks][{dev, stream}];
+    if (!t.defined()) t = new_workspace(dev, chunks);
     return t;
+}
+
+// The caller's workspace, or the current stream's.
+Tensor workspace(PyObject *o, int dev, c10::cuda::CUDAStream current, bool chunks) {
+    if (o == Py_None) return workspace_of(dev, current.stream(), chunks);
+    const Tensor &ws = tensor(o, "workspace");
+    on(ws, "workspace", dev);
+    if (ws.scalar_type() != at::kByte || !ws.is_contiguous()) throw TypeError("workspace must be contiguous bytes");
+    // made on another stream perhaps: its memory is not handed on before this call is through
+    c10::cuda::CUDACachingAllocator::recordStream(ws.storage().data_ptr(), current);
+    return ws;
+}
+
+// An attention's softmax scale: dim^-0.5 for None; false with a Python error set.
+bool scale_of(PyObject *o, int64_t dim, float *scale) {
+    const double v = o == Py_None ? 1.0 / std::sqrt((double)dim) : PyFloat_AsDouble(o);
+    *scale = (float)v;
+    return !(v == -1.0 && PyErr_Occurred());
+}
+
+PyObject *with_or_without(Tensor out, Tensor more) {
+    if (!more.defined()) return THPVariable_Wrap(std::move(out));
+    PyObject *r = PyTuple_New(2);
+    if (!r) return nullptr;
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out)));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(more)));
+    return r;
 }
 
 // (q, k_cache, v_cache, page_table, lens, scale, workspace, out, return_lse) -> out or (out, lse)
@@ -388,13 +458,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     if (kc.size(3) != dim) throw ValueError("the caches have another head dimension");
     if (kv_heads < 1 || heads < 1 || heads % kv_heads) throw ValueError("heads must be a positive multiple of kv_heads");
     if (table.size(0) != seqs || lens.size(0) != seqs) throw ValueError("page_table and lens have one row per sequence");
-    double scale = 0;
-    if (o[5] != Py_None) {
-        scale = PyFloat_AsDouble(o[5]);
-        if (scale == -1.0 && PyErr_Occurred()) return nullptr;
-    } else {
-        scale = 1.0 / std::sqrt((double)dim);
-    }
+    float scale = 0;
+    if (!scale_of(o[5], dim, &scale)) return nullptr;
     const int with_lse = PyObject_IsTrue(o[8]);
     if (with_lse < 0) return nullptr;
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
@@ -408,16 +473,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     } else {
         out = empty(q.sizes(), q.scalar_type(), q);
     }
-    Tensor ws;
-    if (o[6] != Py_None) {
-        ws = tensor(o[6], "workspace");
-        on(ws, "workspace", dev);
-        if (ws.scalar_type() != at::kByte || !ws.is_contiguous()) throw TypeError("workspace must be contiguous bytes");
-        // made on another stream perhaps: its memory is not handed on before this call is through
-        c10::cuda::CUDACachingAllocator::recordStream(ws.storage().data_ptr(), current);
-    } else {
-        ws = workspace_of(dev, stream);
-    }
+    const Tensor ws = workspace(o[6], dev, current, false);
     Tensor lse;
     if (with_lse) lse = empty({seqs, heads}, at::kFloat, q);
     hv_attention_args a{};
@@ -432,21 +488,140 @@ PyObject *paged_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
     a.seqs = int_of(seqs, "seqs"), a.heads = int_of(heads, "heads"), a.kv_heads = int_of(kv_heads, "kv_heads");
     a.dim = int_of(dim, "dim"), a.dtype = code;
     a.num_pages = int_of(kc.size(0), "pages"), a.page_size = int_of(kc.size(1), "page size");
-    a.max_pages = int_of(table.size(1), "page_table"), a.scale = (float)scale;
+    a.max_pages = int_of(table.size(1), "page_table"), a.scale = scale;
     if (const int rc = hv_paged_attention(&a, stream)) return PyLong_FromLong(rc);
     if (o[7] != Py_None) written(out);
-    if (!with_lse) return THPVariable_Wrap(std::move(out));
-    PyObject *r = PyTuple_New(2);
-    if (!r) return nullptr;
-    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out)));
-    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(lse)));
-    return r;
+    return with_or_without(std::move(out), std::move(lse));
+    END
+}
+
+// (q, k_cache, v_cache, page_table, lens, starts, causal, scale, workspace, out, return_lse) -> out or (out, lse)
+PyObject *paged_chunk_attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
+    BEGIN
+    ARGUMENTS(11)
+    const Tensor &q = tensor(o[0], "q"), &kc = tensor(o[1], "k_cache"), &vc = tensor(o[2], "v_cache");
+    const Tensor &table = tensor(o[3], "page_table"), &lens = tensor(o[4], "lens"), &starts = tensor(o[5], "starts");
+    const int dev = device_of(q, "q");
+    need(q, "q", 3, dev);
+    need_caches(kc, vc, dev);
+    need_ints(table, "page_table", 2, dev);
+    need_ints(lens, "lens", 1, dev);
+    need_ints(starts, "starts", 1, dev);
+    const int code = type_code(q.scalar_type());
+    if (code != HV_BF16 && code != HV_F16) throw TypeError("q must be bfloat16 or float16");
+    if (kc.scalar_type() != q.scalar_type()) throw TypeError("q and the caches must have the same type");
+    const int64_t tokens = q.size(0), heads = q.size(1), dim = q.size(2), kv_heads = kc.size(2), seqs = lens.size(0);
+    if (kc.size(3) != dim) throw ValueError("the caches have another head dimension");
+    if (kv_heads < 1 || heads < 1 || heads % kv_heads) throw ValueError("heads must be a positive multiple of kv_heads");
+    if (table.size(0) != seqs) throw ValueError("page_table and lens have one row per sequence");
+    if (starts.size(0) != seqs + 1) throw ValueError("starts has one more entry than there are sequences");
+    const int causal = PyObject_IsTrue(o[6]), with_lse = PyObject_IsTrue(o[10]);
+    if (causal < 0 || with_lse < 0) return nullptr;
+    float scale = 0;
+    if (!scale_of(o[7], dim, &scale)) return nullptr;
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+    const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev);
+    Tensor out;
+    if (o[9] != Py_None) {
+        out = tensor(o[9], "out");
+        need_like(out, "out", q, "q", dev);
+        need_apart(out, "out");
+    } else {
+        out = empty(q.sizes(), q.scalar_type(), q);
+    }
+    const Tensor ws = workspace(o[8], dev, current, true);
+    Tensor lse;
+    if (with_lse) lse = empty({tokens, heads}, at::kFloat, q);
+    hv_chunk_args a{};
+    a.d_q = q.data_ptr(), a.d_out = out.data_ptr(), a.d_lse = with_lse ? lse.data_ptr<float>() : nullptr;
+    a.d_k_cache = kc.data_ptr(), a.d_v_cache = vc.data_ptr();
+    a.d_page_table = table.data_ptr<int32_t>(), a.d_lens = lens.data_ptr<int32_t>(), a.d_starts = starts.data_ptr<int32_t>();
+    a.d_workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+    for (int i = 0; i < 2; ++i) a.q_strides[i] = q.stride(i), a.out_strides[i] = out.stride(i);
+    a.lse_strides[0] = heads, a.lse_strides[1] = 1;
+    for (int i = 0; i < 3; ++i) a.k_cache_strides[i] = kc.stride(i), a.v_cache_strides[i] = vc.stride(i);
+    a.page_table_stride = table.stride(0);
+    a.tokens = int_of(tokens, "tokens"), a.seqs = int_of(seqs, "seqs"), a.heads = int_of(heads, "heads");
+    a.kv_heads = int_of(kv_heads, "kv_heads"), a.dim = int_of(dim, "dim"), a.dtype = code, a.causal = causal;
+    a.num_pages = int_of(kc.size(0), "pages"), a.page_size = int_of(kc.size(1), "page size");
+    a.max_pages = int_of(table.size(1), "page_table"), a.scale = scale;
+    if (const int rc = hv_paged_chunk_attention(&a, current.stream())) return PyLong_FromLong(rc);
+    if (o[9] != Py_None) written(out);
+    return with_or_without(std::move(out), std::move(lse));
+    END
+}
+
+// A setting of sample_tokens: None (`otherwise`), a number for all rows, or a tensor [rows] of `type`.  False with a
+// Python error set.
+template <typename N>
+bool setting(PyObject *o, const char *name, at::ScalarType type, int64_t rows, int dev, N otherwise, N *number, const N **each) {
+    *number = otherwise, *each = nullptr;
+    if (o == Py_None) return true;
+    if (THPVariable_Check(o)) {
+        const Tensor &t = THPVariable_Unpack(o);
+        if (t.scalar_type() != type) throw TypeError("%s must be %s", name, type == at::kInt ? "int32" : "float32");
+        need(t, name, 1, dev);
+        if (t.size(0) != rows) throw ValueError("%s must be a number or have one entry per row", name);
+        *each = t.data_ptr<N>();
+        return true;
+    }
+    if (type == at::kInt) {
+        const long v = PyLong_AsLong(o);
+        if (v == -1 && PyErr_Occurred()) return false;
+        *number = (N)std::min(std::max(v, (long)INT32_MIN), (long)INT32_MAX);
+    } else {
+        const double v = PyFloat_AsDouble(o);
+        if (v == -1.0 && PyErr_Occurred()) return false;
+        *number = (N)v;
+    }
+    return true;
+}
+
+// (logits, uniform, temperature, top_k, top_p, min_p, out, return_logprob) -> tokens or (tokens, logprobs)
+PyObject *sample_tokens(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
+    BEGIN
+    ARGUMENTS(8)
+    const Tensor &z = tensor(o[0], "logits"), &u = tensor(o[1], "uniform");
+    const int dev = device_of(z, "logits");
+    need(z, "logits", 2, dev);
+    const int code = type_code(z.scalar_type());
+    if (code < 0) throw TypeError("logits must be bfloat16, float16 or float32");
+    const int64_t rows = z.size(0), vocab = z.size(1);
+    if (u.scalar_type() != at::kFloat) throw TypeError("uniform must be float32");
+    need(u, "uniform", 1, dev);
+    if (u.size(0) != rows) throw ValueError("one uniform number per row");
+    const int with_logprob = PyObject_IsTrue(o[7]);
+    if (with_logprob < 0) return nullptr;
+    hv_sample_args a{};
+    if (!setting(o[2], "temperature", at::kFloat, rows, dev, 1.f, &a.temperature, &a.d_temperature) ||
+        !setting(o[3], "top_k", at::kInt, rows, dev, 0, &a.top_k, &a.d_top_k) ||
+        !setting(o[4], "top_p", at::kFloat, rows, dev, 1.f, &a.top_p, &a.d_top_p) ||
+        !setting(o[5], "min_p", at::kFloat, rows, dev, 0.f, &a.min_p, &a.d_min_p))
+        return nullptr;
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+    Tensor out, logprobs;
+    if (o[6] != Py_None) {
+        out = tensor(o[6], "out");
+        if (out.scalar_type() != at::kLong) throw TypeError("out must be int64");
+        need(out, "out", 1, dev);
+        if (out.size(0) != rows) throw ValueError("out must have one entry per row");
+    } else {
+        out = empty({rows}, at::kLong, z);
+    }
+    if (with_logprob) logprobs = empty({rows}, at::kFloat, z);
+    a.d_logits = z.data_ptr(), a.d_uniform = u.data_ptr<float>(), a.d_tokens = out.data_ptr<int64_t>();
+    a.d_logprobs = with_logprob ? logprobs.data_ptr<float>() : nullptr;
+    a.row_stride = z.stride(0), a.rows = int_of(rows, "rows"), a.vocab = int_of(vocab, "vocab"), a.dtype = code;
+    if (const int rc = hv_sample_tokens(&a, stream_of(dev))) return PyLong_FromLong(rc);
+    if (o[6] != Py_None) written(out);
+    return with_or_without(std::move(out), std::move(logprobs));
     END
 }
 
 #define METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {METHOD(add_rmsnorm_fp8), METHOD(gemm_fp8), METHOD(append_kv), METHOD(attention_workspace),
-                           METHOD(paged_attention), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef g_methods[] = {METHOD(add_rmsnorm_fp8), METHOD(gemm_fp8), METHOD(append_kv), METHOD(norm_append_kv),
+                           METHOD(attention_workspace), METHOD(chunk_attention_workspace), METHOD(paged_attention),
+                           METHOD(paged_chunk_attention), METHOD(sample_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_decode_native", "Calls of heatvit_b200.decode.", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};
 

@@ -128,7 +128,7 @@ def rope_table(positions, rot, base=10000.0, device="cuda"):
 
 
 def append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, rope=None, q=None, interleaved=False,
-              q_out=None):
+              q_out=None, q_weight=None, k_weight=None, eps=1e-6):
     """Store new keys and values in a paged cache, rotating q and k by position.
 
     k, v [tokens, kv_heads, dim], q [tokens, heads, dim] (views of one projection's
@@ -138,24 +138,33 @@ def append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, rope=
     padding token (nothing stored, zeros in q_out).  ``rope`` [positions, rot]
     float32 (see ``rope_table``) turns the first rot elements of each head in pairs
     (i, i + rot/2), or (2i, 2i + 1) when interleaved; v is stored as it is.  Returns the
-    rotated q (a new tensor, or q_out, which may be q), None without q."""
-    return _done((_native or _load()).append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids, rope, q,
-                                                interleaved, q_out))
+    rotated q (a new tensor, or q_out, which may be q), None without q.
+
+    ``q_weight``, ``k_weight`` [dim] of k's type: an RMS norm of each q or k head goes ahead of the
+    rotation, ``x * rsqrt(mean(x^2) + eps) * weight`` over the head's elements, all in 32 bits and
+    rounded once; where one is None its heads are as they come."""
+    native = _native or _load()
+    if q_weight is None and k_weight is None:
+        return _done(native.append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids, rope, q, interleaved, q_out))
+    return _done(native.norm_append_kv(k, v, k_cache, v_cache, page_table, positions, seq_ids, rope, q, interleaved, q_out,
+                                       q_weight, k_weight, eps))
 
 
 class AttentionWorkspace:
     """Device memory that ``paged_attention`` joins split sequences in, for one device
     (the current one unless named) and any sizes.  Calls that share one must not overlap
     in time (one per stream).  Waits for the device to have zeroed its counters, so that
-    any stream may use it."""
+    any stream may use it.  With ``chunks`` a larger one (5 MB become 39), which
+    ``paged_chunk_attention`` can use as well."""
 
-    def __init__(self, device=None):
+    def __init__(self, device=None, chunks=False):
         torch = _torch()
         device = torch.device("cuda" if device is None else device)
         if device.type != "cuda":
             raise ValueError("an attention workspace lives on a CUDA device")
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
-        self.buffer = _load().attention_workspace(self.device.index)
+        make = _load().chunk_attention_workspace if chunks else _load().attention_workspace
+        self.buffer = make(self.device.index)
         torch.cuda.current_stream(self.device).synchronize()
 
 
@@ -175,3 +184,38 @@ def paged_attention(q, k_cache, v_cache, page_table, lens, scale=None, workspace
     return _done((_native or _load()).paged_attention(
         q, k_cache, v_cache, page_table, lens, scale, None if workspace is None else workspace.buffer, out,
         return_lse))
+
+
+def paged_chunk_attention(q, k_cache, v_cache, page_table, lens, starts, causal=True, scale=None, workspace=None, out=None,
+                          return_lse=False):
+    """Attention of a chunk of new tokens of each sequence over a paged cache that holds them
+    already (``append_kv`` comes first): a prompt, a piece of one, or drafted tokens.
+
+    q [tokens, heads, dim], packed: rows ``starts[i]`` to ``starts[i + 1]`` (int32 [seqs + 1]) are
+    the newest tokens of sequence i, of which the cache has ``lens[i]`` in all; a sequence may
+    bring none.  ``causal``: a token sees those up to itself; otherwise each sees all
+    ``lens[i]``.  A row that sees no token gives zeros (log-sum-exp -inf); rows of no sequence are not
+    written, neither in ``out`` nor in a new tensor.  The rest as ``paged_attention``.
+
+    ``workspace``: an AttentionWorkspace made with ``chunks=True``."""
+    return _done((_native or _load()).paged_chunk_attention(
+        q, k_cache, v_cache, page_table, lens, starts, causal, scale, None if workspace is None else workspace.buffer, out,
+        return_lse))
+
+
+def sample_tokens(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None, return_logprob=False):
+    """Draw a token for each row of logits [rows, vocab] (bfloat16, float16, float32) with that
+    row's number of ``uniform`` (float32 [rows], in [0, 1)) -> int64 [rows].
+
+    With ``w = exp((logit - largest) / temperature)`` and tokens ordered by logit, equal ones by
+    index: ``top_k`` keeps the first top_k (0: all), ``min_p`` those with w >= min_p, ``top_p`` the
+    shortest prefix of what these keep whose weights reach top_p of their sum (at least one token).
+    The token is the first, in the vocabulary's order, at which the kept weights add up to more than
+    ``uniform`` of their total.  Sums are exact, so the same numbers give the same token on any device.
+    Temperature 0 takes the largest logit, the first of equal ones.
+
+    Each setting is None (temperature 1, all tokens), a number, or a tensor [rows] (float32; top_k
+    int32), so that every row may have its own.  With ``return_logprob`` also the logarithm of the token's
+    probability among what was kept, float32 [rows].  A row with a NaN, or with nothing
+    above -inf, gives token 0 and a logprob of NaN, and ``device_error`` reports it."""
+    return _done((_native or _load()).sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, out, return_logprob))

@@ -406,6 +406,8 @@ HV_API int hv_selector_h2(hv_model *model, int selector_index, const int8_t *d_x
                                     stored) or the rotation table (nor is its q_out row) */
 #define HV_DECODE_BAD_LENGTH 4   /* a length above max_pages * page_size or HV_ATTENTION_MAX_LENGTH: taken as that */
 #define HV_DECODE_STALLED 8      /* a bounded wait gave up: that call's output is invalid */
+#define HV_DECODE_BAD_LOGITS 16  /* a row of logits with a NaN or with nothing above -inf: its token is 0, its logprob NaN */
+#define HV_DECODE_BAD_START 32   /* starts that fall, or lie outside [0, tokens]: taken as the nearest that do not */
 
 /* Read and clear the current device's error word (synchronises with the device). */
 HV_API int hv_decode_error(int *bits);
@@ -473,6 +475,17 @@ typedef struct hv_append_args {
 } hv_append_args;
 HV_API int hv_append_kv(const hv_append_args *args, void *stream);
 
+/* The same with an RMS norm of each q and each k head ahead of the rotation:
+ * y = x * rsqrt(mean(x^2) + eps) * weight over a head's dim elements, in 32 bits up to the one
+ * rounding of the rotated result.  d_q_weight, d_k_weight: [dim] of `dtype`; a NULL one leaves its
+ * heads as they are. */
+typedef struct hv_norm_append_args {
+    hv_append_args append;
+    const void *d_q_weight, *d_k_weight;
+    float eps;
+} hv_norm_append_args;
+HV_API int hv_norm_append_kv(const hv_norm_append_args *args, void *stream);
+
 /* Attention of one new token per sequence over a paged cache: softmax(scale * q K^T) V over the
  * first d_lens[seq] cached tokens, `heads / kv_heads` query heads sharing a key head.  A length
  * of zero (or less) gives zeros, and -inf in d_lse.
@@ -500,6 +513,53 @@ typedef struct hv_attention_args {
 } hv_attention_args;
 HV_API int hv_paged_attention_workspace(int dim, int64_t *bytes);
 HV_API int hv_paged_attention(const hv_attention_args *args, void *stream);
+
+/* Attention of a chunk of new tokens of each sequence over a paged cache that holds them already.
+ * Rows d_starts[seq] to d_starts[seq + 1] of q are the newest tokens of the first d_lens[seq] cached
+ * ones; with `causal` a row sees the tokens up to its own, else all d_lens[seq].  A row that sees
+ * none gives zeros, and -inf in d_lse; rows of no sequence are not written.  Everything else, the
+ * workspace's rules among it, as hv_paged_attention; the workspace may be shared with it. */
+typedef struct hv_chunk_args {
+    const void *d_q;                   /* [tokens][heads][dim] */
+    void *d_out;                       /* [tokens][heads][dim] */
+    float *d_lse;                      /* [tokens][heads], may be NULL */
+    const void *d_k_cache, *d_v_cache; /* [num_pages][page_size][kv_heads][dim], by strides */
+    const int32_t *d_page_table;       /* [seqs][max_pages] */
+    const int32_t *d_lens;             /* [seqs] */
+    const int32_t *d_starts;           /* [seqs + 1] */
+    void *d_workspace;
+    int64_t workspace_bytes;
+    int64_t q_strides[2], out_strides[2], lse_strides[2]; /* token, head */
+    int64_t k_cache_strides[3], v_cache_strides[3];       /* page, slot, head */
+    int64_t page_table_stride;
+    int32_t tokens, seqs, heads, kv_heads, dim, dtype, causal;
+    int32_t num_pages, page_size, max_pages;
+    float scale;
+} hv_chunk_args;
+HV_API int hv_paged_chunk_attention_workspace(int dim, int64_t *bytes);
+HV_API int hv_paged_chunk_attention(const hv_chunk_args *args, void *stream);
+
+/* A token for each row of logits, drawn with the row's own uniform number u in [0, 1).
+ * With z the logits, w = exp((z - max z) / temperature).  Tokens are ordered by z, equal ones by
+ * index; top_k keeps the first top_k of them (all when <= 0), min_p those with w >= min_p, and
+ * top_p the shortest prefix of what the two keep whose weights reach top_p of their sum (all when
+ * >= 1; one at least).  The token is the first in the vocabulary's order at which the sum of the
+ * kept weights passes u times their total; d_logprobs receives the log of its share of that total.  A
+ * temperature that is not above zero takes the largest logit, the first of equal ones.  A logit of
+ * +inf leaves only those.
+ * Each setting comes for all rows or, where its pointer is not NULL, for each row. */
+typedef struct hv_sample_args {
+    const void *d_logits;       /* [rows][vocab] of `dtype`, rows row_stride elements apart */
+    const float *d_uniform;     /* [rows] */
+    const float *d_temperature, *d_top_p, *d_min_p; /* [rows] or NULL */
+    const int32_t *d_top_k;     /* [rows] or NULL */
+    int64_t *d_tokens;          /* [rows] */
+    float *d_logprobs;          /* [rows], may be NULL */
+    int64_t row_stride;
+    int32_t rows, vocab, dtype, top_k;
+    float temperature, top_p, min_p;
+} hv_sample_args;
+HV_API int hv_sample_tokens(const hv_sample_args *args, void *stream);
 
 #ifdef __cplusplus
 }
