@@ -4,17 +4,58 @@
 //   seen(t) = lens - n + i + 1 for the i-th of a sequence's n new tokens (causal), or lens;
 //   a row that sees nothing gives zeros (and a log-sum-exp of -inf).
 //
-// A warp takes a row, its lanes the head's dimensions.
+// Rows are (token, query head of a key head's group), so that a tile of 128 rows shares its keys
+// whatever the group is.  One CTA an SM: 4 warps copy (cp.async, 16 bytes a lane, from any page size
+// and stride, zeros past a sequence's end) into a ring of key and value tiles; one thread issues
+// tcgen05.mma kind::f16; a warpgroup a row tile has a row in each thread.  It reads the scores of 128
+// keys from TMEM, keeps the running maximum and sum, and writes the weights over the scores, where
+// the second product takes them as its A operand; the sums stay in TMEM.
+//
+// Heads of up to 128 dimensions have two row tiles in flight (NT), whose products and weights take
+// turns: two tiles of rows against the same keys, or, where an item has no more than 128
+// rows, the same rows against the even and the odd key tiles, joined at the end.  Wider heads have one
+// row tile and two score buffers.
+//
+// Work: an item is a tile of NT * 128 rows of one sequence and key head; its key tiles are steps.  The
+// steps of all items are laid end to end and every CTA takes an equal share of that line, so that
+// ragged and causal batches are even and one long sequence uses every SM.  An item inside a share
+// is written straight out; one that is cut leaves parts (unnormalised sums, maximum, sum of weights, in 32
+// bits) in the workspace, and the CTA that finishes last joins them in the order of the shares.
+//
+// A row's maximum moves only when it is passed by 2^SOFT, so that the sums are rarely rescaled.  The weights go
+// into the second product rounded to the cache's type, and their sum is that of the rounded numbers: weights that are
+// alike, and so rounded alike, cancel.  (As two numbers each, as attention of one token has them, they would
+// take the tensor cores half as long again.)
+//
+// The second product multiplies masked values by zero, which a NaN or an infinity survives.  Slots past a
+// sequence's end are zeros in shared memory; where a row does not see a token that others see, the warpgroup looks
+// through the value tile, and one that holds such a number is added by its threads, each taking what its row sees.
 #include <math_constants.h>
 
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
 #include "hv_decode.cuh"
+#include "hv_tc05.cuh"
 
 namespace hv {
 namespace {
 
 using namespace dec;
 
-constexpr float LOWEST = -3.402823466e38f;  // a running maximum before the first score
+// A running maximum before the first score, finite so that a score of -inf weighs exp2(-inf) = 0 and not NaN.
+constexpr float LOWEST = -3.402823466e38f;
+// fp16 weights begin at 2^9, so that those of a long tail keep their bits (normal numbers from 2^-14 to 2^15).
+template <typename T>
+constexpr float TOP = 0.f;
+template <>
+constexpr float TOP<__half> = 9.f;
+constexpr float SOFT = 6.f;
+constexpr int BK = 128;       // keys of a step
+constexpr int MIN_SHARE = 2;  // steps
+constexpr int MAX_GRID = 512;
+constexpr int LAG = 2;        // copies of a producer that are under way ahead of the one that is waited for
 
 struct ChunkArgs {
     const void *q, *kc, *vc;
@@ -23,81 +64,997 @@ struct ChunkArgs {
     const int32_t *pages, *lens, *starts;
     long long q_tok, q_head, o_tok, o_head, lse_tok, lse_head;
     long long kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head, pages_stride;
-    int tokens, seqs, heads, kv_heads, group, num_pages, page, max_pages, causal;
-    float scale_log2;
+    int tokens, seqs, heads, kv_heads, group, num_pages, page, page_shift, max_pages, causal, q_vec, o_vec, negate;
+    float scale_log2;   // not negative: `negate` has the sign
+    uint32_t skip;      // see skipped_copy
+    float *parts;       // [grid][2][R][D], then [grid][2][R][2]
+    uint32_t *counts;   // [2][MAX_GRID], zero between calls
     int *err;
 };
 
-// Start of sequence b (or its end: b + 1), brought into [0, tokens] and past none before it.
-__device__ __forceinline__ int length_of(const ChunkArgs &a, int b) {
-    const int n = max(a.lens[b], 0);
-    const long long cap = min((long long)a.max_pages * a.page, (long long)HV_ATTENTION_MAX_LENGTH);
-    if (n > cap) {
-        atomicOr(a.err, HV_DECODE_BAD_LENGTH);
-        return (int)cap;
+template <int D>
+struct Lay {
+    static constexpr int DP = (D + 63) / 64 * 64;  // dimensions in shared memory: 128-byte blocks of 64
+    static constexpr int NT = D <= 128 ? 2 : 1, R = 128 * NT;
+    static constexpr int SLOT = DP <= 128 ? 128 : 64, PARTS = BK / SLOT;  // keys of a ring slot
+    static constexpr int SLOT_BYTES = SLOT * DP * 2, Q_TILE = 128 * DP * 2, Q_BYTES = NT * Q_TILE;
+    static constexpr int STAGES = DP == 64 ? 8 : DP == 128 ? 5 : DP == 192 ? 7 : 5;
+    static constexpr int STAT = Q_BYTES + STAGES * SLOT_BYTES;  // [2][128] float2: maxima and sums of the other half
+    static constexpr int BARS = STAT + (NT == 2 ? 2048 : 0), MISC = BARS + 256, BYTES = MISC + 64;
+    static constexpr int SOFT_WARPS = 4 * NT, MMA_WARP = SOFT_WARPS + 4, WARPS = SOFT_WARPS + 8, THREADS = WARPS * 32;
+    // Registers of a thread at launch, and of the roles from then on (shares of what the block was launched with).
+    static constexpr int REGS = NT == 2 ? 128 : 168, COPY_REGS = 72, MMA_REGS = 56, SOFT_REGS = NT == 2 ? 192 : 240;
+    static_assert(128 * (COPY_REGS + MMA_REGS + NT * SOFT_REGS) <= REGS * THREADS, "registers");
+    static constexpr int O_COL = 256;  // TMEM: scores at 0 and 128, sums from here
+    static constexpr int PART = R * D, CH = D / 8;  // numbers of a part; 16-byte pieces of a row
+    static_assert(BYTES <= 227 * 1024, "shared memory");
+    static_assert(O_COL + NT * DP <= 512, "tensor memory");
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float exp2_(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void arrive(uint64_t *mbar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(tc05::smem_u32(mbar)) : "memory");
+}
+// Bounded wait that also ends when another role of the CTA has given up.
+__device__ __forceinline__ bool wait_or_stop(uint64_t *bar, uint32_t parity, volatile int *stop) {
+    for (uint32_t i = 0; i < WAIT_ITERS / 64; ++i) {
+        if (tc05::mbar_wait(bar, parity, 64)) return true;
+        if (*stop) return false;
     }
-    return n;
+    *stop = 1;
+    return false;
+}
+// 128-byte swizzled operands: K-major (eight rows of 128 bytes an atom, `sbo` 1024), or MN-major with blocks of 64
+// along N `lbo` bytes apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16, f32 accumulator.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
+    const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *(uint32_t *)&v;
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *(uint32_t *)&v;
+}
+__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*(const __half2 *)&v); }
+// The largest magnitude's bits from which on numbers are infinite or NaN, twice.
+__device__ __forceinline__ uint32_t infinite(__nv_bfloat16) { return 0x7f807f80u; }
+__device__ __forceinline__ uint32_t infinite(__half) { return 0x7c007c00u; }
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void split2(uint64_t pair, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(pair));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// A sequence's rows of q and cached tokens, brought into range (what is not is reported once, by `tell`).
+struct Seq {
+    int s0, n, len;
+    __device__ __forceinline__ void set(const ChunkArgs &a, int b, bool tell) {
+        const int r0 = a.starts[b], r1 = a.starts[b + 1], l = a.lens[b];
+        s0 = min(max(r0, 0), a.tokens);
+        const int s1 = min(max(r1, 0), a.tokens);
+        n = max(s1 - s0, 0);
+        const long long cap = min((long long)a.max_pages * a.page, (long long)HV_ATTENTION_MAX_LENGTH);
+        len = (int)min((long long)max(l, 0), cap);
+        if (tell) {
+            if (s0 != r0 || s1 != r1 || s1 < s0) atomicOr(a.err, HV_DECODE_BAD_START);
+            if (l > cap) atomicOr(a.err, HV_DECODE_BAD_LENGTH);
+        }
+    }
+    // Tokens that the i-th new one sees.
+    __device__ __forceinline__ int seen(const ChunkArgs &a, int i) const {
+        return a.causal ? min(max(len - n + i + 1, 0), len) : len;
+    }
+    __device__ __forceinline__ int row_tiles(const ChunkArgs &a, int R) const {
+        return (int)(((long long)n * a.group + R - 1) / R);
+    }
+    // Steps of a row tile: one at least, so that rows which see nothing are written.
+    __device__ __forceinline__ int steps(const ChunkArgs &a, int R, int qt) const {
+        if (!a.causal) return max(1, (len + BK - 1) / BK);
+        const int last = (int)min((long long)(qt + 1) * R, (long long)n * a.group) - 1;
+        return max(1, (seen(a, last / a.group) + BK - 1) / BK);
+    }
+};
+
+// Steps [t0, t1) of the item (sequence b, key head h, row tile qt), of `steps` in all, as a share cuts them.
+template <int R>
+struct Segment {
+    Seq seq;
+    int b, h, qt, qts, steps, t0, t1;
+    long long left;  // of the share, from t0 on
+    __device__ __forceinline__ void clip() {
+        t1 = (int)min((long long)steps, t0 + left);
+    }
+    __device__ __forceinline__ bool next(const ChunkArgs &a) {
+        left -= t1 - t0;
+        if (left <= 0) return false;
+        t0 = 0;
+        if (++qt == qts) {
+            qt = 0;
+            if (++h == a.kv_heads) {
+                h = 0;
+                do {
+                    seq.set(a, ++b, false);  // only called where a further step exists
+                    qts = seq.row_tiles(a, R);
+                } while (qts == 0);
+            }
+        }
+        steps = seq.steps(a, R, qt);
+        clip();
+        return true;
+    }
+    __device__ __forceinline__ int rows(const ChunkArgs &a) const {
+        return (int)min((long long)R, (long long)seq.n * a.group - (long long)qt * R);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void store_row16(T *p, bool vec, const float (&v)[16]) {
+    alignas(16) T e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) e[i] = from_f32<T>(v[i]);
+    if (vec) {
+        ((uint4 *)p)[0] = ((const uint4 *)e)[0];
+        ((uint4 *)p)[1] = ((const uint4 *)e)[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = e[i];
+    }
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) chunk_simple_kernel(const __grid_constant__ ChunkArgs a) {
+__global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_constant__ ChunkArgs a) {
+    using L = Lay<D>;
+    constexpr int NT = L::NT, R = L::R, DP = L::DP, SLOT = L::SLOT, PARTS = L::PARTS, STAGES = L::STAGES;
+    extern __shared__ __align__(1024) uint8_t smem[];  // (with no static shared memory ahead of it)
+    uint8_t *ring = smem + L::Q_BYTES;
+    float2 *half_stat = (float2 *)(smem + L::STAT);
+    uint64_t *full = (uint64_t *)(smem + L::BARS), *empty = full + STAGES, *qfull = empty + STAGES, *qempty = qfull + 1;
+    uint64_t *sfull = qempty + 1, *pready = sfull + 2, *ofull = pready + 2, *wgbar = ofull + 2, *both = wgbar + 2;
+    uint64_t *drain = both + 1, *odone = drain + 1;
+    static_assert((2 * STAGES + 15) * 8 <= 256, "barriers");
+    long long *line = (long long *)(smem + L::MISC);  // total, share, steps ahead of the first step's sequence, that sequence
+    uint32_t *tslot = (uint32_t *)(line + 4);
+    volatile int *stop = (volatile int *)(tslot + 1);
+    volatile int *by_hand = stop + 1;        // [2]: this step's values are added by the warpgroup
+    volatile int *last_flag = by_hand + 2;   // [2]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (warp == L::MMA_WARP) {
+        tc05::tmem_alloc(tslot, 512);
+        tc05::tmem_relinquish();
+    }
+    if (tid == 0) {
+        *stop = tc05::smem_u32(smem) % 1024 != 0;  // operands would lie elsewhere than their descriptors say
+        for (int i = 0; i < STAGES; ++i) {
+            tc05::mbar_init(&full[i], 4);
+            tc05::mbar_init(&empty[i], 1);
+        }
+        tc05::mbar_init(qfull, 4);
+        tc05::mbar_init(qempty, 1);
+        for (int i = 0; i < 2; ++i) {
+            by_hand[i] = 0;
+            tc05::mbar_init(&sfull[i], 1);
+            tc05::mbar_init(&pready[i], 4);
+            tc05::mbar_init(&ofull[i], 1);
+            tc05::mbar_init(&wgbar[i], 4);
+        }
+        tc05::mbar_init(both, 8);
+        tc05::mbar_init(drain, 1);
+        tc05::mbar_init(odone, 1);
+        tc05::fence_mbar_init();
+    }
     griddep_wait();
     griddep_launch();
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long id = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-    const int b = blockIdx.y;
-    const int s0 = min(max(a.starts[b], 0), a.tokens), s1 = min(max(a.starts[b + 1], 0), a.tokens);
-    if (s1 < s0 || s0 != a.starts[b] || s1 != a.starts[b + 1]) atomicOr(a.err, HV_DECODE_BAD_START);
-    const int n = max(s1 - s0, 0);
-    const int len = length_of(a, b);
-    for (long long w = id; w < (long long)n * a.heads; w += (long long)gridDim.x * 8) {
-        const int i = (int)(w / a.heads), h = (int)(w - (long long)i * a.heads), kvh = h / a.group;
-        const int seen = a.causal ? max(len - n + i + 1, 0) : len;
-        const T *q = (const T *)a.q + (long long)(s0 + i) * a.q_tok + h * a.q_head + lane * E;
-        float qv[E], o[E], m = LOWEST, l = 0.f;
-        for (int e = 0; e < E; ++e) qv[e] = to_f32(q[e]) * a.scale_log2, o[e] = 0.f;
-        for (int j = 0; j < seen; ++j) {
-            const int pg = a.pages[b * a.pages_stride + j / a.page], slot = j % a.page;
-            const bool ok = pg >= 0 && pg < a.num_pages;
-            if (!ok && lane == 0) atomicOr(a.err, HV_DECODE_BAD_PAGE);
-            const T *k = (const T *)a.kc + (ok ? pg * a.kc_page + slot * a.kc_slot + kvh * a.kc_head + lane * E : 0);
-            const T *v = (const T *)a.vc + (ok ? pg * a.vc_page + slot * a.vc_slot + kvh * a.vc_head + lane * E : 0);
-            float s = 0.f;
-            if (ok)
-                for (int e = 0; e < E; ++e) s += qv[e] * to_f32(k[e]);
-            for (int x = 16; x; x /= 2) s += __shfl_xor_sync(~0u, s, x);
-            const float mn = fmaxf(m, s), f = exp2f(m - mn), p = exp2f(s - mn);
-            m = mn;
-            l = l * f + p;
-            for (int e = 0; e < E; ++e) o[e] = o[e] * f + (ok ? p * to_f32(v[e]) : 0.f);
+
+    // The line's length, this CTA's share of it, and the sequence of the share's first step.
+    if (warp == 0) {
+        // steps of each lane's sequence, for one key head
+        auto steps_of = [&](int b, bool tell) {
+            Seq s{0, 0, 0};
+            if (b < a.seqs) s.set(a, b, tell);
+            const int qts = s.n ? s.row_tiles(a, R) : 0;
+            long long sum = 0;
+            if (!a.causal) {
+                sum = qts ? (long long)qts * s.steps(a, R, 0) : 0;
+            } else {
+                for (int qt = 0; qt < min(qts, 16); ++qt) sum += s.steps(a, R, qt);
+                unsigned many = __ballot_sync(~0u, qts > 16);  // those of long chunks by the whole warp
+                while (many) {
+                    const int l = __ffs(many) - 1;
+                    many &= many - 1;
+                    const Seq o{0, __shfl_sync(~0u, s.n, l), __shfl_sync(~0u, s.len, l)};
+                    const int its = __shfl_sync(~0u, qts, l);
+                    long long part = 0;
+                    for (int qt = 16 + lane; qt < its; qt += 32) part += o.steps(a, R, qt);
+                    for (int x = 16; x; x /= 2) part += __shfl_xor_sync(~0u, part, x);
+                    if (lane == l) sum += part;
+                }
+            }
+            return sum;
+        };
+        long long total = 0, held = 0;
+        for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+            held = steps_of(b0 + lane, blockIdx.x == 0);
+            long long sum = held;
+            for (int x = 16; x; x /= 2) sum += __shfl_xor_sync(~0u, sum, x);
+            total += sum;
         }
-        T *out = (T *)a.out + (long long)(s0 + i) * a.o_tok + h * a.o_head + lane * E;
-        for (int e = 0; e < E; ++e) out[e] = from_f32<T>(seen ? o[e] / l : 0.f);
-        if (a.lse && lane == 0)
-            a.lse[(long long)(s0 + i) * a.lse_tok + h * a.lse_head] =
-                seen ? (m + log2f(l)) * 0.69314718055994531f : -CUDART_INF_F;
+        total *= a.kv_heads;
+        long long share = (total + gridDim.x - 1) / gridDim.x;
+        if (share < MIN_SHARE) share = MIN_SHARE;
+        const long long first = share * blockIdx.x;
+        long long before = 0;
+        int found = -1;
+        for (int b0 = 0; b0 < a.seqs && found < 0 && first < total; b0 += 32) {
+            const long long n = a.seqs <= 32 ? held : steps_of(b0 + lane, false);
+            long long incl = n;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(~0u, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const unsigned m = __ballot_sync(~0u, (before + incl) * a.kv_heads > first);
+            if (m) {
+                const int l = __ffs(m) - 1;
+                found = b0 + l;
+                before += __shfl_sync(~0u, incl - n, l);
+            } else {
+                before += __shfl_sync(~0u, incl, 31);
+            }
+        }
+        if (lane == 0) {
+            line[0] = total;
+            line[1] = share;
+            line[2] = before * a.kv_heads;
+            line[3] = found;
+        }
+    }
+    __syncwarp();
+    tc05::fence_before();
+    __syncthreads();
+    tc05::fence_after();
+    const uint32_t tmem = *tslot;
+    const long long total = line[0], share = line[1], first = share * blockIdx.x;
+    const bool works = first < total && !*stop;
+
+    Segment<R> seg;
+    if (works) {
+        seg.b = (int)line[3];
+        seg.seq.set(a, seg.b, false);
+        seg.qts = seg.seq.row_tiles(a, R);
+        seg.left = min(share, total - first);
+        long long in = first - line[2];
+        // the key head, and the row tile within it
+        long long per = 0;
+        if (a.causal) {
+            for (int qt = lane; qt < seg.qts; qt += 32) per += seg.seq.steps(a, R, qt);
+            for (int x = 16; x; x /= 2) per += __shfl_xor_sync(~0u, per, x);
+        } else {
+            per = (long long)seg.qts * seg.seq.steps(a, R, 0);
+        }
+        seg.h = (int)(in / per);
+        in -= seg.h * per;
+        seg.qt = 0;
+        if (!a.causal) {
+            const int s = seg.seq.steps(a, R, 0);
+            seg.qt = (int)(in / s);
+            in -= (long long)seg.qt * s;
+        } else {
+            for (; seg.qt < seg.qts; seg.qt += 32) {  // 32 row tiles at a time
+                const int qt = seg.qt + lane, s = qt < seg.qts ? seg.seq.steps(a, R, qt) : 0;
+                long long incl = s;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long v = __shfl_up_sync(~0u, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                const unsigned m = __ballot_sync(~0u, incl > in);
+                if (m) {
+                    const int l = __ffs(m) - 1;
+                    in -= __shfl_sync(~0u, incl - s, l);
+                    seg.qt += l;
+                    break;
+                }
+                in -= __shfl_sync(~0u, incl, 31);
+            }
+        }
+        seg.steps = seg.seq.steps(a, R, seg.qt);
+        seg.t0 = (int)in;
+        seg.clip();
+    }
+    __syncwarp();
+    // Which ring fill, from the segment's first, holds the keys (values) of its step j of n: keys of a step ahead
+    // of the values before them; with alternating tiles two steps ahead.
+    auto k_fill = [](int j, bool alt) { return (alt ? (j ? 2 * j - 1 : 0) : 2 * j) * PARTS; };
+    auto v_fill = [](int j, int n, bool alt) { return (!alt || n == 1 ? 2 * j + 1 : j < n - 1 ? 2 * j + 2 : 2 * n - 1) * PARTS; };
+
+    if (warp >= L::SOFT_WARPS && warp < L::SOFT_WARPS + 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::COPY_REGS));
+        const int w = warp - L::SOFT_WARPS;
+        uint32_t fills = 0, qn = 0, waiting = 0;  // slots filled, items, copies not yet reported
+        uint64_t *pend[LAG + 1];
+        bool ok = works;
+        auto report = [&](uint64_t *bar) {
+            tc05::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) arrive(bar);
+        };
+        auto flush = [&]() {
+            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+#pragma unroll
+            for (int i = 0; i <= LAG; ++i)
+                if (i < (int)waiting) report(pend[i]);
+            waiting = 0;
+        };
+        auto issued = [&](uint64_t *bar) {
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+#pragma unroll
+            for (int i = 0; i <= LAG; ++i)
+                if (i == (int)waiting) pend[i] = bar;
+            if (++waiting > LAG) {
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(LAG) : "memory");
+                report(pend[0]);
+#pragma unroll
+                for (int i = 0; i < LAG; ++i) pend[i] = pend[i + 1];
+                --waiting;
+            }
+        };
+        // Before a wait for room all that is on its way is reported, since room may depend on it.
+        auto room = [&](uint64_t *bar, uint32_t parity) {
+            if (__all_sync(~0u, tc05::mbar_wait(bar, parity, 1))) return true;
+            flush();
+            return (bool)__all_sync(~0u, wait_or_stop(bar, parity, stop));
+        };
+        constexpr int RW = SLOT / 4, N = RW * L::CH / 32;  // rows of a warp in a slot, accesses of a lane
+        // Keys or values of this lane's row (lane < RW) into the slot.
+        auto copy = [&](const T *base, long long off) {
+            const uint32_t s = fills % STAGES, dst = tc05::smem_u32(ring + s * L::SLOT_BYTES) + w * RW * 128;
+            if (fills >= STAGES && !room(&empty[s], (fills / STAGES - 1) & 1)) return false;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = i * 32 + lane, row = c / L::CH, col = c % L::CH;
+                const long long o = __shfl_sync(~0u, off, row);
+                cp16(dst + (col >> 3) * (SLOT * 128) + row * 128 + (((col ^ row) & 7) << 4), base + (o < 0 ? 0 : o + col * 8),
+                     o < 0 ? 0 : 16);
+            }
+            if (fills++ == a.skip) asm volatile("cp.async.commit_group;\n" ::: "memory");
+            else issued(&full[s]);
+            return true;
+        };
+        const T *kc = (const T *)a.kc, *vc = (const T *)a.vc;
+        if (ok) do {
+                const int n = seg.t1 - seg.t0, rows = seg.rows(a);
+                const bool alt = NT == 2 && rows <= 128;
+                // rows of q
+                if (qn && !room(qempty, (qn - 1) & 1)) { ok = false; break; }
+                {
+                    const T *q = (const T *)a.q + (long long)seg.seq.s0 * a.q_tok;
+                    const int h0 = seg.h * a.group;
+                    const long long r0 = (long long)seg.qt * R;
+                    const int held = alt ? 128 : R;
+                    for (int g = w * 32; g < held; g += 128) {
+                        const int r = g + lane;
+                        long long off = -1;
+                        if (r < rows) {
+                            const int at = (int)(r0 + r), tok = at / a.group;
+                            off = tok * a.q_tok + (h0 + at - tok * a.group) * a.q_head;
+                        }
+                        const uint32_t dst = tc05::smem_u32(smem) + (g >> 7) * L::Q_TILE + (g & 127) * 128;
+#pragma unroll 4
+                        for (int i = 0; i < L::CH; ++i) {
+                            const int c = i * 32 + lane, row = c / L::CH, col = c % L::CH;
+                            const long long o = __shfl_sync(~0u, off, row);
+                            const uint32_t to = dst + (col >> 3) * (128 * 128) + row * 128 + (((col ^ row) & 7) << 4);
+                            if (a.q_vec) {
+                                cp16(to, q + (o < 0 ? 0 : o + col * 8), o < 0 ? 0 : 16);
+                            } else {
+                                alignas(16) T e[8];
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) e[k] = o < 0 ? from_f32<T>(0.f) : q[o + col * 8 + k];
+                                const uint4 v = *(const uint4 *)e;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                                             : "memory");
+                            }
+                        }
+                    }
+                    issued(qfull);
+                    ++qn;
+                }
+                // Pages of this lane's rows of four steps: the one whose values come next, two whose keys do, and one
+                // on its way.  -1 past the end.
+                struct Pages {
+                    int of[PARTS];
+                };
+                const int head = seg.h;
+                const long long table = seg.b * a.pages_stride;
+                auto pages_of = [&](int j) {
+                    Pages r;
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        const int t = (seg.t0 + min(j, n - 1)) * BK + p * SLOT + w * RW + lane;
+                        r.of[p] = lane < RW && j < n && t < seg.seq.len
+                                      ? a.pages[table + (a.page_shift >= 0 ? t >> a.page_shift : t / a.page)] : INT32_MIN;
+                    }
+                    return r;
+                };
+                auto fill = [&](int j, const Pages &pg, bool keys) {
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        const int t = (seg.t0 + j) * BK + p * SLOT + w * RW + lane;
+                        const bool live = lane < RW && t < seg.seq.len;
+                        bool good = live;
+                        if (live && (pg.of[p] < 0 || pg.of[p] >= a.num_pages)) {
+                            atomicOr(a.err, HV_DECODE_BAD_PAGE);
+                            good = false;
+                        }
+                        const int slot = a.page_shift >= 0 ? t & (a.page - 1) : t % a.page;
+                        const long long off = !good ? -1
+                                              : keys ? pg.of[p] * a.kc_page + slot * a.kc_slot + head * a.kc_head
+                                                     : pg.of[p] * a.vc_page + slot * a.vc_slot + head * a.vc_head;
+                        if (!copy(keys ? kc : vc, off)) return false;
+                    }
+                    return true;
+                };
+                Pages p0 = pages_of(0), p1 = pages_of(1), p2 = pages_of(2), p3;
+                ok = fill(0, p0, true) && (!alt || n == 1 || fill(1, p1, true));
+                for (int j = 0; j < n && ok; ++j) {
+                    p3 = pages_of(j + 3);
+                    ok = fill(j, p0, false);
+                    if (ok) ok = alt ? j + 2 >= n || fill(j + 2, p2, true) : j + 1 >= n || fill(j + 1, p1, true);
+                    p0 = p1, p1 = p2, p2 = p3;
+                }
+            } while (ok && seg.next(a));
+        flush();
+    } else if (warp >= L::MMA_WARP) {  // one thread of its warpgroup
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::MMA_REGS));
+        if (warp == L::MMA_WARP && lane == 0) {
+            constexpr uint32_t qk = idesc_f16<T>(128, SLOT, false), pv = idesc_f16<T>(128, DP, true);
+            const uint32_t qk_idesc = qk | (a.negate ? 1u << 13 : 0);
+            const uint32_t qs = tc05::smem_u32(smem), rs = tc05::smem_u32(ring);
+            uint32_t base = 0, qn = 0, pn[2] = {0, 0};
+            bool ok = works;
+            auto slot_full = [&](uint32_t f) { return wait_or_stop(&full[f % STAGES], (f / STAGES) & 1, stop); };
+            // scores of buffer s: rows of q tile t against the keys of ring fill f
+            auto scores = [&](int s, int t, uint32_t f) {
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const uint32_t at = rs + (f + p) % STAGES * L::SLOT_BYTES;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(tmem + s * BK + p * SLOT, desc_sw128(qs + t * L::Q_TILE + (k >> 2) * (128 * 128) + (k & 3) * 32, 16),
+                               desc_sw128(at + (k >> 2) * (SLOT * 128) + (k & 3) * 32, 16), qk_idesc, k > 0);
+                }
+                tc05::commit(&sfull[s]);
+            };
+            auto release = [&](uint32_t f) {
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) tc05::commit(&empty[(f + p) % STAGES]);
+            };
+            auto keys_full = [&](uint32_t f) {
+                bool r = true;
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) r = r && slot_full(f + p);
+                tc05::fence_after();
+                return r;
+            };
+            // sums of tile t: weights in buffer s times the values of ring fill f
+            auto sums = [&](int s, int t, uint32_t f, bool add) {
+                if (!wait_or_stop(&pready[s], pn[s]++ & 1, stop)) return false;
+                tc05::fence_after();
+                if (by_hand[s]) return true;
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const uint32_t at = rs + (f + p) % STAGES * L::SLOT_BYTES;
+#pragma unroll
+                    for (int k = 0; k < SLOT / 16; ++k)
+                        mma_ts(tmem + L::O_COL + t * DP, tmem + s * BK + (p * SLOT + k * 16) / 2, desc_sw128(at + k * 2048, SLOT * 128),
+                               pv, add || p || k);
+                }
+                return true;
+            };
+            if (ok) do {
+                    const int n = seg.t1 - seg.t0;
+                    const bool alt = NT == 2 && seg.rows(a) <= 128;
+                    ok = wait_or_stop(qfull, qn++ & 1, stop);
+                    if (!ok) break;
+                    if (NT == 2 && !alt) {
+                        ok = keys_full(base);
+                        if (!ok) break;
+                        scores(0, 0, base);
+                        scores(1, 1, base);
+                        release(base);
+                        if (n == 1) tc05::commit(qempty);
+                        for (int j = 0; j < n; ++j) {
+                            const uint32_t v = base + v_fill(j, n, false), k = base + k_fill(j + 1, false);
+                            const bool more = j + 1 < n;
+                            ok = keys_full(v) && sums(0, 0, v, j > 0);
+                            if (!ok) break;
+                            if (more) {
+                                ok = keys_full(k);
+                                if (!ok) break;
+                                scores(0, 0, k);
+                            } else {
+                                tc05::commit(&ofull[0]);
+                            }
+                            ok = sums(1, 1, v, j > 0);
+                            if (!ok) break;
+                            release(v);
+                            if (more) {
+                                scores(1, 1, k);
+                                release(k);
+                                if (j + 2 == n) tc05::commit(qempty);
+                            } else {
+                                tc05::commit(&ofull[1]);
+                            }
+                        }
+                    } else {
+                        // alternating buffers: with two row tiles' worth of sums each its own, with one the same
+                        constexpr int AHEAD = 2;
+                        for (int j = 0; j < min(n, NT == 2 ? AHEAD : 1) && ok; ++j) {
+                            const uint32_t k = base + k_fill(j, NT == 2);
+                            ok = keys_full(k);
+                            if (!ok) break;
+                            scores(j, 0, k);
+                            release(k);
+                        }
+                        if (!ok) break;
+                        if (n <= (NT == 2 ? AHEAD : 1)) tc05::commit(qempty);
+                        for (int j = 0; j < n; ++j) {
+                            const int s = j & 1;
+                            const uint32_t v = base + v_fill(j, n, NT == 2);
+                            if (NT == 1 && j + 1 < n) {  // the next scores go ahead of these sums
+                                const uint32_t k = base + k_fill(j + 1, false);
+                                ok = keys_full(k);
+                                if (!ok) break;
+                                scores(s ^ 1, 0, k);
+                                release(k);
+                                if (j + 2 == n) tc05::commit(qempty);
+                            }
+                            ok = keys_full(v) && sums(s, NT == 2 ? s : 0, v, j >= NT);
+                            if (!ok) break;
+                            if (NT == 1) tc05::commit(odone);
+                            release(v);
+                            if (NT == 2 && j + 2 < n) {
+                                const uint32_t k = base + k_fill(j + 2, true);
+                                ok = keys_full(k);
+                                if (!ok) break;
+                                scores(s, 0, k);
+                                release(k);
+                                if (j + 3 == n) tc05::commit(qempty);
+                            }
+                            if (j + NT >= n) tc05::commit(&ofull[NT == 2 ? s : 0]);
+                        }
+                    }
+                    base += 2 * n * PARTS;
+                } while (ok && seg.next(a));
+            tc05::commit(drain);  // what was issued has read shared memory and written tensor memory
+            tc05::mbar_wait(drain, 0, DRAIN_ITERS);
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(L::SOFT_REGS));
+        const int wg = warp >> 2, row = tid & 127;  // this warpgroup, and this thread's lane of TMEM
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const float c = a.scale_log2;
+        uint32_t sn[2] = {0, 0}, on = 0, wn = 0, bn = 0, base = 0, steps_done = 0, hand = 0;
+        bool ok = works;
+        auto meet = [&](uint64_t *bar, uint32_t &n) {  // the warps of a warpgroup, or of both
+            __syncwarp();
+            if (lane == 0) arrive(bar);
+            return (bool)__all_sync(~0u, wait_or_stop(bar, n++ & 1, stop));
+        };
+        long long item_first = first - (works ? seg.t0 : 0);  // the line's index of the item's first step
+        bool counted = false;
+        if (ok) do {
+                const int n = seg.t1 - seg.t0, rows = seg.rows(a);
+                const bool alt = NT == 2 && rows <= 128;
+                const int r = (alt ? 0 : wg * 128) + row;
+                const bool exists = r < rows;
+                const int at = (int)((long long)seg.qt * R + r), tok = at / a.group;
+                const int seen = exists ? seg.seq.seen(a, tok) : seg.seq.len;
+                const int first_seen = seg.seq.seen(a, (int)((long long)seg.qt * R + r - row) / a.group);  // the tile's first row
+                const uint32_t otm = tmem + lanes + L::O_COL + (NT == 2 ? wg * DP : 0);
+                counted = false;
+                float m = LOWEST, l = 0.f;
+                bool fresh = true;
+                for (int j = alt ? wg : 0; j < n; j += alt ? 2 : 1) {
+                    const int s = NT == 2 ? wg : j & 1;
+                    const uint32_t stm = tmem + lanes + s * BK;
+                    ok = __all_sync(~0u, wait_or_stop(&sfull[s], sn[s]++ & 1, stop));
+                    if (!ok) break;
+                    tc05::fence_after();
+                    if (hand >> s & 1) {  // the product's thread has read it
+                        if (row == 0) by_hand[s] = 0;
+                        hand &= ~(1u << s);
+                        ok = meet(&wgbar[wg], wn);
+                        if (!ok) break;
+                    }
+                    uint32_t x[4][32];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tc05::ld32(stm + i * 32, x[i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tc05::wait_ld_regs(x[i]);
+                    const int k0 = (seg.t0 + j) * BK, lim = seen - k0;
+                    if (__any_sync(~0u, lim < BK)) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (i >= lim) x[i / 32][i % 32] = __float_as_uint(-CUDART_INF_F);
+                    }
+                    float t[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        t[i] = __uint_as_float(x[i][0]);
+#pragma unroll
+                        for (int k = 1; k < 31; k += 2) t[i] = fmaxf(t[i], fmaxf(__uint_as_float(x[i][k]), __uint_as_float(x[i][k + 1])));
+                        t[i] = fmaxf(t[i], __uint_as_float(x[i][31]));
+                    }
+                    const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c;
+                    if (__any_sync(~0u, top > m + (TOP<T> + SOFT))) {
+                        const float to = fmaxf(top - TOP<T>, m), f = exp2_(m - to);
+                        m = to;
+                        l *= f;
+                        if (!fresh) {  // nothing else writes the sums before this step's weights are there
+                            // ... but with one row tile the product before may still be under way
+                            if (NT == 1) {
+                                ok = __all_sync(~0u, wait_or_stop(odone, (steps_done - 1) & 1, stop));
+                                if (!ok) break;
+                                tc05::fence_after();
+                            }
+#pragma unroll 1
+                            for (int k = 0; k < D; k += 16) {
+                                uint32_t o[16];
+                                __syncwarp();
+                                tc05::ld16(otm + k, o);
+                                tc05::wait_ld_regs(o);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tc05::st16(otm + k, o);
+                            }
+                        }
+                    }
+                    const uint64_t c2 = two(c, c), m2 = two(-m, -m);
+                    uint64_t sum2 = 0;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        float lo, hi;
+                        split2(fma2(two(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), c2, m2), lo, hi);
+                        const uint32_t p = pack(exp2_(lo), exp2_(hi), T());
+                        const float2 v = unpack(p, T());
+                        sum2 = add2(sum2, two(v.x, v.y));
+                        x[i / 32][i % 32] = p;
+                    }
+                    float lo, hi;
+                    split2(sum2, lo, hi);
+                    l += lo + hi;
+                    __syncwarp();
+                    tc05::st32(stm, x[0]);
+                    tc05::st32(stm + 32, x[1]);
+                    tc05::wait_st();
+                    // Values that some row of the tile does not see: any that are no numbers?
+                    if (first_seen < seg.seq.len && first_seen < k0 + BK) {
+                        const uint32_t f = base + v_fill(j, n, alt);
+                        uint32_t top2 = 0;
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            const uint32_t fp = f + p;
+                            ok = ok && __all_sync(~0u, wait_or_stop(&full[fp % STAGES], (fp / STAGES) & 1, stop));
+                            const uint4 *v = (const uint4 *)(ring + fp % STAGES * L::SLOT_BYTES);
+                            for (int i = row; i < SLOT * L::CH; i += 128) {
+                                const uint4 u = v[(i / SLOT >> 3) * (SLOT * 8) + i % SLOT * 8 + (((i / SLOT) ^ (i % SLOT)) & 7)];
+                                top2 = __vmaxu2(top2, u.x & 0x7fff7fffu), top2 = __vmaxu2(top2, u.y & 0x7fff7fffu);
+                                top2 = __vmaxu2(top2, u.z & 0x7fff7fffu), top2 = __vmaxu2(top2, u.w & 0x7fff7fffu);
+                            }
+                        }
+                        if (!ok) break;
+                        const bool bad = __vmaxu2(top2, infinite(T()) - 0x00010001u) != infinite(T()) - 0x00010001u;
+                        if (__any_sync(~0u, bad) && lane == 0) by_hand[s] = 1;
+                        ok = meet(&wgbar[wg], wn);
+                        if (!ok) break;
+                        if (by_hand[s]) {
+                            hand |= 1u << s;
+                            if (NT == 1 && !fresh) {
+                                ok = __all_sync(~0u, wait_or_stop(odone, (steps_done - 1) & 1, stop));
+                                if (!ok) break;
+                                tc05::fence_after();
+                            }
+#pragma unroll 1
+                            for (int k = 0; k < D; k += 16) {
+                                uint32_t o[16], w8[8];
+                                if (fresh) {
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) o[i] = 0;
+                                } else {
+                                    tc05::ld16(otm + k, o);
+                                    tc05::wait_ld_regs(o);
+                                }
+#pragma unroll 1
+                                for (int key = 0; key < BK; key += 16) {
+                                    tc05::ld8(stm + key / 2, w8);
+                                    tc05::wait_ld_regs(w8);
+                                    const uint32_t fp = f + key / SLOT;
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) {
+                                        const float2 w2 = unpack(w8[i / 2], T());
+                                        const float wt = i & 1 ? w2.y : w2.x;
+                                        const int kr = (key + i) % SLOT;
+                                        const uint8_t *vr = ring + fp % STAGES * L::SLOT_BYTES + (k >> 6) * (SLOT * 128) + kr * 128;
+#pragma unroll
+                                        for (int q = 0; q < 2 && key + i < lim; ++q) {
+                                            const uint4 u = *(const uint4 *)(vr + (((((k & 63) >> 3) + q) ^ (kr & 7)) << 4));
+                                            const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                                            for (int e = 0; e < 4; ++e) {
+                                                const float2 y = unpack(uu[e], T());
+                                                o[q * 8 + e * 2] = __float_as_uint(fmaf(wt, y.x, __uint_as_float(o[q * 8 + e * 2])));
+                                                o[q * 8 + e * 2 + 1] = __float_as_uint(fmaf(wt, y.y, __uint_as_float(o[q * 8 + e * 2 + 1])));
+                                            }
+                                        }
+                                    }
+                                    __syncwarp();
+                                }
+                                tc05::st16(otm + k, o);
+                            }
+                            tc05::wait_st();
+                        }
+                    }
+                    fresh = false;
+                    ++steps_done;
+                    tc05::fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(&pready[s]);
+                }
+                if (!ok) break;
+                // the sums
+                const bool some = alt ? n > wg : true;
+                if (some) {
+                    ok = __all_sync(~0u, wait_or_stop(&ofull[NT == 2 ? wg : 0], on++ & 1, stop));
+                    if (!ok) break;
+                    tc05::fence_after();
+                }
+                float f[2] = {1.f, 0.f};  // of this warpgroup's sums, and of the other's
+                if (alt) {  // the even and the odd steps'
+                    half_stat[wg * 128 + row] = make_float2(m, l);
+                    tc05::fence_before();
+                    ok = meet(both, bn);
+                    if (!ok) break;
+                    tc05::fence_after();
+                    const float2 other = half_stat[(wg ^ 1) * 128 + row];
+                    const float M = fmaxf(m, other.x);
+                    f[0] = exp2_(m - M), f[1] = exp2_(other.x - M);
+                    l = l * f[0] + other.y * f[1];
+                    m = M;
+                    if (!some) f[0] = 0.f;
+                }
+                const bool two_halves = alt && n > 1, other_alone = alt && !some;
+                const int col0 = alt ? wg * (D / 2) : 0, col1 = alt ? col0 + D / 2 : D;
+                auto columns = [&](int col, float (&v)[16]) {
+                    uint32_t o[16];
+                    __syncwarp();  // rows that do not exist store nothing: the warp's lanes meet again
+                    const uint32_t mine = otm + col, its = tmem + lanes + L::O_COL + (wg ^ 1) * DP + col;
+                    tc05::ld16(other_alone ? its : mine, o);
+                    tc05::wait_ld_regs(o);
+                    const float w = other_alone ? f[1] : f[0];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * w;
+                    if (two_halves) {
+                        tc05::ld16(its, o);
+                        tc05::wait_ld_regs(o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(o[i]), f[1], v[i]);
+                    }
+                };
+                T *out = (T *)a.out;
+                float *lse = a.lse;
+                if (exists) {
+                    const long long tk = seg.seq.s0 + tok;
+                    const int hd = seg.h * a.group + at - tok * a.group;
+                    out += tk * a.o_tok + hd * a.o_head;
+                    if (lse) lse += tk * a.lse_tok + hd * a.lse_head;
+                }
+                const int c_first = (int)(item_first / share), c_last = (int)((item_first + seg.steps - 1) / share);
+                if (c_first == c_last) {
+                    const float inv = seen > 0 ? 1.f / l : 0.f;
+#pragma unroll 1
+                    for (int col = col0; col < col1; col += 16) {
+                        float v[16];
+                        columns(col, v);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = seen > 0 ? v[i] * inv : 0.f;
+                        if (exists) store_row16(out + col, a.o_vec, v);
+                    }
+                    if (exists && lse && col0 == 0) *lse = seen > 0 ? (m + log2f(l)) * 0.69314718055994531f : -CUDART_INF_F;
+                } else {
+                    // A share leaves its second slot to the item that starts in it, its first to one that started before.
+                    auto slot = [&](int k) { return 2ll * k + (k == c_first); };
+                    const int tile0 = alt ? 0 : wg * 128;  // rows of this warpgroup
+                    float4 *po = (float4 *)a.parts;  // a slot: [D / 4][R]
+                    float2 *pst = (float2 *)(a.parts + 2ll * gridDim.x * L::PART);  // a slot: [R], with alternating halves [2][128]
+                    const int strow = alt ? wg * 128 + row : tile0 + row;
+                    const long long mine = slot(blockIdx.x);
+#pragma unroll 1
+                    for (int col = col0; col < col1; col += 16) {
+                        float v[16];
+                        columns(col, v);
+                        if (exists)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                __stcg(po + mine * (L::PART / 4) + (long long)(col / 4 + i) * R + tile0 + row,
+                                       make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+                    }
+                    if (exists) __stcg(pst + mine * R + strow, make_float2(m, l));
+                    const int k_parts = c_last - c_first + 1;
+                    ok = meet(&wgbar[wg], wn);
+                    if (!ok) break;
+                    if (row == 0) {
+                        __threadfence();
+                        last_flag[wg] = atomicInc(a.counts + wg * MAX_GRID + c_first, k_parts - 1) == (uint32_t)k_parts - 1;
+                        __threadfence();
+                    }
+                    counted = true;
+                    ok = meet(&wgbar[wg], wn);
+                    if (!ok) break;
+                    if (last_flag[wg]) {
+                        // a row's maximum and sum over the parts; then each part's weight in the place of its maximum
+                        if (exists) {
+                            float M = LOWEST, S = 0.f;
+                            for (int k = 0; k < k_parts; ++k) M = fmaxf(M, __ldcg(pst + slot(c_first + k) * R + strow).x);
+                            for (int k = 0; k < k_parts; ++k) {
+                                const float2 v = __ldcg(pst + slot(c_first + k) * R + strow);
+                                S += exp2_(v.x - M) * v.y;
+                            }
+                            const float inv = seen > 0 ? 1.f / S : 0.f;
+                            for (int k = 0; k < k_parts; ++k) {
+                                float2 *p = pst + slot(c_first + k) * R + strow;
+                                __stcg(&p->x, seen > 0 ? exp2_(__ldcg(&p->x) - M) : 0.f);
+                                __stcg(&p->y, inv);
+                            }
+                            if (lse && col0 == 0) *lse = seen > 0 ? (M + log2f(S)) * 0.69314718055994531f : -CUDART_INF_F;
+                        }
+                        __threadfence_block();
+                        ok = meet(&wgbar[wg], wn);
+                        if (!ok) break;
+                        const int nr = min(128, rows - tile0), n4 = nr * (col1 - col0) / 4;
+                        for (int i = row; i < n4; i += 128) {
+                            const int rr = i % nr, c4 = col0 / 4 + i / nr;
+                            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                            float inv = 0.f;
+#pragma unroll 4
+                            for (int k = 0; k < k_parts; ++k) {
+                                const long long sl = slot(c_first + k);
+                                const float2 wv = __ldcg(pst + sl * R + (alt ? wg * 128 : tile0) + rr);
+                                const float4 v = __ldcg(po + sl * (L::PART / 4) + (long long)c4 * R + tile0 + rr);
+                                inv = wv.y;
+                                acc.x = fmaf(wv.x, v.x, acc.x), acc.y = fmaf(wv.x, v.y, acc.y);
+                                acc.z = fmaf(wv.x, v.z, acc.z), acc.w = fmaf(wv.x, v.w, acc.w);
+                            }
+                            const int at2 = (int)((long long)seg.qt * R + tile0 + rr), tk = at2 / a.group;
+                            T *o = (T *)a.out + (seg.seq.s0 + (long long)tk) * a.o_tok +
+                                   (seg.h * a.group + at2 - tk * a.group) * a.o_head + c4 * 4;
+                            const bool sees = seg.seq.seen(a, tk) > 0;
+                            alignas(8) T e[4] = {from_f32<T>(sees ? acc.x * inv : 0.f), from_f32<T>(sees ? acc.y * inv : 0.f),
+                                                 from_f32<T>(sees ? acc.z * inv : 0.f), from_f32<T>(sees ? acc.w * inv : 0.f)};
+                            if (a.o_vec) {
+                                *(uint2 *)o = *(const uint2 *)e;
+                            } else {
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) o[q] = e[q];
+                            }
+                        }
+                    }
+                }
+                if (alt) {  // the other warpgroup has read this one's sums
+                    tc05::fence_before();
+                    ok = meet(both, bn);
+                    if (!ok) break;
+                    tc05::fence_after();
+                }
+                item_first += seg.steps;
+                base += 2 * n * PARTS;
+                if (!seg.next(a)) break;
+            } while (true);
+        if (!ok && works && row == 0) {
+            // Gave up: the counters of the cut items of this share are counted on, so that they end at zero.
+            do {
+                const int c_first = (int)(item_first / share), c_last = (int)((item_first + seg.steps - 1) / share);
+                if (c_first != c_last && !counted) atomicInc(a.counts + wg * MAX_GRID + c_first, c_last - c_first);
+                counted = false;
+                item_first += seg.steps;
+            } while (seg.next(a));
+        }
+        tc05::fence_before();
+    }
+    __syncwarp();
+    __syncthreads();
+    if (tid == 0 && *stop) atomicOr(a.err, HV_DECODE_STALLED);  // every role has been through
+    if (warp == L::MMA_WARP) {
+        tc05::fence_after();
+        tc05::tmem_dealloc(tmem, 512);
     }
 }
 
 template <typename T, int D>
-cudaError_t launch(const ChunkArgs &a, cudaStream_t st) {
-    return launch_pdl(chunk_simple_kernel<T, D>, dim3(1024, (unsigned)a.seqs), dim3(256), 0, st, a);
+cudaError_t launch(ChunkArgs a, int grid, cudaStream_t st) {
+    using L = Lay<D>;
+    static std::atomic<uint64_t> ready;
+    static std::atomic<int> regs;
+    cudaError_t e = allow_shared(chunk_kernel<T, D>, ready);
+    if (e != cudaSuccess) return e;
+    if (!regs.load(std::memory_order_relaxed)) {  // what the warps' shares are taken from
+        cudaFuncAttributes f;
+        e = cudaFuncGetAttributes(&f, chunk_kernel<T, D>);
+        if (e != cudaSuccess) return e;
+        if (f.numRegs != L::REGS) return cudaErrorInvalidConfiguration;
+        regs.store(f.numRegs, std::memory_order_relaxed);
+    }
+    return launch_pdl(chunk_kernel<T, D>, dim3((unsigned)grid), dim3(L::THREADS), L::BYTES, st, a);
 }
 
 template <typename T>
-cudaError_t by_dim(const ChunkArgs &a, int dim, cudaStream_t st) {
+cudaError_t by_dim(const ChunkArgs &a, int dim, int grid, cudaStream_t st) {
     switch (dim) {
-        case 32: return launch<T, 32>(a, st);
-        case 64: return launch<T, 64>(a, st);
-        case 96: return launch<T, 96>(a, st);
-        case 128: return launch<T, 128>(a, st);
-        case 192: return launch<T, 192>(a, st);
-        default: return launch<T, 256>(a, st);
+        case 32: return launch<T, 32>(a, grid, st);
+        case 64: return launch<T, 64>(a, grid, st);
+        case 96: return launch<T, 96>(a, grid, st);
+        case 128: return launch<T, 128>(a, grid, st);
+        case 192: return launch<T, 192>(a, grid, st);
+        default: return launch<T, 256>(a, grid, st);
     }
 }
 
 bool known_dim(int d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
+
+int wave() {
+    const int sms = sm_count();
+    return sms < MAX_GRID ? sms : MAX_GRID;
+}
+
+static_assert(2 * MAX_GRID * 4 <= HV_ATTENTION_COUNTER_BYTES, "the counters that the caller zeroes");
+static_assert(HV_ATTENTION_MAX_LENGTH + (long long)BK <= INT32_MAX, "token numbers of a last step are ints");
 
 }  // namespace
 }  // namespace hv
@@ -107,7 +1064,9 @@ using namespace hv;
 extern "C" int hv_paged_chunk_attention_workspace(int dim, int64_t *bytes) {
     if (!bytes) return fail(HV_ERR_VALUE, "null argument");
     if (!known_dim(dim)) return fail(HV_ERR_VALUE, "dim must be 32, 64, 96, 128, 192 or 256");
-    *bytes = HV_ATTENTION_COUNTER_BYTES;
+    const int grid = wave(), rows = dim <= 128 ? 256 : 128;
+    if (!grid) return fail(HV_ERR_CUDA, "cannot read the device's SM count");
+    *bytes = HV_ATTENTION_COUNTER_BYTES + 2ll * grid * rows * (dim + 2) * 4;
     return HV_OK;
 }
 
@@ -145,10 +1104,20 @@ extern "C" int hv_paged_chunk_attention(const hv_chunk_args *p, void *stream) {
     a.pages_stride = p->page_table_stride;
     a.tokens = p->tokens, a.seqs = p->seqs, a.heads = p->heads, a.kv_heads = p->kv_heads, a.group = p->heads / p->kv_heads;
     a.num_pages = p->num_pages, a.page = p->page_size, a.max_pages = p->max_pages, a.causal = p->causal;
-    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
+    a.q_vec = dec::aligned(a.q, 16) && a.q_tok % 8 == 0 && a.q_head % 8 == 0;
+    a.o_vec = dec::aligned(a.out, 16) && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
+    // A score is taken times a scale above zero, with q negated for one below, so that the largest stays the
+    // largest and -inf that; for zero the least normal number gives the weights of 0.
+    a.negate = p->scale < 0;
+    a.scale_log2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, FLT_MIN);
+    a.skip = dec::skipped_copy();
+    a.counts = (uint32_t *)p->d_workspace;
+    a.parts = (float *)((char *)p->d_workspace + HV_ATTENTION_COUNTER_BYTES);
     a.err = err;
-    const cudaError_t e = p->dtype == HV_BF16 ? by_dim<__nv_bfloat16>(a, p->dim, (cudaStream_t)stream)
-                                              : by_dim<__half>(a, p->dim, (cudaStream_t)stream);
+    const int grid = wave();
+    const cudaError_t e = p->dtype == HV_BF16 ? by_dim<__nv_bfloat16>(a, p->dim, grid, (cudaStream_t)stream)
+                                              : by_dim<__half>(a, p->dim, grid, (cudaStream_t)stream);
     if (e != cudaSuccess) return fail(HV_ERR_CUDA, "paged_chunk_attention: %s", cudaGetErrorString(e));
     return HV_OK;
 }

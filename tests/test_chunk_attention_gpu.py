@@ -366,3 +366,38 @@ def test_chunk_refusals():
     out = torch.zeros_like(q)
     decode.paged_chunk_attention(*good, out=out)
     assert out._version == 1 + 0 and q._version == v
+
+
+def test_chunk_workspace_is_large_enough():
+    from heatvit_b200 import decode
+    case = chunk_case(16, [5], [700], 4, 4, 64, 16, HF)
+    for small in (decode.AttentionWorkspace(),):
+        with pytest.raises(ValueError, match="workspace"):
+            check(*case, workspace=small)
+    check(*case, workspace=decode.AttentionWorkspace(chunks=True))
+
+
+@pytest.fixture
+def stall():
+    from heatvit_b200 import _lib, decode
+    assert _lib.lib().hv_test_decode_stall(-1) == 0
+    yield _lib.lib().hv_test_decode_stall
+    _lib.lib().hv_test_decode_stall(-1)
+    decode.device_error()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new,past", [(600, 0), (3, 40000)])
+@pytest.mark.parametrize("copy", [0, 1, 3])
+def test_chunk_wait_runs_out_reports_and_recovers(stall, dim, new, past, copy):
+    """A tile of keys or values that is not reported (in a workspace that is used on): the error word, then the same
+    call right."""
+    from heatvit_b200 import abi, decode
+    q, kc, vc, table, lens, starts = chunk_case(26, [new, 10], [past, 300], 4, 2, dim, 16, BF)
+    ws = decode.AttentionWorkspace(chunks=True)
+    assert stall(copy) == 0
+    decode.paged_chunk_attention(q, kc, vc, table, ints(lens), ints(starts), workspace=ws)
+    assert stall(-1) == 0
+    assert decode.device_error() == abi.HV_DECODE_STALLED
+    assert int(ws.buffer[:12288].max()) == 0
+    check(q, kc, vc, table, lens, starts, workspace=ws)
