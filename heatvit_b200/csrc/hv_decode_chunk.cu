@@ -85,10 +85,15 @@ struct Lay {
     // Registers of a thread at launch, and of the roles from then on (shares of what the block was launched with).
     static constexpr int REGS = NT == 2 ? 128 : 168, COPY_REGS = 72, MMA_REGS = 56, SOFT_REGS = NT == 2 ? 192 : 240;
     static_assert(128 * (COPY_REGS + MMA_REGS + NT * SOFT_REGS) <= REGS * THREADS, "registers");
-    static constexpr int O_COL = 256;  // TMEM: scores at 0 and 128, sums from here
+    // TMEM columns: scores, sums, weights.  APART: the weights have columns of their own, so that the next scores are
+    // under way while they are made; with two row tiles of 128 dimensions they have to take the scores' place.
+    static constexpr bool APART = NT == 1 || DP == 64;
+    __host__ __device__ static constexpr int s_col(int w) { return w * BK; }
+    __host__ __device__ static constexpr int o_col(int w) { return 256 + w * DP; }
+    __host__ __device__ static constexpr int p_col(int w) { return NT == 1 ? BK : APART ? 384 + w * 64 : w * BK; }
     static constexpr int PART = R * D, CH = D / 8;  // numbers of a part; 16-byte pieces of a row
     static_assert(BYTES <= 227 * 1024, "shared memory");
-    static_assert(O_COL + NT * DP <= 512, "tensor memory");
+    static_assert(o_col(NT) <= (APART && NT == 2 ? 384 : 512), "tensor memory");
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
@@ -102,21 +107,30 @@ __device__ __forceinline__ float exp2_(float x) {
 __device__ __forceinline__ void arrive(uint64_t *mbar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(tc05::smem_u32(mbar)) : "memory");
 }
+// One poll of phase `parity` of `bar`, for up to `ns` (the thread sleeps meanwhile).
+__device__ __forceinline__ bool poll(uint64_t *bar, uint32_t parity, uint32_t ns) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(tc05::smem_u32(bar)), "r"(parity), "r"(ns)
+        : "memory");
+    return done;
+}
 // Bounded wait that also ends when another role of the CTA has given up.
 __device__ __forceinline__ bool wait_or_stop(uint64_t *bar, uint32_t parity, volatile int *stop) {
-    for (uint32_t i = 0; i < WAIT_ITERS / 64; ++i) {
-        if (tc05::mbar_wait(bar, parity, 64)) return true;
+    for (uint32_t i = 0; i < WAIT_ITERS; ++i) {
+        if (poll(bar, parity, 2000)) return true;
         if (*stop) return false;
     }
     *stop = 1;
     return false;
 }
-// 128-byte swizzled operands: K-major (eight rows of 128 bytes an atom, `sbo` 1024), or MN-major with blocks of 64
-// along N `lbo` bytes apart.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+// A 128-byte swizzled operand's descriptor: its high word, and its low one for an address.  K-major: atoms of eight rows
+// of 128 bytes, 1024 apart; MN-major: the same atoms of eight k of 64 elements, the blocks of 64 along N `lbo` bytes apart.
+// Steps within an operand are added to the low word, in 16 bytes.
+constexpr uint32_t DESC_HI = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
 // kind::f16, f32 accumulator.
 template <typename T>
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) {
@@ -124,19 +138,27 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn_major) 
     return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Issued by the one lane for which `leads`; the whole warp comes here, so that operands stay in uniform registers.
+__device__ __forceinline__ void mma_ss(uint32_t leads, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n.reg .pred p, q;\n.reg .b64 x, y;\nsetp.ne.b32 p, %5, 0;\nsetp.ne.b32 q, %6, 0;\n"
+        "mov.b64 x, {%1, %4};\nmov.b64 y, {%2, %4};\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(DESC_HI), "r"(acc), "r"(leads)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t leads, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n.reg .pred p, q;\n.reg .b64 y;\nsetp.ne.b32 p, %5, 0;\nsetp.ne.b32 q, %6, 0;\n"
+        "mov.b64 y, {%2, %4};\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(DESC_HI), "r"(acc), "r"(leads)
         : "memory");
+}
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
 }
 __device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -170,6 +192,32 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// One pair of weights in EMULATED is not the special function unit's, which makes 16 exponentials a clock where the
+// tensor core takes 8192 multiply-adds, but 2^x as 2^n 2^f, n the nearest integer, by a polynomial of degree 4 fitted
+// to 2^f on [-1/2, 1/2] (2.6e-6 = 2^-18 off at most; half a step of bf16 is 2^-9, of fp16 2^-12).  Under -126
+// it gives 2^-126; of a NaN the largest number, which as a weight is infinite.
+constexpr int EMULATED = 4;
+__device__ __forceinline__ void exp2_pair(uint64_t x, float &lo, float &hi) {
+    split2(x, lo, hi);
+    const uint64_t y = two(max_nan(lo, -126.f), max_nan(hi, -126.f));
+    const uint64_t magic = two(12582912.f, 12582912.f), back = two(-12582912.f, -12582912.f);  // 1.5 * 2^23
+    const uint64_t n = add2(y, magic), f = fma2(add2(n, back), two(-1.f, -1.f), y);
+    uint64_t p = fma2(f, two(0x1.3997d6p-7f, 0x1.3997d6p-7f), two(0x1.ca1442p-5f, 0x1.ca1442p-5f));
+    p = fma2(p, f, two(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    p = fma2(p, f, two(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    p = fma2(p, f, two(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    float nl, nh;
+    split2(n, nl, nh);
+    split2(p, lo, hi);
+    lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(nl) << 23));
+    hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(nh) << 23));
 }
 
 // A sequence's rows of q and cached tokens, brought into range (what is not is reported once, by `tell`).
@@ -234,6 +282,15 @@ struct Segment {
     }
 };
 
+// What a row's sums are multiplied by, and its log-sum-exp: a row that sees nothing has zeros; one whose scores are
+// all -inf (its maximum never moved), or with a NaN among them (a weight without bounds), has NaN.
+__device__ __forceinline__ float row_factor(int seen, float m, float l) {
+    return seen <= 0 ? 0.f : m == LOWEST || !(l < CUDART_INF_F) ? CUDART_NAN_F : 1.f / l;
+}
+__device__ __forceinline__ float row_lse(int seen, float m, float l) {
+    return seen <= 0 || m == LOWEST ? -CUDART_INF_F : l < CUDART_INF_F ? (m + log2f(l)) * 0.69314718055994531f : CUDART_NAN_F;
+}
+
 template <typename T>
 __device__ __forceinline__ void store_row16(T *p, bool vec, const float (&v)[16]) {
     alignas(16) T e[16];
@@ -256,9 +313,9 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
     uint8_t *ring = smem + L::Q_BYTES;
     float2 *half_stat = (float2 *)(smem + L::STAT);
     uint64_t *full = (uint64_t *)(smem + L::BARS), *empty = full + STAGES, *qfull = empty + STAGES, *qempty = qfull + 1;
-    uint64_t *sfull = qempty + 1, *pready = sfull + 2, *ofull = pready + 2, *wgbar = ofull + 2, *both = wgbar + 2;
-    uint64_t *drain = both + 1, *odone = drain + 1;
-    static_assert((2 * STAGES + 15) * 8 <= 256, "barriers");
+    uint64_t *sfull = qempty + 1, *sfree = sfull + 2, *pready = sfree + 2, *odone = pready + 4, *wgbar = odone + 2, *both = wgbar + 2;
+    uint64_t *drain = both + 1;
+    static_assert((2 * STAGES + 16) * 8 <= 256, "barriers");
     long long *line = (long long *)(smem + L::MISC);  // total, share, steps ahead of the first step's sequence, that sequence
     uint32_t *tslot = (uint32_t *)(line + 4);
     volatile int *stop = (volatile int *)(tslot + 1);
@@ -281,13 +338,14 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
         for (int i = 0; i < 2; ++i) {
             by_hand[i] = 0;
             tc05::mbar_init(&sfull[i], 1);
-            tc05::mbar_init(&pready[i], 4);
-            tc05::mbar_init(&ofull[i], 1);
+            tc05::mbar_init(&sfree[i], 4);
+            tc05::mbar_init(&pready[2 * i], 4);  // weights of the first 64 keys, and of the others
+            tc05::mbar_init(&pready[2 * i + 1], 4);
+            tc05::mbar_init(&odone[i], 1);
             tc05::mbar_init(&wgbar[i], 4);
         }
         tc05::mbar_init(both, 8);
         tc05::mbar_init(drain, 1);
-        tc05::mbar_init(odone, 1);
         tc05::fence_mbar_init();
     }
     griddep_wait();
@@ -408,10 +466,13 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
         seg.clip();
     }
     __syncwarp();
-    // Which ring fill, from the segment's first, holds the keys (values) of its step j of n: keys of a step ahead
-    // of the values before them; with alternating tiles two steps ahead.
-    auto k_fill = [](int j, bool alt) { return (alt ? (j ? 2 * j - 1 : 0) : 2 * j) * PARTS; };
-    auto v_fill = [](int j, int n, bool alt) { return (!alt || n == 1 ? 2 * j + 1 : j < n - 1 ? 2 * j + 2 : 2 * n - 1) * PARTS; };
+    // Which ring fill, from the segment's first, holds the keys (values) of its step j of n.  The keys of the first `lead`
+    // steps come first, then those of step j + lead and the values of step j, in the order of their use: keys ahead
+    // where scores go ahead of sums (APART), else values.
+    constexpr bool APART = L::APART;
+    auto lead_of = [](bool alt) { return alt ? 2 : 1; };
+    auto k_fill = [](int j, int lead) { return (j < lead ? j : 2 * j - lead + !APART) * PARTS; };
+    auto v_fill = [](int j, int n, int lead) { return (j + lead < n + !APART ? lead + 2 * j + APART : n + j) * PARTS; };
 
     if (warp >= L::SOFT_WARPS && warp < L::SOFT_WARPS + 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::COPY_REGS));
@@ -544,135 +605,101 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                 ok = fill(0, p0, true) && (!alt || n == 1 || fill(1, p1, true));
                 for (int j = 0; j < n && ok; ++j) {
                     p3 = pages_of(j + 3);
-                    ok = fill(j, p0, false);
+                    if (!APART) ok = fill(j, p0, false);
                     if (ok) ok = alt ? j + 2 >= n || fill(j + 2, p2, true) : j + 1 >= n || fill(j + 1, p1, true);
+                    if (APART && ok) ok = fill(j, p0, false);
                     p0 = p1, p1 = p2, p2 = p3;
                 }
             } while (ok && seg.next(a));
         flush();
     } else if (warp >= L::MMA_WARP) {  // one thread of its warpgroup
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::MMA_REGS));
-        if (warp == L::MMA_WARP && lane == 0) {
+        if (warp == L::MMA_WARP) {
+            const uint32_t leads = elected();
+            auto commit = [&](uint64_t *bar) {
+                if (leads) tc05::commit(bar);
+                __syncwarp();
+            };
             constexpr uint32_t qk = idesc_f16<T>(128, SLOT, false), pv = idesc_f16<T>(128, DP, true);
             const uint32_t qk_idesc = qk | (a.negate ? 1u << 13 : 0);
             const uint32_t qs = tc05::smem_u32(smem), rs = tc05::smem_u32(ring);
-            uint32_t base = 0, qn = 0, pn[2] = {0, 0};
+            uint32_t base = 0, qn = 0, pn = 0, sn = 0;  // pn, sn: phase bits of either row tile's weights and scores
+            bool scored[2] = {false, false};
             bool ok = works;
-            auto slot_full = [&](uint32_t f) { return wait_or_stop(&full[f % STAGES], (f / STAGES) & 1, stop); };
-            // scores of buffer s: rows of q tile t against the keys of ring fill f
-            auto scores = [&](int s, int t, uint32_t f) {
+            auto wait_all = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(~0u, wait_or_stop(bar, parity, stop)); };
+            auto tile_full = [&](uint32_t f) {
+                bool r = true;
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    const uint32_t at = rs + (f + p) % STAGES * L::SLOT_BYTES;
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_ss(tmem + s * BK + p * SLOT, desc_sw128(qs + t * L::Q_TILE + (k >> 2) * (128 * 128) + (k & 3) * 32, 16),
-                               desc_sw128(at + (k >> 2) * (SLOT * 128) + (k & 3) * 32, 16), qk_idesc, k > 0);
-                }
-                tc05::commit(&sfull[s]);
+                for (int p = 0; p < PARTS; ++p) r = r && wait_all(&full[(f + p) % STAGES], ((f + p) / STAGES) & 1);
+                return r;
             };
             auto release = [&](uint32_t f) {
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) tc05::commit(&empty[(f + p) % STAGES]);
+                for (int p = 0; p < PARTS; ++p) commit(&empty[(f + p) % STAGES]);
             };
-            auto keys_full = [&](uint32_t f) {
-                bool r = true;
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p) r = r && slot_full(f + p);
+            // scores for warpgroup w: rows of q tile t against the keys of ring fill f
+            auto scores = [&](int w, int t, uint32_t f) {
+                if (APART) {  // the scores before have been read
+                    if ((w ? scored[1] : scored[0]) && !wait_all(&sfree[w], sn >> w & 1 ^ 1)) return false;
+                    sn ^= 1u << w;
+                    scored[0] |= w == 0, scored[1] |= w == 1;
+                }
+                if (!tile_full(f)) return false;
                 tc05::fence_after();
-                return r;
-            };
-            // sums of tile t: weights in buffer s times the values of ring fill f
-            auto sums = [&](int s, int t, uint32_t f, bool add) {
-                if (!wait_or_stop(&pready[s], pn[s]++ & 1, stop)) return false;
-                tc05::fence_after();
-                if (by_hand[s]) return true;
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) {
-                    const uint32_t at = rs + (f + p) % STAGES * L::SLOT_BYTES;
+                    const uint32_t x = desc_lo(qs + t * L::Q_TILE, 16), y = desc_lo(rs + (f + p) % STAGES * L::SLOT_BYTES, 16);
 #pragma unroll
-                    for (int k = 0; k < SLOT / 16; ++k)
-                        mma_ts(tmem + L::O_COL + t * DP, tmem + s * BK + (p * SLOT + k * 16) / 2, desc_sw128(at + k * 2048, SLOT * 128),
-                               pv, add || p || k);
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(leads, tmem + w * BK + p * SLOT, x + (k >> 2) * 1024 + (k & 3) * 2, y + (k >> 2) * (SLOT * 8) + (k & 3) * 2,
+                               qk_idesc, k > 0);
                 }
+                commit(&sfull[w]);
+                return true;
+            };
+            // sums of warpgroup w: its weights times the values of ring fill f
+            auto sums = [&](int w, uint32_t f, bool add) {
+                if (!tile_full(f)) return false;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // halves of the keys
+                    if (!wait_all(&pready[2 * w + h], pn >> w & 1)) return false;
+                    tc05::fence_after();
+                    if (by_hand[w]) continue;
+                    const uint32_t y = desc_lo(rs + (f + h * (PARTS - 1)) % STAGES * L::SLOT_BYTES, SLOT * 128) + (PARTS == 1 ? h * 512 : 0);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_ts(leads, tmem + (w ? L::o_col(1) : L::o_col(0)), tmem + (w ? L::p_col(1) : L::p_col(0)) + h * 32 + k * 8,
+                               y + k * 128, pv, add || h || k);
+                }
+                pn ^= 1u << w;
+                commit(&odone[w]);
                 return true;
             };
             if (ok) do {
+                    // Units: either row tile in turn against each step's keys, or the one against the steps in turn.
                     const int n = seg.t1 - seg.t0;
-                    const bool alt = NT == 2 && seg.rows(a) <= 128;
-                    ok = wait_or_stop(qfull, qn++ & 1, stop);
-                    if (!ok) break;
-                    if (NT == 2 && !alt) {
-                        ok = keys_full(base);
+                    const bool alt = NT == 2 && seg.rows(a) <= 128, pair = NT == 2 && !alt;
+                    const int lead = lead_of(alt), all = pair ? 2 * n : n;
+                    ok = wait_all(qfull, qn++ & 1);
+                    auto score_unit = [&](int u) {
+                        const uint32_t f = base + k_fill(pair ? u >> 1 : u, lead);
+                        if (!scores(NT == 2 ? u & 1 : 0, pair ? u & 1 : 0, f)) return false;
+                        if (!pair || u & 1) release(f);
+                        if (u + 1 == all) commit(qempty);
+                        return true;
+                    };
+                    for (int u = 0; u < min(all, NT) && ok; ++u) ok = score_unit(u);
+                    for (int u = 0; u < all && ok; ++u) {
+                        if (APART && u + NT < all) ok = score_unit(u + NT);
                         if (!ok) break;
-                        scores(0, 0, base);
-                        scores(1, 1, base);
-                        release(base);
-                        if (n == 1) tc05::commit(qempty);
-                        for (int j = 0; j < n; ++j) {
-                            const uint32_t v = base + v_fill(j, n, false), k = base + k_fill(j + 1, false);
-                            const bool more = j + 1 < n;
-                            ok = keys_full(v) && sums(0, 0, v, j > 0);
-                            if (!ok) break;
-                            if (more) {
-                                ok = keys_full(k);
-                                if (!ok) break;
-                                scores(0, 0, k);
-                            } else {
-                                tc05::commit(&ofull[0]);
-                            }
-                            ok = sums(1, 1, v, j > 0);
-                            if (!ok) break;
-                            release(v);
-                            if (more) {
-                                scores(1, 1, k);
-                                release(k);
-                                if (j + 2 == n) tc05::commit(qempty);
-                            } else {
-                                tc05::commit(&ofull[1]);
-                            }
-                        }
-                    } else {
-                        // alternating buffers: with two row tiles' worth of sums each its own, with one the same
-                        constexpr int AHEAD = 2;
-                        for (int j = 0; j < min(n, NT == 2 ? AHEAD : 1) && ok; ++j) {
-                            const uint32_t k = base + k_fill(j, NT == 2);
-                            ok = keys_full(k);
-                            if (!ok) break;
-                            scores(j, 0, k);
-                            release(k);
-                        }
-                        if (!ok) break;
-                        if (n <= (NT == 2 ? AHEAD : 1)) tc05::commit(qempty);
-                        for (int j = 0; j < n; ++j) {
-                            const int s = j & 1;
-                            const uint32_t v = base + v_fill(j, n, NT == 2);
-                            if (NT == 1 && j + 1 < n) {  // the next scores go ahead of these sums
-                                const uint32_t k = base + k_fill(j + 1, false);
-                                ok = keys_full(k);
-                                if (!ok) break;
-                                scores(s ^ 1, 0, k);
-                                release(k);
-                                if (j + 2 == n) tc05::commit(qempty);
-                            }
-                            ok = keys_full(v) && sums(s, NT == 2 ? s : 0, v, j >= NT);
-                            if (!ok) break;
-                            if (NT == 1) tc05::commit(odone);
-                            release(v);
-                            if (NT == 2 && j + 2 < n) {
-                                const uint32_t k = base + k_fill(j + 2, true);
-                                ok = keys_full(k);
-                                if (!ok) break;
-                                scores(s, 0, k);
-                                release(k);
-                                if (j + 3 == n) tc05::commit(qempty);
-                            }
-                            if (j + NT >= n) tc05::commit(&ofull[NT == 2 ? s : 0]);
-                        }
+                        const uint32_t f = base + v_fill(pair ? u >> 1 : u, n, lead);
+                        ok = sums(NT == 2 ? u & 1 : 0, f, u >= NT);
+                        if (ok && (!pair || u & 1)) release(f);
+                        if (!APART && ok && u + NT < all) ok = score_unit(u + NT);
                     }
                     base += 2 * n * PARTS;
                 } while (ok && seg.next(a));
-            tc05::commit(drain);  // what was issued has read shared memory and written tensor memory
+            commit(drain);  // what was issued has read shared memory and written tensor memory
             tc05::mbar_wait(drain, 0, DRAIN_ITERS);
         }
         __syncwarp();
@@ -681,7 +708,8 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
         const int wg = warp >> 2, row = tid & 127;  // this warpgroup, and this thread's lane of TMEM
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float c = a.scale_log2;
-        uint32_t sn[2] = {0, 0}, on = 0, wn = 0, bn = 0, base = 0, steps_done = 0, hand = 0;
+        uint32_t un = 0, wn = 0, bn = 0, base = 0;  // un: units of this warpgroup
+        bool hand = false;
         bool ok = works;
         auto meet = [&](uint64_t *bar, uint32_t &n) {  // the warps of a warpgroup, or of both
             __syncwarp();
@@ -698,53 +726,101 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                 const int at = (int)((long long)seg.qt * R + r), tok = at / a.group;
                 const int seen = exists ? seg.seq.seen(a, tok) : seg.seq.len;
                 const int first_seen = seg.seq.seen(a, (int)((long long)seg.qt * R + r - row) / a.group);  // the tile's first row
-                const uint32_t otm = tmem + lanes + L::O_COL + (NT == 2 ? wg * DP : 0);
+                const uint32_t otm = tmem + lanes + (wg ? L::o_col(1) : L::o_col(0)), stm = tmem + lanes + wg * BK;
+                const uint32_t ptm = tmem + lanes + (wg ? L::p_col(1) : L::p_col(0));
                 counted = false;
                 float m = LOWEST, l = 0.f;
                 bool fresh = true;
+                // The weights (in TMEM) times the values of ring fill f, for the keys under `lim` alone.
+                auto add_by_hand = [&](bool first, uint32_t f, int lim) {
+#pragma unroll 1
+                    for (int k = 0; k < D; k += 16) {
+                        uint32_t o[16], w8[8];
+                        if (first) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = 0;
+                        } else {
+                            tc05::ld16(otm + k, o);
+                            tc05::wait_ld_regs(o);
+                        }
+#pragma unroll 1
+                        for (int key = 0; key < BK; key += 16) {
+                            tc05::ld8(ptm + key / 2, w8);
+                            tc05::wait_ld_regs(w8);
+                            const uint8_t *slot = ring + (f + key / SLOT) % STAGES * L::SLOT_BYTES + (k >> 6) * (SLOT * 128);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float2 w2 = unpack(w8[i / 2], T());
+                                const float wt = i & 1 ? w2.y : w2.x;
+                                const int kr = (key + i) % SLOT;
+#pragma unroll
+                                for (int q = 0; q < 2 && key + i < lim; ++q) {
+                                    const uint4 u = *(const uint4 *)(slot + kr * 128 + (((((k & 63) >> 3) + q) ^ (kr & 7)) << 4));
+                                    const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        const float2 y = unpack(uu[e], T());
+                                        o[q * 8 + e * 2] = __float_as_uint(fmaf(wt, y.x, __uint_as_float(o[q * 8 + e * 2])));
+                                        o[q * 8 + e * 2 + 1] = __float_as_uint(fmaf(wt, y.y, __uint_as_float(o[q * 8 + e * 2 + 1])));
+                                    }
+                                }
+                            }
+                            __syncwarp();
+                        }
+                        tc05::st16(otm + k, o);
+                    }
+                    tc05::wait_st();
+                };
                 for (int j = alt ? wg : 0; j < n; j += alt ? 2 : 1) {
-                    const int s = NT == 2 ? wg : j & 1;
-                    const uint32_t stm = tmem + lanes + s * BK;
-                    ok = __all_sync(~0u, wait_or_stop(&sfull[s], sn[s]++ & 1, stop));
+                    ok = __all_sync(~0u, wait_or_stop(&sfull[wg], un & 1, stop));
                     if (!ok) break;
                     tc05::fence_after();
-                    if (hand >> s & 1) {  // the product's thread has read it
-                        if (row == 0) by_hand[s] = 0;
-                        hand &= ~(1u << s);
-                        ok = meet(&wgbar[wg], wn);
-                        if (!ok) break;
-                    }
-                    uint32_t x[4][32];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tc05::ld32(stm + i * 32, x[i]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tc05::wait_ld_regs(x[i]);
+                    // The sums of the unit before, and its weights, are the tensor core's until this.
+                    auto before_done = [&]() {
+                        if (!APART || !un) return true;  // (else scores come after it)
+                        const bool r = __all_sync(~0u, wait_or_stop(&odone[wg], (un - 1) & 1, stop));
+                        tc05::fence_after();
+                        return r;
+                    };
                     const int k0 = (seg.t0 + j) * BK, lim = seen - k0;
-                    if (__any_sync(~0u, lim < BK)) {
+                    // The scores are read twice, 32 at a time: in registers all 128 would have the loops unrolled, and
+                    // those outgrow the instruction cache (a step of heads of 128 took 2.5 to 3.3 thousand clocks so).
+                    const bool masked = __any_sync(~0u, lim < BK);
+                    float top = -CUDART_INF_F;
+                    if (!masked) {
+                        uint32_t x[4][32];
+                        float t[4];
 #pragma unroll
-                        for (int i = 0; i < 128; ++i)
-                            if (i >= lim) x[i / 32][i % 32] = __float_as_uint(-CUDART_INF_F);
+                        for (int g = 0; g < 4; ++g) tc05::ld32(stm + g * 32, x[g]);
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) tc05::wait_ld_regs(x[g]);
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) t[g] = fmaxf(__uint_as_float(x[g][0]), __uint_as_float(x[g][1]));
+#pragma unroll
+                        for (int i = 2; i < 32; i += 2)
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) t[g] = fmaxf(fmaxf(t[g], __uint_as_float(x[g][i])), __uint_as_float(x[g][i + 1]));
+                        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                    } else {
+#pragma unroll 1
+                        for (int g = 0; g < 4; ++g) {
+                            uint32_t x[32];
+                            __syncwarp();
+                            tc05::ld32(stm + g * 32, x);
+                            tc05::wait_ld_regs(x);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (g * 32 + i < lim) top = fmaxf(top, __uint_as_float(x[i]));
+                        }
                     }
-                    float t[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        t[i] = __uint_as_float(x[i][0]);
-#pragma unroll
-                        for (int k = 1; k < 31; k += 2) t[i] = fmaxf(t[i], fmaxf(__uint_as_float(x[i][k]), __uint_as_float(x[i][k + 1])));
-                        t[i] = fmaxf(t[i], __uint_as_float(x[i][31]));
-                    }
-                    const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c;
+                    top *= c;
                     if (__any_sync(~0u, top > m + (TOP<T> + SOFT))) {
                         const float to = fmaxf(top - TOP<T>, m), f = exp2_(m - to);
                         m = to;
                         l *= f;
-                        if (!fresh) {  // nothing else writes the sums before this step's weights are there
-                            // ... but with one row tile the product before may still be under way
-                            if (NT == 1) {
-                                ok = __all_sync(~0u, wait_or_stop(odone, (steps_done - 1) & 1, stop));
-                                if (!ok) break;
-                                tc05::fence_after();
-                            }
+                        if (!fresh) {
+                            ok = before_done();
+                            if (!ok) break;
 #pragma unroll 1
                             for (int k = 0; k < D; k += 16) {
                                 uint32_t o[16];
@@ -757,31 +833,22 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                             }
                         }
                     }
-                    const uint64_t c2 = two(c, c), m2 = two(-m, -m);
-                    uint64_t sum2 = 0;
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        float lo, hi;
-                        split2(fma2(two(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), c2, m2), lo, hi);
-                        const uint32_t p = pack(exp2_(lo), exp2_(hi), T());
-                        const float2 v = unpack(p, T());
-                        sum2 = add2(sum2, two(v.x, v.y));
-                        x[i / 32][i % 32] = p;
+                    if (hand) {  // the products' thread has read it
+                        ok = before_done();
+                        if (!ok) break;
+                        if (row == 0) by_hand[wg] = 0;
+                        hand = false;
+                        ok = meet(&wgbar[wg], wn);
+                        if (!ok) break;
                     }
-                    float lo, hi;
-                    split2(sum2, lo, hi);
-                    l += lo + hi;
-                    __syncwarp();
-                    tc05::st32(stm, x[0]);
-                    tc05::st32(stm + 32, x[1]);
-                    tc05::wait_st();
-                    // Values that some row of the tile does not see: any that are no numbers?
+                    uint32_t vf = 0;
                     if (first_seen < seg.seq.len && first_seen < k0 + BK) {
-                        const uint32_t f = base + v_fill(j, n, alt);
+                        // Values that some row of the tile does not see: any that are no numbers?
+                        vf = base + v_fill(j, n, lead_of(alt));
                         uint32_t top2 = 0;
 #pragma unroll
                         for (int p = 0; p < PARTS; ++p) {
-                            const uint32_t fp = f + p;
+                            const uint32_t fp = vf + p;
                             ok = ok && __all_sync(~0u, wait_or_stop(&full[fp % STAGES], (fp / STAGES) & 1, stop));
                             const uint4 *v = (const uint4 *)(ring + fp % STAGES * L::SLOT_BYTES);
                             for (int i = row; i < SLOT * L::CH; i += 128) {
@@ -792,67 +859,106 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                         }
                         if (!ok) break;
                         const bool bad = __vmaxu2(top2, infinite(T()) - 0x00010001u) != infinite(T()) - 0x00010001u;
-                        if (__any_sync(~0u, bad) && lane == 0) by_hand[s] = 1;
+                        if (__any_sync(~0u, bad) && lane == 0) by_hand[wg] = 1;
                         ok = meet(&wgbar[wg], wn);
                         if (!ok) break;
-                        if (by_hand[s]) {
-                            hand |= 1u << s;
-                            if (NT == 1 && !fresh) {
-                                ok = __all_sync(~0u, wait_or_stop(odone, (steps_done - 1) & 1, stop));
-                                if (!ok) break;
-                                tc05::fence_after();
-                            }
+                        hand = by_hand[wg];
+                    }
+                    ok = before_done();
+                    if (!ok) break;
+                    const uint64_t c2 = two(c, c), m2 = two(-m, -m);
+                    uint64_t sum2 = 0;
+                    auto put = [&](int g, uint32_t (&w)[16]) {  // weights of keys 32 g to 32 g + 31 (over scores that have been read)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 v = unpack(w[i], T());
+                            sum2 = add2(sum2, two(v.x, v.y));
+                        }
+                        tc05::st16(ptm + g * 16, w);
+                    };
+                    auto read = [&]() {  // the scores are
+                        if (APART) {
+                            tc05::fence_before();
+                            __syncwarp();
+                            if (lane == 0) arrive(&sfree[wg]);
+                        }
+                    };
+                    auto half_made = [&](int h) {  // a half of the weights goes to the product while the other is made
+                        tc05::wait_st();
+                        if (hand) return;
+                        tc05::fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive(&pready[2 * wg + h]);
+                        __syncwarp();
+                    };
+                    if (!masked) {
+                        uint32_t x[2][32];
+                        tc05::ld32(stm, x[0]);
 #pragma unroll 1
-                            for (int k = 0; k < D; k += 16) {
-                                uint32_t o[16], w8[8];
-                                if (fresh) {
+                        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                                    for (int i = 0; i < 16; ++i) o[i] = 0;
-                                } else {
-                                    tc05::ld16(otm + k, o);
-                                    tc05::wait_ld_regs(o);
-                                }
-#pragma unroll 1
-                                for (int key = 0; key < BK; key += 16) {
-                                    tc05::ld8(stm + key / 2, w8);
-                                    tc05::wait_ld_regs(w8);
-                                    const uint32_t fp = f + key / SLOT;
+                            for (int e = 0; e < 2; ++e) {
+                                tc05::wait_ld_regs(x[e]);
+                                if (e == 0) tc05::ld32(stm + h * 64 + 32, x[1]);
+                                else if (h == 0) tc05::ld32(stm + 64, x[0]);
+                                else read();
+                                uint32_t w[16];
 #pragma unroll
-                                    for (int i = 0; i < 16; ++i) {
-                                        const float2 w2 = unpack(w8[i / 2], T());
-                                        const float wt = i & 1 ? w2.y : w2.x;
-                                        const int kr = (key + i) % SLOT;
-                                        const uint8_t *vr = ring + fp % STAGES * L::SLOT_BYTES + (k >> 6) * (SLOT * 128) + kr * 128;
-#pragma unroll
-                                        for (int q = 0; q < 2 && key + i < lim; ++q) {
-                                            const uint4 u = *(const uint4 *)(vr + (((((k & 63) >> 3) + q) ^ (kr & 7)) << 4));
-                                            const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                                            for (int e = 0; e < 4; ++e) {
-                                                const float2 y = unpack(uu[e], T());
-                                                o[q * 8 + e * 2] = __float_as_uint(fmaf(wt, y.x, __uint_as_float(o[q * 8 + e * 2])));
-                                                o[q * 8 + e * 2 + 1] = __float_as_uint(fmaf(wt, y.y, __uint_as_float(o[q * 8 + e * 2 + 1])));
-                                            }
-                                        }
+                                for (int i = 0; i < 16; ++i) {
+                                    const uint64_t y = fma2(two(__uint_as_float(x[e][2 * i]), __uint_as_float(x[e][2 * i + 1])), c2, m2);
+                                    float lo, hi;
+                                    if (i % EMULATED == EMULATED - 1) {
+                                        exp2_pair(y, lo, hi);
+                                    } else {
+                                        split2(y, lo, hi);
+                                        lo = exp2_(lo), hi = exp2_(hi);
                                     }
-                                    __syncwarp();
+                                    w[i] = pack(lo, hi, T());
                                 }
-                                tc05::st16(otm + k, o);
+                                put(h * 2 + e, w);
                             }
-                            tc05::wait_st();
+                            half_made(h);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int g = 0; g < 4; ++g) {
+                            uint32_t x[32], w[16];
+                            __syncwarp();
+                            tc05::ld32(stm + g * 32, x);
+                            tc05::wait_ld_regs(x);
+                            if (g == 3) read();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float e = exp2_(fmaf(__uint_as_float(x[i]), c, -m));
+                                x[i] = __float_as_uint(g * 32 + i < lim ? e : 0.f);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) w[i] = pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]), T());
+                            __syncwarp();
+                            put(g, w);
+                            if (g & 1) half_made(g >> 1);
+                        }
+                    }
+                    float lo, hi;
+                    split2(sum2, lo, hi);
+                    l += lo + hi;
+                    if (hand) {
+                        add_by_hand(fresh, vf, lim);
+                        tc05::fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            arrive(&pready[2 * wg]);
+                            arrive(&pready[2 * wg + 1]);
                         }
                     }
                     fresh = false;
-                    ++steps_done;
-                    tc05::fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive(&pready[s]);
+                    ++un;
                 }
                 if (!ok) break;
                 // the sums
                 const bool some = alt ? n > wg : true;
                 if (some) {
-                    ok = __all_sync(~0u, wait_or_stop(&ofull[NT == 2 ? wg : 0], on++ & 1, stop));
+                    ok = __all_sync(~0u, wait_or_stop(&odone[wg], (un - 1) & 1, stop));
                     if (!ok) break;
                     tc05::fence_after();
                 }
@@ -875,7 +981,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                 auto columns = [&](int col, float (&v)[16]) {
                     uint32_t o[16];
                     __syncwarp();  // rows that do not exist store nothing: the warp's lanes meet again
-                    const uint32_t mine = otm + col, its = tmem + lanes + L::O_COL + (wg ^ 1) * DP + col;
+                    const uint32_t mine = otm + col, its = tmem + lanes + (wg ? L::o_col(0) : L::o_col(1)) + col;
                     tc05::ld16(other_alone ? its : mine, o);
                     tc05::wait_ld_regs(o);
                     const float w = other_alone ? f[1] : f[0];
@@ -898,7 +1004,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                 }
                 const int c_first = (int)(item_first / share), c_last = (int)((item_first + seg.steps - 1) / share);
                 if (c_first == c_last) {
-                    const float inv = seen > 0 ? 1.f / l : 0.f;
+                    const float inv = row_factor(seen, m, l);
 #pragma unroll 1
                     for (int col = col0; col < col1; col += 16) {
                         float v[16];
@@ -907,7 +1013,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                         for (int i = 0; i < 16; ++i) v[i] = seen > 0 ? v[i] * inv : 0.f;
                         if (exists) store_row16(out + col, a.o_vec, v);
                     }
-                    if (exists && lse && col0 == 0) *lse = seen > 0 ? (m + log2f(l)) * 0.69314718055994531f : -CUDART_INF_F;
+                    if (exists && lse && col0 == 0) *lse = row_lse(seen, m, l);
                 } else {
                     // A share leaves its second slot to the item that starts in it, its first to one that started before.
                     auto slot = [&](int k) { return 2ll * k + (k == c_first); };
@@ -947,13 +1053,13 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                                 const float2 v = __ldcg(pst + slot(c_first + k) * R + strow);
                                 S += exp2_(v.x - M) * v.y;
                             }
-                            const float inv = seen > 0 ? 1.f / S : 0.f;
+                            const float inv = row_factor(seen, M, S);
                             for (int k = 0; k < k_parts; ++k) {
                                 float2 *p = pst + slot(c_first + k) * R + strow;
                                 __stcg(&p->x, seen > 0 ? exp2_(__ldcg(&p->x) - M) : 0.f);
                                 __stcg(&p->y, inv);
                             }
-                            if (lse && col0 == 0) *lse = seen > 0 ? (M + log2f(S)) * 0.69314718055994531f : -CUDART_INF_F;
+                            if (lse && col0 == 0) *lse = row_lse(seen, M, S);
                         }
                         __threadfence_block();
                         ok = meet(&wgbar[wg], wn);

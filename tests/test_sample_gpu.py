@@ -250,3 +250,25 @@ def test_sample_refusals():
     bad(TypeError, "int64", z, u, out=torch.zeros(4, dtype=torch.int32, device="cuda"))
     bad(ValueError, "one entry", z, u, out=torch.zeros(5, dtype=torch.int64, device="cuda"))
     bad(ValueError, "contiguous", z, u, out=torch.zeros(1, dtype=torch.int64, device="cuda").expand(4))
+
+
+@pytest.mark.parametrize("dtype", [BF, FF])
+def test_sample_cut_around_zero(dtype):
+    """Logits of both zeros and of the smallest numbers about them, where the search's intervals end."""
+    tiny = 2.0 ** -133 if dtype == BF else 2.0 ** -149
+    z = torch.zeros(4, 20000, device="cuda", dtype=dtype)
+    z[:, ::3] = -0.0
+    z[:, 1::7] = tiny
+    z[:, 2::11] = -tiny
+    z[:, 5::13] = -1.0
+    z[:, 3] = 0.5
+    for kw in (dict(top_p=0.3), dict(top_p=0.8), dict(top_k=2000), dict(top_k=6000), dict(top_k=15000), dict(top_k=19990, top_p=0.9)):
+        check(z, uniform(29, 4), **kw)
+
+
+@pytest.mark.parametrize("dtype,vocab", [(FF, 500009), (BF, 1000003)])
+def test_sample_rows_past_shared_memory(dtype, vocab):
+    """Rows that a cluster's shared memory does not hold."""
+    z = rand(30, 2, vocab, dtype=dtype, scale=2.0)
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=3000, top_p=0.7), dict(temperature=0.0), dict(min_p=0.1)):
+        check(z, uniform(31, 2), **kw)
