@@ -30,6 +30,7 @@
 // The second product multiplies masked values by zero, which a NaN or an infinity survives.  Slots past a
 // sequence's end are zeros in shared memory; where a row does not see a token that others see, the warpgroup looks
 // through the value tile, and one that holds such a number is added by its threads, each taking what its row sees.
+#include <cudaTypedefs.h>
 #include <math_constants.h>
 
 #include <cfloat>
@@ -67,10 +68,17 @@ struct ChunkArgs {
     int tokens, seqs, heads, kv_heads, group, num_pages, page, page_shift, max_pages, causal, q_vec, o_vec, negate;
     float scale_log2;   // not negative: `negate` has the sign
     uint32_t skip;      // see skipped_copy
-    float *parts;       // [grid][2][R][D], then [grid][2][R][2]
-    uint32_t *counts;   // [2][MAX_GRID], zero between calls
+    float *parts;       // [grid][2][D / 4][R][4], then [grid][2][4][128][2]
+    uint32_t *counts;   // [4][MAX_GRID], zero between calls
+    int box;            // rows of a TMA box of the cache; 0: none
+    int q_box;          // q by TMA
     int *err;
 };
+
+// a / b, of numbers that nearly always fit in 32 bits.
+__device__ __forceinline__ long long ratio(long long a, long long b) {
+    return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 
 template <int D>
 struct Lay {
@@ -79,20 +87,24 @@ struct Lay {
     static constexpr int SLOT = DP <= 128 ? 128 : 64, PARTS = BK / SLOT;  // keys of a ring slot
     static constexpr int SLOT_BYTES = SLOT * DP * 2, Q_TILE = 128 * DP * 2, Q_BYTES = NT * Q_TILE;
     static constexpr int STAGES = DP == 64 ? 8 : DP == 128 ? 5 : DP == 192 ? 7 : 5;
-    static constexpr int STAT = Q_BYTES + STAGES * SLOT_BYTES;  // [2][128] float2: maxima and sums of the other half
-    static constexpr int BARS = STAT + (NT == 2 ? 2048 : 0), MISC = BARS + 256, BYTES = MISC + 64;
-    static constexpr int SOFT_WARPS = 4 * NT, MMA_WARP = SOFT_WARPS + 4, WARPS = SOFT_WARPS + 8, THREADS = WARPS * 32;
+    static constexpr int STAT = Q_BYTES + STAGES * SLOT_BYTES;  // [4][128] float: what the softmax warpgroups tell one another
+    static constexpr int BARS = STAT + 2048, MISC = BARS + 336, BYTES = MISC + 128;
+    // A row tile has two softmax warpgroups, with 64 keys of a step each; then four copying warps, then the products'.
+    static constexpr int GROUPS = 2 * NT, SOFT_WARPS = 4 * GROUPS, MMA_WARP = SOFT_WARPS + 4, WARPS = SOFT_WARPS + 8, THREADS = WARPS * 32;
     // Registers of a thread at launch, and of the roles from then on (shares of what the block was launched with).
-    static constexpr int REGS = NT == 2 ? 128 : 168, COPY_REGS = 72, MMA_REGS = 56, SOFT_REGS = NT == 2 ? 192 : 240;
-    static_assert(128 * (COPY_REGS + MMA_REGS + NT * SOFT_REGS) <= REGS * THREADS, "registers");
+    static constexpr int REGS = NT == 2 ? 80 : 128, COPY_REGS = NT == 2 ? 56 : 72, MMA_REGS = NT == 2 ? 40 : 56;
+    static constexpr int SOFT_REGS = NT == 2 ? 96 : 192;
+    static_assert(128 * (COPY_REGS + MMA_REGS + GROUPS * SOFT_REGS) <= REGS * THREADS, "registers");
     // TMEM columns: scores, sums, weights.  APART: the weights have columns of their own, so that the next scores are
     // under way while they are made; with two row tiles of 128 dimensions they have to take the scores' place.
     static constexpr bool APART = NT == 1 || DP == 64;
     __host__ __device__ static constexpr int s_col(int w) { return w * BK; }
     __host__ __device__ static constexpr int o_col(int w) { return 256 + w * DP; }
-    __host__ __device__ static constexpr int p_col(int w) { return NT == 1 ? BK : APART ? 384 + w * 64 : w * BK; }
+    __host__ __device__ static constexpr int p_col(int w, int h) {  // of the first and the last 64 keys
+        return NT == 1 ? BK + h * 32 : APART ? 384 + w * 64 + h * 32 : w * BK + h * 64;
+    }
     static constexpr int PART = R * D, CH = D / 8;  // numbers of a part; 16-byte pieces of a row
-    static_assert(BYTES <= 227 * 1024, "shared memory");
+    static_assert(BYTES <= 227 * 1024 - 512, "shared memory");
     static_assert(o_col(NT) <= (APART && NT == 2 ? 384 : 512), "tensor memory");
 };
 
@@ -291,36 +303,32 @@ __device__ __forceinline__ float row_lse(int seen, float m, float l) {
     return seen <= 0 || m == LOWEST ? -CUDART_INF_F : l < CUDART_INF_F ? (m + log2f(l)) * 0.69314718055994531f : CUDART_NAN_F;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_row16(T *p, bool vec, const float (&v)[16]) {
-    alignas(16) T e[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) e[i] = from_f32<T>(v[i]);
-    if (vec) {
-        ((uint4 *)p)[0] = ((const uint4 *)e)[0];
-        ((uint4 *)p)[1] = ((const uint4 *)e)[1];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = e[i];
-    }
+__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_constant__ ChunkArgs a) {
+__global__ void __launch_bounds__(Lay<D>::THREADS, 1)
+    chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                 const __grid_constant__ CUtensorMap tmq) {
     using L = Lay<D>;
     constexpr int NT = L::NT, R = L::R, DP = L::DP, SLOT = L::SLOT, PARTS = L::PARTS, STAGES = L::STAGES;
     extern __shared__ __align__(1024) uint8_t smem[];  // (with no static shared memory ahead of it)
     uint8_t *ring = smem + L::Q_BYTES;
-    float2 *half_stat = (float2 *)(smem + L::STAT);
+    float *told = (float *)(smem + L::STAT);  // [softmax warpgroup][row]
     uint64_t *full = (uint64_t *)(smem + L::BARS), *empty = full + STAGES, *qfull = empty + STAGES, *qempty = qfull + 1;
-    uint64_t *sfull = qempty + 1, *sfree = sfull + 2, *pready = sfree + 2, *odone = pready + 4, *wgbar = odone + 2, *both = wgbar + 2;
-    uint64_t *drain = both + 1;
-    static_assert((2 * STAGES + 16) * 8 <= 256, "barriers");
-    long long *line = (long long *)(smem + L::MISC);  // total, share, steps ahead of the first step's sequence, that sequence
-    uint32_t *tslot = (uint32_t *)(line + 4);
+    uint64_t *sfull = qempty + 1, *sfree = sfull + 2, *pready = sfree + 2, *odone = pready + 2, *tbar = odone + 2, *gbar = tbar + 2;
+    uint64_t *both = gbar + 4, *drain = both + 1, *pair_bar = drain + 1;  // tbar: a row tile's warps, gbar: a warpgroup's
+    static_assert((2 * STAGES + 26) * 8 <= 336, "barriers");
+    long long *line = (long long *)(smem + L::MISC);  // the line's length, a share of it
+    uint32_t *tslot = (uint32_t *)(line + 2);
     volatile int *stop = (volatile int *)(tslot + 1);
     volatile int *by_hand = stop + 1;        // [2]: this step's values are added by the warpgroup
     volatile int *last_flag = by_hand + 2;   // [2]
+    Segment<R> *start = (Segment<R> *)(last_flag + 2);
+    static_assert(sizeof(Segment<R>) <= 128 - 40 && L::MISC % 8 == 0, "the first segment");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (warp == L::MMA_WARP) {
@@ -338,13 +346,14 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
         for (int i = 0; i < 2; ++i) {
             by_hand[i] = 0;
             tc05::mbar_init(&sfull[i], 1);
-            tc05::mbar_init(&sfree[i], 4);
-            tc05::mbar_init(&pready[2 * i], 4);  // weights of the first 64 keys, and of the others
-            tc05::mbar_init(&pready[2 * i + 1], 4);
+            tc05::mbar_init(&sfree[i], 8);
+            tc05::mbar_init(&pready[i], 8);
             tc05::mbar_init(&odone[i], 1);
-            tc05::mbar_init(&wgbar[i], 4);
+            tc05::mbar_init(&tbar[i], 8);
         }
-        tc05::mbar_init(both, 8);
+        for (int i = 0; i < 4; ++i) tc05::mbar_init(&gbar[i], 4);
+        for (int i = 0; i < 8; ++i) tc05::mbar_init(&pair_bar[i], 2);
+        tc05::mbar_init(both, 16);
         tc05::mbar_init(drain, 1);
         tc05::fence_mbar_init();
     }
@@ -362,15 +371,33 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
             if (!a.causal) {
                 sum = qts ? (long long)qts * s.steps(a, R, 0) : 0;
             } else {
-                for (int qt = 0; qt < min(qts, 16); ++qt) sum += s.steps(a, R, qt);
-                unsigned many = __ballot_sync(~0u, qts > 16);  // those of long chunks by the whole warp
+                // Row tiles of tp whole tokens, of which the i-th sees off + i tp: the sum of ceil((off + i tp) / 128), in
+                // closed form where one of tp and 128 is a multiple of the other.
+                const int tp = R / a.group, off = s.len - s.n;
+                const bool closed = tp * a.group == R && (tp & (tp - 1)) == 0 && off >= 0;
+                if (qts && closed) {
+                    const long long full = s.n / tp;
+                    if (tp >= BK) {
+                        sum = full * ((off + BK - 1) / BK) + full * (full + 1) / 2 * (tp / BK);
+                    } else {
+                        const int m = BK / tp;  // (off + 127 + i tp) / 128 = ((off + 127) / tp + i) / m
+                        auto down = [&](long long k) {  // 0 / m + 1 / m + ... + k / m, rounded down each
+                            const long long q = k / m;
+                            return m * (q * (q - 1) / 2) + q * (k - q * m + 1);
+                        };
+                        const long long x = (off + BK - 1) / tp;
+                        sum = down(x + full) - down(x);
+                    }
+                    if (full * tp < s.n) sum += s.steps(a, R, qts - 1);
+                }
+                unsigned many = __ballot_sync(~0u, qts && !closed);  // the others by the whole warp
                 while (many) {
                     const int l = __ffs(many) - 1;
                     many &= many - 1;
                     const Seq o{0, __shfl_sync(~0u, s.n, l), __shfl_sync(~0u, s.len, l)};
                     const int its = __shfl_sync(~0u, qts, l);
                     long long part = 0;
-                    for (int qt = 16 + lane; qt < its; qt += 32) part += o.steps(a, R, qt);
+                    for (int qt = lane; qt < its; qt += 32) part += o.steps(a, R, qt);
                     for (int x = 16; x; x /= 2) part += __shfl_xor_sync(~0u, part, x);
                     if (lane == l) sum += part;
                 }
@@ -385,10 +412,8 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
             total += sum;
         }
         total *= a.kv_heads;
-        long long share = (total + gridDim.x - 1) / gridDim.x;
-        if (share < MIN_SHARE) share = MIN_SHARE;
-        const long long first = share * blockIdx.x;
-        long long before = 0;
+        const long long share = max((long long)MIN_SHARE, ratio(total + gridDim.x - 1, gridDim.x)), first = share * blockIdx.x;
+        long long before = 0, per = 0;  // steps of the sequences ahead, and of the one that is found, for one key head
         int found = -1;
         for (int b0 = 0; b0 < a.seqs && found < 0 && first < total; b0 += 32) {
             const long long n = a.seqs <= 32 ? held : steps_of(b0 + lane, false);
@@ -402,16 +427,49 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                 const int l = __ffs(m) - 1;
                 found = b0 + l;
                 before += __shfl_sync(~0u, incl - n, l);
+                per = __shfl_sync(~0u, n, l);
             } else {
                 before += __shfl_sync(~0u, incl, 31);
             }
         }
-        if (lane == 0) {
-            line[0] = total;
-            line[1] = share;
-            line[2] = before * a.kv_heads;
-            line[3] = found;
+        if (found >= 0) {  // its first step: the key head, and the row tile within it
+            Segment<R> seg;
+            seg.b = found;
+            seg.seq.set(a, found, false);
+            seg.qts = seg.seq.row_tiles(a, R);
+            seg.left = min(share, total - first);
+            long long in = first - before * a.kv_heads;
+            seg.h = (int)ratio(in, per);
+            in -= seg.h * per;
+            seg.qt = 0;
+            if (!a.causal) {
+                const int n = seg.seq.steps(a, R, 0);
+                seg.qt = (int)ratio(in, n);
+                in -= (long long)seg.qt * n;
+            } else {
+                for (; seg.qt < seg.qts; seg.qt += 32) {  // 32 row tiles at a time
+                    const int qt = seg.qt + lane, n = qt < seg.qts ? seg.seq.steps(a, R, qt) : 0;
+                    long long incl = n;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const long long v = __shfl_up_sync(~0u, incl, o);
+                        if (lane >= o) incl += v;
+                    }
+                    const unsigned m = __ballot_sync(~0u, incl > in);
+                    if (m) {
+                        const int l = __ffs(m) - 1;
+                        in -= __shfl_sync(~0u, incl - n, l);
+                        seg.qt += l;
+                        break;
+                    }
+                    in -= __shfl_sync(~0u, incl, 31);
+                }
+            }
+            seg.steps = seg.seq.steps(a, R, seg.qt);
+            seg.t0 = (int)in;
+            seg.clip();
+            if (lane == 0) *start = seg;
         }
+        if (lane == 0) line[0] = total, line[1] = share;
     }
     __syncwarp();
     tc05::fence_before();
@@ -420,51 +478,8 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
     const uint32_t tmem = *tslot;
     const long long total = line[0], share = line[1], first = share * blockIdx.x;
     const bool works = first < total && !*stop;
-
     Segment<R> seg;
-    if (works) {
-        seg.b = (int)line[3];
-        seg.seq.set(a, seg.b, false);
-        seg.qts = seg.seq.row_tiles(a, R);
-        seg.left = min(share, total - first);
-        long long in = first - line[2];
-        // the key head, and the row tile within it
-        long long per = 0;
-        if (a.causal) {
-            for (int qt = lane; qt < seg.qts; qt += 32) per += seg.seq.steps(a, R, qt);
-            for (int x = 16; x; x /= 2) per += __shfl_xor_sync(~0u, per, x);
-        } else {
-            per = (long long)seg.qts * seg.seq.steps(a, R, 0);
-        }
-        seg.h = (int)(in / per);
-        in -= seg.h * per;
-        seg.qt = 0;
-        if (!a.causal) {
-            const int s = seg.seq.steps(a, R, 0);
-            seg.qt = (int)(in / s);
-            in -= (long long)seg.qt * s;
-        } else {
-            for (; seg.qt < seg.qts; seg.qt += 32) {  // 32 row tiles at a time
-                const int qt = seg.qt + lane, s = qt < seg.qts ? seg.seq.steps(a, R, qt) : 0;
-                long long incl = s;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long v = __shfl_up_sync(~0u, incl, o);
-                    if (lane >= o) incl += v;
-                }
-                const unsigned m = __ballot_sync(~0u, incl > in);
-                if (m) {
-                    const int l = __ffs(m) - 1;
-                    in -= __shfl_sync(~0u, incl - s, l);
-                    seg.qt += l;
-                    break;
-                }
-                in -= __shfl_sync(~0u, incl, 31);
-            }
-        }
-        seg.steps = seg.seq.steps(a, R, seg.qt);
-        seg.t0 = (int)in;
-        seg.clip();
-    }
+    if (works) seg = *start;
     __syncwarp();
     // Which ring fill, from the segment's first, holds the keys (values) of its step j of n.  The keys of the first `lead`
     // steps come first, then those of step j + lead and the values of step j, in the order of their use: keys ahead
@@ -474,10 +489,10 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
     auto k_fill = [](int j, int lead) { return (j < lead ? j : 2 * j - lead + !APART) * PARTS; };
     auto v_fill = [](int j, int n, int lead) { return (j + lead < n + !APART ? lead + 2 * j + APART : n + j) * PARTS; };
 
-    if (warp >= L::SOFT_WARPS && warp < L::SOFT_WARPS + 4) {
+    if (warp >= L::SOFT_WARPS && warp < L::MMA_WARP) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::COPY_REGS));
         const int w = warp - L::SOFT_WARPS;
-        uint32_t fills = 0, qn = 0, waiting = 0;  // slots filled, items, copies not yet reported
+        uint32_t fills = 0, qn = 0, waiting = 0;  // slots filled, items, copies by cp.async not yet reported
         uint64_t *pend[LAG + 1];
         bool ok = works;
         auto report = [&](uint64_t *bar) {
@@ -486,6 +501,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
             if (lane == 0) arrive(bar);
         };
         auto flush = [&]() {
+            if (!waiting) return;
             asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 #pragma unroll
             for (int i = 0; i <= LAG; ++i)
@@ -511,42 +527,133 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
             flush();
             return (bool)__all_sync(~0u, wait_or_stop(bar, parity, stop));
         };
-        constexpr int RW = SLOT / 4, N = RW * L::CH / 32;  // rows of a warp in a slot, accesses of a lane
-        // Keys or values of this lane's row (lane < RW) into the slot.
-        auto copy = [&](const T *base, long long off) {
-            const uint32_t s = fills % STAGES, dst = tc05::smem_u32(ring + s * L::SLOT_BYTES) + w * RW * 128;
-            if (fills >= STAGES && !room(&empty[s], (fills / STAGES - 1) & 1)) return false;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int c = i * 32 + lane, row = c / L::CH, col = c % L::CH;
-                const long long o = __shfl_sync(~0u, off, row);
-                cp16(dst + (col >> 3) * (SLOT * 128) + row * 128 + (((col ^ row) & 7) << 4), base + (o < 0 ? 0 : o + col * 8),
-                     o < 0 ? 0 : 16);
-            }
-            if (fills++ == a.skip) asm volatile("cp.async.commit_group;\n" ::: "memory");
-            else issued(&full[s]);
-            return true;
+        auto expect = [&](uint64_t *bar, uint32_t bytes, bool arrives) {
+            if (arrives)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(tc05::smem_u32(bar)), "r"(bytes) : "memory");
+            else
+                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(tc05::smem_u32(bar)), "r"(bytes) : "memory");
         };
+        constexpr int RW = SLOT / 4, N = RW * L::CH / 32;  // rows of a warp in a slot, accesses of a lane
+        constexpr int NB = DP / 64;                         // blocks of 64 dimensions
+        const int nb = a.box ? RW / a.box : 0;              // boxes of a warp's rows
+        const int my_box = lane / NB, box_shift = __ffs(a.box) - 1;
         const T *kc = (const T *)a.kc, *vc = (const T *)a.vc;
         if (ok) do {
-                const int n = seg.t1 - seg.t0, rows = seg.rows(a);
+                const int n = seg.t1 - seg.t0, rows = seg.rows(a), head = seg.h;
                 const bool alt = NT == 2 && rows <= 128;
+                const int lead = lead_of(alt);
+                const long long table = seg.b * a.pages_stride;
+                auto page_at = [&](int t) { return a.pages[table + (a.page_shift >= 0 ? t >> a.page_shift : t / a.page)]; };
+                // Pages.  With boxes a lane holds one of a window of `steps` steps' boxes, so that loads are far ahead; else
+                // that of its own row in the step whose values come next and two further ones.
+                const int per_step = a.box ? PARTS * nb : 32, steps = 32 / per_step, step_shift = __ffs(steps) - 1;
+                auto window = [&](int g) {
+                    const int j = g * steps + lane / per_step, e = lane % per_step;
+                    const int p = e / (a.box ? nb : 1), box = e - p * nb;
+                    const int t = (seg.t0 + min(j, n - 1)) * BK + p * SLOT + w * RW + (box << box_shift);
+                    return j < n && t < seg.seq.len ? page_at(t) : INT32_MIN;
+                };
+                struct Pages {
+                    int of[PARTS];
+                };
+                auto own_pages = [&](int j) {
+                    Pages r;
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        const int t = (seg.t0 + min(j, n - 1)) * BK + p * SLOT + w * RW + lane;
+                        r.of[p] = lane < RW && j < n && t < seg.seq.len ? page_at(t) : INT32_MIN;
+                    }
+                    return r;
+                };
+                int now = 0, next = 0, at_window = 0;
+                Pages p0 = {}, p1 = {}, p2 = {};
+                if (a.box) now = window(0), next = window(1);
+                else p0 = own_pages(0), p1 = own_pages(1), p2 = own_pages(2);
+                // Keys or values of step j: by TMA the boxes that are live as a whole, row by row with cp.async what is not.
+                auto fill = [&](int j, const Pages &own, bool keys) {
+                    for (int p = 0; p < PARTS; ++p) {
+                        const uint32_t s = fills % STAGES, dst = tc05::smem_u32(ring + s * L::SLOT_BYTES) + w * RW * 128;
+                        const int t0 = (seg.t0 + j) * BK + p * SLOT + w * RW;
+                        const int t = t0 + (a.box ? my_box << box_shift : lane);  // of this lane's box, or row
+                        int page = PARTS == 1 || p == 0 ? own.of[0] : own.of[PARTS - 1];
+                        if (a.box) {
+                            const int from = (j & (steps - 1)) * per_step + p * nb + min(my_box, nb - 1);
+                            page = __shfl_sync(~0u, j >> step_shift == at_window ? now : next, from);
+                        }
+                        bool good = (a.box ? my_box < nb : lane < RW) && t < seg.seq.len;
+                        if (good && (page < 0 || page >= a.num_pages)) {
+                            atomicOr(a.err, HV_DECODE_BAD_PAGE);
+                            good = false;
+                        }
+                        const int slot = a.page_shift >= 0 ? t & (a.page - 1) : t % a.page;
+                        const unsigned boxes = __ballot_sync(~0u, a.box && good && t + a.box <= seg.seq.len);
+                        const bool all = a.box && __popc(boxes) == nb * NB;
+                        if (fills >= STAGES && !room(&empty[s], (fills / STAGES - 1) & 1)) return false;
+                        if (fills++ == a.skip) continue;
+                        if (boxes) {
+                            if (lane == 0) expect(&full[s], __popc(boxes) * a.box * 128, all);
+                            __syncwarp();
+                            if (boxes >> lane & 1)
+                                asm volatile(
+                                    "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+                                    "[%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst + lane % NB * (SLOT * 128) + (my_box << box_shift) * 128),
+                                    "l"(reinterpret_cast<uint64_t>(keys ? &tmk : &tmv)), "r"(lane % NB * 64), "r"(slot), "r"(head),
+                                    "r"(page), "r"(tc05::smem_u32(&full[s]))
+                                    : "memory");
+                            __syncwarp();
+                        }
+                        if (all) continue;
+                        const int of = a.box ? (lane >> box_shift) * NB & 31 : lane;  // the lane that knows row `lane`
+                        const int its = __shfl_sync(~0u, good ? page : -1, of), its_slot = __shfl_sync(~0u, slot, of);
+                        const int at = a.box ? its_slot + (lane & (a.box - 1)) : its_slot;
+                        long long off = -1;
+                        if (lane < RW && its >= 0 && t0 + lane < seg.seq.len)
+                            off = keys ? its * a.kc_page + at * a.kc_slot + head * a.kc_head : its * a.vc_page + at * a.vc_slot + head * a.vc_head;
+#pragma unroll 4
+                        for (int i = 0; i < N; ++i) {
+                            const int c = i * 32 + lane, row = c / L::CH, col = c % L::CH;
+                            const long long o = __shfl_sync(~0u, off, row);
+                            if (a.box && boxes >> ((row >> box_shift) * NB) & 1) continue;
+                            cp16(dst + (col >> 3) * (SLOT * 128) + row * 128 + (((col ^ row) & 7) << 4), (keys ? kc : vc) + (o < 0 ? 0 : o + col * 8),
+                                 o < 0 ? 0 : 16);
+                        }
+                        issued(&full[s]);
+                    }
+                    return true;
+                };
+                ok = fill(0, p0, true) && (!alt || n == 1 || fill(1, p1, true));
+                if (!ok) break;
                 // rows of q
                 if (qn && !room(qempty, (qn - 1) & 1)) { ok = false; break; }
-                {
+                const int tiles = NT == 2 && !alt ? 2 : 1;
+                if (a.q_box) {  // [tokens][group][64] boxes; what is past the sequence is in no row that is written
+                    if (w == 0) {
+                        if (lane == 0) expect(qfull, tiles * L::Q_TILE, true);
+                        __syncwarp();
+                        if (lane < tiles * NB)
+                            asm volatile(
+                                "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+                                "[%5];\n" ::"r"(tc05::smem_u32(smem) + lane / NB * L::Q_TILE + lane % NB * (128 * 128)),
+                                "l"(reinterpret_cast<uint64_t>(&tmq)), "r"(lane % NB * 64), "r"(head * a.group),
+                                "r"(seg.seq.s0 + seg.qt * (R / a.group) + lane / NB * (128 / a.group)), "r"(tc05::smem_u32(qfull))
+                                : "memory");
+                        __syncwarp();
+                    } else if (lane == 0) {
+                        arrive(qfull);
+                    }
+                } else {
                     const T *q = (const T *)a.q + (long long)seg.seq.s0 * a.q_tok;
-                    const int h0 = seg.h * a.group;
                     const long long r0 = (long long)seg.qt * R;
-                    const int held = alt ? 128 : R;
-                    for (int g = w * 32; g < held; g += 128) {
+#pragma unroll 1
+                    for (int g = w * 32; g < tiles * 128; g += 128) {
                         const int r = g + lane;
                         long long off = -1;
                         if (r < rows) {
                             const int at = (int)(r0 + r), tok = at / a.group;
-                            off = tok * a.q_tok + (h0 + at - tok * a.group) * a.q_head;
+                            off = tok * a.q_tok + (head * a.group + at - tok * a.group) * a.q_head;
                         }
                         const uint32_t dst = tc05::smem_u32(smem) + (g >> 7) * L::Q_TILE + (g & 127) * 128;
-#pragma unroll 4
+#pragma unroll 2
                         for (int i = 0; i < L::CH; ++i) {
                             const int c = i * 32 + lane, row = c / L::CH, col = c % L::CH;
                             const long long o = __shfl_sync(~0u, off, row);
@@ -564,55 +671,34 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                         }
                     }
                     issued(qfull);
-                    ++qn;
                 }
-                // Pages of this lane's rows of four steps: the one whose values come next, two whose keys do, and one
-                // on its way.  -1 past the end.
-                struct Pages {
-                    int of[PARTS];
-                };
-                const int head = seg.h;
-                const long long table = seg.b * a.pages_stride;
-                auto pages_of = [&](int j) {
-                    Pages r;
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        const int t = (seg.t0 + min(j, n - 1)) * BK + p * SLOT + w * RW + lane;
-                        r.of[p] = lane < RW && j < n && t < seg.seq.len
-                                      ? a.pages[table + (a.page_shift >= 0 ? t >> a.page_shift : t / a.page)] : INT32_MIN;
-                    }
-                    return r;
-                };
-                auto fill = [&](int j, const Pages &pg, bool keys) {
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        const int t = (seg.t0 + j) * BK + p * SLOT + w * RW + lane;
-                        const bool live = lane < RW && t < seg.seq.len;
-                        bool good = live;
-                        if (live && (pg.of[p] < 0 || pg.of[p] >= a.num_pages)) {
-                            atomicOr(a.err, HV_DECODE_BAD_PAGE);
-                            good = false;
-                        }
-                        const int slot = a.page_shift >= 0 ? t & (a.page - 1) : t % a.page;
-                        const long long off = !good ? -1
-                                              : keys ? pg.of[p] * a.kc_page + slot * a.kc_slot + head * a.kc_head
-                                                     : pg.of[p] * a.vc_page + slot * a.vc_slot + head * a.vc_head;
-                        if (!copy(keys ? kc : vc, off)) return false;
-                    }
-                    return true;
-                };
-                Pages p0 = pages_of(0), p1 = pages_of(1), p2 = pages_of(2), p3;
-                ok = fill(0, p0, true) && (!alt || n == 1 || fill(1, p1, true));
+                ++qn;
                 for (int j = 0; j < n && ok; ++j) {
-                    p3 = pages_of(j + 3);
+                    Pages p3 = {};
+                    if (!a.box) {
+                        p3 = own_pages(j + 3);
+                    } else if (j >> step_shift != at_window) {
+                        at_window = j >> step_shift;
+                        now = next;
+                        next = window(at_window + 1);
+                    }
                     if (!APART) ok = fill(j, p0, false);
-                    if (ok) ok = alt ? j + 2 >= n || fill(j + 2, p2, true) : j + 1 >= n || fill(j + 1, p1, true);
+                    if (ok && j + lead < n) ok = fill(j + lead, alt ? p2 : p1, true);
                     if (APART && ok) ok = fill(j, p0, false);
                     p0 = p1, p1 = p2, p2 = p3;
                 }
             } while (ok && seg.next(a));
         flush();
-    } else if (warp >= L::MMA_WARP) {  // one thread of its warpgroup
+        if (a.box)  // what was issued has landed before shared memory goes, whichever role gives up
+            for (uint32_t k = fills > STAGES ? fills - STAGES : 0; k < fills; ++k)
+                if (k != a.skip)
+                    for (uint32_t i = 0; i < DRAIN_ITERS && !poll(&full[k % STAGES], (k / STAGES) & 1, 2000); ++i)
+                        if (*stop && i > 1000) break;
+        if (a.q_box && qn)
+            for (uint32_t i = 0; i < DRAIN_ITERS && !poll(qfull, (qn - 1) & 1, 2000); ++i)
+                if (*stop && i > 1000) break;
+        __syncwarp();
+    } else if (warp >= L::MMA_WARP) {  // the products: one warp of its warpgroup
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::MMA_REGS));
         if (warp == L::MMA_WARP) {
             const uint32_t leads = elected();
@@ -623,8 +709,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
             constexpr uint32_t qk = idesc_f16<T>(128, SLOT, false), pv = idesc_f16<T>(128, DP, true);
             const uint32_t qk_idesc = qk | (a.negate ? 1u << 13 : 0);
             const uint32_t qs = tc05::smem_u32(smem), rs = tc05::smem_u32(ring);
-            uint32_t base = 0, qn = 0, pn = 0, sn = 0;  // pn, sn: phase bits of either row tile's weights and scores
-            bool scored[2] = {false, false};
+            uint32_t base = 0, qn = 0, pn = 0, sn = 0, scored = 0;  // pn, sn: phase bits of either row tile's weights and scores
             bool ok = works;
             auto wait_all = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(~0u, wait_or_stop(bar, parity, stop)); };
             auto tile_full = [&](uint32_t f) {
@@ -637,12 +722,12 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) commit(&empty[(f + p) % STAGES]);
             };
-            // scores for warpgroup w: rows of q tile t against the keys of ring fill f
+            // scores of row tile w: rows of q tile t against the keys of ring fill f
             auto scores = [&](int w, int t, uint32_t f) {
                 if (APART) {  // the scores before have been read
-                    if ((w ? scored[1] : scored[0]) && !wait_all(&sfree[w], sn >> w & 1 ^ 1)) return false;
+                    if ((scored >> w & 1) && !wait_all(&sfree[w], sn >> w & 1 ^ 1)) return false;
                     sn ^= 1u << w;
-                    scored[0] |= w == 0, scored[1] |= w == 1;
+                    scored |= 1u << w;
                 }
                 if (!tile_full(f)) return false;
                 tc05::fence_after();
@@ -657,19 +742,19 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                 commit(&sfull[w]);
                 return true;
             };
-            // sums of warpgroup w: its weights times the values of ring fill f
+            // sums of row tile w: its weights times the values of ring fill f
             auto sums = [&](int w, uint32_t f, bool add) {
-                if (!tile_full(f)) return false;
+                if (!tile_full(f) || !wait_all(&pready[w], pn >> w & 1)) return false;
+                tc05::fence_after();
+                if (!by_hand[w]) {
+                    const uint32_t to = tmem + (w ? L::o_col(1) : L::o_col(0));
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {  // halves of the keys
-                    if (!wait_all(&pready[2 * w + h], pn >> w & 1)) return false;
-                    tc05::fence_after();
-                    if (by_hand[w]) continue;
-                    const uint32_t y = desc_lo(rs + (f + h * (PARTS - 1)) % STAGES * L::SLOT_BYTES, SLOT * 128) + (PARTS == 1 ? h * 512 : 0);
+                    for (int h = 0; h < 2; ++h) {  // halves of the keys
+                        const uint32_t x = tmem + (w ? L::p_col(1, h) : L::p_col(0, h));
+                        const uint32_t y = desc_lo(rs + (f + h * (PARTS - 1)) % STAGES * L::SLOT_BYTES, SLOT * 128) + (PARTS == 1 ? h * 512 : 0);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_ts(leads, tmem + (w ? L::o_col(1) : L::o_col(0)), tmem + (w ? L::p_col(1) : L::p_col(0)) + h * 32 + k * 8,
-                               y + k * 128, pv, add || h || k);
+                        for (int k = 0; k < 4; ++k) mma_ts(leads, to, x + k * 8, y + k * 128, pv, add || h || k);
+                    }
                 }
                 pn ^= 1u << w;
                 commit(&odone[w]);
@@ -681,21 +766,25 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                     const bool alt = NT == 2 && seg.rows(a) <= 128, pair = NT == 2 && !alt;
                     const int lead = lead_of(alt), all = pair ? 2 * n : n;
                     ok = wait_all(qfull, qn++ & 1);
-                    auto score_unit = [&](int u) {
-                        const uint32_t f = base + k_fill(pair ? u >> 1 : u, lead);
-                        if (!scores(NT == 2 ? u & 1 : 0, pair ? u & 1 : 0, f)) return false;
-                        if (!pair || u & 1) release(f);
-                        if (u + 1 == all) commit(qempty);
-                        return true;
-                    };
-                    for (int u = 0; u < min(all, NT) && ok; ++u) ok = score_unit(u);
-                    for (int u = 0; u < all && ok; ++u) {
-                        if (APART && u + NT < all) ok = score_unit(u + NT);
-                        if (!ok) break;
-                        const uint32_t f = base + v_fill(pair ? u >> 1 : u, n, lead);
-                        ok = sums(NT == 2 ? u & 1 : 0, f, u >= NT);
-                        if (ok && (!pair || u & 1)) release(f);
-                        if (!APART && ok && u + NT < all) ok = score_unit(u + NT);
+                    // the scores of unit i, and the sums of unit i - NT behind them (APART) or ahead of them
+                    for (int i = 0; i < all + NT && ok; ++i) {
+#pragma unroll 1
+                        for (int e = 0; e < 2 && ok; ++e) {
+                            if ((e == 0) == APART) {
+                                if (i >= all) continue;
+                                const uint32_t f = base + k_fill(pair ? i >> 1 : i, lead);
+                                ok = scores(NT == 2 ? i & 1 : 0, pair ? i & 1 : 0, f);
+                                if (!ok) break;
+                                if (!pair || i & 1) release(f);
+                                if (i + 1 == all) commit(qempty);
+                            } else {
+                                const int u = i - NT;
+                                if (u < 0) continue;
+                                const uint32_t f = base + v_fill(pair ? u >> 1 : u, n, lead);
+                                ok = sums(NT == 2 ? u & 1 : 0, f, u >= NT);
+                                if (ok && (!pair || u & 1)) release(f);
+                            }
+                        }
                     }
                     base += 2 * n * PARTS;
                 } while (ok && seg.next(a));
@@ -705,115 +794,78 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
         __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(L::SOFT_REGS));
-        const int wg = warp >> 2, row = tid & 127;  // this warpgroup, and this thread's lane of TMEM
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        // A warpgroup: half `h` of the keys of row tile `w`, a row in each thread.
+        const int wg = warp >> 2, w = wg >> 1, h = wg & 1, row = tid & 127;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t otm = lanes + (w ? L::o_col(1) : L::o_col(0)), stm = lanes + w * BK + h * 64;
+        const uint32_t ptm = lanes + (w ? (h ? L::p_col(1, 1) : L::p_col(1, 0)) : (h ? L::p_col(0, 1) : L::p_col(0, 0)));
         const float c = a.scale_log2;
-        uint32_t un = 0, wn = 0, bn = 0, base = 0;  // un: units of this warpgroup
-        bool hand = false;
-        bool ok = works;
-        auto meet = [&](uint64_t *bar, uint32_t &n) {  // the warps of a warpgroup, or of both
+        uint32_t un = 0, tn = 0, gn = 0, bn = 0, base = 0;  // units of this row tile; turns of the barriers
+        bool hand = false, ok = works;
+        auto meet = [&](uint64_t *bar, uint32_t &turn) {  // the warps that share a barrier
             __syncwarp();
             if (lane == 0) arrive(bar);
-            return (bool)__all_sync(~0u, wait_or_stop(bar, n++ & 1, stop));
+            return (bool)__all_sync(~0u, wait_or_stop(bar, turn++ & 1, stop));
+        };
+        // The sums of the unit before, and its weights, are the tensor core's until this.
+        auto before_done = [&]() {
+            if (!APART || !un) return true;  // (else scores come after it)
+            const bool r = __all_sync(~0u, wait_or_stop(&odone[w], (un - 1) & 1, stop));
+            tc05::fence_after();
+            return r;
         };
         long long item_first = first - (works ? seg.t0 : 0);  // the line's index of the item's first step
         bool counted = false;
         if (ok) do {
                 const int n = seg.t1 - seg.t0, rows = seg.rows(a);
                 const bool alt = NT == 2 && rows <= 128;
-                const int r = (alt ? 0 : wg * 128) + row;
+                const int r = (alt ? 0 : w * 128) + row;
                 const bool exists = r < rows;
                 const int at = (int)((long long)seg.qt * R + r), tok = at / a.group;
                 const int seen = exists ? seg.seq.seen(a, tok) : seg.seq.len;
                 const int first_seen = seg.seq.seen(a, (int)((long long)seg.qt * R + r - row) / a.group);  // the tile's first row
-                const uint32_t otm = tmem + lanes + (wg ? L::o_col(1) : L::o_col(0)), stm = tmem + lanes + wg * BK;
-                const uint32_t ptm = tmem + lanes + (wg ? L::p_col(1) : L::p_col(0));
                 counted = false;
                 float m = LOWEST, l = 0.f;
                 bool fresh = true;
-                // The weights (in TMEM) times the values of ring fill f, for the keys under `lim` alone.
-                auto add_by_hand = [&](bool first, uint32_t f, int lim) {
-#pragma unroll 1
-                    for (int k = 0; k < D; k += 16) {
-                        uint32_t o[16], w8[8];
-                        if (first) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = 0;
-                        } else {
-                            tc05::ld16(otm + k, o);
-                            tc05::wait_ld_regs(o);
-                        }
-#pragma unroll 1
-                        for (int key = 0; key < BK; key += 16) {
-                            tc05::ld8(ptm + key / 2, w8);
-                            tc05::wait_ld_regs(w8);
-                            const uint8_t *slot = ring + (f + key / SLOT) % STAGES * L::SLOT_BYTES + (k >> 6) * (SLOT * 128);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const float2 w2 = unpack(w8[i / 2], T());
-                                const float wt = i & 1 ? w2.y : w2.x;
-                                const int kr = (key + i) % SLOT;
-#pragma unroll
-                                for (int q = 0; q < 2 && key + i < lim; ++q) {
-                                    const uint4 u = *(const uint4 *)(slot + kr * 128 + (((((k & 63) >> 3) + q) ^ (kr & 7)) << 4));
-                                    const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        const float2 y = unpack(uu[e], T());
-                                        o[q * 8 + e * 2] = __float_as_uint(fmaf(wt, y.x, __uint_as_float(o[q * 8 + e * 2])));
-                                        o[q * 8 + e * 2 + 1] = __float_as_uint(fmaf(wt, y.y, __uint_as_float(o[q * 8 + e * 2 + 1])));
-                                    }
-                                }
-                            }
-                            __syncwarp();
-                        }
-                        tc05::st16(otm + k, o);
-                    }
-                    tc05::wait_st();
-                };
-                for (int j = alt ? wg : 0; j < n; j += alt ? 2 : 1) {
-                    ok = __all_sync(~0u, wait_or_stop(&sfull[wg], un & 1, stop));
+                for (int j = alt ? w : 0; j < n; j += alt ? 2 : 1) {
+                    ok = __all_sync(~0u, wait_or_stop(&sfull[w], un & 1, stop));
                     if (!ok) break;
                     tc05::fence_after();
-                    // The sums of the unit before, and its weights, are the tensor core's until this.
-                    auto before_done = [&]() {
-                        if (!APART || !un) return true;  // (else scores come after it)
-                        const bool r = __all_sync(~0u, wait_or_stop(&odone[wg], (un - 1) & 1, stop));
-                        tc05::fence_after();
-                        return r;
-                    };
-                    const int k0 = (seg.t0 + j) * BK, lim = seen - k0;
-                    // The scores are read twice, 32 at a time: in registers all 128 would have the loops unrolled, and
-                    // those outgrow the instruction cache (a step of heads of 128 took 2.5 to 3.3 thousand clocks so).
-                    const bool masked = __any_sync(~0u, lim < BK);
+                    const int k0 = (seg.t0 + j) * BK + h * 64, lim = seen - k0;  // of this half
+                    // The scores are read twice, 32 at a time: in registers all would have the loops unrolled, and those
+                    // outgrow the instruction cache.
+                    const bool masked = __any_sync(~0u, lim < 64);
                     float top = -CUDART_INF_F;
                     if (!masked) {
-                        uint32_t x[4][32];
-                        float t[4];
+                        uint32_t x[2][32];
+                        float t = -CUDART_INF_F;
+                        tc05::ld32(stm, x[0]);
+                        tc05::ld32(stm + 32, x[1]);
+                        tc05::wait_ld_regs(x[0]);
+                        tc05::wait_ld_regs(x[1]);
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) tc05::ld32(stm + g * 32, x[g]);
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) tc05::wait_ld_regs(x[g]);
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) t[g] = fmaxf(__uint_as_float(x[g][0]), __uint_as_float(x[g][1]));
-#pragma unroll
-                        for (int i = 2; i < 32; i += 2)
-#pragma unroll
-                            for (int g = 0; g < 4; ++g) t[g] = fmaxf(fmaxf(t[g], __uint_as_float(x[g][i])), __uint_as_float(x[g][i + 1]));
-                        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                        for (int i = 0; i < 32; i += 2) {
+                            top = fmaxf(fmaxf(top, __uint_as_float(x[0][i])), __uint_as_float(x[0][i + 1]));
+                            t = fmaxf(fmaxf(t, __uint_as_float(x[1][i])), __uint_as_float(x[1][i + 1]));
+                        }
+                        top = fmaxf(top, t);
                     } else {
 #pragma unroll 1
-                        for (int g = 0; g < 4; ++g) {
-                            uint32_t x[32];
+                        for (int g = 0; g < 64; g += 16) {
+                            uint32_t x[16];
                             __syncwarp();
-                            tc05::ld32(stm + g * 32, x);
+                            tc05::ld16(stm + g, x);
                             tc05::wait_ld_regs(x);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (g * 32 + i < lim) top = fmaxf(top, __uint_as_float(x[i]));
+                            for (int i = 0; i < 16; ++i) top = fmaxf(top, g + i < lim ? __uint_as_float(x[i]) : -CUDART_INF_F);
                         }
                     }
-                    top *= c;
+                    // the row's over both halves
+                    told[wg * 128 + row] = top;
+                    uint32_t turn = un;
+                    ok = meet(&pair_bar[w * 4 + (warp & 3)], turn);
+                    if (!ok) break;
+                    top = fmaxf(top, told[(wg ^ 1) * 128 + row]) * c;
                     if (__any_sync(~0u, top > m + (TOP<T> + SOFT))) {
                         const float to = fmaxf(top - TOP<T>, m), f = exp2_(m - to);
                         m = to;
@@ -822,7 +874,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                             ok = before_done();
                             if (!ok) break;
 #pragma unroll 1
-                            for (int k = 0; k < D; k += 16) {
+                            for (int k = h * (D / 2); k < (h + 1) * (D / 2); k += 16) {
                                 uint32_t o[16];
                                 __syncwarp();
                                 tc05::ld16(otm + k, o);
@@ -833,165 +885,197 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                             }
                         }
                     }
-                    if (hand) {  // the products' thread has read it
-                        ok = before_done();
+                    if (hand) {  // the products' warp has read it
+                        ok = before_done() && meet(&tbar[w], tn);
                         if (!ok) break;
-                        if (row == 0) by_hand[wg] = 0;
+                        if (row == 0 && h == 0) by_hand[w] = 0;
                         hand = false;
-                        ok = meet(&wgbar[wg], wn);
+                        ok = meet(&tbar[w], tn);
                         if (!ok) break;
                     }
                     uint32_t vf = 0;
-                    if (first_seen < seg.seq.len && first_seen < k0 + BK) {
+                    if (first_seen < seg.seq.len && first_seen < k0 - h * 64 + BK) {
                         // Values that some row of the tile does not see: any that are no numbers?
                         vf = base + v_fill(j, n, lead_of(alt));
+                        const uint32_t fp = vf + h * (PARTS - 1);
+                        ok = __all_sync(~0u, wait_or_stop(&full[fp % STAGES], (fp / STAGES) & 1, stop));
+                        if (!ok) break;
+                        const uint4 *v = (const uint4 *)(ring + fp % STAGES * L::SLOT_BYTES) + (PARTS == 1 ? h * 512 : 0);
                         uint32_t top2 = 0;
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            const uint32_t fp = vf + p;
-                            ok = ok && __all_sync(~0u, wait_or_stop(&full[fp % STAGES], (fp / STAGES) & 1, stop));
-                            const uint4 *v = (const uint4 *)(ring + fp % STAGES * L::SLOT_BYTES);
-                            for (int i = row; i < SLOT * L::CH; i += 128) {
-                                const uint4 u = v[(i / SLOT >> 3) * (SLOT * 8) + i % SLOT * 8 + (((i / SLOT) ^ (i % SLOT)) & 7)];
-                                top2 = __vmaxu2(top2, u.x & 0x7fff7fffu), top2 = __vmaxu2(top2, u.y & 0x7fff7fffu);
-                                top2 = __vmaxu2(top2, u.z & 0x7fff7fffu), top2 = __vmaxu2(top2, u.w & 0x7fff7fffu);
-                            }
+#pragma unroll 2
+                        for (int i = row; i < 64 * L::CH; i += 128) {
+                            const uint4 u = v[(i / 64 >> 3) * (SLOT * 8) + i % 64 * 8 + (((i / 64) ^ i) & 7)];
+                            top2 = __vmaxu2(top2, u.x & 0x7fff7fffu), top2 = __vmaxu2(top2, u.y & 0x7fff7fffu);
+                            top2 = __vmaxu2(top2, u.z & 0x7fff7fffu), top2 = __vmaxu2(top2, u.w & 0x7fff7fffu);
                         }
-                        if (!ok) break;
                         const bool bad = __vmaxu2(top2, infinite(T()) - 0x00010001u) != infinite(T()) - 0x00010001u;
-                        if (__any_sync(~0u, bad) && lane == 0) by_hand[wg] = 1;
-                        ok = meet(&wgbar[wg], wn);
+                        if (__any_sync(~0u, bad) && lane == 0) by_hand[w] = 1;
+                        ok = meet(&tbar[w], tn);
                         if (!ok) break;
-                        hand = by_hand[wg];
+                        hand = by_hand[w];
                     }
                     ok = before_done();
                     if (!ok) break;
                     const uint64_t c2 = two(c, c), m2 = two(-m, -m);
                     uint64_t sum2 = 0;
-                    auto put = [&](int g, uint32_t (&w)[16]) {  // weights of keys 32 g to 32 g + 31 (over scores that have been read)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 v = unpack(w[i], T());
-                            sum2 = add2(sum2, two(v.x, v.y));
-                        }
-                        tc05::st16(ptm + g * 16, w);
+                    auto put = [&](uint32_t v) {
+                        const float2 p = unpack(v, T());
+                        sum2 = add2(sum2, two(p.x, p.y));
                     };
                     auto read = [&]() {  // the scores are
                         if (APART) {
                             tc05::fence_before();
                             __syncwarp();
-                            if (lane == 0) arrive(&sfree[wg]);
+                            if (lane == 0) arrive(&sfree[w]);
                         }
-                    };
-                    auto half_made = [&](int h) {  // a half of the weights goes to the product while the other is made
-                        tc05::wait_st();
-                        if (hand) return;
-                        tc05::fence_before();
-                        __syncwarp();
-                        if (lane == 0) arrive(&pready[2 * wg + h]);
-                        __syncwarp();
                     };
                     if (!masked) {
-                        uint32_t x[2][32];
-                        tc05::ld32(stm, x[0]);
 #pragma unroll 1
-                        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                tc05::wait_ld_regs(x[e]);
-                                if (e == 0) tc05::ld32(stm + h * 64 + 32, x[1]);
-                                else if (h == 0) tc05::ld32(stm + 64, x[0]);
-                                else read();
-                                uint32_t w[16];
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    const uint64_t y = fma2(two(__uint_as_float(x[e][2 * i]), __uint_as_float(x[e][2 * i + 1])), c2, m2);
-                                    float lo, hi;
-                                    if (i % EMULATED == EMULATED - 1) {
-                                        exp2_pair(y, lo, hi);
-                                    } else {
-                                        split2(y, lo, hi);
-                                        lo = exp2_(lo), hi = exp2_(hi);
-                                    }
-                                    w[i] = pack(lo, hi, T());
-                                }
-                                put(h * 2 + e, w);
-                            }
-                            half_made(h);
-                        }
-                    } else {
-#pragma unroll 1
-                        for (int g = 0; g < 4; ++g) {
-                            uint32_t x[32], w[16];
+                        for (int g = 0; g < 2; ++g) {
+                            uint32_t x[32], v[16];
                             __syncwarp();
                             tc05::ld32(stm + g * 32, x);
                             tc05::wait_ld_regs(x);
-                            if (g == 3) read();
+                            if (g) read();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float e = exp2_(fmaf(__uint_as_float(x[i]), c, -m));
-                                x[i] = __float_as_uint(g * 32 + i < lim ? e : 0.f);
+                            for (int i = 0; i < 16; ++i) {
+                                const uint64_t y = fma2(two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c2, m2);
+                                float lo, hi;
+                                if (i % EMULATED == EMULATED - 1) {
+                                    exp2_pair(y, lo, hi);
+                                } else {
+                                    split2(y, lo, hi);
+                                    lo = exp2_(lo), hi = exp2_(hi);
+                                }
+                                v[i] = pack(lo, hi, T());
+                                put(v[i]);
                             }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) w[i] = pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]), T());
                             __syncwarp();
-                            put(g, w);
-                            if (g & 1) half_made(g >> 1);
+                            tc05::st16(ptm + g * 16, v);  // (over scores that have been read)
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int g = 0; g < 64; g += 16) {
+                            uint32_t x[16];
+                            __syncwarp();
+                            tc05::ld16(stm + g, x);
+                            tc05::wait_ld_regs(x);
+                            if (g == 48) read();
+                            uint32_t v[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float lo = exp2_(fmaf(__uint_as_float(x[2 * i]), c, -m));
+                                const float hi = exp2_(fmaf(__uint_as_float(x[2 * i + 1]), c, -m));
+                                v[i] = pack(g + 2 * i < lim ? lo : 0.f, g + 2 * i + 1 < lim ? hi : 0.f, T());
+                                put(v[i]);
+                            }
+                            __syncwarp();
+                            st8(ptm + g / 2, v);
                         }
                     }
+                    tc05::wait_st();
                     float lo, hi;
                     split2(sum2, lo, hi);
                     l += lo + hi;
                     if (hand) {
-                        add_by_hand(fresh, vf, lim);
+                        // The weights times the values of ring fill vf, for the keys that a row sees alone: this half's
+                        // dimensions, of all keys.
                         tc05::fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            arrive(&pready[2 * wg]);
-                            arrive(&pready[2 * wg + 1]);
+                        ok = meet(&tbar[w], tn);
+                        if (!ok) break;
+                        tc05::fence_after();
+                        const int most = seen - (k0 - h * 64);
+#pragma unroll 1
+                        for (int k = h * (D / 2); k < (h + 1) * (D / 2); k += 8) {
+                            uint32_t o[8];
+                            __syncwarp();
+                            if (fresh) {
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) o[i] = 0;
+                            } else {
+                                tc05::ld8(otm + k, o);
+                                tc05::wait_ld_regs(o);
+                            }
+#pragma unroll 1
+                            for (int key = 0; key < BK; key += 8) {
+                                const int half = key >> 6;
+                                uint32_t v[4];
+                                __syncwarp();
+                                tc05::ld4(lanes + (w ? (half ? L::p_col(1, 1) : L::p_col(1, 0)) : (half ? L::p_col(0, 1) : L::p_col(0, 0))) + (key & 63) / 2, v);
+                                tc05::wait_ld_regs(v);
+                                const uint8_t *at_slot = ring + (vf + key / SLOT) % STAGES * L::SLOT_BYTES + (k >> 6) * (SLOT * 128) +
+                                                         key % SLOT * 128;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const float2 p2 = unpack(v[i / 2], T());
+                                    const float wt = i & 1 ? p2.y : p2.x;
+                                    const uint4 u = *(const uint4 *)(at_slot + i * 128 + ((((k & 63) >> 3) ^ i) << 4));
+                                    const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+                                    if (key + i < most)
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e) {
+                                            const float2 y = unpack(uu[e], T());
+                                            o[e * 2] = __float_as_uint(fmaf(wt, y.x, __uint_as_float(o[e * 2])));
+                                            o[e * 2 + 1] = __float_as_uint(fmaf(wt, y.y, __uint_as_float(o[e * 2 + 1])));
+                                        }
+                                }
+                            }
+                            __syncwarp();
+                            st8(otm + k, o);
                         }
+                        tc05::wait_st();
                     }
                     fresh = false;
                     ++un;
+                    tc05::fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(&pready[w]);
                 }
                 if (!ok) break;
-                // the sums
-                const bool some = alt ? n > wg : true;
+                // The row tile's sums are done; the row's weights over both halves, and, where the tiles had the even and the
+                // odd steps of the same rows, over both tiles.
+                const bool some = alt ? n > w : true;
                 if (some) {
-                    ok = __all_sync(~0u, wait_or_stop(&odone[wg], (un - 1) & 1, stop));
+                    ok = __all_sync(~0u, wait_or_stop(&odone[w], (un - 1) & 1, stop));
                     if (!ok) break;
-                    tc05::fence_after();
                 }
-                float f[2] = {1.f, 0.f};  // of this warpgroup's sums, and of the other's
-                if (alt) {  // the even and the odd steps'
-                    half_stat[wg * 128 + row] = make_float2(m, l);
-                    tc05::fence_before();
+                auto everyone = [&]() { return alt ? meet(both, bn) : meet(&tbar[w], tn); };
+                told[wg * 128 + row] = l;
+                tc05::fence_before();
+                ok = everyone();
+                if (!ok) break;
+                tc05::fence_after();
+                l += told[(wg ^ 1) * 128 + row];
+                float mine = 1.f, its = 0.f;  // what the sums of this row tile, and of the other, are multiplied by
+                if (alt) {
+                    const float other = told[(wg ^ 2) * 128 + row] + told[(wg ^ 3) * 128 + row];
                     ok = meet(both, bn);
                     if (!ok) break;
-                    tc05::fence_after();
-                    const float2 other = half_stat[(wg ^ 1) * 128 + row];
-                    const float M = fmaxf(m, other.x);
-                    f[0] = exp2_(m - M), f[1] = exp2_(other.x - M);
-                    l = l * f[0] + other.y * f[1];
+                    told[wg * 128 + row] = m;
+                    ok = meet(both, bn);
+                    if (!ok) break;
+                    const float M = fmaxf(m, told[(wg ^ 2) * 128 + row]);
+                    mine = exp2_(m - M), its = exp2_(told[(wg ^ 2) * 128 + row] - M);
+                    l = l * mine + other * its;
                     m = M;
-                    if (!some) f[0] = 0.f;
                 }
-                const bool two_halves = alt && n > 1, other_alone = alt && !some;
-                const int col0 = alt ? wg * (D / 2) : 0, col1 = alt ? col0 + D / 2 : D;
-                auto columns = [&](int col, float (&v)[16]) {
-                    uint32_t o[16];
+                const bool two_tiles = alt && n > 1, other_alone = alt && !some;
+                constexpr int QUARTER = D / 4;
+                const int col0 = alt ? wg * QUARTER : h * (D / 2), col1 = col0 + (alt ? QUARTER : D / 2);  // this warpgroup's
+                const uint32_t its_otm = lanes + (w ? L::o_col(0) : L::o_col(1));
+                auto columns = [&](int col, float (&v)[8]) {
+                    uint32_t o[8];
                     __syncwarp();  // rows that do not exist store nothing: the warp's lanes meet again
-                    const uint32_t mine = otm + col, its = tmem + lanes + (wg ? L::o_col(0) : L::o_col(1)) + col;
-                    tc05::ld16(other_alone ? its : mine, o);
+                    tc05::ld8(other_alone ? its_otm + col : otm + col, o);
                     tc05::wait_ld_regs(o);
-                    const float w = other_alone ? f[1] : f[0];
+                    const float f = other_alone ? its : mine;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * w;
-                    if (two_halves) {
-                        tc05::ld16(its, o);
+                    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[i]) * f;
+                    if (two_tiles) {
+                        tc05::ld8(its_otm + col, o);
                         tc05::wait_ld_regs(o);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(o[i]), f[1], v[i]);
+                        for (int i = 0; i < 8; ++i) v[i] = fmaf(__uint_as_float(o[i]), its, v[i]);
                     }
                 };
                 T *out = (T *)a.out;
@@ -1002,39 +1086,45 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                     out += tk * a.o_tok + hd * a.o_head;
                     if (lse) lse += tk * a.lse_tok + hd * a.lse_head;
                 }
-                const int c_first = (int)(item_first / share), c_last = (int)((item_first + seg.steps - 1) / share);
+                const int c_first = (int)ratio(item_first, share), c_last = (int)ratio(item_first + seg.steps - 1, share);
                 if (c_first == c_last) {
                     const float inv = row_factor(seen, m, l);
 #pragma unroll 1
-                    for (int col = col0; col < col1; col += 16) {
-                        float v[16];
+                    for (int col = col0; col < col1; col += 8) {
+                        float v[8];
                         columns(col, v);
+                        alignas(16) T e[8];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = seen > 0 ? v[i] * inv : 0.f;
-                        if (exists) store_row16(out + col, a.o_vec, v);
+                        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(seen > 0 ? v[i] * inv : 0.f);
+                        if (!exists) continue;
+                        if (a.o_vec) {
+                            *(uint4 *)(out + col) = *(const uint4 *)e;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) out[col + i] = e[i];
+                        }
                     }
                     if (exists && lse && col0 == 0) *lse = row_lse(seen, m, l);
                 } else {
                     // A share leaves its second slot to the item that starts in it, its first to one that started before.
                     auto slot = [&](int k) { return 2ll * k + (k == c_first); };
-                    const int tile0 = alt ? 0 : wg * 128;  // rows of this warpgroup
-                    float4 *po = (float4 *)a.parts;  // a slot: [D / 4][R]
-                    float2 *pst = (float2 *)(a.parts + 2ll * gridDim.x * L::PART);  // a slot: [R], with alternating halves [2][128]
-                    const int strow = alt ? wg * 128 + row : tile0 + row;
-                    const long long mine = slot(blockIdx.x);
+                    const int tile0 = alt ? 0 : w * 128;  // rows of this warpgroup
+                    float4 *po = (float4 *)a.parts;       // a slot: [D / 4][R]
+                    float2 *pst = (float2 *)(a.parts + 2ll * gridDim.x * L::PART) + wg * 128;  // a slot: [4][128]
+                    const long long own = slot(blockIdx.x);
 #pragma unroll 1
-                    for (int col = col0; col < col1; col += 16) {
-                        float v[16];
+                    for (int col = col0; col < col1; col += 8) {
+                        float v[8];
                         columns(col, v);
                         if (exists)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                __stcg(po + mine * (L::PART / 4) + (long long)(col / 4 + i) * R + tile0 + row,
+                            for (int i = 0; i < 2; ++i)
+                                __stcg(po + own * (L::PART / 4) + (long long)(col / 4 + i) * R + tile0 + row,
                                        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
                     }
-                    if (exists) __stcg(pst + mine * R + strow, make_float2(m, l));
+                    if (exists) __stcg(pst + own * 512 + row, make_float2(m, l));
                     const int k_parts = c_last - c_first + 1;
-                    ok = meet(&wgbar[wg], wn);
+                    ok = meet(&gbar[wg], gn);
                     if (!ok) break;
                     if (row == 0) {
                         __threadfence();
@@ -1042,29 +1132,32 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                         __threadfence();
                     }
                     counted = true;
-                    ok = meet(&wgbar[wg], wn);
+                    ok = meet(&gbar[wg], gn);
                     if (!ok) break;
                     if (last_flag[wg]) {
                         // a row's maximum and sum over the parts; then each part's weight in the place of its maximum
                         if (exists) {
                             float M = LOWEST, S = 0.f;
-                            for (int k = 0; k < k_parts; ++k) M = fmaxf(M, __ldcg(pst + slot(c_first + k) * R + strow).x);
+#pragma unroll 4
+                            for (int k = 0; k < k_parts; ++k) M = fmaxf(M, __ldcg(pst + slot(c_first + k) * 512 + row).x);
+#pragma unroll 4
                             for (int k = 0; k < k_parts; ++k) {
-                                const float2 v = __ldcg(pst + slot(c_first + k) * R + strow);
+                                const float2 v = __ldcg(pst + slot(c_first + k) * 512 + row);
                                 S += exp2_(v.x - M) * v.y;
                             }
                             const float inv = row_factor(seen, M, S);
+#pragma unroll 1
                             for (int k = 0; k < k_parts; ++k) {
-                                float2 *p = pst + slot(c_first + k) * R + strow;
-                                __stcg(&p->x, seen > 0 ? exp2_(__ldcg(&p->x) - M) : 0.f);
-                                __stcg(&p->y, inv);
+                                float2 *p = pst + slot(c_first + k) * 512 + row;
+                                __stcg(p, make_float2(seen > 0 ? exp2_(__ldcg(p).x - M) : 0.f, inv));
                             }
                             if (lse && col0 == 0) *lse = row_lse(seen, M, S);
                         }
                         __threadfence_block();
-                        ok = meet(&wgbar[wg], wn);
+                        ok = meet(&gbar[wg], gn);
                         if (!ok) break;
                         const int nr = min(128, rows - tile0), n4 = nr * (col1 - col0) / 4;
+#pragma unroll 1
                         for (int i = row; i < n4; i += 128) {
                             const int rr = i % nr, c4 = col0 / 4 + i / nr;
                             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1072,7 +1165,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
 #pragma unroll 4
                             for (int k = 0; k < k_parts; ++k) {
                                 const long long sl = slot(c_first + k);
-                                const float2 wv = __ldcg(pst + sl * R + (alt ? wg * 128 : tile0) + rr);
+                                const float2 wv = __ldcg(pst + sl * 512 + rr);
                                 const float4 v = __ldcg(po + sl * (L::PART / 4) + (long long)c4 * R + tile0 + rr);
                                 inv = wv.y;
                                 acc.x = fmaf(wv.x, v.x, acc.x), acc.y = fmaf(wv.x, v.y, acc.y);
@@ -1093,12 +1186,11 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
                         }
                     }
                 }
-                if (alt) {  // the other warpgroup has read this one's sums
-                    tc05::fence_before();
-                    ok = meet(both, bn);
-                    if (!ok) break;
-                    tc05::fence_after();
-                }
+                // What the others have of this warpgroup (in `told`, and its sums) has been read.
+                tc05::fence_before();
+                ok = everyone();
+                if (!ok) break;
+                tc05::fence_after();
                 item_first += seg.steps;
                 base += 2 * n * PARTS;
                 if (!seg.next(a)) break;
@@ -1106,7 +1198,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
         if (!ok && works && row == 0) {
             // Gave up: the counters of the cut items of this share are counted on, so that they end at zero.
             do {
-                const int c_first = (int)(item_first / share), c_last = (int)((item_first + seg.steps - 1) / share);
+                const int c_first = (int)ratio(item_first, share), c_last = (int)ratio(item_first + seg.steps - 1, share);
                 if (c_first != c_last && !counted) atomicInc(a.counts + wg * MAX_GRID + c_first, c_last - c_first);
                 counted = false;
                 item_first += seg.steps;
@@ -1123,9 +1215,67 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1) chunk_kernel(const __grid_
     }
 }
 
+PFN_cuTensorMapEncodeTiled encoder() {
+    static PFN_cuTensorMapEncodeTiled encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return (PFN_cuTensorMapEncodeTiled)fn;
+    }();
+    return encode;
+}
+
+// A cache in boxes of `rows` slots x 64 dimensions of one head of a page; false where its strides do not allow that.
+template <typename T, int D>
+bool tensor_map(CUtensorMap *map, const void *base, const ChunkArgs &a, long long page, long long slot, long long head, int rows) {
+    const PFN_cuTensorMapEncodeTiled encode = encoder();
+    if (!encode || !base || !a.num_pages) return false;
+    const cuuint64_t dims[4] = {D, (cuuint64_t)a.page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.num_pages};
+    const long long strides[3] = {slot, head, page};
+    cuuint64_t bytes[3];
+    for (int i = 0; i < 3; ++i) {
+        if (dims[i + 1] > 1 && (strides[i] < D || strides[i] >= 1ll << 38)) return false;
+        bytes[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] * 2 : 512;
+    }
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type =
+        std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode(map, type, 4, const_cast<void *>(base), dims, bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// q in boxes of the heads of a group x as many tokens as make 128 rows; false where they do not.
+template <typename T, int D>
+bool q_map(CUtensorMap *map, const ChunkArgs &a) {
+    const PFN_cuTensorMapEncodeTiled encode = encoder();
+    if (!encode || a.group > 128 || 128 % a.group) return false;
+    const cuuint64_t dims[3] = {D, (cuuint64_t)a.heads, (cuuint64_t)a.tokens};
+    const long long strides[2] = {a.q_head, a.q_tok};
+    cuuint64_t bytes[2];
+    for (int i = 0; i < 2; ++i) {
+        if (dims[i + 1] > 1 && (strides[i] < D || strides[i] >= 1ll << 38)) return false;
+        bytes[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] * 2 : 512;
+    }
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(128 / a.group)}, estr[3] = {1, 1, 1};
+    const CUtensorMapDataType type =
+        std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode(map, type, 3, const_cast<void *>(a.q), dims, bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
 cudaError_t launch(ChunkArgs a, int grid, cudaStream_t st) {
     using L = Lay<D>;
+    // Pages of a multiple of eight tokens come by TMA, in boxes of as many as a page and a copying warp's rows share.
+    CUtensorMap tmk = {}, tmv = {};
+    for (a.box = L::SLOT / 4; a.page % a.box; a.box /= 2) {}
+    if (a.box < 8 || !tensor_map<T, D>(&tmk, a.kc, a, a.kc_page, a.kc_slot, a.kc_head, a.box) ||
+        !tensor_map<T, D>(&tmv, a.vc, a, a.vc_page, a.vc_slot, a.vc_head, a.box))
+        a.box = 0;
+    CUtensorMap tmq = {};
+    a.q_box = a.q_vec && q_map<T, D>(&tmq, a);
     static std::atomic<uint64_t> ready;
     static std::atomic<int> regs;
     cudaError_t e = allow_shared(chunk_kernel<T, D>, ready);
@@ -1137,7 +1287,7 @@ cudaError_t launch(ChunkArgs a, int grid, cudaStream_t st) {
         if (f.numRegs != L::REGS) return cudaErrorInvalidConfiguration;
         regs.store(f.numRegs, std::memory_order_relaxed);
     }
-    return launch_pdl(chunk_kernel<T, D>, dim3((unsigned)grid), dim3(L::THREADS), L::BYTES, st, a);
+    return launch_pdl(chunk_kernel<T, D>, dim3((unsigned)grid), dim3(L::THREADS), L::BYTES, st, a, tmk, tmv, tmq);
 }
 
 template <typename T>
@@ -1159,7 +1309,7 @@ int wave() {
     return sms < MAX_GRID ? sms : MAX_GRID;
 }
 
-static_assert(2 * MAX_GRID * 4 <= HV_ATTENTION_COUNTER_BYTES, "the counters that the caller zeroes");
+static_assert(4 * MAX_GRID * 4 <= HV_ATTENTION_COUNTER_BYTES, "the counters that the caller zeroes");
 static_assert(HV_ATTENTION_MAX_LENGTH + (long long)BK <= INT32_MAX, "token numbers of a last step are ints");
 
 }  // namespace
@@ -1172,7 +1322,7 @@ extern "C" int hv_paged_chunk_attention_workspace(int dim, int64_t *bytes) {
     if (!known_dim(dim)) return fail(HV_ERR_VALUE, "dim must be 32, 64, 96, 128, 192 or 256");
     const int grid = wave(), rows = dim <= 128 ? 256 : 128;
     if (!grid) return fail(HV_ERR_CUDA, "cannot read the device's SM count");
-    *bytes = HV_ATTENTION_COUNTER_BYTES + 2ll * grid * rows * (dim + 2) * 4;
+    *bytes = HV_ATTENTION_COUNTER_BYTES + 2ll * grid * (rows * dim + 1024) * 4;
     return HV_OK;
 }
 
