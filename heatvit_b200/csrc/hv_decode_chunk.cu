@@ -55,6 +55,7 @@ constexpr float TOP<__half> = 9.f;
 constexpr float SOFT = 6.f;
 constexpr int BK = 128;       // keys of a step
 constexpr int MIN_SHARE = 2;  // steps
+constexpr int ITEM = 3;       // steps' time that an item takes beside its steps: its rows of q, the join and its output
 constexpr int MAX_GRID = 512;
 constexpr int LAG = 2;        // copies of a producer that are under way ahead of the one that is waited for
 
@@ -72,6 +73,7 @@ struct ChunkArgs {
     uint32_t *counts;   // [4][MAX_GRID], zero between calls
     int box;            // rows of a TMA box of the cache; 0: none
     int q_box;          // q by TMA
+    int tp_shift;       // log2 of a row tile's tokens, where that is a whole power of two, or -1
     int *err;
 };
 
@@ -88,7 +90,7 @@ struct Lay {
     static constexpr int SLOT_BYTES = SLOT * DP * 2, Q_TILE = 128 * DP * 2, Q_BYTES = NT * Q_TILE;
     static constexpr int STAGES = DP == 64 ? 8 : DP == 128 ? 5 : DP == 192 ? 7 : 5;
     static constexpr int STAT = Q_BYTES + STAGES * SLOT_BYTES;  // [4][128] float: what the softmax warpgroups tell one another
-    static constexpr int BARS = STAT + 2048, MISC = BARS + 336, BYTES = MISC + 128;
+    static constexpr int BARS = STAT + 2048, MISC = BARS + 336, BYTES = MISC + 160;
     // A row tile has two softmax warpgroups, with 64 keys of a step each; then four copying warps, then the products'.
     static constexpr int GROUPS = 2 * NT, SOFT_WARPS = 4 * GROUPS, MMA_WARP = SOFT_WARPS + 4, WARPS = SOFT_WARPS + 8, THREADS = WARPS * 32;
     // Registers of a thread at launch, and of the roles from then on (shares of what the block was launched with).
@@ -206,32 +208,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-// One pair of weights in EMULATED is not the special function unit's, which makes 16 exponentials a clock where the
-// tensor core takes 8192 multiply-adds, but 2^x as 2^n 2^f, n the nearest integer, by a polynomial of degree 4 fitted
-// to 2^f on [-1/2, 1/2] (2.6e-6 = 2^-18 off at most; half a step of bf16 is 2^-9, of fp16 2^-12).  Under -126
-// it gives 2^-126; of a NaN the largest number, which as a weight is infinite.
-constexpr int EMULATED = 4;
-__device__ __forceinline__ void exp2_pair(uint64_t x, float &lo, float &hi) {
-    split2(x, lo, hi);
-    const uint64_t y = two(max_nan(lo, -126.f), max_nan(hi, -126.f));
-    const uint64_t magic = two(12582912.f, 12582912.f), back = two(-12582912.f, -12582912.f);  // 1.5 * 2^23
-    const uint64_t n = add2(y, magic), f = fma2(add2(n, back), two(-1.f, -1.f), y);
-    uint64_t p = fma2(f, two(0x1.3997d6p-7f, 0x1.3997d6p-7f), two(0x1.ca1442p-5f, 0x1.ca1442p-5f));
-    p = fma2(p, f, two(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    p = fma2(p, f, two(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    p = fma2(p, f, two(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    float nl, nh;
-    split2(n, nl, nh);
-    split2(p, lo, hi);
-    lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(nl) << 23));
-    hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(nh) << 23));
-}
-
 // A sequence's rows of q and cached tokens, brought into range (what is not is reported once, by `tell`).
 struct Seq {
     int s0, n, len;
@@ -262,45 +238,50 @@ struct Seq {
     }
 };
 
-// Steps [t0, t1) of the item (sequence b, key head h, row tile qt), of `steps` in all, as a share cuts them.
+// Steps [t0, t1) of the item (sequence b, key head h, row tile qt), of `steps` in all, as a share cuts them.  On the line an
+// item has ITEM further places ahead of its steps: what it costs beside them.
 template <int R>
 struct Segment {
     Seq seq;
-    int b, h, qt, qts, steps, t0, t1;
-    long long left;  // of the share, from t0 on
+    int b, h, qt, qts, steps, t0, t1, x0, x1;  // x0, x1: its places of the line
+    long long item, left;  // the line's index of the item's first place; places of the share from x0 on
     __device__ __forceinline__ void clip() {
-        t1 = (int)min((long long)steps, t0 + left);
+        x1 = (int)min((long long)steps + ITEM, x0 + left);
+        t0 = max(0, x0 - ITEM), t1 = max(0, x1 - ITEM);
     }
     __device__ __forceinline__ bool next(const ChunkArgs &a) {
-        left -= t1 - t0;
-        if (left <= 0) return false;
-        t0 = 0;
-        if (++qt == qts) {
-            qt = 0;
-            if (++h == a.kv_heads) {
-                h = 0;
-                do {
-                    seq.set(a, ++b, false);  // only called where a further step exists
-                    qts = seq.row_tiles(a, R);
-                } while (qts == 0);
+        do {
+            left -= x1 - x0;
+            if (left <= 0) return false;
+            item += steps + ITEM;
+            x0 = 0;
+            if (++qt == qts) {
+                qt = 0;
+                if (++h == a.kv_heads) {
+                    h = 0;
+                    do {
+                        seq.set(a, ++b, false);  // only called where a further step exists
+                        qts = seq.row_tiles(a, R);
+                    } while (qts == 0);
+                }
             }
-        }
-        steps = seq.steps(a, R, qt);
-        clip();
+            steps = seq.steps(a, R, qt);
+            clip();
+        } while (t0 == t1);
         return true;
     }
+    // The shares that have its first and its last step.
+    __device__ __forceinline__ int first_share(long long share) const { return (int)ratio(item + ITEM, share); }
+    __device__ __forceinline__ int last_share(long long share) const { return (int)ratio(item + ITEM + steps - 1, share); }
     __device__ __forceinline__ int rows(const ChunkArgs &a) const {
         return (int)min((long long)R, (long long)seq.n * a.group - (long long)qt * R);
     }
 };
 
-// What a row's sums are multiplied by, and its log-sum-exp: a row that sees nothing has zeros; one whose scores are
-// all -inf (its maximum never moved), or with a NaN among them (a weight without bounds), has NaN.
-__device__ __forceinline__ float row_factor(int seen, float m, float l) {
-    return seen <= 0 ? 0.f : m == LOWEST || !(l < CUDART_INF_F) ? CUDART_NAN_F : 1.f / l;
-}
+// What a row's sums are multiplied by, and its log-sum-exp; a row that sees nothing has zeros.
+__device__ __forceinline__ float row_factor(int seen, float l) { return seen > 0 ? 1.f / l : 0.f; }
 __device__ __forceinline__ float row_lse(int seen, float m, float l) {
-    return seen <= 0 || m == LOWEST ? -CUDART_INF_F : l < CUDART_INF_F ? (m + log2f(l)) * 0.69314718055994531f : CUDART_NAN_F;
+    return seen > 0 ? (m + log2f(l)) * 0.69314718055994531f : -CUDART_INF_F;
 }
 
 __device__ __forceinline__ void st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -322,13 +303,13 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
     uint64_t *sfull = qempty + 1, *sfree = sfull + 2, *pready = sfree + 2, *odone = pready + 2, *tbar = odone + 2, *gbar = tbar + 2;
     uint64_t *both = gbar + 4, *drain = both + 1, *pair_bar = drain + 1;  // tbar: a row tile's warps, gbar: a warpgroup's
     static_assert((2 * STAGES + 26) * 8 <= 336, "barriers");
-    long long *line = (long long *)(smem + L::MISC);  // the line's length, a share of it
+    long long *line = (long long *)(smem + L::MISC);  // whether this CTA has work (>= 0), a share of the line
     uint32_t *tslot = (uint32_t *)(line + 2);
     volatile int *stop = (volatile int *)(tslot + 1);
     volatile int *by_hand = stop + 1;        // [2]: this step's values are added by the warpgroup
     volatile int *last_flag = by_hand + 2;   // [2]
     Segment<R> *start = (Segment<R> *)(last_flag + 2);
-    static_assert(sizeof(Segment<R>) <= 128 - 40 && L::MISC % 8 == 0, "the first segment");
+    static_assert(sizeof(Segment<R>) <= 160 - 40 && L::MISC % 8 == 0, "the first segment");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (warp == L::MMA_WARP) {
@@ -363,8 +344,9 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
     // The line's length, this CTA's share of it, and the sequence of the share's first step.
     if (warp == 0) {
         // steps of each lane's sequence, for one key head
+        Seq s{0, 0, 0};  // this lane's of the last 32 sequences
         auto steps_of = [&](int b, bool tell) {
-            Seq s{0, 0, 0};
+            s = {0, 0, 0};
             if (b < a.seqs) s.set(a, b, tell);
             const int qts = s.n ? s.row_tiles(a, R) : 0;
             long long sum = 0;
@@ -373,22 +355,22 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
             } else {
                 // Row tiles of tp whole tokens, of which the i-th sees off + i tp: the sum of ceil((off + i tp) / 128), in
                 // closed form where one of tp and 128 is a multiple of the other.
-                const int tp = R / a.group, off = s.len - s.n;
-                const bool closed = tp * a.group == R && (tp & (tp - 1)) == 0 && off >= 0;
+                const int off = s.len - s.n, shift = a.tp_shift;
+                const bool closed = shift >= 0 && off >= 0;
                 if (qts && closed) {
-                    const long long full = s.n / tp;
-                    if (tp >= BK) {
-                        sum = full * ((off + BK - 1) / BK) + full * (full + 1) / 2 * (tp / BK);
+                    const int full = s.n >> shift;
+                    if (shift >= 7) {
+                        sum = (long long)full * ((off + BK - 1) / BK) + ((long long)full * (full + 1) / 2 << (shift - 7));
                     } else {
-                        const int m = BK / tp;  // (off + 127 + i tp) / 128 = ((off + 127) / tp + i) / m
-                        auto down = [&](long long k) {  // 0 / m + 1 / m + ... + k / m, rounded down each
-                            const long long q = k / m;
-                            return m * (q * (q - 1) / 2) + q * (k - q * m + 1);
+                        const int m = 7 - shift;  // (off + 127 + i tp) / 128 = ((off + 127) / tp + i) / 2^m
+                        auto down = [&](uint32_t k) {  // 0 / 2^m + 1 / 2^m + ... + k / 2^m, rounded down each
+                            const long long q = k >> m;
+                            return ((q * (q - 1) / 2) << m) + q * (long long)((k & ((1u << m) - 1)) + 1);
                         };
-                        const long long x = (off + BK - 1) / tp;
+                        const uint32_t x = (uint32_t)(off + BK - 1) >> shift;
                         sum = down(x + full) - down(x);
                     }
-                    if (full * tp < s.n) sum += s.steps(a, R, qts - 1);
+                    if (full << shift < s.n) sum += s.steps(a, R, qts - 1);
                 }
                 unsigned many = __ballot_sync(~0u, qts && !closed);  // the others by the whole warp
                 while (many) {
@@ -402,7 +384,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                     if (lane == l) sum += part;
                 }
             }
-            return sum;
+            return sum + (long long)qts * ITEM;
         };
         long long total = 0, held = 0;
         for (int b0 = 0; b0 < a.seqs; b0 += 32) {
@@ -412,9 +394,10 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
             total += sum;
         }
         total *= a.kv_heads;
-        const long long share = max((long long)MIN_SHARE, ratio(total + gridDim.x - 1, gridDim.x)), first = share * blockIdx.x;
+        const long long share = max((long long)(ITEM + MIN_SHARE), ratio(total + gridDim.x - 1, gridDim.x)), first = share * blockIdx.x;
         long long before = 0, per = 0;  // steps of the sequences ahead, and of the one that is found, for one key head
         int found = -1;
+        Seq its{0, 0, 0};
         for (int b0 = 0; b0 < a.seqs && found < 0 && first < total; b0 += 32) {
             const long long n = a.seqs <= 32 ? held : steps_of(b0 + lane, false);
             long long incl = n;
@@ -428,6 +411,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                 found = b0 + l;
                 before += __shfl_sync(~0u, incl - n, l);
                 per = __shfl_sync(~0u, n, l);
+                its = {__shfl_sync(~0u, s.s0, l), __shfl_sync(~0u, s.n, l), __shfl_sync(~0u, s.len, l)};
             } else {
                 before += __shfl_sync(~0u, incl, 31);
             }
@@ -435,7 +419,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
         if (found >= 0) {  // its first step: the key head, and the row tile within it
             Segment<R> seg;
             seg.b = found;
-            seg.seq.set(a, found, false);
+            seg.seq = its;
             seg.qts = seg.seq.row_tiles(a, R);
             seg.left = min(share, total - first);
             long long in = first - before * a.kv_heads;
@@ -443,12 +427,12 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
             in -= seg.h * per;
             seg.qt = 0;
             if (!a.causal) {
-                const int n = seg.seq.steps(a, R, 0);
+                const int n = seg.seq.steps(a, R, 0) + ITEM;
                 seg.qt = (int)ratio(in, n);
                 in -= (long long)seg.qt * n;
             } else {
                 for (; seg.qt < seg.qts; seg.qt += 32) {  // 32 row tiles at a time
-                    const int qt = seg.qt + lane, n = qt < seg.qts ? seg.seq.steps(a, R, qt) : 0;
+                    const int qt = seg.qt + lane, n = qt < seg.qts ? seg.seq.steps(a, R, qt) + ITEM : 0;
                     long long incl = n;
                     for (int o = 1; o < 32; o <<= 1) {
                         const long long v = __shfl_up_sync(~0u, incl, o);
@@ -465,19 +449,21 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                 }
             }
             seg.steps = seg.seq.steps(a, R, seg.qt);
-            seg.t0 = (int)in;
+            seg.x0 = (int)in;
+            seg.item = first - in;
             seg.clip();
+            if (seg.t0 == seg.t1 && !seg.next(a)) found = -1;
             if (lane == 0) *start = seg;
         }
-        if (lane == 0) line[0] = total, line[1] = share;
+        if (lane == 0) line[0] = found, line[1] = share;
     }
     __syncwarp();
     tc05::fence_before();
     __syncthreads();
     tc05::fence_after();
     const uint32_t tmem = *tslot;
-    const long long total = line[0], share = line[1], first = share * blockIdx.x;
-    const bool works = first < total && !*stop;
+    const long long share = line[1];
+    const bool works = line[0] >= 0 && !*stop;
     Segment<R> seg;
     if (works) seg = *start;
     __syncwarp();
@@ -618,6 +604,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                                  o < 0 ? 0 : 16);
                         }
                         issued(&full[s]);
+                        if (a.box) flush();  // (the others are not reported behind it)
                     }
                     return true;
                 };
@@ -687,6 +674,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                     if (APART && ok) ok = fill(j, p0, false);
                     p0 = p1, p1 = p2, p2 = p3;
                 }
+                flush();
             } while (ok && seg.next(a));
         flush();
         if (a.box)  // what was issued has landed before shared memory goes, whichever role gives up
@@ -814,7 +802,6 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
             tc05::fence_after();
             return r;
         };
-        long long item_first = first - (works ? seg.t0 : 0);  // the line's index of the item's first step
         bool counted = false;
         if (ok) do {
                 const int n = seg.t1 - seg.t0, rows = seg.rows(a);
@@ -941,13 +928,8 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                             for (int i = 0; i < 16; ++i) {
                                 const uint64_t y = fma2(two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c2, m2);
                                 float lo, hi;
-                                if (i % EMULATED == EMULATED - 1) {
-                                    exp2_pair(y, lo, hi);
-                                } else {
-                                    split2(y, lo, hi);
-                                    lo = exp2_(lo), hi = exp2_(hi);
-                                }
-                                v[i] = pack(lo, hi, T());
+                                split2(y, lo, hi);
+                                v[i] = pack(exp2_(lo), exp2_(hi), T());
                                 put(v[i]);
                             }
                             __syncwarp();
@@ -1086,9 +1068,9 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                     out += tk * a.o_tok + hd * a.o_head;
                     if (lse) lse += tk * a.lse_tok + hd * a.lse_head;
                 }
-                const int c_first = (int)ratio(item_first, share), c_last = (int)ratio(item_first + seg.steps - 1, share);
+                const int c_first = seg.first_share(share), c_last = seg.last_share(share);
                 if (c_first == c_last) {
-                    const float inv = row_factor(seen, m, l);
+                    const float inv = row_factor(seen, l);
 #pragma unroll 1
                     for (int col = col0; col < col1; col += 8) {
                         float v[8];
@@ -1145,7 +1127,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                                 const float2 v = __ldcg(pst + slot(c_first + k) * 512 + row);
                                 S += exp2_(v.x - M) * v.y;
                             }
-                            const float inv = row_factor(seen, M, S);
+                            const float inv = row_factor(seen, S);
 #pragma unroll 1
                             for (int k = 0; k < k_parts; ++k) {
                                 float2 *p = pst + slot(c_first + k) * 512 + row;
@@ -1191,17 +1173,15 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                 ok = everyone();
                 if (!ok) break;
                 tc05::fence_after();
-                item_first += seg.steps;
                 base += 2 * n * PARTS;
                 if (!seg.next(a)) break;
             } while (true);
         if (!ok && works && row == 0) {
             // Gave up: the counters of the cut items of this share are counted on, so that they end at zero.
             do {
-                const int c_first = (int)ratio(item_first, share), c_last = (int)ratio(item_first + seg.steps - 1, share);
+                const int c_first = seg.first_share(share), c_last = seg.last_share(share);
                 if (c_first != c_last && !counted) atomicInc(a.counts + wg * MAX_GRID + c_first, c_last - c_first);
                 counted = false;
-                item_first += seg.steps;
             } while (seg.next(a));
         }
         tc05::fence_before();
@@ -1365,6 +1345,9 @@ extern "C" int hv_paged_chunk_attention(const hv_chunk_args *p, void *stream) {
     a.o_vec = dec::aligned(a.out, 16) && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
     // A score is taken times a scale above zero, with q negated for one below, so that the largest stays the
     // largest and -inf that; for zero the least normal number gives the weights of 0.
+    a.tp_shift = -1;
+    for (int i = 0, rows = p->dim <= 128 ? 256 : 128; rows >> i; ++i)
+        if (rows >> i == rows / a.group && rows % a.group == 0) a.tp_shift = __builtin_ctz(rows / a.group);
     a.negate = p->scale < 0;
     a.scale_log2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, FLT_MIN);
     a.skip = dec::skipped_copy();
