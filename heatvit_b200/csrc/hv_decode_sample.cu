@@ -14,8 +14,8 @@
 // place for every pass, and the same bits come again.  w itself is taken in 64 bits (2^-35 of it off at
 // most): in 32 the sum of a flat row of 131072 would be off by enough to move one draw in a hundred.
 // That exponential, eleven operations in 64 bits of which an SM has 64 a clock, is what a row that is not cut short by
-// top_k or min_p costs beside its bytes, so of two sides of a cut the one with fewer logits is summed.  (A table of roots
-// of two saves three of them and its reads collide in shared memory: 1024 x 65536 272 us.)
+// top_k or min_p costs beside its bytes.  (A table of roots of two saves three of them and its reads collide in shared
+// memory: 1024 x 65536 272 us.)
 //
 // The search: the logits of the interval that holds the cut are counted in NB bins; bounds of the
 // bins' weights give a narrower interval; a pass with exact sums checks it.  When it holds CAP logits
@@ -106,6 +106,11 @@ struct Cut {
     __device__ __forceinline__ bool keeps(float v, int at) const { return v > z || (v == z && at <= i); }
 };
 
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+    for (int o = 16; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
+    return v;
+}
+
 // What a pass finds: sums and counts, and the keys of the extremes, of the whole row after meet().
 struct Found {
     u64 above, in;
@@ -113,6 +118,11 @@ struct Found {
     __device__ __forceinline__ void add(const Found &o) {
         above += o.above, in += o.in, over += o.over, n += o.n;
         least = min(least, o.least), most = max(most, o.most);
+    }
+    __device__ __forceinline__ void over_lanes() {
+        above = warp_sum(above), in = warp_sum(in);
+        over = __reduce_add_sync(~0u, over), n = __reduce_add_sync(~0u, n);
+        least = __reduce_min_sync(~0u, least), most = __reduce_max_sync(~0u, most);
     }
 };
 
@@ -125,14 +135,8 @@ struct Shared {
     Cut cut;
     double bounds[WARPS][2];
     float lo, hi;
-    uint32_t below, over, through;
     int at, first_b, last_b;
 };
-
-__device__ __forceinline__ u64 warp_sum(u64 v) {
-    for (int o = 16; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
-    return v;
-}
 
 // A row's slice as the cluster's CTA has it, and what the CTAs tell one another.
 template <typename T, bool HELD>
@@ -180,40 +184,52 @@ struct Row {
             f(z, first + c * CHUNK + (int)(threadIdx.x & 31) * VEC);
         }
     }
-    // The same for the chunks with a logit from l to h alone.
+    // f(logit, index) for the logits from l to h; a lane goes through its own.
     template <typename F>
     __device__ __forceinline__ void each_with(float l, float h, F f) const {
         each_vec([&](const float (&z)[VEC], int at) {
-            bool any = false;
+            uint32_t some = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) any |= z[j] >= l && z[j] <= h;
-            if (__any_sync(~0u, any)) f(z, at);
+            for (int j = 0; j < VEC; ++j) some |= (uint32_t)(z[j] >= l && z[j] <= h) << j;
+#pragma unroll 1
+            for (; some; some &= some - 1) {
+                const int i = at + __ffs(some) - 1;
+                f(to_f32(HELD ? held[i - first] : global[i]), i);
+            }
+            __syncwarp();
         });
     }
     // The sum of a warp's, then of every warp's and CTA's, findings.
     __device__ __forceinline__ Found meet(Found f) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        f.above = warp_sum(f.above), f.in = warp_sum(f.in);
-        f.over = __reduce_add_sync(~0u, f.over), f.n = __reduce_add_sync(~0u, f.n);
-        f.least = __reduce_min_sync(~0u, f.least), f.most = __reduce_max_sync(~0u, f.most);
+        f.over_lanes();
         __syncthreads();
         if (lane == 0) sh.parts[warp] = f;
         __syncthreads();
         const int b = turn++ & 1;
-        if (threadIdx.x < ranks) {
-            f = sh.parts[0];
-            for (int w = 1; w < WARPS; ++w) f.add(sh.parts[w]);
-            cluster.map_shared_rank(&sh, threadIdx.x)->of_rank[b][rank] = f;
+        if (warp == 0) {
+            f = lane < WARPS ? sh.parts[lane] : Found{0, 0, 0, 0, ~0u, 0};
+            f.over_lanes();
+            if (lane < ranks) cluster.map_shared_rank(&sh, lane)->of_rank[b][rank] = f;
         }
         sync();
         f = sh.of_rank[b][0];
         for (int r = 1; r < ranks; ++r) f.add(sh.of_rank[b][r]);
         return f;
     }
+    // (What is read of another CTA's memory, and written to it, is so ahead of a meeting: a CTA may leave after its last.)
     // After meet(): what the CTAs ahead of this one found.
     __device__ __forceinline__ Found ahead() const {
         Found f{0, 0, 0, 0, ~0u, 0};
         for (int r = 0; r < rank; ++r) f.add(sh.of_rank[(turn & 1) ^ 1][r]);
+        return f;
+    }
+
+    // And what the warps ahead of this one did.
+    __device__ __forceinline__ Found warps_ahead() const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        Found f = lane < warp ? sh.parts[lane] : Found{0, 0, 0, 0, ~0u, 0};
+        f.over_lanes();
         return f;
     }
 
@@ -222,14 +238,14 @@ struct Row {
     __device__ __forceinline__ Found look(const Cut &cut, float l, float h, float hi, W weigh) {
         Found f{0, 0, 0, 0, ~0u, 0};
         float least = CUDART_INF_F, most = -CUDART_INF_F;
-        each_with(fmaxf(l, cut.z), hi, [&](const float (&z)[VEC], int at) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const bool is = z[j] >= l && z[j] <= hi && cut.keeps(z[j], at + j), over = is && z[j] > h, in = is && z[j] <= h;
-                const u64 w = weigh(z[j]);
-                f.above += over ? w : 0, f.over += over;
-                f.in += in ? w : 0, f.n += in;
-                least = in ? fminf(least, z[j]) : least, most = in ? fmaxf(most, z[j]) : most;
+        each_with(fmaxf(l, cut.z), hi, [&](float z, int i) {
+            if (!cut.keeps(z, i)) return;
+            const u64 w = weigh(z);
+            if (z > h) {
+                f.above += w, ++f.over;
+            } else {
+                f.in += w, ++f.n;
+                least = fminf(least, z), most = fmaxf(most, z);
             }
         });
         f.least = key_of(least), f.most = key_of(most);
@@ -239,13 +255,8 @@ struct Row {
     template <typename W>
     __device__ __forceinline__ Found sum(const Cut &cut, const Cut *but, W weigh) {
         Found f{0, 0, 0, 0, ~0u, 0};
-        each_with(cut.z, but ? but->z : CUDART_INF_F, [&](const float (&z)[VEC], int at) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const bool is = cut.keeps(z[j], at + j) && !(but && but->keeps(z[j], at + j));
-                const u64 w = weigh(z[j]);
-                f.in += is ? w : 0, f.n += is;
-            }
+        each_with(cut.z, but ? but->z : CUDART_INF_F, [&](float z, int i) {
+            if (cut.keeps(z, i) && !(but && but->keeps(z, i))) f.in += weigh(z), ++f.n;
         });
         return meet(f);
     }
@@ -264,16 +275,12 @@ struct Row {
 
     // The index of the r-th (from 1) of the kept logits equal to z, in the row's order.
     __device__ __forceinline__ int nth_equal(const Cut &cut, float z, u64 r) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int lane = threadIdx.x & 31;
         Found f{0, 0, 0, 0, ~0u, 0};
-        each_with(z, z, [&](const float (&v)[VEC], int at) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) f.n += v[j] == z && cut.keeps(v[j], at + j);
-        });
+        each_with(z, z, [&](float v, int i) { f.n += cut.keeps(v, i); });
         const uint32_t mine = __reduce_add_sync(~0u, f.n);
         meet(f);
-        u64 before = ahead().n;
-        for (int w = 0; w < warp; ++w) before += sh.parts[w].n;
+        u64 before = ahead().n + warps_ahead().n;
         if (before < r && before + mine >= r) {  // in this warp's chunks
             int c0, c1;
             chunks(c0, c1);
@@ -309,22 +316,17 @@ struct Row {
 
     // Counts of the kept logits of [lo, hi] in NB bins from the top, in rank 0, which then sets l and h everywhere: between
     // them lies, by bounds of the bins' weights, what brings `above` to `target`.  bound(z, up): a bound of a weight.
-    // sh.below: how many lie under l, less how many lie above h.
     template <typename B>
-    __device__ __forceinline__ void narrow(const Cut &cut, float lo, float hi, u64 above, u64 target, B bound, float &l, float &h, bool &few_below,
-                                           uint32_t &number) {
+    __device__ __forceinline__ void narrow(const Cut &cut, float lo, float hi, u64 above, u64 target, B bound, float &l, float &h, uint32_t &number) {
         const int tid = threadIdx.x, lane = tid & 31;
         for (int i = tid; i < NB; i += THREADS) sh.hist[i] = 0;
         const float s = (float)NB / (hi - lo);
         sync();
-        each_vec([&](const float (&z)[VEC], int at) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                // the nearest integer to (hi - z) s - 1/2, by an addition whose last bit it is (NaN, of an infinite
-                // interval, and what is out of it: the first bin)
-                const int b = __float_as_int(fmaxf(fmaf(hi - z[j], s, 8388607.5f), 8388608.f)) - 0x4b000000;
-                if (z[j] >= lo && z[j] <= hi && cut.keeps(z[j], at + j)) atomicAdd(&sh.hist[min(NB - 1, b)], 1u);
-            }
+        each_with(lo, hi, [&](float z, int i) {
+            // the nearest integer to (hi - z) s - 1/2, by an addition whose last bit it is (NaN, of an infinite interval: the
+            // first bin)
+            const int b = __float_as_int(fmaxf(fmaf(hi - z, s, 8388607.5f), 8388608.f)) - 0x4b000000;
+            if (cut.keeps(z, i)) atomicAdd(&sh.hist[min(NB - 1, b)], 1u);
         });
         __syncthreads();
         if (rank) {
@@ -339,67 +341,59 @@ struct Row {
             constexpr int PER = NB / THREADS;
             const int warp = tid >> 5;
             double most[PER], least[PER], m0 = 0, l0 = 0;
-            uint32_t count[PER], c0 = 0;
+            uint32_t count[PER], all = 0;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int b = tid * PER + i;
                 count[i] = sh.hist[b];
                 most[i] = count[i] ? count[i] * bound(fminf(hi, hi - (b - 0.05f) / s), true) : 0.0;
                 least[i] = count[i] ? count[i] * bound(fmaxf(lo, hi - (b + 1.05f) / s), false) : 0.0;
-                m0 += most[i], l0 += least[i], c0 += count[i];
+                m0 += most[i], l0 += least[i], all += count[i];
             }
             const double m_own = m0, l_own = l0;
-            const uint32_t c_own = c0;
+            all = __reduce_add_sync(~0u, all);
             for (int o = 1; o < 32; o <<= 1) {
                 const double v = __shfl_up_sync(~0u, m0, o), w = __shfl_up_sync(~0u, l0, o);
-                const uint32_t x = __shfl_up_sync(~0u, c0, o);
-                if (lane >= o) m0 += v, l0 += w, c0 += x;
+                if (lane >= o) m0 += v, l0 += w;
             }
-            if (tid == 0) sh.first_b = sh.last_b = NB, sh.over = sh.through = 0;
-            if (lane == 31) sh.bounds[warp][0] = m0, sh.bounds[warp][1] = l0, sh.parts[warp].n = c0;
+            if (tid == 0) sh.first_b = sh.last_b = NB;
+            if (lane == 31) sh.bounds[warp][0] = m0, sh.bounds[warp][1] = l0, sh.parts[warp].n = all;
             __syncthreads();
-            uint32_t all = 0;
+            all = 0;
             for (int w = 0; w < WARPS; ++w) {
-                if (w < warp) m0 += sh.bounds[w][0], l0 += sh.bounds[w][1], c0 += sh.parts[w].n;
+                if (w < warp) m0 += sh.bounds[w][0], l0 += sh.bounds[w][1];
                 all += sh.parts[w].n;
             }
-            m0 += (double)above - m_own, l0 += (double)above - l_own, c0 -= c_own;  // ahead of this thread's bins
-            uint32_t cum[PER];
+            m0 += (double)above - m_own, l0 += (double)above - l_own;  // ahead of this thread's bins
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                m0 += most[i], l0 += least[i], c0 += count[i], cum[i] = c0;
+                m0 += most[i], l0 += least[i];
                 if (count[i] && m0 >= (double)target * (1 - 1e-9)) atomicMin(&sh.first_b, tid * PER + i);
                 if (count[i] && l0 >= (double)target * (1 + 1e-9)) atomicMin(&sh.last_b, tid * PER + i);
             }
             __syncthreads();
             const int first_b = sh.first_b, last_b = sh.last_b;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (tid * PER + i == first_b) sh.over = cum[i] - count[i];
-                if (tid * PER + i == last_b) sh.through = cum[i];
-            }
-            __syncthreads();
             l = last_b >= NB ? lo : fmaxf(lo, hi - (last_b + 1.05f) / s);
             h = first_b >= NB ? hi : fminf(hi, hi - (first_b - 0.05f) / s);
             if (tid < ranks) {
                 Shared *to = cluster.map_shared_rank(&sh, tid);
-                to->lo = l, to->hi = h, to->below = last_b < NB && all - sh.through < sh.over, to->n = all;
+                to->lo = l, to->hi = h, to->n = all;
             }
         }
         sync();
-        l = sh.lo, h = sh.hi, few_below = sh.below, number = sh.n;
+        l = sh.lo, h = sh.hi, number = sh.n;
         if (!(l <= h)) l = lo, h = hi;
     }
 
     // The cut at which the weights of the kept logits, added in their order, first reach `target` (from 1 up to their
-    // sum).  They lie in [lo, hi], their sum is `total`, and there are `number` of them at most.
-    // kept: how many the cut keeps, or up to CAP fewer.
+    // sum).  It lies in [lo, hi], with none above, and `number` of them at most.  kept: how many the cut keeps, or up to
+    // CAP fewer.
     template <typename W, typename B>
-    __device__ __forceinline__ Cut search(const Cut &cut, float lo, float hi, u64 total, uint32_t number, u64 target, W weigh, B bound,
+    __device__ __forceinline__ Cut search(const Cut &cut, float lo, float hi, uint32_t number, u64 target, W weigh, B bound,
                                           uint32_t &kept) {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-        u64 above = 0, in = total;  // sums of those above hi, and of those in [lo, hi]; `number` of these
-        kept = 0;                   // of those above hi, for now
+        u64 above = 0;  // the sum of those above hi
+        kept = 0;       // their number, for now
         bool halve = false;
         for (;;) {
             if (lo == hi) {  // one value
@@ -411,11 +405,8 @@ struct Row {
                 if (tid == 0) sh.n = 0;
                 sync();
                 Shared *to = cluster.map_shared_rank(&sh, 0);
-                each_with(lo, hi, [&](const float (&z)[VEC], int at) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (z[j] >= lo && z[j] <= hi && cut.keeps(z[j], at + j))
-                            to->cand[atomicAdd(&to->n, 1u)] = (u64)~key_of(z[j]) << 32 | (uint32_t)(at + j);
+                each_with(lo, hi, [&](float z, int i) {
+                    if (cut.keeps(z, i)) to->cand[atomicAdd(&to->n, 1u)] = (u64)~key_of(z) << 32 | (uint32_t)i;
                 });
                 sync();
                 if (rank == 0) {
@@ -456,31 +447,19 @@ struct Row {
             }
             const uint32_t kl = key_of(lo), kh = key_of(hi);
             float l, h;
-            bool few_below = false;
             if (halve) {
                 l = of_key(kl + (kh - kl) / 2 + ((kh - kl) & 1)), h = hi;
             } else {
-                narrow(cut, lo, hi, above, target, bound, l, h, few_below, number);
+                narrow(cut, lo, hi, above, target, bound, l, h, number);
             }
             halve = !halve && key_of(h) - key_of(l) >= (kh - kl) / 2;
-            // Exact sums of [l, h] and of one side of it; the other's is the rest.
-            Found f;
-            if (few_below) {
-                const Found g = look(cut, lo, ahead_of(l), h, weigh);  // "above" is [l, h] here
-                f = look(cut, l, h, h, [](float) -> u64 { return 0; });
-                f.in = g.above, f.above = in - g.above - g.in, f.over = number - g.over - g.n;
-            } else {
-                f = look(cut, l, h, hi, weigh);
-            }
+            const Found f = look(cut, l, h, hi, weigh);
             if (above + f.above < target && target <= above + f.above + f.in) {
-                lo = of_key(f.least), hi = of_key(f.most), above += f.above, kept += f.over, in = f.in, number = f.n;
+                lo = of_key(f.least), hi = of_key(f.most), above += f.above, kept += f.over, number = f.n;
                 continue;
             }
-            if (above + f.above >= target) {  // above what was tried
-                lo = after(h), in = f.above;
-            } else {  // below
-                hi = ahead_of(l), above += f.above + f.in, kept += f.over + f.n, in -= f.above + f.in;
-            }
+            if (above + f.above >= target) lo = after(h);  // above what was tried
+            else hi = ahead_of(l), above += f.above + f.in, kept += f.over + f.n;
             const Found g = look(cut, lo, hi, hi, [](float) -> u64 { return 0; });
             lo = of_key(g.least), hi = of_key(g.most), number = g.n;
         }
@@ -567,7 +546,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
             a.tokens[r] = at;
             if (a.logprobs) a.logprobs[r] = none ? CUDART_NAN_F : 0.f;
         }
-        row.sync();  // no CTA leaves while its memory may be read
         return;
     }
     const Weigh weigh{(double)m, 1.4426950408889634 / (double)temp, m, a.shift};
@@ -586,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         const Found all = row.sum(cut, nullptr, one);
         uint32_t kept;
         if (all.in > (u64)top_k)
-            cut = row.search(cut, cut.z, m, all.in, all.n, (u64)top_k, one, [](float, bool) { return 1.0; }, kept);
+            cut = row.search(cut, cut.z, m, all.n, (u64)top_k, one, [](float, bool) { return 1.0; }, kept);
     }
     // The kept weights, a sum for each warp's chunks, and their total.
     // (2^-900 is still a number in 64 bits)
@@ -594,13 +572,15 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
                        weigh(nothing) == 0;
     const Found all = whole ? row.sum_all(weigh, nothing) : row.sum(cut, nullptr, weigh);
     const uint32_t number = whole ? (uint32_t)a.vocab : all.n;
-    u64 mine = sh.parts[warp].in, before = row.ahead().in, total = all.in;
-    for (int w = 0; w < warp; ++w) before += sh.parts[w].in;
+    u64 mine = sh.parts[warp].in, before = row.ahead().in + row.warps_ahead().in, total = all.in;
     if (top_p < 1.f && number > 1) {
         const u64 target = max(1ull, part_of(fmaxf(top_p, 0.f), total, true));
         const Cut was = cut;
         uint32_t kept;
-        cut = row.search(was, was.z, m, total, number, target, weigh, [&](float z, bool up) {
+        // Logits that all together could not make up the rest of the sum are under the cut.
+        const double rest = (1.0 - fmax(0.0, (double)top_p)) * (double)total / number / (double)(1ull << a.shift);
+        const float floor = __double2float_rd((double)m + (double)temp * log(rest) * (1 + 1e-6) - 1e-6 * (double)temp);
+        cut = row.search(was, floor == floor ? fminf(fmaxf(was.z, floor), m) : was.z, m, number, target, weigh, [&](float z, bool up) {
             const double w = (double)exp2f((float)(((double)z - weigh.m) * weigh.c)) * (double)(1ull << a.shift);
             return up ? w * (1 + 1e-5) + 1 : fmax(0.0, w * (1 - 1e-5) - 1);
         }, kept);
@@ -608,8 +588,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         const bool less = kept > number / 2;
         const Found f = less ? row.sum(was, &cut, weigh) : row.sum(cut, nullptr, weigh);
         const u64 own = sh.parts[warp].in;
-        u64 ahead = row.ahead().in;
-        for (int w = 0; w < warp; ++w) ahead += sh.parts[w].in;
+        const u64 ahead = row.ahead().in + row.warps_ahead().in;
         total = less ? total - f.in : f.in;
         before = less ? before - ahead : ahead;
         mine = less ? mine - own : own;
@@ -653,7 +632,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
             before += __shfl_sync(~0u, s, 31);
         }
     }
-    row.sync();
 }
 
 template <typename T, bool HELD>
