@@ -1,14 +1,17 @@
-"""The serving step of a language decoder that reads the encoder's tokens.
+"""What a language decoder that reads the encoder's tokens runs, from a prompt to its next token.
 
-Four operators that belong together, on torch CUDA tensors, on the caller's
+Operators that belong together, on torch CUDA tensors, on the caller's
 current stream: the norm writes the e4m3 rows that the GEMM multiplies, the GEMM's
-q, k and v are what the append rotates and stores, and the attention reads that
-cache.  Floating point, inference only, with no counterpart in the reference.
+q, k and v are what the append norms, rotates and stores, the attentions (of a prompt's tokens, and of
+one new token a sequence) read that cache, and a token is drawn from the last GEMM's logits.
+Floating point, inference only, with no counterpart in the reference.
 
     rows = add_rmsnorm_fp8(x, weight, residual=r)          # 8 bits, a scale for each 128 channels
     qkv = gemm_fp8(rows.q, rows.scale, w, w_scale)         # [tokens, (heads + 2 kv_heads) * dim]
-    q = append_kv(k, v, k_cache, v_cache, page_table, positions, rope=table, q=q)
-    out = paged_attention(q, k_cache, v_cache, page_table, lens)
+    q = append_kv(k, v, k_cache, v_cache, page_table, positions, rope=table, q=q, q_weight=qw, k_weight=kw)
+    out = paged_chunk_attention(q, k_cache, v_cache, page_table, lens, starts)  # prompts, or pieces of them
+    out = paged_attention(q, k_cache, v_cache, page_table, lens)                # one new token a sequence
+    ids = sample_tokens(logits, uniform, temperature=0.8, top_p=0.95)
 
 The last dimension of every tensor is contiguous; the others may have any stride
 (a cache may be [pages, page, kv_heads, dim] in memory or a transposed view of
@@ -64,7 +67,8 @@ def _done(result):
 
 def device_error(device=None):
     """Read and clear the decode error bits of a device (synchronises with it):
-    abi.HV_DECODE_BAD_PAGE, _BAD_POSITION, _BAD_LENGTH, _STALLED; 0 when all went well."""
+    abi.HV_DECODE_BAD_PAGE, _BAD_POSITION, _BAD_LENGTH, _STALLED, _BAD_LOGITS, _BAD_START; 0 when all
+    went well."""
     torch = _torch()
     bits = C.c_int()
     with torch.cuda.device(device):
@@ -154,7 +158,7 @@ class AttentionWorkspace:
     """Device memory that ``paged_attention`` joins split sequences in, for one device
     (the current one unless named) and any sizes.  Calls that share one must not overlap
     in time (one per stream).  Waits for the device to have zeroed its counters, so that
-    any stream may use it.  With ``chunks`` a larger one (5 MB become 39), which
+    any stream may use it.  With ``chunks`` a larger one (5 MB become 40), which
     ``paged_chunk_attention`` can use as well."""
 
     def __init__(self, device=None, chunks=False):
