@@ -482,6 +482,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    // A CTA's memory may be written by another once it has begun: said here, waited for ahead of the first meeting.
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.release;\n" ::: "memory");
     const long long r = blockIdx.x / ranks;
     const int first = (int)min((long long)a.vocab, (long long)rank * a.slice), end = (int)min((long long)a.vocab, first + (long long)a.slice);
     Row<T, HELD> row{(const T *)a.logits + r * a.stride, held, sh, cluster, first, end, a.wide, rank, ranks, 0};
@@ -536,6 +538,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         });
     }
     Found f{0, 0, 0, 0, ~0u, top == top ? key_of(top) : ~0u};
+    if (ranks > 1) asm volatile("barrier.cluster.wait.acquire;\n" ::: "memory");
     f = row.meet(f);
     const float m = of_key(f.most);
     const bool none = f.most == ~0u || m == -CUDART_INF_F;
