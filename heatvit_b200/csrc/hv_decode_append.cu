@@ -229,8 +229,8 @@ __device__ __forceinline__ uint64_t swapped(uint64_t v) {
 // thread has it once for the NH heads that it takes.
 //
 // Measured on one B200: 8 ragged prompts (24,004 tokens, 40 + 2 x 8 heads of 96 in fp16, two thirds rotated in
-// neighbouring pairs) 119 us, 4.3 TB/s of what is read and written (a quarter of its lanes have no place); 12,004 tokens of
-// 48 heads of 128 63 us, 4.7 TB/s; a decode step of 64 sequences 2.6 us, the launch and three memory latencies.
+// neighbouring pairs) 146 us, 3.6 TB/s of what is read and written (a quarter of its lanes have no place); 12,004 tokens of
+// 48 heads of 128 69 us, 4.3 TB/s; a decode step of 64 sequences 2.6 us, the launch and three memory latencies.
 template <typename T, bool INTER, int NH>
 __global__ void __launch_bounds__(THREADS) norm_append_kernel(const __grid_constant__ AppendArgs a) {
     griddep_wait();
@@ -450,10 +450,12 @@ template <typename T>
 int launch_norm(AppendArgs &a, int tokens, bool wide, bool inter, int sms, cudaStream_t st) {
     // 32 lanes hold 256 elements of a head that is not rotated, or in neighbouring pairs; all three share a layout
     if (!wide || a.dim > 256) return launch_norm_any<T>(a, tokens, inter, st);
-    // One head a thread until that fills the SMs' threads twice, then four: the 8 prompts above took 242 us with one, 157
-    // with two, 119 with four, the 12,004 tokens 87, 68 and 63; the decode step 2.6, 3.1 and 3.9.
-    if ((double)tokens * a.dim / 8 * (a.t[0].heads + 2.0 * a.t[1].heads) <= 2.0 * 2048 * sms)
-        return inter ? launch_norm<T, true, 1>(a, tokens, st) : launch_norm<T, false, 1>(a, tokens, st);
+    // One head a thread until that fills the SMs' threads once, two until four times, then four.  us with one, two and
+    // four: the 8 prompts above 270, 183, 146; 48 heads of 128, 12,004 tokens 91.5, 72.4, 69.1; 2048 15.1, 11.7, 11.4; 1024
+    // 8.5, 6.8, 7.7; 512 5.3, 4.3, 5.1; 256 3.9, 3.8, 4.1; 128 3.1, 3.2, 4.1; the decode step 2.6, 3.2, 3.9.
+    const double threads = (double)tokens * a.dim / 8 * (a.t[0].heads + 2.0 * a.t[1].heads), room = 2048.0 * sms;
+    if (threads <= room) return inter ? launch_norm<T, true, 1>(a, tokens, st) : launch_norm<T, false, 1>(a, tokens, st);
+    if (threads <= 4 * room) return inter ? launch_norm<T, true, 2>(a, tokens, st) : launch_norm<T, false, 2>(a, tokens, st);
     return inter ? launch_norm<T, true, 4>(a, tokens, st) : launch_norm<T, false, 4>(a, tokens, st);
 }
 

@@ -105,6 +105,30 @@ def test_norm_append_many_tokens(heads, kv, interleaved, rot):
     assert torch.equal(vc[pg, slot], v)
 
 
+@pytest.mark.parametrize("dtype,interleaved,rot", [(BF, False, 128), (HF, True, 64)])
+@pytest.mark.parametrize("heads,kv", [(31, 1), (8, 3)])
+@pytest.mark.parametrize("tokens", [700, 1400, 6000])
+def test_norm_append_is_the_same_whatever_comes_with_it(tokens, heads, kv, dtype, interleaved, rot):
+    """A token's bits do not depend on how many heads a thread takes: calls of few, of some and of many tokens."""
+    from heatvit_b200 import decode
+    dim, page = 128, 64
+    table, pages = make_table(1, [tokens], page)
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    seq = torch.zeros_like(pos)
+    q, k, v = (rand(s, tokens, n, dim, dtype=dtype) for s, n in ((2, heads), (3, kv), (4, kv)))
+    qw, kw = ((1 + rand(s, dim, scale=0.3)).to(dtype) for s in (8, 9))
+    rope = decode.rope_table(tokens, rot)
+    results = []
+    for step in (tokens, 64):
+        kc, vc = (make_cache(s, pages, page, kv, dim, dtype, "nhd") for s in (5, 6))
+        parts = [decode.append_kv(k[i:i + step], v[i:i + step], kc, vc, table, pos[i:i + step], seq_ids=seq[i:i + step], rope=rope,
+                                  q=q[i:i + step], interleaved=interleaved, q_weight=qw, k_weight=kw) for i in range(0, tokens, step)]
+        results.append((torch.cat(parts), kc, vc))
+    for whole, pieces in zip(*results):
+        assert torch.equal(whole, pieces)
+    near(results[0][0], rotate64(normed64(q, qw, 1e-6), rope, pos.long(), rot, interleaved), 16.0)
+
+
 @pytest.mark.parametrize("dim", [64, 36])
 def test_norm_append_in_place_without_q_and_extreme_heads(dim):
     """q_out = q; no q; heads of zeros, of the type's largest values, and with a NaN, which stays its head's."""
