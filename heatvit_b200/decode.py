@@ -199,7 +199,7 @@ def paged_chunk_attention(q, k_cache, v_cache, page_table, lens, starts, causal=
     the newest tokens of sequence i, of which the cache has ``lens[i]`` in all; a sequence may
     bring none.  ``causal``: a token sees those up to itself; otherwise each sees all
     ``lens[i]``.  A row that sees no token gives zeros (log-sum-exp -inf); rows of no sequence are not
-    written, neither in ``out`` nor in a new tensor.  The rest as ``paged_attention``.
+    written, neither in ``out`` (which may be q) nor in a new tensor.  The rest as ``paged_attention``.
 
     ``workspace``: an AttentionWorkspace made with ``chunks=True``."""
     return _done((_native or _load()).paged_chunk_attention(

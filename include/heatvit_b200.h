@@ -407,7 +407,7 @@ HV_API int hv_selector_h2(hv_model *model, int selector_index, const int8_t *d_x
 #define HV_DECODE_BAD_LENGTH 4   /* a length above max_pages * page_size or HV_ATTENTION_MAX_LENGTH: taken as that */
 #define HV_DECODE_STALLED 8      /* a bounded wait gave up: that call's output is invalid */
 #define HV_DECODE_BAD_LOGITS 16  /* a row of logits with a NaN or with nothing above -inf: its token is 0, its logprob NaN */
-#define HV_DECODE_BAD_START 32   /* starts that fall, or lie outside [0, tokens]: taken as the nearest that do not */
+#define HV_DECODE_BAD_START 32   /* starts outside [0, tokens], taken as the nearest inside, or that fall: that sequence has no rows */
 
 /* Read and clear the current device's error word (synchronises with the device). */
 HV_API int hv_decode_error(int *bits);

@@ -162,6 +162,24 @@ def test_chunk_strided_q_and_out():
         assert torch.equal(plain_out, out)
 
 
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(4, 2, 64, HF), (5, 1, 128, BF), (8, 1, 256, BF)])
+def test_chunk_out_may_be_q(heads, kv, dim, dtype):
+    """Whole items and items that many shares cut, rows behind the last sequence, and a sequence of no rows."""
+    q, kc, vc, table, lens, starts = chunk_case(28, [300, 0, 2, 90], [50, 10, 9000, 0], heads, kv, dim, 16, dtype, rest=3)
+    want, _ = check(q, kc, vc, table, lens, starts)
+    got, _ = check_in_place(q, kc, vc, table, lens, starts)
+    assert got is q and torch.equal(got[:starts[-1]], want[:starts[-1]])
+
+
+def check_in_place(q, *rest):
+    from heatvit_b200 import decode
+    kc, vc, table, lens, starts = rest
+    behind = q[starts[-1]:].clone()
+    result = decode.paged_chunk_attention(q, kc, vc, table, ints(lens), ints(starts), out=q, return_lse=True)
+    assert torch.equal(q[starts[-1]:], behind)
+    return result
+
+
 def test_chunk_scale_and_wide_scores():
     q, kc, vc, table, lens, starts = chunk_case(9, [50, 200], [300, 0], 4, 2, 128, 16, BF)
     for scale in (0.0, 0.5, -0.25):
