@@ -25,9 +25,9 @@
 // is written straight out; one that is cut leaves parts (unnormalised sums, maximum, sum of weights, in 32
 // bits) in the workspace, and the CTA that finishes last joins them in the order of the shares.
 //
-// Measured on one B200 (calls in a long run): 8192 new tokens over 16384 (32 heads of 128 over 8, bf16) 3.13 ms, 2.80 in
-// bursts (982 TFLOP/s); 16 x 6 tokens over 32768 486 us, 409 in bursts (5.2 TB/s of cache); 24 prompts of up to 4001 tokens
-// (24 heads of 64 over 6, fp16) 1.12 ms; 3 x 1499 of heads of 256 132 us; 4 x 5 tokens over 300 24 us, latency.  The operands
+// Measured on one B200 (calls in a long run): 8192 new tokens over 16384 (32 heads of 128 over 8, bf16) 3.13 ms, 2.73 to
+// 2.80 in bursts (982 to 1007 TFLOP/s); 16 x 6 tokens over 32768 480 us, 382 to 410 in bursts (5.2 to 5.6 TB/s of cache); 24 prompts of up to 4001 tokens
+// (24 heads of 64 over 6, fp16) 1.11 ms; 3 x 1499 of heads of 256 131 us; 4 x 5 tokens over 300 24 us, latency.  The operands
 // of the products in uniform registers (the whole warp goes through the loop, one lane issues) took a 128^3 from 950 clocks
 // to 520.  TMA, the second softmax warpgroup and the line's length in closed form came in together and were not timed
 // apart: the first of these calls from 3.64 to 3.19 ms, the second from 580 to 506 us.

@@ -15,12 +15,16 @@
 // most): in 32 the sum of a flat row of 131072 would be off by enough to move one draw in a hundred.
 // That exponential, eleven operations in 64 bits of which an SM has 64 a clock, is what a row that is not cut short by
 // top_k or min_p costs beside its bytes.  (A table of roots of two saves three of them and its reads collide in shared
-// memory: 1024 x 65536 272 us.)
+// memory: 1024 x 65536 took 272 us with it when it took 225 without.)
 //
 // The search: the logits of the interval that holds the cut are counted in NB bins; bounds of the
 // bins' weights give a narrower interval; a pass with exact sums checks it.  When it holds CAP logits
 // or fewer these are sorted and the cut is read off; when it holds one value, by its count.  An
 // interval that the bins do not narrow is halved by its bit patterns, so that the search ends.
+//
+// Measured on one B200, in a graph: 1024 x 65536 of float32 201 us uncut (1.3 TB/s),
+// 118 greedy, which weighs nothing; 256 x 131072 of bfloat16 with top_p 0.95 219 to 379, the more the flatter; 48 x 50021 of float32 15.5 uncut, 32 with top_k 50, 64 with top_p
+// 0.95; 1 x 1000 3.7 greedy, 6 uncut, 20 with a search, whose steps wait for one another.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
