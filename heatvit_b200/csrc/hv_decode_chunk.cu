@@ -47,6 +47,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "hv_chunk_order.cuh"
 #include "hv_decode.cuh"
 #include "hv_tc05.cuh"
 
@@ -94,11 +95,12 @@ __device__ __forceinline__ long long ratio(long long a, long long b) {
 
 template <int D>
 struct Lay {
-    static constexpr int DP = (D + 63) / 64 * 64;  // dimensions in shared memory: 128-byte blocks of 64
-    static constexpr int NT = D <= 128 ? 2 : 1, R = 128 * NT;
-    static constexpr int SLOT = DP <= 128 ? 128 : 64, PARTS = BK / SLOT;  // keys of a ring slot
+    static constexpr chunk::Order ORDER = chunk::order_of(D);
+    static constexpr int DP = chunk::padded_dim(D);  // dimensions in shared memory: 128-byte blocks of 64
+    static constexpr int NT = ORDER.row_tiles, R = 128 * NT;
+    static constexpr int PARTS = ORDER.parts, SLOT = BK / PARTS;  // keys of a ring slot
     static constexpr int SLOT_BYTES = SLOT * DP * 2, Q_TILE = 128 * DP * 2, Q_BYTES = NT * Q_TILE;
-    static constexpr int STAGES = DP == 64 ? 8 : DP == 128 ? 5 : DP == 192 ? 7 : 5;
+    static constexpr int STAGES = ORDER.stages;
     static constexpr int STAT = Q_BYTES + STAGES * SLOT_BYTES;  // [4][128] float: what the softmax warpgroups tell one another
     static constexpr int BARS = STAT + 2048, MISC = BARS + 336, BYTES = MISC + 160;
     // A row tile has two softmax warpgroups, with 64 keys of a step each; then four copying warps, then the products'.
@@ -109,7 +111,10 @@ struct Lay {
     static_assert(128 * (COPY_REGS + MMA_REGS + GROUPS * SOFT_REGS) <= REGS * THREADS, "registers");
     // TMEM columns: scores, sums, weights.  APART: the weights have columns of their own, so that the next scores are
     // under way while they are made; with two row tiles of 128 dimensions they have to take the scores' place.
-    static constexpr bool APART = NT == 1 || DP == 64;
+    static constexpr bool APART = ORDER.apart;
+    // Heads of 256: the ring is so short that the slot of a step's last values may still await the step before's.
+    static constexpr bool POLL_AFTER_SUMS = !ORDER.values_may_be_polled(false, 12);
+    static_assert(ORDER.values_may_be_polled(POLL_AFTER_SUMS, 12), "a poll that may end on an older fill");
     __host__ __device__ static constexpr int s_col(int w) { return w * BK; }
     __host__ __device__ static constexpr int o_col(int w) { return 256 + w * DP; }
     __host__ __device__ static constexpr int p_col(int w, int h) {  // of the first and the last 64 keys
@@ -477,13 +482,8 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
     Segment<R> seg;
     if (works) seg = *start;
     __syncwarp();
-    // Which ring fill, from the segment's first, holds the keys (values) of its step j of n.  The keys of the first `lead`
-    // steps come first, then those of step j + lead and the values of step j, in the order of their use: keys ahead
-    // where scores go ahead of sums (APART), else values.
     constexpr bool APART = L::APART;
-    auto lead_of = [](bool alt) { return alt ? 2 : 1; };
-    auto k_fill = [](int j, int lead) { return (j < lead ? j : 2 * j - lead + !APART) * PARTS; };
-    auto v_fill = [](int j, int n, int lead) { return (j + lead < n + !APART ? lead + 2 * j + APART : n + j) * PARTS; };
+    constexpr chunk::Order ORDER = L::ORDER;
 
     if (warp >= L::SOFT_WARPS && warp < L::MMA_WARP) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(L::COPY_REGS));
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
         if (ok) do {
                 const int n = seg.t1 - seg.t0, rows = seg.rows(a), head = seg.h;
                 const bool alt = NT == 2 && rows <= 128;
-                const int lead = lead_of(alt);
+                const int lead = ORDER.lead_of(alt);
                 const long long table = seg.b * a.pages_stride;
                 auto page_at = [&](int t) { return a.pages[table + (a.page_shift >= 0 ? t >> a.page_shift : t / a.page)]; };
                 // Pages.  With boxes a lane holds one of a window of `steps` steps' boxes, so that loads are far ahead; else
@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                     // Units: either row tile in turn against each step's keys, or the one against the steps in turn.
                     const int n = seg.t1 - seg.t0;
                     const bool alt = NT == 2 && seg.rows(a) <= 128, pair = NT == 2 && !alt;
-                    const int lead = lead_of(alt), all = pair ? 2 * n : n;
+                    const int lead = ORDER.lead_of(alt), all = pair ? 2 * n : n;
                     ok = wait_all(qfull, qn++ & 1);
                     // the scores of unit i, and the sums of unit i - NT behind them (APART) or ahead of them
                     for (int i = 0; i < all + NT && ok; ++i) {
@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                         for (int e = 0; e < 2 && ok; ++e) {
                             if ((e == 0) == APART) {
                                 if (i >= all) continue;
-                                const uint32_t f = base + k_fill(pair ? i >> 1 : i, lead);
+                                const uint32_t f = base + ORDER.k_fill(pair ? i >> 1 : i, lead);
                                 ok = scores(NT == 2 ? i & 1 : 0, pair ? i & 1 : 0, f);
                                 if (!ok) break;
                                 if (!pair || i & 1) release(f);
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                             } else {
                                 const int u = i - NT;
                                 if (u < 0) continue;
-                                const uint32_t f = base + v_fill(pair ? u >> 1 : u, n, lead);
+                                const uint32_t f = base + ORDER.v_fill(pair ? u >> 1 : u, n, lead);
                                 ok = sums(NT == 2 ? u & 1 : 0, f, u >= NT);
                                 if (ok && (!pair || u & 1)) release(f);
                             }
@@ -893,7 +893,11 @@ __global__ void __launch_bounds__(Lay<D>::THREADS, 1)
                     uint32_t vf = 0;
                     if (first_seen < seg.seq.len && first_seen < k0 - h * 64 + BK) {
                         // Values that some row of the tile does not see: any that are no numbers?
-                        vf = base + v_fill(j, n, lead_of(alt));
+                        if (L::POLL_AFTER_SUMS) {
+                            ok = before_done();
+                            if (!ok) break;
+                        }
+                        vf = base + ORDER.v_fill(j, n, ORDER.lead_of(alt));
                         const uint32_t fp = vf + h * (PARTS - 1);
                         ok = __all_sync(~0u, wait_or_stop(&full[fp % STAGES], (fp / STAGES) & 1, stop));
                         if (!ok) break;

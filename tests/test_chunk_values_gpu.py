@@ -1,0 +1,59 @@
+"""Chunk attention on the GPU where values are infinite or not numbers, against the plain 64-bit form."""
+
+import math
+import os
+import sys
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+
+from test_chunk_attention_gpu import chunk_case, ints, plain  # noqa: E402
+from test_decode_gpu import BF, HF, clean  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+
+def hidden_values_stay_out(case, past, hidden, value):
+    """Values of the tokens `hidden` (from a sequence's first new token on) are `value` in every sequence: rows that do not see
+    the first of them are as if they were not there, the others are no numbers; three calls give the same bits."""
+    from heatvit_b200 import decode
+    q, kc, vc, table, lens, starts = case
+    want, _, bound = plain(q, kc, vc, table, lens, starts, True, q.shape[2] ** -0.5)
+    page = kc.shape[1]
+    row = torch.arange(q.shape[0], device="cuda")
+    for b in range(len(lens)):
+        t = torch.tensor([past[b] + h for h in hidden], device="cuda")
+        vc[table[b, t // page].long(), t % page] = value
+        row[starts[b]:starts[b + 1]] -= starts[b]
+    sees = row >= hidden[0]
+    first = None
+    for _ in range(3):
+        out = decode.paged_chunk_attention(q, kc, vc, table, ints(lens), ints(starts))
+        assert bool(((out.double() - want).abs() <= bound)[~sees].all())
+        assert not bool(out[sees].isfinite().any())
+        first = out if first is None else first
+        assert torch.equal(first.view(torch.int16), out.view(torch.int16))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("page", [1, 12, 16])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("group", [1, 2])
+def test_hidden_values_late_in_a_segment(dim, page, dtype, group):
+    """The border of what rows see lies in the last but one tile of keys, long after the maxima have settled, and the values in
+    its second half; there are more items than shares, so that segments are of up to all nine steps."""
+    seqs, kv = 24, 8
+    case = chunk_case(40, [40] * seqs, [1000] * seqs, kv * group, kv, dim, page, dtype)
+    hidden_values_stay_out(case, [1000] * seqs, [7, 20, 39], math.nan)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF), (128, HF), (192, BF), (256, BF), (256, HF)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("new,past,hidden", [(300, 700, [70, 200]), (130, 1987, [1, 60]), (5, 4000, [3])])
+def test_hidden_values_in_cut_items(dim, dtype, value, new, past, hidden):
+    """The same of a few sequences, whose items many shares cut, and of a border that crosses several tiles."""
+    case = chunk_case(41, [new] * 3, [past] * 3, 4, 2, dim, 16, dtype)
+    hidden_values_stay_out(case, [past] * 3, hidden, value)
