@@ -406,7 +406,7 @@ struct Row {
                 return {lo, r >= number ? cut.z == lo ? cut.i : INT32_MAX : nth_equal(cut, lo, r)};
             }
             if (number <= CAP) {
-                if (tid == 0) sh.n = 0;
+                if (tid == 0) sh.n = 0, sh.cut = cut;  // (what was kept, unless a candidate says less)
                 sync();
                 Shared *to = cluster.map_shared_rank(&sh, 0);
                 each_with(lo, hi, [&](float z, int i) {
@@ -584,8 +584,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         const u64 target = max(1ull, part_of(fmaxf(top_p, 0.f), total, true));
         const Cut was = cut;
         uint32_t kept;
-        // Logits that all together could not make up the rest of the sum are under the cut.
-        const double rest = (1.0 - fmax(0.0, (double)top_p)) * (double)total / number / (double)(1ull << a.shift);
+        // Logits that all together could not make up the rest of the sum are under the cut.  A logit counts for at most half a
+        // unit more than it weighs, which takes half a unit from what each has to weigh; where that leaves nothing (a
+        // logarithm of -inf or NaN) the search has no floor.
+        const double rest = ((1.0 - fmax(0.0, (double)top_p)) * (double)total / number - 0.5) / (double)(1ull << a.shift);
         const float floor = __double2float_rd((double)m + (double)temp * log(rest) * (1 + 1e-6) - 1e-6 * (double)temp);
         cut = row.search(was, floor == floor ? fminf(fmaxf(was.z, floor), m) : was.z, m, number, target, weigh, [&](float z, bool up) {
             const double w = (double)exp2f((float)(((double)z - weigh.m) * weigh.c)) * (double)(1ull << a.shift);
