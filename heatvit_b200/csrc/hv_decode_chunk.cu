@@ -40,6 +40,8 @@
 // The second product multiplies masked values by zero, which a NaN or an infinity survives.  Slots past a
 // sequence's end are zeros in shared memory; where a row does not see a token that others see, the warpgroup looks
 // through the value tile, and one that holds such a number is added by its threads, each taking what its row sees.
+// An infinite value that a row does see is its output's, unless the weight rounds to zero (fp16: under 2^-34 of the row's
+// largest; bf16: under 2^-120), which makes a NaN of it.
 #include <cudaTypedefs.h>
 #include <math_constants.h>
 
@@ -58,12 +60,14 @@ using namespace dec;
 
 // A running maximum before the first score, finite so that a score of -inf weighs exp2(-inf) = 0 and not NaN.
 constexpr float LOWEST = -3.402823466e38f;
-// fp16 weights begin at 2^9, so that those of a long tail keep their bits (normal numbers from 2^-14 to 2^15).
+// A row's largest weight is 2^TOP when its maximum moves, and 2^(TOP + SOFT) before it moves again.  bf16 weights stay at 1
+// and below, so that sums of large values overflow no sooner than those of exact weights; fp16 ones begin at 2^9, so
+// that those of a long tail keep their bits (normal numbers from 2^-14 to 2^15).
+constexpr float SOFT = 6.f;
 template <typename T>
-constexpr float TOP = 0.f;
+constexpr float TOP = -SOFT;
 template <>
 constexpr float TOP<__half> = 9.f;
-constexpr float SOFT = 6.f;
 constexpr int BK = 128;       // keys of a step
 constexpr int MIN_SHARE = 2;  // steps
 constexpr int ITEM = 3;       // steps' time that an item takes beside its steps: its rows of q, the join and its output

@@ -57,3 +57,47 @@ def test_hidden_values_in_cut_items(dim, dtype, value, new, past, hidden):
     """The same of a few sequences, whose items many shares cut, and of a border that crosses several tiles."""
     case = chunk_case(41, [new] * 3, [past] * 3, 4, 2, dim, 16, dtype)
     hidden_values_stay_out(case, [past] * 3, hidden, value)
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 1, 128), (2, 2, 256), (9, 1, 64), (20, 1, 192)])
+@pytest.mark.parametrize("new,n,equal", [(1, 1, True), (3, 70, True), (70, 70, False), (5, 3000, False), (200, 3000, False)])
+def test_infinite_values_that_are_seen(dtype, heads, kv, dim, new, n, equal):
+    """An infinity among the values that a row sees is its output, as in the formula, whatever its weight rounds
+    to (one and halves among them); two of either sign make a NaN."""
+    from heatvit_b200 import decode
+    q, kc, vc, table, lens, starts = chunk_case(42, [new] * 4, [n - new] * 4, heads, kv, dim, 16, dtype)
+    if equal:
+        q.zero_()
+    q[:, :, :8] *= 0.25
+    at = lambda b, t: (table[b, t // 16].long(), t % 16)  # noqa: E731
+    vc[at(0, (n - new) // 2)] = math.inf
+    vc[at(1, n - new)] = -math.inf  # the first row's own, which all see
+    vc[at(2, 0)], vc[at(2, n - 1)] = math.inf, -math.inf
+    if n == 1:
+        vc[at(2, 0)] = math.nan
+    out = decode.paged_chunk_attention(q, kc, vc, table, ints(lens), ints(starts), scale=0.02).unflatten(0, (4, new))
+    assert bool((out[0] == math.inf).all()) and bool((out[1] == -math.inf).all()) and bool(out[2, -1].isnan().all())
+    assert bool((out[2, :-1] == math.inf).all()) and bool(out[3].isfinite().all())
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 192, 256])
+@pytest.mark.parametrize("new,past,causal", [(3, 1021, False), (40, 1000, True), (260, 780, True)])
+def test_large_values_keep_their_sums(dim, new, past, causal):
+    """bf16 values whose sum, each times a weight of one at most, is a number in 32 bits: also where the scores rise, after a
+    row's first steps, by a little less than what its maximum has to be passed by to move."""
+    from heatvit_b200 import decode
+    n, seqs = new + past, 24  # items enough that segments are of many steps
+    q, kc, vc, table, lens, starts = chunk_case(43, [new] * seqs, [past] * seqs, 8, 8, dim, 16, BF)
+    q.zero_()
+    q[:, :, 0] = 1
+    at = torch.arange(n, device="cuda")
+    v = torch.rand(n, 8, dim, generator=torch.Generator("cuda").manual_seed(44), device="cuda")
+    for b in range(seqs):
+        place = table[b, at // 16].long(), at % 16
+        kc[place] = 0
+        kc[place[0][256:], place[1][256:], :, 0] = 4.0  # 5.8 powers of two above the first ones
+        vc[place] = ((v + 1) * 2.0 ** (126 - math.ceil(math.log2(n)))).to(BF)
+    want, _, bound = plain(q, kc, vc, table, lens, starts, causal, 1.0)
+    out = decode.paged_chunk_attention(q, kc, vc, table, ints(lens), ints(starts), causal=causal, scale=1.0)
+    assert bool(out.isfinite().all()) and bool(((out.double() - want).abs() <= bound).all())
