@@ -1362,12 +1362,13 @@ extern "C" int hv_paged_chunk_attention(const hv_chunk_args *p, void *stream) {
     a.q_vec = dec::aligned(a.q, 16) && a.q_tok % 8 == 0 && a.q_head % 8 == 0;
     a.o_vec = dec::aligned(a.out, 16) && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
     // A score is taken times a scale above zero, with q negated for one below, so that the largest stays the
-    // largest and -inf that; for zero the least normal number gives the weights of 0.
+    // largest and -inf that; for zero the least normal number gives the weights of 0.  A NaN stays one.
     a.tp_shift = -1;
     for (int i = 0, rows = p->dim <= 128 ? 256 : 128; rows >> i; ++i)
         if (rows >> i == rows / a.group && rows % a.group == 0) a.tp_shift = __builtin_ctz(rows / a.group);
     a.negate = p->scale < 0;
-    a.scale_log2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, FLT_MIN);
+    a.scale_log2 = fabsf(p->scale) * 1.4426950408889634f;
+    if (a.scale_log2 < FLT_MIN) a.scale_log2 = FLT_MIN;
     a.skip = dec::skipped_copy();
     a.counts = (uint32_t *)p->d_workspace;
     a.parts = (float *)((char *)p->d_workspace + HV_ATTENTION_COUNTER_BYTES);

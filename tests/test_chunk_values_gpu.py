@@ -101,3 +101,16 @@ def test_large_values_keep_their_sums(dim, new, past, causal):
     want, _, bound = plain(q, kc, vc, table, lens, starts, causal, 1.0)
     out = decode.paged_chunk_attention(q, kc, vc, table, ints(lens), ints(starts), causal=causal, scale=1.0)
     assert bool(out.isfinite().all()) and bool(((out.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, HF), (128, BF), (256, BF)])
+def test_scale_that_is_no_number(dim, dtype):
+    """A NaN for a scale is every row's, as in attention of one token; rows that see nothing are zeros all the same."""
+    from heatvit_b200 import decode
+    q, kc, vc, table, lens, starts = chunk_case(45, [40, 1, 150], [0, 700, 20], 4, 2, dim, 16, dtype)
+    lens[0] = 30  # the first ten rows stand before the first token
+    out, lse = decode.paged_chunk_attention(q, kc, vc, table, ints(lens), ints(starts), scale=math.nan, return_lse=True)
+    assert bool((out[:10] == 0).all()) and bool((lse[:10] == -math.inf).all())
+    assert bool(out[10:].isnan().all()) and bool(lse[10:].isnan().all())
+    one = decode.paged_attention(q[40:41], kc, vc, table[1:2], ints(lens[1:2]), scale=math.nan)
+    assert bool(one.isnan().all())
