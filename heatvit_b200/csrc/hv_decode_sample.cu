@@ -557,9 +557,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     }
     const Weigh weigh{(double)m, 1.4426950408889634 / (double)temp, m, a.shift};
 
-    // Logits that weigh nothing are never drawn: the lowest that may, and with min_p the lowest that is kept.
+    // Logits that weigh nothing are never drawn: the lowest that may, and with min_p the lowest that is kept.  (The sum of
+    // all weights has those below as well, so they must be zeros in it: half a unit, less far more than the 2^-35 that a
+    // weight may be off.)
     Cut cut{-CUDART_MAX_NORMAL_F, INT32_MAX};
-    const double lowest = (double)m - (a.shift + 1) / weigh.c;
+    const double lowest = (double)m - (a.shift + 1 + 1e-9) / weigh.c;
     if (lowest > cut.z) cut.z = fminf(__double2float_ru(lowest), m);
     const float live = cut.z, nothing = fmaxf(__double2float_rd((double)m - (a.shift + 2) / weigh.c), -CUDART_MAX_NORMAL_F);
     if (min_p > 0.f) {

@@ -88,3 +88,19 @@ def test_flat_tails_after_other_rows():
     for _ in range(2):
         graph.replay()
         assert bool((out[::2] == 0).all())
+
+
+@pytest.mark.parametrize("temperature,top,low", [
+    (0.9895793795585632, 31.55251121520996, -1.3288322664450902e-09), (0.9181880950927734, 29.276216506958008, -2.5560853433859165e-09),
+    (1.0416868925094604, 33.21394729614258, -2.039854729574131e-09), (0.9366442561149597, 29.864686965942383, 1.5098072791985828e-09)])
+def test_a_weight_of_half_a_unit(temperature, top, low):
+    """A logit that weighs half a unit to the last bit counts for one in every sum or in none: between two likely ones it has the
+    draw that falls on it."""
+    from heatvit_b200 import decode
+    assert all(float(np.float32(v)) == v for v in (temperature, top, low))
+    z = torch.full((3, 2048), -math.inf, device="cuda")
+    z[:, 0], z[:, 130], z[:, 300] = top, low, top
+    token, logprob = decode.sample_tokens(z, torch.tensor([0.4999, 0.5, 0.5001], device="cuda"), temperature=temperature, return_logprob=True)
+    # 2^45, one and 2^45 units: half of them, rounded down, is 2^45
+    assert token.tolist() == [0, 130, 300]
+    assert np.allclose(logprob.tolist(), [-math.log(2), -47 * math.log(2), -math.log(2)], rtol=2.0 ** -23)
