@@ -4,9 +4,10 @@
 //   seen(t) = lens - n + i + 1 for the i-th of a sequence's n new tokens (causal), or lens;
 //   a row that sees nothing gives zeros (and a log-sum-exp of -inf).
 //
-// Bound by the tensor cores for long prompts (4 d multiply-adds a pair of tokens and head, at 128 x 128 x 128 in 520
-// clocks), with heads of 64 by the exponentials (one a pair and head, 16 a clock and SM), and by HBM where few
-// tokens see a long cache.
+// Bound by the tensor cores beside the softmax, and then by power, for long prompts (4 d multiply-adds a pair of tokens and
+// head, at 128 x 128 x 128 in 520 clocks); with heads of 64 by the softmax, whose exponentials (one a pair and head, 16 a clock
+// and SM) are a third of it and reads of tensor memory, maxima, conversions and sums the rest; and where few tokens see a
+// long cache by HBM for a while, in a long run by power, since the rows of a tile that nobody has are worked on as well.
 //
 // Rows are (token, query head of a key head's group), so that a tile of 128 rows shares its keys
 // whatever the group is.  One CTA an SM: 4 warps copy keys and values into a ring of tiles, by TMA in boxes of slots where
@@ -25,9 +26,12 @@
 // is written straight out; one that is cut leaves parts (unnormalised sums, maximum, sum of weights, in 32
 // bits) in the workspace, and the CTA that finishes last joins them in the order of the shares.
 //
-// Measured on one B200 (calls in a long run): 8192 new tokens over 16384 (32 heads of 128 over 8, bf16) 3.13 ms, 2.73 to
-// 2.80 in bursts (982 to 1007 TFLOP/s); 16 x 6 tokens over 32768 480 us, 382 to 410 in bursts (5.2 to 5.6 TB/s of cache); 24 prompts of up to 4001 tokens
-// (24 heads of 64 over 6, fp16) 1.11 ms; 3 x 1499 of heads of 256 131 us; 4 x 5 tokens over 300 24 us, latency.  The operands
+// Measured on one B200 (calls in a long run): 8192 new tokens over 16384 (32 heads of 128 over 8, bf16) 3.08 to 3.13 ms at the
+// power limit (1.7 GHz), 2.73 to 2.83 in bursts (972 to 1007 TFLOP/s); 16 x 6 tokens over 32768 482 us, likewise (991 W, 1.48 GHz),
+// 382 to 410 in bursts (5.2 to 5.6 TB/s of cache); 24 prompts of up to 4001 tokens (24 heads of 64 over 6, fp16) 1.11 ms, short of that
+// limit; 3 x 1499 of heads of 256 130 us with pages of 24 (boxes of 8 slots), 117 with pages of 16, 64 and 256, 202 with pages of one
+// (cp.async): 18 steps an SM, of which the products are 1.1 us each, the ring (five slots, four a step) holding little ahead; 4 x 5 tokens
+// over 300 24 us, latency; 3 tokens each of 256, 1024 and 4096 sequences 56, 154 and 608 us, as one warp of each CTA goes through them.  The operands
 // of the products in uniform registers (the whole warp goes through the loop, one lane issues) took a 128^3 from 950 clocks
 // to 520.  TMA, the second softmax warpgroup and the line's length in closed form came in together and were not timed
 // apart: the first of these calls from 3.64 to 3.19 ms, the second from 580 to 506 us.

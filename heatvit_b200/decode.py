@@ -201,7 +201,8 @@ def paged_chunk_attention(q, k_cache, v_cache, page_table, lens, starts, causal=
     ``lens[i]``.  A row that sees no token gives zeros (log-sum-exp -inf); rows of no sequence are not
     written, neither in ``out`` (which may be q) nor in a new tensor.  The rest as ``paged_attention``.
 
-    ``workspace``: an AttentionWorkspace made with ``chunks=True``."""
+    ``workspace``: an AttentionWorkspace made with ``chunks=True`` (by default the module keeps one of
+    40 MB per stream, beside that of ``paged_attention``)."""
     return _done((_native or _load()).paged_chunk_attention(
         q, k_cache, v_cache, page_table, lens, starts, causal, scale, None if workspace is None else workspace.buffer, out,
         return_lse))
